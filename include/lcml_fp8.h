@@ -420,6 +420,114 @@ LCML_API int lcml_fp8_binary(int op, int dtype, const void *a, const int64_t *a_
                              void *stream);
 
 /*
+ * Residual addition, root-mean-square norm and the E4M3 codes of the result,
+ * the input of the next FP8 linear:
+ *   h[m,i] = x[m,i] + residual[m,i], rounded to the residual's type and
+ *            written to residual_out (x itself without a residual)
+ *   v[m,i] = h[m,i] * (1 / sqrt(mean_i h[m,i]^2 + eps)) * gamma[i]    (fp32)
+ *   y[m,i] = from_float(v[m,i] / s)    (IEEE fp32 divide, the encoder above)
+ * mode: LCML_SCALE_STATIC  s = scale[0], an input;
+ *       LCML_SCALE_TENSOR  s = max |v| / 448 of the tensor, written to
+ *                          scale[0]: lcml_fp8_gemm's a_scale;
+ *       LCML_SCALE_ROW     s = max |v| / 448 of row m, written to scale[m];
+ *   NaN is left out of the maximum, and s is 1 where that is not a positive
+ *   finite number.
+ * x: M rows of H, FLOAT or BFLOAT16, row pitch ldx elements; residual (may be
+ * NULL) and residual_out (may be NULL, may be `residual` itself): r_dtype
+ * FLOAT or BFLOAT16, pitches ldr, ldro; gamma: H floats; y: row pitch ldy
+ * bytes (lcml_fp8_gemm wants ldy % 16 == 0).  Any H >= 1; pointers aligned to
+ * their elements.  A row whose sum of squares overflows fp32 gives zeros
+ * (and NaN where its elements are infinite), as the formula does.
+ * workspace: lcml_fp8_rms_norm_workspace_bytes(M, H, mode) bytes, written
+ * before they are read (0: may be NULL).
+ * No counterpart in the reference, which has no norm operators.
+ */
+#define LCML_SCALE_STATIC 0
+#define LCML_SCALE_TENSOR 1
+#define LCML_SCALE_ROW 2
+LCML_API int64_t lcml_fp8_rms_norm_workspace_bytes(int64_t M, int64_t H, int mode);
+LCML_API int lcml_fp8_rms_norm(int64_t M, int64_t H, const void *x, int x_dtype, int64_t ldx, const void *residual,
+                               void *residual_out, int r_dtype, int64_t ldr, int64_t ldro, const float *gamma,
+                               float eps, uint8_t *y, int64_t ldy, int mode, float *scale, void *workspace,
+                               int64_t workspace_bytes, void *stream);
+
+/*
+ * The E4M3 KV cache: pages of page_tokens tokens (16, 32, 64, 128 or 256),
+ * with one fp32 scale for each page and KV head, a power of two.  No
+ * counterpart in the reference.
+ *   k_cache, v_cache: [pages][kv_heads] blocks of page_tokens * head_dim codes
+ *     (head_dim 16 to 256 in steps of 16); element e of slot t lies at byte
+ *       K: (t/16) * 16*head_dim + (e/16) * 256 + (t%16) * 16 + e%16
+ *       V: (t/4)  *  4*head_dim + e * 4 + t%4
+ *     of its block, the order in which attention's matrix instructions read;
+ *   k_scale, v_scale: [pages][kv_heads];
+ *   block_table: [seqs] rows of table_cols pages (row pitch table_stride),
+ *     the token at position p of sequence b is slot p % page_tokens of page
+ *     block_table[b][p / page_tokens];
+ *   kv_len[b]: tokens of sequence b, the call's own included;
+ *   cu_q[b] .. cu_q[b+1]: the call's rows of sequence b (cu_q[0] = 0), which
+ *     are its last tokens: row cu_q[b] + i is position kv_len[b] - n + i with
+ *     n = cu_q[b+1] - cu_q[b] <= max_q.
+ * The index arrays are int32 on the device.  A row whose position is negative
+ * or whose page is not in [0, pages) has no token: it is neither written nor
+ * read back, and attention does not see it.
+ *
+ * lcml_fp8_kv_cache_write stores rows of k and v [tokens][kv_heads][head_dim]
+ * (dtype FLOAT or BFLOAT16, strides in elements, elements of a head
+ * contiguous: slices of a QKV projection do).  The scale of a page and head is
+ * the smallest power of two s >= 2^-126 with |x| <= 448 s for its finite
+ * values, and y = from_float(x / s) (infinities saturate).  A page that is
+ * written from its first slot starts anew; one that holds earlier tokens keeps
+ * its scale while that is enough, else it takes the larger one and the codes
+ * that stay become from_float(to_float(c) * s_old / s), which is exact down to
+ * the smallest normal code.  Slots past the last token keep their bytes.
+ * Two sequences must not share a page that the call writes.
+ *
+ * lcml_fp8_kv_cache_read is its inverse: to_float(c) * s for the same rows.
+ */
+LCML_API int lcml_fp8_kv_cache_write(const void *k, const void *v, int dtype, int64_t tokens, int64_t k_token_stride,
+                                     int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                                     uint8_t *k_cache, uint8_t *v_cache, float *k_scale, float *v_scale, int64_t pages,
+                                     int64_t kv_heads, int64_t head_dim, int64_t page_tokens,
+                                     const int32_t *block_table, int64_t table_stride, int64_t table_cols,
+                                     const int32_t *kv_len, const int32_t *cu_q, int64_t seqs, int64_t max_q,
+                                     void *stream);
+LCML_API int lcml_fp8_kv_cache_read(const uint8_t *k_cache, const uint8_t *v_cache, const float *k_scale,
+                                    const float *v_scale, int64_t pages, int64_t kv_heads, int64_t head_dim,
+                                    int64_t page_tokens, const int32_t *block_table, int64_t table_stride,
+                                    int64_t table_cols, const int32_t *kv_len, const int32_t *cu_q, int64_t seqs,
+                                    int64_t max_q, void *k, void *v, int dtype, int64_t tokens, int64_t k_token_stride,
+                                    int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, void *stream);
+
+/*
+ * Attention over the E4M3 KV cache, for prompts, chunks of prompts and single
+ * tokens alike: for row cu_q[b] + i at position p = kv_len[b] - n + i,
+ *   o = sum_j w_j v_j / sum_j w_j,   w_j = exp(scale * q.k_j)
+ * over the positions j of sequence b with j < kv_len[b], j <= p if `causal`,
+ * and j > p - window if window > 0.  A row that sees no position, or only
+ * scores of -inf, gives 0.
+ * q, o: [tokens][q_heads][head_dim], FLOAT or BFLOAT16, strides in elements,
+ *   elements of a head contiguous; q head h reads KV head
+ *   h / (q_heads / kv_heads).
+ * Cache and index arguments as above; kv_len[b] <= max_kv and
+ * cu_q[b+1] - cu_q[b] <= max_q are the host's bounds (rows and positions past
+ * them are left out).  scale > 0.
+ * workspace: lcml_fp8_attention_workspace_bytes(...) bytes, 16-byte aligned,
+ * written before they are read (0: may be NULL).
+ * No counterpart in the reference.
+ */
+LCML_API int64_t lcml_fp8_attention_workspace_bytes(int64_t tokens, int64_t seqs, int64_t q_heads, int64_t kv_heads,
+                                                    int64_t head_dim, int64_t max_q, int64_t max_kv);
+LCML_API int lcml_fp8_attention(const void *q, int q_dtype, int64_t tokens, int64_t q_heads, int64_t q_token_stride,
+                                int64_t q_head_stride, void *o, int o_dtype, int64_t o_token_stride,
+                                int64_t o_head_stride, const uint8_t *k_cache, const uint8_t *v_cache,
+                                const float *k_scale, const float *v_scale, int64_t pages, int64_t kv_heads,
+                                int64_t head_dim, int64_t page_tokens, const int32_t *block_table,
+                                int64_t table_stride, int64_t table_cols, const int32_t *kv_len, const int32_t *cu_q,
+                                int64_t seqs, int64_t max_q, int64_t max_kv, float scale, int causal, int64_t window,
+                                void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
  * Measurement aid, no counterpart in the reference: reads `bytes` bytes
  * (a multiple of 16) at 16-byte aligned device pointer p with `workgroups`
  * workgroups of 512 threads, each streaming one contiguous, equal share

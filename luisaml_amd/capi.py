@@ -23,6 +23,7 @@ ACT_NONE, ACT_RELU, ACT_GELU_ERF, ACT_GELU_TANH = 0, 1, 2, 3
 KERNEL_AUTO, KERNEL_MFMA, KERNEL_SKINNY, KERNEL_VALU, KERNEL_MFMA_FP8, KERNEL_SKINNY_FP8 = 0, 1, 2, 3, 4, 5
 KERNEL_MFMA_128, KERNEL_MFMA_128_FP8 = 6, 7
 KERNEL_AUTO_FP8 = 8  # AUTO's tiling with the native FP8 MFMA kernels (opt-in)
+SCALE_STATIC, SCALE_TENSOR, SCALE_ROW = 0, 1, 2
 DYNAMIC_WORKSPACE_BYTES = 4096
 DYNAMIC_SMALL_MAX = 65536
 PACK_K, PANEL_COLS = 128, 64
@@ -76,6 +77,17 @@ _SIGS = {
     "lcml_fp8_sgemm": (_int, [_i64, _i64, _i64, _vp, _i64, _int, _vp, _i64, _int, _f32, _vp, _int, _i64,
                               _i64, _f32, _int, _vp, _int, _i64, _vp]),
     "lcml_fp8_activation": (_int, [_vp, _vp, _i64, _int, _vp]),
+    "lcml_fp8_rms_norm_workspace_bytes": (_i64, [_i64, _i64, _int]),
+    "lcml_fp8_rms_norm": (_int, [_i64, _i64, _vp, _int, _i64, _vp, _vp, _int, _i64, _i64, _vp, _f32, _vp, _i64, _int,
+                                 _vp, _vp, _i64, _vp]),
+    "lcml_fp8_kv_cache_write": (_int, [_vp, _vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64,
+                                       _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp]),
+    "lcml_fp8_kv_cache_read": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64,
+                                      _i64, _vp, _vp, _int, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "lcml_fp8_attention_workspace_bytes": (_i64, [_i64] * 7),
+    "lcml_fp8_attention": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _vp, _int, _i64, _i64, _vp, _vp, _vp, _vp, _i64,
+                                  _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _f32, _int, _i64,
+                                  _vp, _i64, _vp]),
     "lcml_fp8_stream_read": (_int, [_vp, _i64, _int, _vp, _vp]),
 }
 
@@ -469,3 +481,117 @@ def binary(op: int, a: torch.Tensor, b: torch.Tensor, dtype: int, out: torch.Ten
     _check(lib().lcml_fp8_binary(int(op), int(dtype), _ptr(a), sh(tuple(a.shape)), a.dim(), _ptr(b),
                                  sh(tuple(b.shape)), b.dim(), _ptr(y), sh(tuple(y.shape)), y.dim(), _stream(stream)))
     return y
+
+
+# ------------------------------------- norm, KV cache, attention -----------
+
+def rms_norm(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual: torch.Tensor | None = None,
+             residual_out: torch.Tensor | None = None, mode: int = SCALE_TENSOR, scale: torch.Tensor | None = None,
+             out: torch.Tensor | None = None, workspace: torch.Tensor | None = None, stream=None):
+    """h = x + residual, RMS norm of h, E4M3 codes of it: the input of an FP8
+    linear.  x [M,H] fp32/bf16; residual fp32/bf16; gamma [H] fp32.  mode
+    SCALE_STATIC takes scale[1]; SCALE_TENSOR gives it; SCALE_ROW gives [M].
+    Returns (codes uint8 [M,H], scale, h or None)."""
+    assert x.dim() == 2 and x.stride(1) == 1 and gamma.dtype == torch.float32 and gamma.is_contiguous()
+    M, H = x.shape
+    assert gamma.numel() == H
+    if residual is not None:
+        assert residual.shape == x.shape and residual.stride(1) == 1
+        if residual_out is None:
+            residual_out = torch.empty((M, H), dtype=residual.dtype, device=x.device)
+        assert residual_out.shape == x.shape and residual_out.stride(1) == 1 and residual_out.dtype == residual.dtype
+    elif residual_out is not None:
+        raise ValueError("residual_out without residual")
+    y = out if out is not None else torch.empty((M, H), dtype=torch.uint8, device=x.device)
+    assert y.dtype == torch.uint8 and y.shape == x.shape and y.stride(1) == 1
+    if scale is None:
+        assert mode != SCALE_STATIC, "SCALE_STATIC takes a scale"
+        scale = torch.empty(M if mode == SCALE_ROW else 1, dtype=torch.float32, device=x.device)
+    assert scale.dtype == torch.float32 and scale.is_contiguous() and scale.numel() >= (M if mode == SCALE_ROW else 1)
+    if workspace is None and mode == SCALE_TENSOR and M > 1:
+        workspace = torch.empty(lib().lcml_fp8_rms_norm_workspace_bytes(M, H, mode), dtype=torch.uint8, device=x.device)
+    r = residual is not None
+    _check(lib().lcml_fp8_rms_norm(M, H, _ptr(x), _DTYPE_CODE.get(x.dtype, 0), x.stride(0), _ptr(residual),
+                                   _ptr(residual_out), _DTYPE_CODE.get(residual.dtype, 0) if r else 0,
+                                   residual.stride(0) if r else 0, residual_out.stride(0) if r else 0, _ptr(gamma),
+                                   float(eps), _ptr(y), y.stride(0), int(mode), _ptr(scale), _ptr(workspace),
+                                   workspace.numel() * workspace.element_size() if workspace is not None else 0,
+                                   _stream(stream)))
+    return y, scale, residual_out
+
+
+def _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q):
+    assert k_cache.dtype == torch.uint8 and v_cache.dtype == torch.uint8 and k_cache.dim() == 4
+    assert k_cache.shape == v_cache.shape and k_cache.is_contiguous() and v_cache.is_contiguous()
+    assert k_scale.dtype == torch.float32 and v_scale.dtype == torch.float32
+    assert k_scale.shape == k_cache.shape[:2] == v_scale.shape and k_scale.is_contiguous() and v_scale.is_contiguous()
+    assert block_table.dtype == torch.int32 and kv_len.dtype == torch.int32 and cu_q.dtype == torch.int32
+    assert block_table.dim() == 2 and block_table.stride(1) == 1 and kv_len.is_contiguous() and cu_q.is_contiguous()
+    seqs = kv_len.numel()
+    assert block_table.shape[0] == seqs and cu_q.numel() == seqs + 1
+    pages, heads, page_tokens, dim = k_cache.shape
+    return ((_ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale)), (pages, heads, dim, page_tokens),
+            (_ptr(block_table), max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], _ptr(kv_len),
+             _ptr(cu_q), seqs))
+
+
+def _token_rows(x: torch.Tensor, heads: int, dim: int):
+    assert x.dim() == 3 and x.shape[1:] == (heads, dim) and (x.stride(2) == 1 or x.numel() == 0)
+    return x.stride(0), x.stride(1)
+
+
+def kv_cache(pages: int, kv_heads: int, page_tokens: int, head_dim: int, device):
+    """An empty E4M3 KV cache: (k_cache, v_cache, k_scale, v_scale)."""
+    shape = (pages, kv_heads, page_tokens, head_dim)
+    return (torch.zeros(shape, dtype=torch.uint8, device=device), torch.zeros(shape, dtype=torch.uint8, device=device),
+            torch.ones(shape[:2], device=device), torch.ones(shape[:2], device=device))
+
+
+def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   k_scale: torch.Tensor, v_scale: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,
+                   cu_q: torch.Tensor, max_q: int, stream=None) -> None:
+    """New tokens' k, v [tokens, kv_heads, head_dim] (fp32/bf16, any token and
+    head strides) into the cache [pages, kv_heads, page_tokens, head_dim], as
+    the last tokens of their sequences (kv_len counts them)."""
+    c, geo, idx = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q)
+    assert k.dtype == v.dtype and k.shape == v.shape
+    (kt, kh), (vt, vh) = _token_rows(k, geo[1], geo[2]), _token_rows(v, geo[1], geo[2])
+    _check(lib().lcml_fp8_kv_cache_write(_ptr(k), _ptr(v), _DTYPE_CODE.get(k.dtype, 0), k.shape[0], kt, kh, vt, vh, *c,
+                                         *geo, *idx, int(max_q), _stream(stream)))
+
+
+def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                  block_table: torch.Tensor, kv_len: torch.Tensor, cu_q: torch.Tensor, max_q: int, k_out: torch.Tensor,
+                  v_out: torch.Tensor, stream=None) -> None:
+    """The inverse of kv_cache_write: the same rows' tokens into k_out, v_out
+    [tokens, kv_heads, head_dim] (fp32 or bf16)."""
+    c, geo, idx = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q)
+    assert k_out.dtype == v_out.dtype and k_out.shape == v_out.shape
+    (kt, kh), (vt, vh) = _token_rows(k_out, geo[1], geo[2]), _token_rows(v_out, geo[1], geo[2])
+    _check(lib().lcml_fp8_kv_cache_read(*c, *geo, *idx, int(max_q), _ptr(k_out), _ptr(v_out),
+                                        _DTYPE_CODE.get(k_out.dtype, 0), k_out.shape[0], kt, kh, vt, vh,
+                                        _stream(stream)))
+
+
+def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+              v_scale: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor, cu_q: torch.Tensor, max_q: int,
+              max_kv: int, scale: float, causal: bool = True, window: int = 0, out: torch.Tensor | None = None,
+              out_dtype=None, workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """softmax(scale * q k^T) v over the E4M3 cache: q [tokens, q_heads,
+    head_dim] (fp32/bf16) are the last tokens of their sequences, which the
+    cache already holds.  window > 0: only the last `window` positions."""
+    c, geo, idx = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q)
+    tokens, heads, dim = q.shape
+    o = out if out is not None else torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
+    assert o.shape == q.shape
+    qt, qh = _token_rows(q, heads, geo[2])
+    ot, oh = _token_rows(o, heads, geo[2])
+    need = lib().lcml_fp8_attention_workspace_bytes(tokens, idx[5], heads, geo[1], dim, int(max_q), int(max_kv))
+    if need and workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _check(lib().lcml_fp8_attention(_ptr(q), _DTYPE_CODE.get(q.dtype, 0), tokens, heads, qt, qh, _ptr(o),
+                                    _DTYPE_CODE.get(o.dtype, 0), ot, oh, *c, *geo, *idx, int(max_q), int(max_kv),
+                                    float(scale), int(causal), int(window), _ptr(workspace),
+                                    workspace.numel() * workspace.element_size() if workspace is not None else 0,
+                                    _stream(stream)))
+    return o

@@ -8,6 +8,7 @@
 #include <atomic>
 
 #include "../../include/lcml_fp8.h"
+#include "kv_cache.hpp"
 #include "lcml_internal.hpp"
 
 namespace {
@@ -46,6 +47,8 @@ int hip_status(hipError_t err, const char *what, const char *label = nullptr) {
 }
 
 bool aligned(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+bool float_or_bf16(int dtype) { return dtype == LCML_DTYPE_FLOAT || dtype == LCML_DTYPE_BFLOAT16; }
+bool elem_aligned(const void *p, int dtype) { return aligned(p, dtype == LCML_DTYPE_BFLOAT16 ? 2 : 4); }
 
 int check_view(int64_t outer, int64_t axis_len, int64_t inner, const char *fn) {
     if (outer < 0 || axis_len < 1 || inner < 0)
@@ -806,6 +809,178 @@ int lcml_fp8_binary(int op, int dtype, const void *a, const int64_t *a_shape, in
     if (dtype == LCML_DTYPE_FLOAT && (!aligned(a, 4) || !aligned(b, 4) || !aligned(y, 4)))
         return fail(LCML_ERR_INVALID_ARG, "%s: fp32 tensors must be 4-byte aligned", fn);
     return hip_status(lcml::launch_fp8_binary(op, dtype, a, b, y, n, same, g, (hipStream_t)stream), fn);
+}
+
+int64_t lcml_fp8_rms_norm_workspace_bytes(int64_t M, int64_t H, int mode) {
+    return M > 1 && H > 0 && mode == LCML_SCALE_TENSOR ? lcml::rms_norm_workspace(M) : 0;
+}
+
+int lcml_fp8_rms_norm(int64_t M, int64_t H, const void *x, int x_dtype, int64_t ldx, const void *residual,
+                      void *residual_out, int r_dtype, int64_t ldr, int64_t ldro, const float *gamma, float eps,
+                      uint8_t *y, int64_t ldy, int mode, float *scale, void *workspace, int64_t workspace_bytes,
+                      void *stream) {
+    const char *fn = "lcml_fp8_rms_norm";
+    if (M < 0 || H <= 0) return fail(LCML_ERR_INVALID_ARG, "%s: M=%lld H=%lld", fn, (long long)M, (long long)H);
+    if (!float_or_bf16(x_dtype)) return fail(LCML_ERR_UNSUPPORTED, "%s: x dtype %d", fn, x_dtype);
+    if (mode < LCML_SCALE_STATIC || mode > LCML_SCALE_ROW) return fail(LCML_ERR_INVALID_ARG, "%s: mode %d", fn, mode);
+    if (!(eps >= 0.0f)) return fail(LCML_ERR_INVALID_ARG, "%s: eps %g", fn, (double)eps);
+    if (residual) {
+        if (!float_or_bf16(r_dtype)) return fail(LCML_ERR_UNSUPPORTED, "%s: residual dtype %d", fn, r_dtype);
+        if (ldr < H || (residual_out && ldro < H))
+            return fail(LCML_ERR_INVALID_ARG, "%s: residual pitch below H=%lld", fn, (long long)H);
+    } else if (residual_out) {
+        return fail(LCML_ERR_INVALID_ARG, "%s: residual_out without residual", fn);
+    }
+    if (ldx < H || ldy < H) return fail(LCML_ERR_INVALID_ARG, "%s: pitch below H=%lld", fn, (long long)H);
+    if (M >= (int64_t)1 << 31 || H >= (int64_t)1 << 31)
+        return fail(LCML_ERR_UNSUPPORTED, "%s: M=%lld H=%lld", fn, (long long)M, (long long)H);
+    if (M == 0) return LCML_OK;
+    if (!x || !gamma || !y || !scale) return fail(LCML_ERR_INVALID_ARG, "%s: NULL pointer", fn);
+    if (!elem_aligned(x, x_dtype) || (residual && (!elem_aligned(residual, r_dtype) || !elem_aligned(residual_out, r_dtype))) ||
+        !aligned(gamma, 4) || !aligned(scale, 4))
+        return fail(LCML_ERR_INVALID_ARG, "%s: pointer not aligned to its elements", fn);
+    if (const int64_t need = lcml_fp8_rms_norm_workspace_bytes(M, H, mode);
+        need && (!workspace || workspace_bytes < need || !aligned(workspace, 4)))
+        return fail(LCML_ERR_INVALID_ARG, "%s: needs a workspace of %lld bytes", fn, (long long)need);
+    return hip_status(lcml::launch_rms_norm(M, H, x, x_dtype == LCML_DTYPE_BFLOAT16, ldx, residual, residual_out,
+                                            r_dtype == LCML_DTYPE_BFLOAT16, ldr, ldro, gamma, eps, y, ldy, mode, scale,
+                                            workspace, (hipStream_t)stream),
+                      fn);
+}
+
+namespace {
+// The cache arguments of the three KV entry points.
+int make_tokens(lcml::KvTokens &t, const char *fn, int64_t tokens, const void *k_cache, const void *v_cache,
+                const float *k_scale, const float *v_scale, int64_t pages, int64_t kv_heads, int64_t head_dim,
+                int64_t page_tokens, const int32_t *block_table, int64_t table_stride, int64_t table_cols,
+                const int32_t *kv_len, const int32_t *cu_q, int64_t seqs, int64_t max_q) {
+    if (tokens < 0 || seqs < 0 || max_q < 0 || pages < 0 || table_cols < 0 || kv_heads <= 0)
+        return fail(LCML_ERR_INVALID_ARG, "%s: tokens=%lld seqs=%lld max_q=%lld pages=%lld table_cols=%lld kv_heads=%lld",
+                    fn, (long long)tokens, (long long)seqs, (long long)max_q, (long long)pages, (long long)table_cols,
+                    (long long)kv_heads);
+    if (head_dim < 16 || head_dim > 256 || head_dim % 16)
+        return fail(LCML_ERR_UNSUPPORTED, "%s: head_dim=%lld (16 to 256, in steps of 16)", fn, (long long)head_dim);
+    if (page_tokens < 16 || page_tokens > 256 || (page_tokens & (page_tokens - 1)))
+        return fail(LCML_ERR_UNSUPPORTED, "%s: page_tokens=%lld (16, 32, 64, 128 or 256)", fn, (long long)page_tokens);
+    const int64_t most = ((int64_t)1 << 31) - 1;
+    if (tokens > most || seqs > most || pages > most || table_cols > most || kv_heads > 65535 || max_q > most)
+        return fail(LCML_ERR_UNSUPPORTED, "%s: a size of 2^31 or more", fn);
+    if (table_stride < table_cols)
+        return fail(LCML_ERR_INVALID_ARG, "%s: table_stride=%lld < table_cols=%lld", fn, (long long)table_stride,
+                    (long long)table_cols);
+    if (tokens == 0 || seqs == 0 || max_q == 0) return LCML_OK;
+    if ((table_cols && !block_table) || !kv_len || !cu_q) return fail(LCML_ERR_INVALID_ARG, "%s: NULL index array", fn);
+    if (!aligned(block_table, 4) || !aligned(kv_len, 4) || !aligned(cu_q, 4))
+        return fail(LCML_ERR_INVALID_ARG, "%s: index arrays not 4-byte aligned", fn);
+    if (pages && (!k_cache || !v_cache || !k_scale || !v_scale)) return fail(LCML_ERR_INVALID_ARG, "%s: NULL cache", fn);
+    if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(k_scale, 4) || !aligned(v_scale, 4))
+        return fail(LCML_ERR_INVALID_ARG, "%s: caches must be 16-byte aligned, scales 4-byte aligned", fn);
+    t = lcml::KvTokens{block_table,         kv_len,           cu_q,           table_stride,      (int32_t)table_cols,
+                       (int32_t)seqs,       (int32_t)tokens,  (int32_t)pages, (int32_t)kv_heads, (int32_t)head_dim,
+                       __builtin_ctzll((unsigned long long)page_tokens)};
+    return LCML_OK;
+}
+
+int check_kv_grid(const char *fn, const lcml::KvTokens &t, int64_t max_q) {
+    const int64_t per_seq = lcml::kv_pages_per_seq(max_q, t.tshift) * 2 * t.heads;
+    if (per_seq > (((int64_t)1 << 23) - 1) / t.seqs)  // 256 threads each, 2^32 work items a launch
+        return fail(LCML_ERR_UNSUPPORTED, "%s: seqs=%lld max_q=%lld exceeds one launch", fn, (long long)t.seqs,
+                    (long long)max_q);
+    return LCML_OK;
+}
+}  // namespace
+
+int lcml_fp8_kv_cache_write(const void *k, const void *v, int dtype, int64_t tokens, int64_t k_token_stride,
+                            int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, uint8_t *k_cache,
+                            uint8_t *v_cache, float *k_scale, float *v_scale, int64_t pages, int64_t kv_heads,
+                            int64_t head_dim, int64_t page_tokens, const int32_t *block_table, int64_t table_stride,
+                            int64_t table_cols, const int32_t *kv_len, const int32_t *cu_q, int64_t seqs,
+                            int64_t max_q, void *stream) {
+    const char *fn = "lcml_fp8_kv_cache_write";
+    if (!float_or_bf16(dtype)) return fail(LCML_ERR_UNSUPPORTED, "%s: dtype %d", fn, dtype);
+    lcml::KvTokens t;
+    if (int rc = make_tokens(t, fn, tokens, k_cache, v_cache, k_scale, v_scale, pages, kv_heads, head_dim, page_tokens,
+                             block_table, table_stride, table_cols, kv_len, cu_q, seqs, max_q))
+        return rc;
+    if (tokens == 0 || seqs == 0 || max_q == 0 || pages == 0) return LCML_OK;
+    if (!k || !v || !elem_aligned(k, dtype) || !elem_aligned(v, dtype))
+        return fail(LCML_ERR_INVALID_ARG, "%s: k or v NULL or not aligned to its elements", fn);
+    if (int rc = check_kv_grid(fn, t, max_q)) return rc;
+    return hip_status(lcml::launch_kv_write(t, max_q, k, v, dtype == LCML_DTYPE_BFLOAT16, k_token_stride, k_head_stride,
+                                            v_token_stride, v_head_stride, k_cache, v_cache, k_scale, v_scale,
+                                            (hipStream_t)stream),
+                      fn);
+}
+
+int lcml_fp8_kv_cache_read(const uint8_t *k_cache, const uint8_t *v_cache, const float *k_scale, const float *v_scale,
+                           int64_t pages, int64_t kv_heads, int64_t head_dim, int64_t page_tokens,
+                           const int32_t *block_table, int64_t table_stride, int64_t table_cols, const int32_t *kv_len,
+                           const int32_t *cu_q, int64_t seqs, int64_t max_q, void *k, void *v, int dtype,
+                           int64_t tokens, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                           int64_t v_head_stride, void *stream) {
+    const char *fn = "lcml_fp8_kv_cache_read";
+    if (!float_or_bf16(dtype)) return fail(LCML_ERR_UNSUPPORTED, "%s: dtype %d", fn, dtype);
+    lcml::KvTokens t;
+    if (int rc = make_tokens(t, fn, tokens, k_cache, v_cache, k_scale, v_scale, pages, kv_heads, head_dim, page_tokens,
+                             block_table, table_stride, table_cols, kv_len, cu_q, seqs, max_q))
+        return rc;
+    if (tokens == 0 || seqs == 0 || max_q == 0 || pages == 0) return LCML_OK;
+    if (!k || !v || !elem_aligned(k, dtype) || !elem_aligned(v, dtype))
+        return fail(LCML_ERR_INVALID_ARG, "%s: k or v NULL or not aligned to its elements", fn);
+    if (int rc = check_kv_grid(fn, t, max_q)) return rc;
+    return hip_status(lcml::launch_kv_read(t, max_q, k, v, dtype == LCML_DTYPE_BFLOAT16, k_token_stride, k_head_stride,
+                                           v_token_stride, v_head_stride, k_cache, v_cache, k_scale, v_scale,
+                                           (hipStream_t)stream),
+                      fn);
+}
+
+int64_t lcml_fp8_attention_workspace_bytes(int64_t tokens, int64_t seqs, int64_t q_heads, int64_t kv_heads,
+                                           int64_t head_dim, int64_t max_q, int64_t max_kv) {
+    if (tokens <= 0 || seqs <= 0 || kv_heads <= 0 || q_heads < kv_heads || head_dim <= 0 || max_q <= 0 || max_kv <= 0)
+        return 0;
+    return lcml::attention_workspace(tokens, seqs, q_heads, kv_heads, head_dim, max_q, max_kv);
+}
+
+int lcml_fp8_attention(const void *q, int q_dtype, int64_t tokens, int64_t q_heads, int64_t q_token_stride,
+                       int64_t q_head_stride, void *o, int o_dtype, int64_t o_token_stride, int64_t o_head_stride,
+                       const uint8_t *k_cache, const uint8_t *v_cache, const float *k_scale, const float *v_scale,
+                       int64_t pages, int64_t kv_heads, int64_t head_dim, int64_t page_tokens,
+                       const int32_t *block_table, int64_t table_stride, int64_t table_cols, const int32_t *kv_len,
+                       const int32_t *cu_q, int64_t seqs, int64_t max_q, int64_t max_kv, float scale, int causal,
+                       int64_t window, void *workspace, int64_t workspace_bytes, void *stream) {
+    const char *fn = "lcml_fp8_attention";
+    if (!float_or_bf16(q_dtype) || !float_or_bf16(o_dtype))
+        return fail(LCML_ERR_UNSUPPORTED, "%s: dtypes q %d, o %d", fn, q_dtype, o_dtype);
+    if (!(scale > 0.0f) || scale > 3.0e38f) return fail(LCML_ERR_INVALID_ARG, "%s: scale %g", fn, (double)scale);
+    if (window < 0 || max_kv < 0)
+        return fail(LCML_ERR_INVALID_ARG, "%s: window=%lld max_kv=%lld", fn, (long long)window, (long long)max_kv);
+    lcml::AttentionArgs a{};
+    if (int rc = make_tokens(a.t, fn, tokens, k_cache, v_cache, k_scale, v_scale, pages, kv_heads, head_dim, page_tokens,
+                             block_table, table_stride, table_cols, kv_len, cu_q, seqs, max_q))
+        return rc;
+    if (q_heads <= 0 || q_heads % kv_heads)
+        return fail(LCML_ERR_INVALID_ARG, "%s: q_heads=%lld is not a multiple of kv_heads=%lld", fn, (long long)q_heads,
+                    (long long)kv_heads);
+    if (q_heads > 65535 || max_kv >= (int64_t)1 << 31)
+        return fail(LCML_ERR_UNSUPPORTED, "%s: q_heads=%lld max_kv=%lld", fn, (long long)q_heads, (long long)max_kv);
+    if (tokens == 0 || seqs == 0 || max_q == 0) return LCML_OK;
+    if (!q || !o || !elem_aligned(q, q_dtype) || !elem_aligned(o, o_dtype))
+        return fail(LCML_ERR_INVALID_ARG, "%s: q or o NULL or not aligned to its elements", fn);
+    if (tokens * q_heads >= (int64_t)1 << 24)  // 256 threads each, 2^32 work items a launch
+        return fail(LCML_ERR_UNSUPPORTED, "%s: tokens=%lld q_heads=%lld exceeds one launch", fn, (long long)tokens,
+                    (long long)q_heads);
+    const int64_t need = lcml::attention_workspace(tokens, seqs, q_heads, kv_heads, head_dim, max_q, max_kv);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+        return fail(LCML_ERR_INVALID_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", fn, (long long)need);
+    a.q = q, a.o = o, a.k = k_cache, a.v = v_cache, a.ks = k_scale, a.vs = v_scale;
+    a.q_token = q_token_stride, a.q_head = q_head_stride, a.o_token = o_token_stride, a.o_head = o_head_stride;
+    a.max_q = max_q, a.max_kv = max_kv, a.window = window;
+    a.q_heads = (int32_t)q_heads, a.causal = causal != 0;
+    a.q_bf16 = q_dtype == LCML_DTYPE_BFLOAT16, a.o_bf16 = o_dtype == LCML_DTYPE_BFLOAT16;
+    a.scale = scale;
+    const char *label = nullptr;
+    const hipError_t err = lcml::launch_attention(a, workspace, (hipStream_t)stream, &label);
+    return hip_status(err, fn, label);
 }
 
 }  // extern "C"

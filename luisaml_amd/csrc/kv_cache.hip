@@ -1,0 +1,286 @@
+// kv_cache.hip -- tokens into an E4M3 cache of pages, and back (gfx950).
+//
+// Both directions stream: a written token costs 2 or 4 bytes in and one out
+// for each element, a read one the inverse.  One workgroup takes one page of
+// one head, of K or of V, so the page's maximum, its scale and the codes that
+// stay are its own and no order between workgroups matters.  A thread's unit
+// is 4 tokens x 8 elements: four row loads of 16 or 32 bytes, and in the
+// cache 4 x 8 bytes of K or 32 contiguous bytes of V, which transposes V in
+// registers.
+#include "kv_cache.hpp"
+#include "lcml_internal.hpp"
+
+namespace lcml {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct __attribute__((packed, aligned(2))) H8 {
+    uint16_t v[8];
+};
+struct __attribute__((packed, aligned(4))) F8x32 {
+    float v[8];
+};
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+
+struct Rows {
+    const char *k, *v;      // write: the call's K and V
+    char *ko, *vo;          // read: its outputs
+    int64_t kt, kh, vt, vh;  // strides in elements: token, head
+};
+
+template <bool BF16>
+__device__ inline void load8(const char *p, float *x) {
+    if constexpr (BF16) {
+        const H8 q = *reinterpret_cast<const H8 *>(p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = bits_f32((uint32_t)q.v[e] << 16);
+    } else {
+        const F8x32 q = *reinterpret_cast<const F8x32 *>(p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = q.v[e];
+    }
+}
+
+// where the workgroup is: K or V, head, page, and the page's new slots
+struct Spot {
+    bool is_v;
+    int32_t head, page, lo, hi;  // new slots lo .. hi-1
+    int64_t row;                 // the call's row of slot 0
+};
+
+__device__ inline bool find_spot(const KvTokens &t, int32_t pages_per_seq, Spot *s) {
+    uint32_t i = blockIdx.x;
+    s->is_v = i & 1;
+    i >>= 1;
+    s->head = i % t.heads;
+    i /= t.heads;
+    const int32_t r = i % pages_per_seq, b = i / pages_per_seq;
+    const SeqRows q = seq_rows(t, b);
+    if (q.n <= 0) return false;
+    const int32_t p0 = q.pos0 > 0 ? q.pos0 : 0;
+    const int32_t c = (p0 >> t.tshift) + r, T = 1 << t.tshift;
+    const int64_t base = (int64_t)c << t.tshift;
+    if (base >= q.len) return false;
+    s->lo = p0 > base ? (int32_t)(p0 - base) : 0;
+    s->hi = q.len - base < T ? (int32_t)(q.len - base) : T;
+    s->page = page_of(t, b, c);
+    s->row = q.row0 + (base - q.pos0);
+    return s->page >= 0 && s->lo < s->hi;
+}
+
+// a thread's unit in the cache: 4 slots from t0, 8 elements from e0
+template <bool V>
+__device__ inline void load_codes(const uint8_t *blk, int32_t t0, int32_t e0, int32_t D, uint32_t w[8]) {
+    if constexpr (V) {
+        const u4 *p = reinterpret_cast<const u4 *>(blk + v_place(t0, e0, D));
+        const u4 a = p[0], b = p[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = a[e], w[4 + e] = b[e];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const u2 a = *reinterpret_cast<const u2 *>(blk + k_place(t0 + i, e0, D));
+            w[2 * i] = a[0], w[2 * i + 1] = a[1];
+        }
+    }
+}
+
+// the code of token i, element e within a unit's eight words
+template <bool V>
+__device__ constexpr int word_of(int i, int e) {
+    return V ? e : 2 * i + (e >> 2);
+}
+template <bool V>
+__device__ constexpr int byte_of(int i, int e) {
+    return V ? i : e & 3;
+}
+
+__device__ inline uint32_t encode_again(uint32_t w, float k) {
+    const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    return e4m3x2_hw(a[0] * k, a[1] * k) | (e4m3x2_hw(b[0] * k, b[1] * k) << 16);
+}
+
+template <bool V, bool BF16>
+__device__ inline void write_page(const KvTokens &t, const Spot &sp, const Rows &rows, uint8_t *cache, float *scales,
+                                  float *red) {
+    const int32_t D = t.dim, T = 1 << t.tshift, d8 = D >> 3;
+    const int64_t at = (int64_t)sp.page * t.heads + sp.head;
+    uint8_t *blk = cache + (at << t.tshift) * D;
+    const char *src = V ? rows.v + (sp.row * rows.vt + sp.head * rows.vh) * (BF16 ? 2 : 4)
+                        : rows.k + (sp.row * rows.kt + sp.head * rows.kh) * (BF16 ? 2 : 4);
+    const int64_t pitch = (V ? rows.vt : rows.kt) * (BF16 ? 2 : 4);
+    const int32_t units = (T >> 2) * d8;
+    auto load = [&](int32_t g, int i, float *x) {
+        load8<BF16>(src + (int64_t)(g / d8 * 4 + i) * pitch + (int64_t)(g % d8) * 8 * (BF16 ? 2 : 4), x);
+    };
+    float m = 0.0f;
+    for (int32_t g = threadIdx.x; g < units; g += kThreads) {
+        const int32_t t0 = g / d8 * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (t0 + i >= sp.lo && t0 + i < sp.hi) {
+                float x[8];
+                load(g, i, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float a = fabsf(x[e]);
+                    m = a > m && a < __builtin_inff() ? a : m;
+                }
+            }
+    }
+    float s = page_scale(block_max<kThreads>(m, red)), grow = 1.0f;
+    if (sp.lo > 0) {  // tokens that stay
+        const float old = scales[at];
+        if (old >= s)
+            s = old;
+        else
+            grow = old / s;
+    }
+    __syncthreads();  // every thread has read the old scale
+    if (threadIdx.x == 0) scales[at] = s;
+    const float inv = 1.0f / s;  // a power of two: x * inv is x / s
+    for (int32_t g = threadIdx.x; g < units; g += kThreads) {
+        const int32_t t0 = g / d8 * 4, e0 = g % d8 * 8;
+        const bool fresh = t0 < sp.hi && t0 + 4 > sp.lo, stays = t0 < sp.lo && grow != 1.0f;
+        if (!fresh && !stays) continue;
+        uint32_t w[8];
+        load_codes<V>(blk, t0, e0, D, w);
+        uint32_t n[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) n[q] = stays ? encode_again(w[q], grow) : w[q];
+        uint32_t out[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) out[q] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int32_t slot = t0 + i;
+            float x[8];
+            const bool now = slot >= sp.lo && slot < sp.hi;
+            if (now) load(g, i, x);
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const int wi = word_of<V>(i, e), wj = word_of<V>(i, e + 1);
+                const int bi = 8 * byte_of<V>(i, e), bj = 8 * byte_of<V>(i, e + 1);
+                uint32_t c0, c1;
+                if (now) {
+                    const uint32_t c = e4m3x2_hw(x[e] * inv, x[e + 1] * inv);
+                    c0 = c & 0xffu, c1 = c >> 8;
+                } else {  // a kept token, or a slot past the last one as it was
+                    c0 = ((slot < sp.lo ? n[wi] : w[wi]) >> bi) & 0xffu;
+                    c1 = ((slot < sp.lo ? n[wj] : w[wj]) >> bj) & 0xffu;
+                }
+                out[wi] |= c0 << bi;
+                out[wj] |= c1 << bj;
+            }
+        }
+        if constexpr (V) {
+            u4 *p = reinterpret_cast<u4 *>(blk + v_place(t0, e0, D));
+            p[0] = u4{out[0], out[1], out[2], out[3]};
+            p[1] = u4{out[4], out[5], out[6], out[7]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<u2 *>(blk + k_place(t0 + i, e0, D)) = u2{out[2 * i], out[2 * i + 1]};
+        }
+    }
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kThreads) void k_kv_write(KvTokens t, Rows rows, uint8_t *kc, uint8_t *vc, float *ks,
+                                                       float *vs, int32_t pages_per_seq) {
+    __shared__ float red[kThreads / 64];
+    Spot sp;
+    if (!find_spot(t, pages_per_seq, &sp)) return;
+    if (sp.is_v)
+        write_page<true, BF16>(t, sp, rows, vc, vs, red);
+    else
+        write_page<false, BF16>(t, sp, rows, kc, ks, red);
+}
+
+template <bool V, bool BF16>
+__device__ inline void read_page(const KvTokens &t, const Spot &sp, const Rows &rows, const uint8_t *cache,
+                                 const float *scales) {
+    const int32_t D = t.dim, T = 1 << t.tshift, d8 = D >> 3;
+    const int64_t at = (int64_t)sp.page * t.heads + sp.head;
+    const uint8_t *blk = cache + (at << t.tshift) * D;
+    char *dst = V ? rows.vo + (sp.row * rows.vt + sp.head * rows.vh) * (BF16 ? 2 : 4)
+                  : rows.ko + (sp.row * rows.kt + sp.head * rows.kh) * (BF16 ? 2 : 4);
+    const int64_t pitch = (V ? rows.vt : rows.kt) * (BF16 ? 2 : 4);
+    const float s = scales[at];
+    for (int32_t g = threadIdx.x; g < (T >> 2) * d8; g += kThreads) {
+        const int32_t t0 = g / d8 * 4, e0 = g % d8 * 8;
+        if (t0 + 4 <= sp.lo || t0 >= sp.hi) continue;
+        uint32_t w[8];
+        load_codes<V>(blk, t0, e0, D, w);
+        float x[8][4];  // [word][byte]
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[q], false);
+            const f2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[q], true);
+            x[q][0] = a[0] * s, x[q][1] = a[1] * s, x[q][2] = b[0] * s, x[q][3] = b[1] * s;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (t0 + i < sp.lo || t0 + i >= sp.hi) continue;
+            char *p = dst + (int64_t)(t0 + i) * pitch + (int64_t)e0 * (BF16 ? 2 : 4);
+            if constexpr (BF16) {
+                H8 o;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o.v[e] = bf16_rne(x[word_of<V>(i, e)][byte_of<V>(i, e)]);
+                *reinterpret_cast<H8 *>(p) = o;
+            } else {
+                F8x32 o;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o.v[e] = x[word_of<V>(i, e)][byte_of<V>(i, e)];
+                *reinterpret_cast<F8x32 *>(p) = o;
+            }
+        }
+    }
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kThreads) void k_kv_read(KvTokens t, Rows rows, const uint8_t *kc, const uint8_t *vc,
+                                                      const float *ks, const float *vs, int32_t pages_per_seq) {
+    Spot sp;
+    if (!find_spot(t, pages_per_seq, &sp)) return;
+    if (sp.is_v)
+        read_page<true, BF16>(t, sp, rows, vc, vs);
+    else
+        read_page<false, BF16>(t, sp, rows, kc, ks);
+}
+
+}  // namespace
+
+// pages that max_q tokens of one sequence can touch
+int64_t kv_pages_per_seq(int64_t max_q, int tshift) { return ((max_q - 2 + ((int64_t)1 << tshift)) >> tshift) + 1; }
+
+hipError_t launch_kv_write(const KvTokens &t, int64_t max_q, const void *k, const void *v, bool bf16, int64_t kt,
+                           int64_t kh, int64_t vt, int64_t vh, uint8_t *kc, uint8_t *vc, float *ks, float *vs,
+                           hipStream_t s) {
+    const Rows rows{(const char *)k, (const char *)v, nullptr, nullptr, kt, kh, vt, vh};
+    const int64_t pp = kv_pages_per_seq(max_q, t.tshift);
+    const dim3 grid((unsigned)(2 * t.heads * pp * t.seqs));
+    if (bf16)
+        hipLaunchKernelGGL((k_kv_write<true>), grid, dim3(kThreads), 0, s, t, rows, kc, vc, ks, vs, (int32_t)pp);
+    else
+        hipLaunchKernelGGL((k_kv_write<false>), grid, dim3(kThreads), 0, s, t, rows, kc, vc, ks, vs, (int32_t)pp);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_read(const KvTokens &t, int64_t max_q, void *k, void *v, bool bf16, int64_t kt, int64_t kh,
+                          int64_t vt, int64_t vh, const uint8_t *kc, const uint8_t *vc, const float *ks,
+                          const float *vs, hipStream_t s) {
+    const Rows rows{nullptr, nullptr, (char *)k, (char *)v, kt, kh, vt, vh};
+    const int64_t pp = kv_pages_per_seq(max_q, t.tshift);
+    const dim3 grid((unsigned)(2 * t.heads * pp * t.seqs));
+    if (bf16)
+        hipLaunchKernelGGL((k_kv_read<true>), grid, dim3(kThreads), 0, s, t, rows, kc, vc, ks, vs, (int32_t)pp);
+    else
+        hipLaunchKernelGGL((k_kv_read<false>), grid, dim3(kThreads), 0, s, t, rows, kc, vc, ks, vs, (int32_t)pp);
+    return hipGetLastError();
+}
+
+}  // namespace lcml

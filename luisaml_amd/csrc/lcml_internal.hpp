@@ -124,6 +124,29 @@ hipError_t launch_fp8_binary(int op, int fmt, const void *a, const void *b, void
 // the fold of the data equals a fixed constant
 hipError_t launch_stream_read(const void *p, int64_t bytes, int workgroups, uint32_t *sink, hipStream_t s);
 
+// residual addition, RMS norm and E4M3 codes; mode: LCML_SCALE_*; work (mode
+// TENSOR, M > 1): rms_norm_workspace(M) bytes
+int64_t rms_norm_workspace(int64_t M);
+hipError_t launch_rms_norm(int64_t M, int64_t H, const void *x, bool x_bf16, int64_t ldx, const void *res,
+                           void *res_out, bool res_bf16, int64_t ldr, int64_t ldro, const float *gamma, float eps,
+                           uint8_t *y, int64_t ldy, int mode, float *scale, void *work, hipStream_t s);
+
+// the E4M3 KV cache (kv_cache.hpp); kt, kh, vt, vh: strides of k and v in
+// elements, from token to token and from head to head
+struct KvTokens;
+struct AttentionArgs;
+int64_t kv_pages_per_seq(int64_t max_q, int tshift);
+hipError_t launch_kv_write(const KvTokens &t, int64_t max_q, const void *k, const void *v, bool bf16, int64_t kt,
+                           int64_t kh, int64_t vt, int64_t vh, uint8_t *kc, uint8_t *vc, float *ks, float *vs,
+                           hipStream_t s);
+hipError_t launch_kv_read(const KvTokens &t, int64_t max_q, void *k, void *v, bool bf16, int64_t kt, int64_t kh,
+                          int64_t vt, int64_t vh, const uint8_t *kc, const uint8_t *vc, const float *ks,
+                          const float *vs, hipStream_t s);
+// workspace bytes, and a call (work: that many bytes)
+int64_t attention_workspace(int64_t tokens, int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                            int64_t max_q, int64_t max_kv);
+hipError_t launch_attention(const AttentionArgs &a, void *work, hipStream_t s, const char **kernel);
+
 // A kernel's dynamic-LDS limit (hipFuncSetAttribute) is per device: set it
 // once per (kernel, device), tracked in `done` (bit d = device d; devices past
 // 63 set it on every call).  The call is idempotent, so two threads racing on
