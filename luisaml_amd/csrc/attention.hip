@@ -14,6 +14,8 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr float kInf = __builtin_inff();
@@ -63,6 +65,19 @@ __device__ inline float v_ratio(uint32_t vs, uint32_t vref) {
     return bits_f32((uint32_t)(e < 1 ? 1 : e) << 23);
 }
 
+// 2^kPBits 2^(t - m).  Two pieces take the factor after the exponential: with
+// it in the argument, the rounding of a sum near 14 costs three bits.
+template <int NP>
+__device__ inline float weights_at(float m) {
+    m = m == -kInf ? 0.0f : m;
+    return NP == 1 ? m - (float)kPBits : m;
+}
+template <int NP>
+__device__ inline float weight_of(float t, float mm) {
+    const float e = __builtin_amdgcn_exp2f(t - mm);
+    return NP == 1 ? e : e * (float)(1 << kPBits);
+}
+
 __device__ inline float load_q(const AttentionArgs &a, int64_t i) {
     return a.q_bf16 ? bits_f32((uint32_t)static_cast<const uint16_t *>(a.q)[i] << 16) : static_cast<const float *>(a.q)[i];
 }
@@ -84,8 +99,6 @@ __device__ inline Block find_block(const AttentionArgs &a, int32_t b, int32_t he
     }
     return r;
 }
-
-typedef float f2 __attribute__((ext_vector_type(2)));
 
 struct __attribute__((packed, aligned(4))) F4 {
     float v[4];
@@ -303,13 +316,13 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
             scale_o(bits_f32((uint32_t)(e < 0 ? 0 : e) << 23));
             vref = top;
         }
-        const float mm = (m == -kInf ? 0.0f : m) - (float)kPBits;
+        const float mm = weights_at<NP>(m);
         h8 p[NP][2];
 #pragma unroll
         for (int sb = 0; sb < 4; ++sb)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float e = __builtin_amdgcn_exp2f(t[sb][i] - mm);
+                const float e = weight_of<NP>(t[sb][i], mm);
                 l += e;
                 const _Float16 eh = (_Float16)e;
                 p[0][sb >> 1][(sb & 1) * 4 + i] = eh;
@@ -406,6 +419,303 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
     }
 }
 
+// ---------------------------------------------------------------- many rows --
+//
+// One workgroup: 128 rows (queries x heads of the group) of one sequence and
+// KV head, 32 for each wavefront, over one part of the tokens.  K and V go
+// through LDS as codes, 64 tokens a step and two steps in turn, and are widened
+// to fp16 in registers, where a wavefront uses each for all its rows.  As
+// above, S^T = K Q^T and O^T = V^T P^T, on 32x32x16 instructions.
+constexpr int kManyWaves = 4, kManyRows = 32 * kManyWaves;
+
+template <int DP, bool EXACT, int NQ, int NP>
+__global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attention_many(AttentionArgs a, Split sp) {
+    constexpr int KJ = DP / 32;                // pairs of 16-element pieces of K
+    constexpr int MT = DP / 32;                // tiles of 32 columns of V
+    constexpr int CPL = DP >= 128 ? 4 : 2;     // columns of V that a lane reads at once
+    constexpr int VR = MT / CPL;               // such reads for a group of four tokens
+    constexpr int kHalf = 64 * DP + 4 * DP;    // K's or V's bytes of a step, and room for reads past D
+    constexpr int PL = (16 * DP / 16 + 63) / 64;  // 16-byte loads for a lane of a 16-token block
+    __shared__ __attribute__((aligned(16))) uint8_t stage[2][2][kHalf];
+    __shared__ uint32_t info[2][4][3];  // of a block: K's and V's scale, V has NaN codes
+    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int32_t D = EXACT ? DP : a.t.dim, G = a.q_heads / a.t.heads;
+    // workgroups of one sequence and KV head on one XCD (blockIdx modulo 8),
+    // whose L2 then holds their K and V; the longest rows first
+    const uint32_t pairs = (uint32_t)a.t.seqs * a.t.heads, per = (uint32_t)sp.tiles * sp.splits;
+    uint32_t pair, rest;
+    if (pairs % 8 == 0) {
+        pair = blockIdx.x % 8 + 8 * (blockIdx.x / (8 * per));
+        rest = blockIdx.x / 8 % per;
+    } else {
+        pair = blockIdx.x / per;
+        rest = blockIdx.x % per;
+    }
+    const int32_t head = pair % a.t.heads, b = pair / a.t.heads;
+    const int32_t split = rest % sp.splits, tile = sp.tiles - 1 - (int32_t)(rest / sp.splits);
+    const SeqRows s = seq_rows(a.t, b);
+    const int64_t rows = (int64_t)s.n * G, row0 = (int64_t)tile * kManyRows;
+    if (row0 >= rows) return;
+    const int64_t last = rows - row0 < kManyRows ? rows - 1 : row0 + kManyRows - 1;
+    // this wavefront's rows and this lane's
+    const int64_t w0 = row0 + 32 * wave < last ? row0 + 32 * wave : last, w1 = w0 + 31 < last ? w0 + 31 : last;
+    const bool live = row0 + 32 * wave + r <= last;
+    const int64_t row = live ? row0 + 32 * wave + r : w1;
+    const int32_t qi = (int32_t)(row / G), qh = head * G + (int32_t)(row % G);
+    int32_t lo, hi, lo_min, hi_min, lo_max, hi_max, w_lo, w_hi, skip0, skip1;
+    sees(a, s, qi, &lo, &hi);
+    sees(a, s, (int32_t)(row0 / G), &lo_min, &skip0);
+    sees(a, s, (int32_t)(last / G), &skip1, &hi_max);
+    sees(a, s, (int32_t)(w0 / G), &w_lo, &hi_min);  // of the wavefront: all tokens, and those that every row sees
+    sees(a, s, (int32_t)(w1 / G), &lo_max, &w_hi);
+    const int64_t from = (lo_min & ~63) + (int64_t)split * sp.chunk;
+    int64_t to = split + 1 < sp.splits ? from + sp.chunk : (int64_t)1 << 31;
+    to = to < hi_max ? to : hi_max;
+    const int32_t start = from < to ? (int32_t)from : 0;
+    const int32_t steps = from < to && a.t.pages > 0 ? (int32_t)((to - from + 63) >> 6) : 0;
+    const int64_t out_row = ((int64_t)s.row0 + qi) * a.q_heads + qh;
+    if (steps == 0 && sp.splits > 1) {
+        if (h == 0 && live) sp.lse[out_row * sp.splits + split] = -kInf;
+        return;
+    }
+
+    // a step's 64 tokens: this wavefront brings block `wave` of them
+    u4 kr[PL], vr[PL];
+    uint32_t ksr = 0, vsr = 0;
+    auto fetch = [&](int32_t k) {
+        const Block blk = find_block(a, b, head, start + (k << 6) + 16 * wave, (int32_t)to);
+        ksr = blk.ks, vsr = blk.vs;
+        const uint64_t at = (blk.lo | (uint64_t)blk.hi << 32) * (uint64_t)(16 * D);
+#pragma unroll
+        for (int x = 0; x < PL; ++x) {
+            const bool in = blk.vs != 0 && (EXACT && DP % 64 == 0 ? true : 64 * x + lane < D);
+            kr[x] = in ? *reinterpret_cast<const u4 *>(a.k + at + (64 * x + lane) * 16) : u4{0, 0, 0, 0};
+            vr[x] = in ? *reinterpret_cast<const u4 *>(a.v + at + (64 * x + lane) * 16) : u4{0, 0, 0, 0};
+        }
+    };
+    auto deposit = [&](int buf) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int x = 0; x < PL; ++x) {
+            if (EXACT || 64 * x + lane < D) {
+                *reinterpret_cast<u4 *>(&stage[buf][0][wave * 16 * D + (64 * x + lane) * 16]) = kr[x];
+                *reinterpret_cast<u4 *>(&stage[buf][1][wave * 16 * D + (64 * x + lane) * 16]) = vr[x];
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) bad |= nan_bits(vr[x][c]);
+        }
+        const bool any = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+        if (lane == 0) info[buf][wave][0] = ksr, info[buf][wave][1] = vsr, info[buf][wave][2] = any;
+    };
+
+    if (steps > 0) fetch(0);
+
+    h8 qf[NQ][KJ][2];
+    float cq;
+    {
+        const int64_t at = ((int64_t)s.row0 + qi) * a.q_token + (int64_t)qh * a.q_head;
+        float amax = 0.0f;
+#pragma unroll
+        for (int j = 0; j < KJ; ++j)
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                const int d = 32 * j + 16 * h + u;
+                const float v = d < D ? fabsf(load_q(a, at + d)) : 0.0f;
+                amax = v > amax && v < kInf ? v : amax;
+            }
+        const auto sw = __builtin_amdgcn_permlane32_swap(f32_bits(amax), f32_bits(amax), false, false);
+        const float f = query_factor(fmaxf(bits_f32(sw[0]), bits_f32(sw[1])));
+        cq = a.scale * kLog2e * (1.0f / f);
+#pragma unroll
+        for (int j = 0; j < KJ; ++j)
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                const int d = 32 * j + 16 * h + u;
+                const float v = (d < D ? load_q(a, at + d) : 0.0f) * f;
+                qf[0][j][u >> 3][u & 7] = (_Float16)v;
+                if constexpr (NQ == 2) qf[NQ - 1][j][u >> 3][u & 7] = (_Float16)(v - (float)(_Float16)v);
+            }
+    }
+
+    f16v o[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+    float m = -kInf, l = 0.0f;
+    uint32_t vref = 0;
+    auto scale_o = [&](float f) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) o[t] *= f;
+    };
+    if (steps > 0) deposit(0);
+    __syncthreads();
+
+    for (int32_t k = 0; k < steps; ++k) {
+        const int32_t tok = start + (k << 6);
+        const int buf = k & 1;
+        if (k + 1 < steps) fetch(k + 1);
+        if (tok < w_hi && tok + 64 > w_lo) {
+            const uint8_t *sk = stage[buf][0], *sv = stage[buf][1];
+            uint32_t ks[4], vs[4], nan = 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                ks[q] = __builtin_amdgcn_readfirstlane(info[buf][q][0]);
+                vs[q] = __builtin_amdgcn_readfirstlane(info[buf][q][1]);
+                nan |= __builtin_amdgcn_readfirstlane(info[buf][q][2]);
+            }
+            f16v t[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                f16v acc;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+                const uint8_t *p = sk + (2 * q + (r >> 4)) * 16 * D + h * 256 + (r & 15) * 16;
+#pragma unroll
+                for (int j = 0; j < KJ; ++j) {
+                    if (!EXACT && 32 * j >= D) break;
+                    u4 w = *reinterpret_cast<const u4 *>(p + j * 512);
+                    if (!EXACT && 32 * j + 16 * h >= D) w = u4{0, 0, 0, 0};
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const h8 kh = widen8(w[2 * u], w[2 * u + 1], 1.0f);
+#pragma unroll
+                        for (int x = 0; x < NQ; ++x) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qf[x][j][u], acc, 0, 0, 0);
+                    }
+                }
+                const float c0 = cq * bits_f32(ks[2 * q]), c1 = cq * bits_f32(ks[2 * q + 1]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) t[q][i] = acc[i] * (i < 8 ? c0 : c1);
+            }
+            const bool full = tok >= lo_max && tok + 64 <= hi_min && vs[0] && vs[1] && vs[2] && vs[3];
+            if (!full) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int32_t j = tok + 32 * q + 8 * (i >> 2) + 4 * h + (i & 3);
+                        const bool ok = j >= lo && j < hi && vs[2 * q + (i >> 3)] != 0;
+                        t[q][i] = ok ? t[q][i] : -kInf;
+                    }
+            }
+            float mx = m;
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, t[q][i]);
+            const auto sw = __builtin_amdgcn_permlane32_swap(f32_bits(mx), f32_bits(mx), false, false);
+            mx = fmaxf(bits_f32(sw[0]), bits_f32(sw[1]));
+            if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
+                const float f = mx > m ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
+                l *= f;
+                scale_o(f);
+                m = mx;
+            }
+            uint32_t top = vs[0] > vs[1] ? vs[0] : vs[1];
+            top = vs[2] > top ? vs[2] : top;
+            top = vs[3] > top ? vs[3] : top;
+            if (top > vref) {
+                const int e = (int)(vref >> 23) - (int)(top >> 23) + 127;
+                scale_o(bits_f32((uint32_t)(e < 0 ? 0 : e) << 23));
+                vref = top;
+            }
+            const float mm = weights_at<NP>(m);
+            h8 p[NP][4];
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float e = weight_of<NP>(t[q][i], mm);
+                    l += e;
+                    const _Float16 eh = (_Float16)e;
+                    p[0][2 * q + (i >> 3)][i & 7] = eh;
+                    if constexpr (NP == 2) p[NP - 1][2 * q + (i >> 3)][i & 7] = (_Float16)(e - (float)eh);
+                }
+            const bool mend = !full && nan;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float ratio = v_ratio(vs[q], vref);
+#pragma unroll
+                for (int x = 0; x < VR; ++x) {
+                    const uint8_t *pv = sv + q * 16 * D + h * 4 * D + (128 * x + CPL * r) * 4;
+                    uint32_t w0[CPL], w1[CPL];
+                    if constexpr (CPL == 4) {
+                        const u4 u0 = *reinterpret_cast<const u4 *>(pv), u1 = *reinterpret_cast<const u4 *>(pv + 8 * D);
+#pragma unroll
+                        for (int c = 0; c < CPL; ++c) w0[c] = u0[c], w1[c] = u1[c];
+                    } else {
+                        const u2 u0 = *reinterpret_cast<const u2 *>(pv), u1 = *reinterpret_cast<const u2 *>(pv + 8 * D);
+#pragma unroll
+                        for (int c = 0; c < CPL; ++c) w0[c] = u0[c], w1[c] = u1[c];
+                    }
+#pragma unroll
+                    for (int c = 0; c < CPL; ++c) {
+                        if (!mend) {
+                            const h8 va = widen8(w0[c], w1[c], ratio);
+#pragma unroll
+                            for (int y = 0; y < NP; ++y)
+                                o[x * CPL + c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, p[y][q], o[x * CPL + c], 0, 0, 0);
+                        } else {
+                            // as above: NaN codes among tokens that not every row sees
+                            const uint32_t n0 = nan_bits(w0[c]) >> 7, n1 = nan_bits(w1[c]) >> 7;
+                            const h8 va = widen8(w0[c] & ~(n0 * 0xffu), w1[c] & ~(n1 * 0xffu), ratio);
+                            h8 is, on;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                is[e] = ((e < 4 ? n0 : n1) >> (8 * (e & 3))) & 1 ? (_Float16)1.0f : (_Float16)0.0f;
+                                const int32_t j = tok + 16 * q + 8 * (e >> 2) + 4 * h + (e & 3);
+                                on[e] = j >= lo && j < hi && vs[q] != 0 ? (_Float16)1.0f : (_Float16)0.0f;
+                            }
+#pragma unroll
+                            for (int y = 0; y < NP; ++y)
+                                o[x * CPL + c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, p[y][q], o[x * CPL + c], 0, 0, 0);
+                            f16v hit;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) hit[i] = 0.0f;
+                            hit = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, on, hit, 0, 0, 0);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                o[x * CPL + c][i] = hit[i] > 0.0f ? __builtin_nanf("") : o[x * CPL + c][i];
+                        }
+                    }
+                }
+            }
+        }
+        if (k + 1 < steps) deposit(buf ^ 1);
+        __syncthreads();
+    }
+
+    const auto sw = __builtin_amdgcn_permlane32_swap(f32_bits(l), f32_bits(l), false, false);
+    l = bits_f32(sw[0]) + bits_f32(sw[1]);
+    if (!live) return;
+    const float f = l == 0.0f ? 0.0f : bits_f32(vref) * (1.0f / (1 << kVBits)) / l;
+    float *po = nullptr;
+    if (sp.splits > 1) {
+        po = sp.o + (out_row * sp.splits + split) * D;
+        if (h == 0) sp.lse[out_row * sp.splits + split] = l == 0.0f ? -kInf : m + __builtin_amdgcn_logf(l);
+    }
+    const int64_t oo = ((int64_t)s.row0 + qi) * a.o_token + (int64_t)qh * a.o_head;
+    // row 8 a + 4 h + b of tile c: columns 128 x + CPL * that + c
+#pragma unroll
+    for (int x = 0; x < VR; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < CPL; ++e) {
+                const int d = 128 * x + CPL * (8 * i + 4 * h) + 4 * e;
+                f4 v;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    v[u] = l == 0.0f ? 0.0f : o[x * CPL + (4 * e + u) % CPL][4 * i + (4 * e + u) / CPL] * f;
+                if (!EXACT && d >= D) continue;
+                if (po)
+                    *reinterpret_cast<f4 *>(po + d) = v;
+                else
+                    store_o4(a, oo + d, v);
+            }
+}
+
 // Joins a row's parts: one wavefront a row.
 __global__ __launch_bounds__(256) void k_attention_join(AttentionArgs a, Split sp) {
     const int32_t D = a.t.dim, lane = threadIdx.x & 63;
@@ -431,97 +741,6 @@ __global__ __launch_bounds__(256) void k_attention_join(AttentionArgs a, Split s
         store_o4(a, (s.row0 + i) * a.o_token + h * a.o_head + lane * 4, sum == 0.0f ? f4{0.f, 0.f, 0.f, 0.f} : v * (1.0f / sum));
 }
 
-constexpr int kThreads = 256;
-
-// One query row and head for each workgroup: scores of 256 tokens at a time,
-// one token a thread, then the columns of V, one a thread.
-__global__ __launch_bounds__(kThreads) void k_attention_rows(AttentionArgs a) {
-    __shared__ float q[256], p[kThreads];
-    const KvTokens &t = a.t;
-    const int32_t row = blockIdx.x / a.q_heads, h = blockIdx.x % a.q_heads, D = t.dim;
-    const int32_t kvh = h / (a.q_heads / t.heads);
-    int32_t b = 0;  // the row's sequence: the first with cu[b + 1] > row
-    for (int32_t lo = 0, hi = t.seqs; lo < hi;) {
-        b = (lo + hi) >> 1;
-        if (t.cu[b + 1] > row)
-            hi = b;
-        else
-            lo = b = b + 1;
-    }
-    if (b >= t.seqs) return;
-    const SeqRows s = seq_rows(t, b);
-    if (row < s.row0 || row >= s.row0 + s.n) return;
-    const int32_t pos = s.pos0 + (row - s.row0);
-    if ((int32_t)threadIdx.x < D) {
-        const int64_t i = row * a.q_token + h * a.q_head + threadIdx.x;
-        q[threadIdx.x] = a.q_bf16 ? bits_f32((uint32_t)static_cast<const uint16_t *>(a.q)[i] << 16)
-                                  : static_cast<const float *>(a.q)[i];
-    }
-    __syncthreads();
-    int64_t first = a.window > 0 ? (int64_t)pos - a.window + 1 : 0;
-    if (first < 0) first = 0;
-    const int64_t end = a.causal && pos + 1 < s.len ? pos + 1 : s.len;
-    float m = -__builtin_inff(), l = 0.0f, o = 0.0f;
-    for (int64_t j0 = first & ~(int64_t)15; j0 < end; j0 += kThreads) {
-        const int64_t j = j0 + threadIdx.x;
-        float x = -__builtin_inff();
-        const int32_t page = j < end ? page_of(t, b, (int32_t)(j >> t.tshift)) : -1;
-        if (j >= first && page >= 0) {
-            const int64_t at = (int64_t)page * t.heads + kvh;
-            const uint8_t *blk = a.k + (at << t.tshift) * D;
-            const int32_t slot = (int32_t)j & ((1 << t.tshift) - 1);
-            float acc = 0.0f;
-            for (int32_t e = 0; e < D; e += 16) {
-                const u4 w = *reinterpret_cast<const u4 *>(blk + k_place(slot, e, D));
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const f2 u = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[c], false);
-                    const f2 v = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[c], true);
-                    acc = fmaf(u[0], q[e + 4 * c], acc);
-                    acc = fmaf(u[1], q[e + 4 * c + 1], acc);
-                    acc = fmaf(v[0], q[e + 4 * c + 2], acc);
-                    acc = fmaf(v[1], q[e + 4 * c + 3], acc);
-                }
-            }
-            x = acc * a.ks[at] * a.scale;
-        }
-        float top = -__builtin_inff();
-        p[threadIdx.x] = x;
-        __syncthreads();
-        for (int w = 0; w < kThreads; ++w) top = fmaxf(top, p[w]);
-        __syncthreads();
-        const float m1 = fmaxf(m, top), base = m1 == -__builtin_inff() ? 0.0f : m1;
-        const float e = expf(x - base);
-        p[threadIdx.x] = e;
-        __syncthreads();
-        const float keep = m == -__builtin_inff() ? 0.0f : expf(m - base);
-        o *= keep;
-        l *= keep;
-        for (int w = 0; w < kThreads; ++w) l += p[w];
-        if ((int32_t)threadIdx.x < D) {
-            for (int w = 0; w < kThreads && j0 + w < end; ++w) {
-                if (j0 + w < first) continue;
-                const int32_t pg = page_of(t, b, (int32_t)((j0 + w) >> t.tshift));
-                if (pg < 0) continue;
-                const int64_t at = (int64_t)pg * t.heads + kvh;
-                const int32_t slot = (int32_t)(j0 + w) & ((1 << t.tshift) - 1);
-                const uint8_t c = a.v[(at << t.tshift) * D + v_place(slot, threadIdx.x, D)];
-                o = fmaf(p[w] * a.vs[at], __builtin_amdgcn_cvt_f32_fp8((int)c, 0), o);
-            }
-        }
-        m = m1;
-        __syncthreads();
-    }
-    if ((int32_t)threadIdx.x < D) {
-        const int64_t i = row * a.o_token + h * a.o_head + threadIdx.x;
-        const float y = l == 0.0f ? 0.0f : o / l;
-        if (a.o_bf16)
-            static_cast<uint16_t *>(a.o)[i] = bf16_rne(y);
-        else
-            static_cast<float *>(a.o)[i] = y;
-    }
-}
-
 // ------------------------------------------------------------------- plan --
 
 constexpr int kFewWaves = 4;
@@ -535,31 +754,42 @@ Plan make_plan(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t max_q, i
     Plan p{};
     const int64_t rows = max_q * (q_heads / kv_heads);
     p.few = rows <= 64;
-    p.sp.tiles = (int32_t)((rows + 15) / 16);
+    const int64_t tile = p.few ? 16 : kManyRows;
+    p.sp.tiles = (int32_t)((rows + tile - 1) / tile);
     // tokens that a row tile can see
     int64_t span = max_kv;
     if (window > 0 && window < span && window + max_q + 64 < span) span = window + max_q + 64;
     const int64_t groups = seqs * kv_heads * p.sp.tiles, steps = (span + 63) / 64;
-    int64_t splits = (1024 + groups - 1) / groups;
-    if (splits > (steps + kFewWaves - 1) / kFewWaves) splits = (steps + kFewWaves - 1) / kFewWaves;
+    int64_t splits = ((p.few ? 1024 : 512) + groups - 1) / groups;
+    const int64_t most = (steps + 3) / 4;  // a step for each wavefront, or four for the workgroup
+    if (splits > most) splits = most;
     if (splits > 128) splits = 128;
-    if (splits < 1 || !p.few) splits = 1;
+    if (splits < 1) splits = 1;
     p.sp.chunk = (int32_t)(((steps + splits - 1) / splits) * 64);
     p.sp.splits = (int32_t)splits;
     return p;
 }
 
 template <int DC, int NQ, int NP>
-hipError_t launch_few(const AttentionArgs &a, const Split &sp, hipStream_t s) {
-    const unsigned grid = (unsigned)((int64_t)a.t.heads * sp.splits * sp.tiles * a.t.seqs);
+void start_few(const AttentionArgs &a, const Split &sp, unsigned grid, hipStream_t s) {
     hipLaunchKernelGGL((k_attention_few<DC, NQ, NP, kFewWaves>), dim3(grid), dim3(kFewWaves * 64), 0, s, a, sp);
-    return hipGetLastError();
 }
 
-template <int DC>
-hipError_t launch_few_t(const AttentionArgs &a, const Split &sp, hipStream_t s) {
-    if (a.q_bf16) return a.o_bf16 ? launch_few<DC, 1, 1>(a, sp, s) : launch_few<DC, 1, 2>(a, sp, s);
-    return a.o_bf16 ? launch_few<DC, 2, 1>(a, sp, s) : launch_few<DC, 2, 2>(a, sp, s);
+template <int DP, int NQ, int NP>
+void start_many(const AttentionArgs &a, const Split &sp, unsigned grid, hipStream_t s) {
+    if (a.t.dim == DP)
+        hipLaunchKernelGGL((k_attention_many<DP, true, NQ, NP>), dim3(grid), dim3(kManyWaves * 64), 0, s, a, sp);
+    else
+        hipLaunchKernelGGL((k_attention_many<DP, false, NQ, NP>), dim3(grid), dim3(kManyWaves * 64), 0, s, a, sp);
+}
+
+template <int NQ, int NP>
+void start(const AttentionArgs &a, const Plan &p, unsigned grid, hipStream_t s) {
+    const int32_t D = a.t.dim;
+    if (p.few)
+        D <= 64 ? start_few<1, NQ, NP>(a, p.sp, grid, s) : D <= 128 ? start_few<2, NQ, NP>(a, p.sp, grid, s) : start_few<4, NQ, NP>(a, p.sp, grid, s);
+    else
+        D <= 64 ? start_many<64, NQ, NP>(a, p.sp, grid, s) : D <= 128 ? start_many<128, NQ, NP>(a, p.sp, grid, s) : start_many<256, NQ, NP>(a, p.sp, grid, s);
 }
 
 }  // namespace
@@ -570,17 +800,25 @@ int64_t attention_workspace(int64_t tokens, int64_t seqs, int64_t q_heads, int64
     return p.sp.splits > 1 ? tokens * q_heads * p.sp.splits * (dim + 1) * 4 : 0;
 }
 
+int64_t attention_groups(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t max_q, int64_t max_kv) {
+    const Plan p = make_plan(seqs, q_heads, kv_heads, max_q, max_kv, 0);
+    return seqs * kv_heads * p.sp.tiles * p.sp.splits;
+}
+
 hipError_t launch_attention(const AttentionArgs &a, void *work, hipStream_t s, const char **kernel) {
     Plan p = make_plan(a.t.seqs, a.q_heads, a.t.heads, a.max_q, a.max_kv, a.window);
-    if (!p.few) {
-        *kernel = "attention_rows";
-        hipLaunchKernelGGL(k_attention_rows, dim3((unsigned)((int64_t)a.t.tokens * a.q_heads)), dim3(kThreads), 0, s, a);
-        return hipGetLastError();
-    }
     p.sp.o = static_cast<float *>(work);
     p.sp.lse = p.sp.o + (int64_t)a.t.tokens * a.q_heads * p.sp.splits * a.t.dim;
-    *kernel = p.sp.splits > 1 ? "attention_few, attention_join" : "attention_few";
-    hipError_t err = a.t.dim <= 64 ? launch_few_t<1>(a, p.sp, s) : a.t.dim <= 128 ? launch_few_t<2>(a, p.sp, s) : launch_few_t<4>(a, p.sp, s);
+    if (p.few)
+        *kernel = p.sp.splits > 1 ? "attention_few, attention_join" : "attention_few";
+    else
+        *kernel = p.sp.splits > 1 ? "attention_many, attention_join" : "attention_many";
+    const unsigned grid = (unsigned)((int64_t)a.t.seqs * a.t.heads * p.sp.tiles * p.sp.splits);
+    if (a.q_bf16)
+        a.o_bf16 ? start<1, 1>(a, p, grid, s) : start<1, 2>(a, p, grid, s);
+    else
+        a.o_bf16 ? start<2, 1>(a, p, grid, s) : start<2, 2>(a, p, grid, s);
+    const hipError_t err = hipGetLastError();
     if (err != hipSuccess || p.sp.splits == 1) return err;
     const int64_t rows = (int64_t)a.t.seqs * a.max_q * a.q_heads;
     hipLaunchKernelGGL(k_attention_join, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, p.sp);
