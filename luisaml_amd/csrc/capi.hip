@@ -881,9 +881,12 @@ int make_tokens(lcml::KvTokens &t, const char *fn, int64_t tokens, const void *k
     return LCML_OK;
 }
 
+// 2^32 work items a launch: at most 256 threads for a page and head, or a
+// thread for 4 tokens x 8 elements of it
 int check_kv_grid(const char *fn, const lcml::KvTokens &t, int64_t max_q) {
     const int64_t per_seq = lcml::kv_pages_per_seq(max_q, t.tshift) * 2 * t.heads;
-    if (per_seq > (((int64_t)1 << 23) - 1) / t.seqs)  // 256 threads each, 2^32 work items a launch
+    const int64_t units = (int64_t)(t.dim >> 3) << (t.tshift - 2), threads = units > 256 ? units : 256;
+    if (per_seq > (((int64_t)1 << 32) - 256) / threads / t.seqs)
         return fail(LCML_ERR_UNSUPPORTED, "%s: seqs=%lld max_q=%lld exceeds one launch", fn, (long long)t.seqs,
                     (long long)max_q);
     return LCML_OK;

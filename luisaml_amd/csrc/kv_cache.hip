@@ -1,19 +1,21 @@
 // kv_cache.hip -- tokens into an E4M3 cache of pages, and back (gfx950).
 //
 // Both directions stream: a written token costs 2 or 4 bytes in and one out
-// for each element, a read one the inverse.  One workgroup takes one page of
-// one head, of K or of V, so the page's maximum, its scale and the codes that
-// stay are its own and no order between workgroups matters.  A thread's unit
-// is 4 tokens x 8 elements: four row loads of 16 or 32 bytes, and in the
-// cache 4 x 8 bytes of K or 32 contiguous bytes of V, which transposes V in
-// registers.
+// for each element, a read one the inverse.  A thread's unit is 4 tokens x 8
+// elements: four row loads of 16 or 32 bytes, and in the cache 4 x 8 bytes of K
+// or 32 contiguous bytes of V, which transposes V in registers.  Writing, one
+// workgroup takes one page of one head, of K or of V, so the page's maximum,
+// its scale and the codes that stay are its own and no order between
+// workgroups matters; the new rows stay in registers between the maximum and
+// the codes.  Reading, threads take units of consecutive heads, so that a
+// workgroup's rows are contiguous across them.
 #include "kv_cache.hpp"
 #include "lcml_internal.hpp"
 
 namespace lcml {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;  // of a read
 
 struct __attribute__((packed, aligned(2))) H8 {
     uint16_t v[8];
@@ -44,19 +46,19 @@ __device__ inline void load8(const char *p, float *x) {
     }
 }
 
-// where the workgroup is: K or V, head, page, and the page's new slots
+// one page that the call touches: K or V, head, and the page's new slots
 struct Spot {
     bool is_v;
     int32_t head, page, lo, hi;  // new slots lo .. hi-1
     int64_t row;                 // the call's row of slot 0
 };
 
-__device__ inline bool find_spot(const KvTokens &t, int32_t pages_per_seq, Spot *s) {
-    uint32_t i = blockIdx.x;
-    s->is_v = i & 1;
-    i >>= 1;
+// spot i of [seqs][pages_per_seq][K, V][heads]; false: no new slot there
+__device__ inline bool find_spot(const KvTokens &t, int32_t pages_per_seq, uint32_t i, Spot *s) {
     s->head = i % t.heads;
     i /= t.heads;
+    s->is_v = i & 1;
+    i >>= 1;
     const int32_t r = i % pages_per_seq, b = i / pages_per_seq;
     const SeqRows q = seq_rows(t, b);
     if (q.n <= 0) return false;
@@ -103,7 +105,8 @@ __device__ inline uint32_t encode_again(uint32_t w, float k) {
     return e4m3x2_hw(a[0] * k, a[1] * k) | (e4m3x2_hw(b[0] * k, b[1] * k) << 16);
 }
 
-template <bool V, bool BF16>
+// NT threads, UPT units each in registers; pages of more units load rows again
+template <bool V, bool BF16, int NT, int UPT>
 __device__ inline void write_page(const KvTokens &t, const Spot &sp, const Rows &rows, uint8_t *cache, float *scales,
                                   float *red) {
     const int32_t D = t.dim, T = 1 << t.tshift, d8 = D >> 3;
@@ -113,67 +116,79 @@ __device__ inline void write_page(const KvTokens &t, const Spot &sp, const Rows 
                         : rows.k + (sp.row * rows.kt + sp.head * rows.kh) * (BF16 ? 2 : 4);
     const int64_t pitch = (V ? rows.vt : rows.kt) * (BF16 ? 2 : 4);
     const int32_t units = (T >> 2) * d8;
-    auto load = [&](int32_t g, int i, float *x) {
-        load8<BF16>(src + (int64_t)(g / d8 * 4 + i) * pitch + (int64_t)(g % d8) * 8 * (BF16 ? 2 : 4), x);
-    };
+    float old = scales[at];
     float m = 0.0f;
-    for (int32_t g = threadIdx.x; g < units; g += kThreads) {
+    // the new rows of unit g; zeros for the others
+    auto load = [&](int32_t g, float (*x)[8]) {
         const int32_t t0 = g / d8 * 4;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (t0 + i >= sp.lo && t0 + i < sp.hi) {
-                float x[8];
-                load(g, i, x);
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float a = fabsf(x[e]);
-                    m = a > m && a < __builtin_inff() ? a : m;
-                }
+            for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
+            if (g < units && t0 + i >= sp.lo && t0 + i < sp.hi)
+                load8<BF16>(src + (int64_t)(t0 + i) * pitch + (int64_t)(g % d8) * 8 * (BF16 ? 2 : 4), x[i]);
+        }
+    };
+    auto amax = [&](const float (*x)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float a = fabsf(x[i][e]);
+                m = a > m && a < __builtin_inff() ? a : m;
             }
+    };
+    float x[UPT][4][8];
+#pragma unroll
+    for (int u = 0; u < UPT; ++u) load(u * NT + threadIdx.x, x[u]);
+#pragma unroll
+    for (int u = 0; u < UPT; ++u) amax(x[u]);
+    for (int32_t g = UPT * NT + threadIdx.x; g < units; g += NT) {
+        float y[4][8];
+        load(g, y);
+        amax(y);
     }
-    float s = page_scale(block_max<kThreads>(m, red)), grow = 1.0f;
+    asm volatile("" : "+v"(old));  // every wavefront has it before the barrier that the new one's store follows
+    m = NT == 64 ? wave_max(m) : block_max<NT>(m, red);
+    float s = page_scale(m), grow = 1.0f;
     if (sp.lo > 0) {  // tokens that stay
-        const float old = scales[at];
         if (old >= s)
             s = old;
         else
             grow = old / s;
     }
-    __syncthreads();  // every thread has read the old scale
     if (threadIdx.x == 0) scales[at] = s;
     const float inv = 1.0f / s;  // a power of two: x * inv is x / s
-    for (int32_t g = threadIdx.x; g < units; g += kThreads) {
+    auto put = [&](int32_t g, const float (*x)[8]) {
         const int32_t t0 = g / d8 * 4, e0 = g % d8 * 8;
         const bool fresh = t0 < sp.hi && t0 + 4 > sp.lo, stays = t0 < sp.lo && grow != 1.0f;
-        if (!fresh && !stays) continue;
-        uint32_t w[8];
-        load_codes<V>(blk, t0, e0, D, w);
-        uint32_t n[8];
+        if (g >= units || !(fresh || stays)) return;
+        uint32_t w[8], out[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) n[q] = stays ? encode_again(w[q], grow) : w[q];
-        uint32_t out[8];
+        for (int q = 0; q < 8; ++q) w[q] = out[q] = 0;
+        if (t0 < sp.lo || t0 + 4 > sp.hi) {  // tokens that stay, or slots past the last one, which keep their bytes
+            load_codes<V>(blk, t0, e0, D, w);
+            if (stays)
 #pragma unroll
-        for (int q = 0; q < 8; ++q) out[q] = 0;
+                for (int i = 0; i < 4; ++i)
+                    if (t0 + i < sp.lo)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int wi = word_of<V>(i, e), sh = 8 * byte_of<V>(i, e);
+                            const float c = __builtin_amdgcn_cvt_f32_fp8((int)(w[wi] >> sh), 0);
+                            w[wi] = (w[wi] & ~(0xffu << sh)) | ((e4m3x2_hw(c * grow, 0.0f) & 0xffu) << sh);
+                        }
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int32_t slot = t0 + i;
-            float x[8];
-            const bool now = slot >= sp.lo && slot < sp.hi;
-            if (now) load(g, i, x);
+            const bool now = t0 + i >= sp.lo && t0 + i < sp.hi;
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
                 const int wi = word_of<V>(i, e), wj = word_of<V>(i, e + 1);
-                const int bi = 8 * byte_of<V>(i, e), bj = 8 * byte_of<V>(i, e + 1);
-                uint32_t c0, c1;
-                if (now) {
-                    const uint32_t c = e4m3x2_hw(x[e] * inv, x[e + 1] * inv);
-                    c0 = c & 0xffu, c1 = c >> 8;
-                } else {  // a kept token, or a slot past the last one as it was
-                    c0 = ((slot < sp.lo ? n[wi] : w[wi]) >> bi) & 0xffu;
-                    c1 = ((slot < sp.lo ? n[wj] : w[wj]) >> bj) & 0xffu;
-                }
-                out[wi] |= c0 << bi;
-                out[wj] |= c1 << bj;
+                const int si = 8 * byte_of<V>(i, e), sj = 8 * byte_of<V>(i, e + 1);
+                const uint32_t c = e4m3x2_hw(x[i][e] * inv, x[i][e + 1] * inv);
+                out[wi] |= (now ? c & 0xffu : w[wi] >> si & 0xffu) << si;
+                out[wj] |= (now ? c >> 8 : w[wj] >> sj & 0xffu) << sj;
             }
         }
         if constexpr (V) {
@@ -185,71 +200,78 @@ __device__ inline void write_page(const KvTokens &t, const Spot &sp, const Rows 
             for (int i = 0; i < 4; ++i)
                 *reinterpret_cast<u2 *>(blk + k_place(t0 + i, e0, D)) = u2{out[2 * i], out[2 * i + 1]};
         }
+    };
+#pragma unroll
+    for (int u = 0; u < UPT; ++u) put(u * NT + threadIdx.x, x[u]);
+    for (int32_t g = UPT * NT + threadIdx.x; g < units; g += NT) {
+        float y[4][8];
+        load(g, y);
+        put(g, y);
     }
 }
 
-template <bool BF16>
-__global__ __launch_bounds__(kThreads) void k_kv_write(KvTokens t, Rows rows, uint8_t *kc, uint8_t *vc, float *ks,
-                                                       float *vs, int32_t pages_per_seq) {
-    __shared__ float red[kThreads / 64];
+template <bool BF16, int NT, int UPT>
+__global__ __launch_bounds__(NT) void k_kv_write(KvTokens t, Rows rows, uint8_t *kc, uint8_t *vc, float *ks, float *vs,
+                                                 int32_t pages_per_seq) {
+    __shared__ float red[NT / 64];
     Spot sp;
-    if (!find_spot(t, pages_per_seq, &sp)) return;
+    if (!find_spot(t, pages_per_seq, blockIdx.x, &sp)) return;
     if (sp.is_v)
-        write_page<true, BF16>(t, sp, rows, vc, vs, red);
+        write_page<true, BF16, NT, UPT>(t, sp, rows, vc, vs, red);
     else
-        write_page<false, BF16>(t, sp, rows, kc, ks, red);
+        write_page<false, BF16, NT, UPT>(t, sp, rows, kc, ks, red);
 }
 
 template <bool V, bool BF16>
-__device__ inline void read_page(const KvTokens &t, const Spot &sp, const Rows &rows, const uint8_t *cache,
-                                 const float *scales) {
-    const int32_t D = t.dim, T = 1 << t.tshift, d8 = D >> 3;
+__device__ inline void read_unit(const KvTokens &t, const Spot &sp, const Rows &rows, const uint8_t *cache,
+                                 const float *scales, int32_t g) {
+    const int32_t D = t.dim, d8 = D >> 3, t0 = g / d8 * 4, e0 = g % d8 * 8;
+    if (t0 + 4 <= sp.lo || t0 >= sp.hi) return;
     const int64_t at = (int64_t)sp.page * t.heads + sp.head;
-    const uint8_t *blk = cache + (at << t.tshift) * D;
-    char *dst = V ? rows.vo + (sp.row * rows.vt + sp.head * rows.vh) * (BF16 ? 2 : 4)
-                  : rows.ko + (sp.row * rows.kt + sp.head * rows.kh) * (BF16 ? 2 : 4);
-    const int64_t pitch = (V ? rows.vt : rows.kt) * (BF16 ? 2 : 4);
+    uint32_t w[8];
+    load_codes<V>(cache + (at << t.tshift) * D, t0, e0, D, w);
     const float s = scales[at];
-    for (int32_t g = threadIdx.x; g < (T >> 2) * d8; g += kThreads) {
-        const int32_t t0 = g / d8 * 4, e0 = g % d8 * 8;
-        if (t0 + 4 <= sp.lo || t0 >= sp.hi) continue;
-        uint32_t w[8];
-        load_codes<V>(blk, t0, e0, D, w);
-        float x[8][4];  // [word][byte]
+    char *dst = V ? rows.vo + ((sp.row + t0) * rows.vt + sp.head * rows.vh + e0) * (BF16 ? 2 : 4)
+                  : rows.ko + ((sp.row + t0) * rows.kt + sp.head * rows.kh + e0) * (BF16 ? 2 : 4);
+    const int64_t pitch = (V ? rows.vt : rows.kt) * (BF16 ? 2 : 4);
+    float x[8][4];  // [word][byte]
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[q], false);
-            const f2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[q], true);
-            x[q][0] = a[0] * s, x[q][1] = a[1] * s, x[q][2] = b[0] * s, x[q][3] = b[1] * s;
-        }
+    for (int q = 0; q < 8; ++q) {
+        const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[q], false);
+        const f2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[q], true);
+        x[q][0] = a[0] * s, x[q][1] = a[1] * s, x[q][2] = b[0] * s, x[q][3] = b[1] * s;
+    }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (t0 + i < sp.lo || t0 + i >= sp.hi) continue;
-            char *p = dst + (int64_t)(t0 + i) * pitch + (int64_t)e0 * (BF16 ? 2 : 4);
-            if constexpr (BF16) {
-                H8 o;
+    for (int i = 0; i < 4; ++i) {
+        if (t0 + i < sp.lo || t0 + i >= sp.hi) continue;
+        if constexpr (BF16) {
+            H8 o;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o.v[e] = bf16_rne(x[word_of<V>(i, e)][byte_of<V>(i, e)]);
-                *reinterpret_cast<H8 *>(p) = o;
-            } else {
-                F8x32 o;
+            for (int e = 0; e < 8; ++e) o.v[e] = bf16_rne(x[word_of<V>(i, e)][byte_of<V>(i, e)]);
+            *reinterpret_cast<H8 *>(dst + i * pitch) = o;
+        } else {
+            F8x32 o;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o.v[e] = x[word_of<V>(i, e)][byte_of<V>(i, e)];
-                *reinterpret_cast<F8x32 *>(p) = o;
-            }
+            for (int e = 0; e < 8; ++e) o.v[e] = x[word_of<V>(i, e)][byte_of<V>(i, e)];
+            *reinterpret_cast<F8x32 *>(dst + i * pitch) = o;
         }
     }
 }
 
+// a unit a thread, in the order [spots][units of a page and head]
 template <bool BF16>
 __global__ __launch_bounds__(kThreads) void k_kv_read(KvTokens t, Rows rows, const uint8_t *kc, const uint8_t *vc,
-                                                      const float *ks, const float *vs, int32_t pages_per_seq) {
+                                                      const float *ks, const float *vs, int32_t pages_per_seq,
+                                                      uint32_t spots) {
+    const uint32_t units = (uint32_t)(t.dim >> 3) << (t.tshift - 2);
+    const uint64_t id = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
+    const uint32_t i = (uint32_t)(id / units), g = (uint32_t)(id - (uint64_t)i * units);
     Spot sp;
-    if (!find_spot(t, pages_per_seq, &sp)) return;
+    if (i >= spots || !find_spot(t, pages_per_seq, i, &sp)) return;
     if (sp.is_v)
-        read_page<true, BF16>(t, sp, rows, vc, vs);
+        read_unit<true, BF16>(t, sp, rows, vc, vs, g);
     else
-        read_page<false, BF16>(t, sp, rows, kc, ks);
+        read_unit<false, BF16>(t, sp, rows, kc, ks, g);
 }
 
 }  // namespace
@@ -257,16 +279,26 @@ __global__ __launch_bounds__(kThreads) void k_kv_read(KvTokens t, Rows rows, con
 // pages that max_q tokens of one sequence can touch
 int64_t kv_pages_per_seq(int64_t max_q, int tshift) { return ((max_q - 2 + ((int64_t)1 << tshift)) >> tshift) + 1; }
 
+template <bool BF16>
+static void start_kv_write(const KvTokens &t, const Rows &r, uint8_t *kc, uint8_t *vc, float *ks, float *vs, int32_t pp,
+                           hipStream_t s) {
+    const dim3 grid((unsigned)(2 * t.heads * pp * t.seqs));
+    const int units = (t.dim >> 3) << (t.tshift - 2);
+    // a wavefront where it holds the page (no barriers); else 256 threads
+    if (units <= 64)
+        hipLaunchKernelGGL((k_kv_write<BF16, 64, 1>), grid, dim3(64), 0, s, t, r, kc, vc, ks, vs, pp);
+    else if (units <= 256)
+        hipLaunchKernelGGL((k_kv_write<BF16, 256, 1>), grid, dim3(256), 0, s, t, r, kc, vc, ks, vs, pp);
+    else
+        hipLaunchKernelGGL((k_kv_write<BF16, 256, 4>), grid, dim3(256), 0, s, t, r, kc, vc, ks, vs, pp);
+}
+
 hipError_t launch_kv_write(const KvTokens &t, int64_t max_q, const void *k, const void *v, bool bf16, int64_t kt,
                            int64_t kh, int64_t vt, int64_t vh, uint8_t *kc, uint8_t *vc, float *ks, float *vs,
                            hipStream_t s) {
     const Rows rows{(const char *)k, (const char *)v, nullptr, nullptr, kt, kh, vt, vh};
-    const int64_t pp = kv_pages_per_seq(max_q, t.tshift);
-    const dim3 grid((unsigned)(2 * t.heads * pp * t.seqs));
-    if (bf16)
-        hipLaunchKernelGGL((k_kv_write<true>), grid, dim3(kThreads), 0, s, t, rows, kc, vc, ks, vs, (int32_t)pp);
-    else
-        hipLaunchKernelGGL((k_kv_write<false>), grid, dim3(kThreads), 0, s, t, rows, kc, vc, ks, vs, (int32_t)pp);
+    const int32_t pp = (int32_t)kv_pages_per_seq(max_q, t.tshift);
+    bf16 ? start_kv_write<true>(t, rows, kc, vc, ks, vs, pp, s) : start_kv_write<false>(t, rows, kc, vc, ks, vs, pp, s);
     return hipGetLastError();
 }
 
@@ -274,12 +306,13 @@ hipError_t launch_kv_read(const KvTokens &t, int64_t max_q, void *k, void *v, bo
                           int64_t vt, int64_t vh, const uint8_t *kc, const uint8_t *vc, const float *ks,
                           const float *vs, hipStream_t s) {
     const Rows rows{nullptr, nullptr, (char *)k, (char *)v, kt, kh, vt, vh};
-    const int64_t pp = kv_pages_per_seq(max_q, t.tshift);
-    const dim3 grid((unsigned)(2 * t.heads * pp * t.seqs));
+    const int64_t pp = kv_pages_per_seq(max_q, t.tshift), spots = 2 * t.heads * pp * t.seqs;
+    const int64_t units = (int64_t)(t.dim >> 3) << (t.tshift - 2);
+    const dim3 grid((unsigned)((spots * units + kThreads - 1) / kThreads));
     if (bf16)
-        hipLaunchKernelGGL((k_kv_read<true>), grid, dim3(kThreads), 0, s, t, rows, kc, vc, ks, vs, (int32_t)pp);
+        hipLaunchKernelGGL((k_kv_read<true>), grid, dim3(kThreads), 0, s, t, rows, kc, vc, ks, vs, (int32_t)pp, (uint32_t)spots);
     else
-        hipLaunchKernelGGL((k_kv_read<false>), grid, dim3(kThreads), 0, s, t, rows, kc, vc, ks, vs, (int32_t)pp);
+        hipLaunchKernelGGL((k_kv_read<false>), grid, dim3(kThreads), 0, s, t, rows, kc, vc, ks, vs, (int32_t)pp, (uint32_t)spots);
     return hipGetLastError();
 }
 
