@@ -50,15 +50,28 @@ __device__ inline float load1(const void *p, int64_t i) {
         return static_cast<const float *>(p)[i];
 }
 
-// elements i .. i+3 of a row of H; zero past its end
-template <bool BF16>
+// how a row of H is taken in groups of four
+enum { kWhole = 0, kOdd = 1, kTiny = 2 };  // H % 4 == 0; H > 4; H < 4
+
+// elements i .. i+3 of a row of H, zero past its end, without a branch: past
+// the last whole group the row's last four are loaded, and moved into place
+template <bool BF16, int CUT>
 __device__ inline f4 load_row4(const void *p, int64_t i, int64_t H) {
-    if (i + 4 <= H) return load4<BF16>(p, i);
-    f4 v{0.f, 0.f, 0.f, 0.f};
+    const f4 zero{0.f, 0.f, 0.f, 0.f};
+    if constexpr (CUT == kTiny) {
+        f4 v = zero;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (i + e < H) v[e] = load1<BF16>(p, i + e);
-    return v;
+        for (int e = 0; e < 3; ++e)
+            if (i + e < H) v[e] = load1<BF16>(p, i + e);
+        return v;
+    }
+    f4 v = load4<BF16>(p, i + 4 <= H ? i : H - 4);
+    if constexpr (CUT == kOdd) {
+        const int64_t by = i + 4 - H;  // 1, 2, 3: that many past the end
+        if (by >= 2) v = f4{v[2], v[3], 0.f, 0.f};
+        if (by == 1 || by == 3) v = f4{v[1], v[2], v[3], 0.f};
+    }
+    return i < H ? v : zero;
 }
 
 __device__ inline float wave_sum(float v) {
@@ -98,47 +111,59 @@ enum { kStatic = 0, kTensor = 1, kRow = 2 };
 // residual: none, fp32, bf16
 enum { kNoRes = 0, kResF32 = 1, kResBf16 = 2 };
 
-// h of four elements of row m, rounded to the residual's type
-template <bool XB, int RES>
-__device__ inline f4 load_h(const NormArgs &a, int64_t m, int64_t i) {
-    const char *xr = static_cast<const char *>(a.x) + m * a.ldx * (XB ? 2 : 4);
-    f4 v = load_row4<XB>(xr, i, a.H);
-    if constexpr (RES != kNoRes) {
-        const char *rr = static_cast<const char *>(a.res) + m * a.ldr * (RES == kResBf16 ? 2 : 4);
-        v += load_row4<RES == kResBf16>(rr, i, a.H);
+// x and the residual of four elements of row m, and h from them, rounded to
+// the residual's type
+template <bool XB, int RES, int CUT>
+struct Raw {
+    f4 x, r;
+    __device__ inline void load(const NormArgs &a, int64_t m, int64_t i) {
+        x = load_row4<XB, CUT>(static_cast<const char *>(a.x) + m * a.ldx * (XB ? 2 : 4), i, a.H);
+        if constexpr (RES != kNoRes)
+            r = load_row4<RES == kResBf16, CUT>(static_cast<const char *>(a.res) + m * a.ldr * (RES == kResBf16 ? 2 : 4), i, a.H);
+    }
+    __device__ inline f4 h() const {
+        if constexpr (RES == kNoRes) return x;
+        f4 v = x + r;
         if constexpr (RES == kResBf16)
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = widen(bf16_rne(v[e]));
+        return v;
     }
-    return v;
-}
+};
 
-template <int RES>
+template <int RES, int CUT>
 __device__ inline void store_h(const NormArgs &a, int64_t m, int64_t i, f4 h) {
+    if (i >= a.H) return;
+    const bool whole = CUT == kWhole || i + 4 <= a.H;
     if constexpr (RES == kResBf16) {
         uint16_t *o = static_cast<uint16_t *>(a.res_out) + m * a.ldro + i;
         H4 q;
 #pragma unroll
         for (int e = 0; e < 4; ++e) q.v[e] = (uint16_t)(f32_bits(h[e]) >> 16);
-        if (i + 4 <= a.H)
+        if (whole)
             *reinterpret_cast<H4 *>(o) = q;
         else
-            for (int e = 0; e < 4 && i + e < a.H; ++e) o[e] = q.v[e];
+            for (int e = 0; e < 3; ++e)
+                if (i + e < a.H) o[e] = q.v[e];
     } else if constexpr (RES == kResF32) {
         float *o = static_cast<float *>(a.res_out) + m * a.ldro + i;
-        if (i + 4 <= a.H)
+        if (whole)
             *reinterpret_cast<F4 *>(o) = F4{{h[0], h[1], h[2], h[3]}};
         else
-            for (int e = 0; e < 4 && i + e < a.H; ++e) o[e] = h[e];
+            for (int e = 0; e < 3; ++e)
+                if (i + e < a.H) o[e] = h[e];
     }
 }
 
+template <int CUT>
 __device__ inline void store_codes(const NormArgs &a, int64_t m, int64_t i, uint32_t c) {
+    if (i >= a.H) return;
     uint8_t *o = a.y + m * a.ldy + i;
-    if (i + 4 <= a.H)
+    if (CUT == kWhole || i + 4 <= a.H)
         reinterpret_cast<C4 *>(o)->v = c;
     else
-        for (int e = 0; e < 4 && i + e < a.H; ++e) o[e] = (uint8_t)(c >> (8 * e));
+        for (int e = 0; e < 3; ++e)
+            if (i + e < a.H) o[e] = (uint8_t)(c >> (8 * e));
 }
 
 __device__ inline float abs_max4(float m, f4 v) {
@@ -150,129 +175,206 @@ __device__ inline float abs_max4(float m, f4 v) {
     return m;
 }
 
-// One row at a time; NV groups of four elements for each thread stay in
-// registers.  Rows longer than THREADS * NV * 4 read their tail again.
-template <bool XB, int RES, int THREADS, int NV>
-__global__ __launch_bounds__(THREADS) void k_rms_norm(NormArgs a) {
-    __shared__ float red[THREADS / 64];
-    constexpr int64_t kHeld = (int64_t)THREADS * NV * 4;
+// TPR threads a row (64: four rows of a workgroup side by side, no barriers),
+// NV groups of four elements for each thread in registers.  TAIL: rows longer
+// than TPR * NV * 4, which read the rest again.
+template <bool XB, int RES, int CUT, int TPR, int NV, bool TAIL>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm(NormArgs a) {
+    constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR;
+    constexpr int64_t kHeld = (int64_t)TPR * NV * 4;
+    __shared__ float red[kThreads / 64];
+    const int t = threadIdx.x % TPR;
+    auto tail = [&](int64_t m, auto f) {
+        if constexpr (TAIL)
+            for (int64_t i = kHeld + t * 4; i < a.H; i += TPR * 4) {
+                Raw<XB, RES, CUT> raw;
+                raw.load(a, m, i);
+                f(raw.h(), i);
+            }
+    };
+    const bool store = RES != kNoRes && a.res_out;
     float tensor_max = 0.0f;
-    for (int64_t m = blockIdx.x; m < a.M; m += gridDim.x) {
-        f4 h[NV];
+    for (int64_t m = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR; m < a.M; m += (int64_t)gridDim.x * kRows) {
+        Raw<XB, RES, CUT> raw[NV];
+        f4 h[NV], gamma[NV];
         float ss = 0.0f;
+        auto at = [&](int u) { return ((int64_t)u * TPR + t) * 4; };
 #pragma unroll
-        for (int u = 0; u < NV; ++u) {
-            const int64_t i = ((int64_t)u * THREADS + threadIdx.x) * 4;
-            h[u] = i < a.H ? load_h<XB, RES>(a, m, i) : f4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int u = 0; u < NV; ++u) raw[u].load(a, m, at(u));
 #pragma unroll
-        for (int u = 0; u < NV; ++u) {
-            const int64_t i = ((int64_t)u * THREADS + threadIdx.x) * 4;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) ss = fmaf(h[u][e], h[u][e], ss);
-            if (RES != kNoRes && a.res_out && i < a.H) store_h<RES>(a, m, i, h[u]);
-        }
-        for (int64_t i = kHeld + threadIdx.x * 4; i < a.H; i += THREADS * 4) {
-            const f4 v = load_h<XB, RES>(a, m, i);
+        for (int u = 0; u < NV; ++u) gamma[u] = load_row4<false, CUT>(a.gamma, at(u), a.H);
+        auto sum = [&](f4 v) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) ss = fmaf(v[e], v[e], ss);
-        }
-        ss = block_sum<THREADS>(ss, red);
-        const float r = 1.0f / sqrtf(ss / (float)a.H + a.eps);
-        auto norm = [&](f4 v, int64_t i) { return v * r * load_row4<false>(a.gamma, i, a.H); };
-        float mx = 0.0f;
+        };
 #pragma unroll
-        for (int u = 0; u < NV; ++u) {
-            const int64_t i = ((int64_t)u * THREADS + threadIdx.x) * 4;
-            if (i < a.H) h[u] = norm(h[u], i);
-            mx = abs_max4(mx, h[u]);
-        }
-        float s;
+        for (int u = 0; u < NV; ++u) sum(h[u] = raw[u].h());
+        if (store)
+#pragma unroll
+            for (int u = 0; u < NV; ++u) store_h<RES, CUT>(a, m, at(u), h[u]);
+        tail(m, [&](f4 v, int64_t) { sum(v); });
+        ss = block_sum<TPR>(ss, red);
+        const float r = 1.0f / sqrtf(ss / (float)a.H + a.eps);
+        auto norm = [&](f4 v, int64_t i) { return v * r * load_row4<false, CUT>(a.gamma, i, a.H); };
+        float mx = 0.0f, s;
+#pragma unroll
+        for (int u = 0; u < NV; ++u) mx = abs_max4(mx, h[u] = h[u] * r * gamma[u]);
         if (a.mode == kStatic) {
             s = a.scale[0];
         } else {
-            for (int64_t i = kHeld + threadIdx.x * 4; i < a.H; i += THREADS * 4)
-                mx = abs_max4(mx, norm(load_h<XB, RES>(a, m, i), i));
+            tail(m, [&](f4 v, int64_t i) {
+                mx = abs_max4(mx, norm(v, i));
+                if (store && a.mode == kTensor) store_h<RES, CUT>(a, m, i, v);  // its last reader in this pass
+            });
             if (a.mode == kTensor) {
                 tensor_max = fmaxf(tensor_max, mx);
-                if (threadIdx.x == 0) a.rstd[m] = r;
-                // the tail's h, after its last reader in this row
-                if (RES != kNoRes && a.res_out)
-                    for (int64_t i = kHeld + threadIdx.x * 4; i < a.H; i += THREADS * 4)
-                        store_h<RES>(a, m, i, load_h<XB, RES>(a, m, i));
+                if (t == 0) a.rstd[m] = r;
                 continue;
             }
-            s = scale_from_amax_bits(f32_bits(block_max<THREADS>(mx, red)));
-            if (threadIdx.x == 0) a.scale[m] = s;
+            if constexpr (TPR == 64)
+                mx = wave_max(mx);
+            else
+                mx = block_max<TPR>(mx, red);
+            s = scale_from_amax_bits(f32_bits(mx));
+            if (t == 0) a.scale[m] = s;
         }
         const Recip d = make_recip(s);
+        auto encode = [&](auto fast) {
+            constexpr bool FAST = decltype(fast)::value;
 #pragma unroll
-        for (int u = 0; u < NV; ++u) {
-            const int64_t i = ((int64_t)u * THREADS + threadIdx.x) * 4;
-            const uint32_t c = quantize4(h[u][0], h[u][1], h[u][2], h[u][3], d);
-            if (i < a.H) store_codes(a, m, i, c);
-        }
-        for (int64_t i = kHeld + threadIdx.x * 4; i < a.H; i += THREADS * 4) {
-            const f4 t = load_h<XB, RES>(a, m, i);
-            if (RES != kNoRes && a.res_out) store_h<RES>(a, m, i, t);
-            const f4 v = norm(t, i);
-            store_codes(a, m, i, quantize4(v[0], v[1], v[2], v[3], d));
-        }
+            for (int u = 0; u < NV; ++u)
+                store_codes<CUT>(a, m, at(u), quantize4_t<FAST>(h[u][0], h[u][1], h[u][2], h[u][3], d));
+            tail(m, [&](f4 v, int64_t i) {
+                if (store) store_h<RES, CUT>(a, m, i, v);
+                const f4 n = norm(v, i);
+                store_codes<CUT>(a, m, i, quantize4_t<FAST>(n[0], n[1], n[2], n[3], d));
+            });
+        };
+        if (__builtin_amdgcn_ballot_w64(!d.fast) == 0)
+            encode(std::true_type{});
+        else
+            encode(std::false_type{});
     }
     if (a.mode == kTensor) {
-        const float b = block_max<THREADS>(tensor_max, red);
+        const float b = block_max<kThreads>(tensor_max, red);
         if (threadIdx.x == 0) a.part[blockIdx.x] = f32_bits(b);
     }
 }
 
 // The second pass of one scale for the tensor: codes of h (the stored one, or
 // x + residual again), from the rows' r and the partial maxima.
-template <bool XB, int RES, int THREADS>
-__global__ __launch_bounds__(THREADS) void k_norm_encode(NormArgs a, int npart) {
-    __shared__ float red[THREADS / 64];
-    const float s = scale_from_partials<THREADS>(a.part, npart, red);
+template <bool XB, int RES, int CUT>
+__global__ __launch_bounds__(256) void k_norm_encode(NormArgs a, int npart) {
+    __shared__ float red[4];
+    constexpr int NV = 4;
+    const bool stored = RES != kNoRes && a.res_out;
+    auto load = [&](int64_t m, int64_t i) {
+        if (stored)
+            return load_row4<RES == kResBf16, CUT>(
+                static_cast<const char *>(a.res_out) + m * a.ldro * (RES == kResBf16 ? 2 : 4), i, a.H);
+        Raw<XB, RES, CUT> raw;
+        raw.load(a, m, i);
+        return raw.h();
+    };
+    int64_t m = blockIdx.x;
+    f4 h[NV], gamma[NV];
+    float r;
+    auto begin = [&](int64_t i0) {
+        r = a.rstd[m];
+#pragma unroll
+        for (int u = 0; u < NV; ++u) h[u] = load(m, i0 + u * 1024);
+#pragma unroll
+        for (int u = 0; u < NV; ++u) gamma[u] = load_row4<false, CUT>(a.gamma, i0 + u * 1024, a.H);
+    };
+    const int64_t first = threadIdx.x * 4;
+    begin(first);
+    // the maxima 16 at a time (one after the other they took 8 us of 25)
+    float mx = 0.0f;
+    for (int i0 = 0; i0 < npart; i0 += 16 * 256) {
+        uint32_t v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int i = i0 + k * 256 + threadIdx.x;
+            v[k] = a.part[i < npart ? i : npart - 1];
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) mx = fmaxf(mx, bits_f32(v[k]));
+    }
+    const float s = scale_from_amax_bits(f32_bits(block_max<256>(mx, red)));
     if (blockIdx.x == 0 && threadIdx.x == 0) a.scale[0] = s;
     const Recip d = make_recip(s);
-    for (int64_t m = blockIdx.x; m < a.M; m += gridDim.x) {
-        const float r = a.rstd[m];
-        for (int64_t i = threadIdx.x * 4; i < a.H; i += THREADS * 4) {
-            f4 h;
-            if (RES != kNoRes && a.res_out)
-                h = load_row4<RES == kResBf16>(static_cast<const char *>(a.res_out) +
-                                                   m * a.ldro * (RES == kResBf16 ? 2 : 4), i, a.H);
-            else
-                h = load_h<XB, RES>(a, m, i);
-            const f4 v = h * r * load_row4<false>(a.gamma, i, a.H);
-            store_codes(a, m, i, quantize4(v[0], v[1], v[2], v[3], d));
+    auto run = [&](auto fast) {
+        for (;;) {
+            for (int64_t i0 = first; i0 < a.H; i0 += NV * 1024) {
+                if (i0 != first) begin(i0);
+#pragma unroll
+                for (int u = 0; u < NV; ++u) {
+                    const f4 v = h[u] * r * gamma[u];
+                    store_codes<CUT>(a, m, i0 + u * 1024, quantize4_t<decltype(fast)::value>(v[0], v[1], v[2], v[3], d));
+                }
+            }
+            m += gridDim.x;
+            if (m >= a.M) break;
+            begin(first);
         }
+    };
+    if (d.fast)
+        run(std::true_type{});
+    else
+        run(std::false_type{});
+}
+
+constexpr int kParts = 4096;  // at most: partial maxima of a tensor
+
+template <bool XB, int RES, int CUT>
+hipError_t launch_t(const NormArgs &a, hipStream_t s) {
+    const bool two = a.mode == kTensor;
+    auto grid = [&](int64_t rows, int64_t most) {
+        const int64_t n = (a.M + rows - 1) / rows;
+        return (unsigned)(n < most ? n : most);
+    };
+    const int64_t most = two ? kParts : 1 << 20;
+    unsigned n;
+    if constexpr (CUT == kTiny) {
+        hipLaunchKernelGGL((k_rms_norm<XB, RES, CUT, 64, 1, false>), dim3(n = grid(4, most)), dim3(256), 0, s, a);
+    } else {
+        if (a.H <= 1024)
+            hipLaunchKernelGGL((k_rms_norm<XB, RES, CUT, 64, 4, false>), dim3(n = grid(4, most)), dim3(256), 0, s, a);
+        else if (a.H <= 4096 && a.M >= 256)
+            hipLaunchKernelGGL((k_rms_norm<XB, RES, CUT, 256, 4, false>), dim3(n = grid(1, most)), dim3(256), 0, s, a);
+        else if (a.H <= 4096)  // the rows are waited for
+            hipLaunchKernelGGL((k_rms_norm<XB, RES, CUT, 1024, 1, false>), dim3(n = grid(1, most)), dim3(1024), 0, s, a);
+        else if (a.H <= 8192 && a.M >= 256)
+            hipLaunchKernelGGL((k_rms_norm<XB, RES, CUT, 512, 4, false>), dim3(n = grid(1, most)), dim3(512), 0, s, a);
+        else if (a.H <= 8192)
+            hipLaunchKernelGGL((k_rms_norm<XB, RES, CUT, 1024, 2, false>), dim3(n = grid(1, most)), dim3(1024), 0, s, a);
+        else
+            hipLaunchKernelGGL((k_rms_norm<XB, RES, CUT, 1024, 4, true>), dim3(n = grid(1, most)), dim3(1024), 0, s, a);
     }
+    hipError_t err = hipGetLastError();
+    if (err != hipSuccess || !two) return err;
+    hipLaunchKernelGGL((k_norm_encode<XB, RES, CUT>), dim3(grid(1, 2048)), dim3(256), 0, s, a, (int)n);
+    return hipGetLastError();
 }
 
 template <bool XB, int RES>
 hipError_t launch_t(const NormArgs &a, hipStream_t s) {
-    const bool two = a.mode == kTensor;
-    const int64_t most = two ? kMaxAmaxPartials : 1 << 20;
-    const unsigned grid = (unsigned)(a.M < most ? a.M : most);
-    if (a.H <= 1024)
-        hipLaunchKernelGGL((k_rms_norm<XB, RES, 64, 4>), dim3(grid), dim3(64), 0, s, a);
-    else
-        hipLaunchKernelGGL((k_rms_norm<XB, RES, 256, 4>), dim3(grid), dim3(256), 0, s, a);
-    hipError_t err = hipGetLastError();
-    if (err != hipSuccess || !two) return err;
-    hipLaunchKernelGGL((k_norm_encode<XB, RES, 256>), dim3(grid), dim3(256), 0, s, a, (int)grid);
-    return hipGetLastError();
+    if (a.H < 4) return launch_t<XB, RES, kTiny>(a, s);
+    return a.H % 4 ? launch_t<XB, RES, kOdd>(a, s) : launch_t<XB, RES, kWhole>(a, s);
 }
 
 }  // namespace
 
-int64_t rms_norm_workspace(int64_t M) { return 4 * (M + kMaxAmaxPartials); }
+int64_t rms_norm_workspace(int64_t M) { return 4 * (M + kParts); }
 
 hipError_t launch_rms_norm(int64_t M, int64_t H, const void *x, bool x_bf16, int64_t ldx, const void *res,
                            void *res_out, bool res_bf16, int64_t ldr, int64_t ldro, const float *gamma, float eps,
                            uint8_t *y, int64_t ldy, int mode, float *scale, void *work, hipStream_t s) {
+    uint32_t *part = static_cast<uint32_t *>(work);
+    float *rstd = work ? reinterpret_cast<float *>(part) + kParts : nullptr;
     // one row's scale is its tensor's
-    NormArgs a{x,   res, res_out, gamma, y,   scale, static_cast<float *>(work) + kMaxAmaxPartials, static_cast<uint32_t *>(work),
-               M,   H,   ldx,     ldr,   ldro, ldy,  eps, mode == kTensor && M == 1 ? kRow : mode};
+    const NormArgs a{x,  res, res_out, gamma, y,   scale, rstd, part, M,
+                     H,  ldx, ldr,     ldro,  ldy, eps,   mode == kTensor && M == 1 ? kRow : mode};
     const int r = !res ? kNoRes : res_bf16 ? kResBf16 : kResF32;
     if (x_bf16)
         return r == kNoRes ? launch_t<true, kNoRes>(a, s) : r == kResBf16 ? launch_t<true, kResBf16>(a, s)
