@@ -7,6 +7,7 @@ if the library is missing or a call fails, an exception is raised.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 import re
 
@@ -484,6 +485,16 @@ def binary(op: int, a: torch.Tensor, b: torch.Tensor, dtype: int, out: torch.Ten
 
 
 # ------------------------------------- norm, KV cache, attention -----------
+#
+# These run once or more for every layer and token, so their checks touch each
+# tensor's attributes once: a decode step's calls are as long as their kernels.
+
+_F32, _U8, _I32 = torch.float32, torch.uint8, torch.int32
+
+
+def _bytes_of(t):
+    return t.numel() * t.element_size() if t is not None else 0
+
 
 def rms_norm(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual: torch.Tensor | None = None,
              residual_out: torch.Tensor | None = None, mode: int = SCALE_TENSOR, scale: torch.Tensor | None = None,
@@ -492,58 +503,75 @@ def rms_norm(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual: torch.T
     linear.  x [M,H] fp32/bf16; residual fp32/bf16; gamma [H] fp32.  mode
     SCALE_STATIC takes scale[1]; SCALE_TENSOR gives it; SCALE_ROW gives [M].
     Returns (codes uint8 [M,H], scale, h or None)."""
-    assert x.dim() == 2 and x.stride(1) == 1 and gamma.dtype == torch.float32 and gamma.is_contiguous()
-    M, H = x.shape
-    assert gamma.numel() == H
+    shape = x.shape
+    M, H = shape
+    assert x.is_cuda and gamma.is_cuda, "device tensors expected"
+    assert gamma.dtype is _F32 and gamma.numel() == H and gamma.is_contiguous()
+    ldx, one = x.stride()
+    assert one == 1 or H <= 1
+    rp = rop = None
+    rt = ldr = ldro = 0
     if residual is not None:
-        assert residual.shape == x.shape and residual.stride(1) == 1
         if residual_out is None:
             residual_out = torch.empty((M, H), dtype=residual.dtype, device=x.device)
-        assert residual_out.shape == x.shape and residual_out.stride(1) == 1 and residual_out.dtype == residual.dtype
+        rdt = residual.dtype
+        assert residual.is_cuda and residual_out.is_cuda, "device tensors expected"
+        assert residual.shape == shape == residual_out.shape and residual_out.dtype is rdt
+        (ldr, one), (ldro, one2) = residual.stride(), residual_out.stride()
+        assert one == one2 == 1 or H <= 1
+        rp, rop, rt = residual.data_ptr(), residual_out.data_ptr(), _DTYPE_CODE.get(rdt, 0)
     elif residual_out is not None:
         raise ValueError("residual_out without residual")
-    y = out if out is not None else torch.empty((M, H), dtype=torch.uint8, device=x.device)
-    assert y.dtype == torch.uint8 and y.shape == x.shape and y.stride(1) == 1
+    y = out if out is not None else torch.empty((M, H), dtype=_U8, device=x.device)
+    ldy, one = y.stride()
+    assert y.is_cuda and y.dtype is _U8 and y.shape == shape and (one == 1 or H <= 1)
+    n = M if mode == SCALE_ROW else 1
     if scale is None:
         assert mode != SCALE_STATIC, "SCALE_STATIC takes a scale"
-        scale = torch.empty(M if mode == SCALE_ROW else 1, dtype=torch.float32, device=x.device)
-    assert scale.dtype == torch.float32 and scale.is_contiguous() and scale.numel() >= (M if mode == SCALE_ROW else 1)
-    if workspace is None and mode == SCALE_TENSOR and M > 1:
-        workspace = torch.empty(lib().lcml_fp8_rms_norm_workspace_bytes(M, H, mode), dtype=torch.uint8, device=x.device)
-    r = residual is not None
-    _check(lib().lcml_fp8_rms_norm(M, H, _ptr(x), _DTYPE_CODE.get(x.dtype, 0), x.stride(0), _ptr(residual),
-                                   _ptr(residual_out), _DTYPE_CODE.get(residual.dtype, 0) if r else 0,
-                                   residual.stride(0) if r else 0, residual_out.stride(0) if r else 0, _ptr(gamma),
-                                   float(eps), _ptr(y), y.stride(0), int(mode), _ptr(scale), _ptr(workspace),
-                                   workspace.numel() * workspace.element_size() if workspace is not None else 0,
-                                   _stream(stream)))
+        scale = torch.empty(n, dtype=_F32, device=x.device)
+    assert scale.is_cuda and scale.dtype is _F32 and scale.numel() >= n and scale.is_contiguous()
+    if mode == SCALE_TENSOR and M > 1 and workspace is None:
+        workspace = torch.empty(lib().lcml_fp8_rms_norm_workspace_bytes(M, H, mode), dtype=_U8, device=x.device)
+    _check(lib().lcml_fp8_rms_norm(M, H, x.data_ptr(), _DTYPE_CODE.get(x.dtype, 0), ldx, rp, rop, rt, ldr, ldro,
+                                   gamma.data_ptr(), eps, y.data_ptr(), ldy, mode, scale.data_ptr(), _ptr(workspace),
+                                   _bytes_of(workspace), _stream(stream)))
     return y, scale, residual_out
 
 
 def _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q):
-    assert k_cache.dtype == torch.uint8 and v_cache.dtype == torch.uint8 and k_cache.dim() == 4
-    assert k_cache.shape == v_cache.shape and k_cache.is_contiguous() and v_cache.is_contiguous()
-    assert k_scale.dtype == torch.float32 and v_scale.dtype == torch.float32
-    assert k_scale.shape == k_cache.shape[:2] == v_scale.shape and k_scale.is_contiguous() and v_scale.is_contiguous()
-    assert block_table.dtype == torch.int32 and kv_len.dtype == torch.int32 and cu_q.dtype == torch.int32
-    assert block_table.dim() == 2 and block_table.stride(1) == 1 and kv_len.is_contiguous() and cu_q.is_contiguous()
-    seqs = kv_len.numel()
-    assert block_table.shape[0] == seqs and cu_q.numel() == seqs + 1
-    pages, heads, page_tokens, dim = k_cache.shape
-    return ((_ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale)), (pages, heads, dim, page_tokens),
-            (_ptr(block_table), max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], _ptr(kv_len),
-             _ptr(cu_q), seqs))
+    """The checked cache arguments, in the C ABI's order; kv heads and head size."""
+    shape = k_cache.shape
+    pages, heads, page_tokens, dim = shape
+    assert (k_cache.is_cuda and v_cache.is_cuda and k_scale.is_cuda and v_scale.is_cuda and block_table.is_cuda
+            and kv_len.is_cuda and cu_q.is_cuda), "device tensors expected"
+    assert k_cache.dtype is _U8 and v_cache.dtype is _U8 and k_scale.dtype is _F32 and v_scale.dtype is _F32
+    assert block_table.dtype is _I32 and kv_len.dtype is _I32 and cu_q.dtype is _I32
+    assert v_cache.shape == shape and k_scale.shape == shape[:2] == v_scale.shape
+    assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()
+    seqs, cols = block_table.shape
+    pitch, one = block_table.stride()
+    assert kv_len.numel() == seqs and cu_q.numel() == seqs + 1 and kv_len.is_contiguous() and cu_q.is_contiguous()
+    assert one == 1 or cols <= 1
+    return (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, heads, dim,
+            page_tokens, block_table.data_ptr(), pitch if pitch > cols else cols, cols, kv_len.data_ptr(),
+            cu_q.data_ptr(), seqs)
 
 
-def _token_rows(x: torch.Tensor, heads: int, dim: int):
-    assert x.dim() == 3 and x.shape[1:] == (heads, dim) and (x.stride(2) == 1 or x.numel() == 0)
-    return x.stride(0), x.stride(1)
+def _two_rows(k, v, cache):
+    """Of K's and V's rows: dtype, tokens, strides."""
+    shape = k.shape
+    tokens, heads, dim = shape
+    assert k.is_cuda and v.is_cuda, "device tensors expected"
+    assert heads == cache[5] and dim == cache[6] and v.shape == shape and k.dtype is v.dtype
+    (kt, kh, one), (vt, vh, one2) = k.stride(), v.stride()
+    assert one == one2 == 1
+    return _DTYPE_CODE.get(k.dtype, 0), tokens, kt, kh, vt, vh
 
 
 def kv_cache(pages: int, kv_heads: int, page_tokens: int, head_dim: int, device):
     """An empty E4M3 KV cache: (k_cache, v_cache, k_scale, v_scale)."""
     shape = (pages, kv_heads, page_tokens, head_dim)
-    return (torch.zeros(shape, dtype=torch.uint8, device=device), torch.zeros(shape, dtype=torch.uint8, device=device),
+    return (torch.zeros(shape, dtype=_U8, device=device), torch.zeros(shape, dtype=_U8, device=device),
             torch.ones(shape[:2], device=device), torch.ones(shape[:2], device=device))
 
 
@@ -553,11 +581,8 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     """New tokens' k, v [tokens, kv_heads, head_dim] (fp32/bf16, any token and
     head strides) into the cache [pages, kv_heads, page_tokens, head_dim], as
     the last tokens of their sequences (kv_len counts them)."""
-    c, geo, idx = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q)
-    assert k.dtype == v.dtype and k.shape == v.shape
-    (kt, kh), (vt, vh) = _token_rows(k, geo[1], geo[2]), _token_rows(v, geo[1], geo[2])
-    _check(lib().lcml_fp8_kv_cache_write(_ptr(k), _ptr(v), _DTYPE_CODE.get(k.dtype, 0), k.shape[0], kt, kh, vt, vh, *c,
-                                         *geo, *idx, int(max_q), _stream(stream)))
+    c = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q)
+    _check(lib().lcml_fp8_kv_cache_write(k.data_ptr(), v.data_ptr(), *_two_rows(k, v, c), *c, max_q, _stream(stream)))
 
 
 def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -565,12 +590,14 @@ def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.T
                   v_out: torch.Tensor, stream=None) -> None:
     """The inverse of kv_cache_write: the same rows' tokens into k_out, v_out
     [tokens, kv_heads, head_dim] (fp32 or bf16)."""
-    c, geo, idx = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q)
-    assert k_out.dtype == v_out.dtype and k_out.shape == v_out.shape
-    (kt, kh), (vt, vh) = _token_rows(k_out, geo[1], geo[2]), _token_rows(v_out, geo[1], geo[2])
-    _check(lib().lcml_fp8_kv_cache_read(*c, *geo, *idx, int(max_q), _ptr(k_out), _ptr(v_out),
-                                        _DTYPE_CODE.get(k_out.dtype, 0), k_out.shape[0], kt, kh, vt, vh,
+    c = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q)
+    _check(lib().lcml_fp8_kv_cache_read(*c, max_q, k_out.data_ptr(), v_out.data_ptr(), *_two_rows(k_out, v_out, c),
                                         _stream(stream)))
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_workspace(tokens, seqs, q_heads, kv_heads, dim, max_q, max_kv):
+    return lib().lcml_fp8_attention_workspace_bytes(tokens, seqs, q_heads, kv_heads, dim, max_q, max_kv)
 
 
 def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -580,18 +607,18 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_s
     """softmax(scale * q k^T) v over the E4M3 cache: q [tokens, q_heads,
     head_dim] (fp32/bf16) are the last tokens of their sequences, which the
     cache already holds.  window > 0: only the last `window` positions."""
-    c, geo, idx = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q)
-    tokens, heads, dim = q.shape
-    o = out if out is not None else torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
-    assert o.shape == q.shape
-    qt, qh = _token_rows(q, heads, geo[2])
-    ot, oh = _token_rows(o, heads, geo[2])
-    need = lib().lcml_fp8_attention_workspace_bytes(tokens, idx[5], heads, geo[1], dim, int(max_q), int(max_kv))
-    if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _check(lib().lcml_fp8_attention(_ptr(q), _DTYPE_CODE.get(q.dtype, 0), tokens, heads, qt, qh, _ptr(o),
-                                    _DTYPE_CODE.get(o.dtype, 0), ot, oh, *c, *geo, *idx, int(max_q), int(max_kv),
-                                    float(scale), int(causal), int(window), _ptr(workspace),
-                                    workspace.numel() * workspace.element_size() if workspace is not None else 0,
-                                    _stream(stream)))
+    c = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q)
+    shape = q.shape
+    tokens, heads, dim = shape
+    o = out if out is not None else torch.empty(shape, dtype=out_dtype or q.dtype, device=q.device)
+    assert q.is_cuda and o.is_cuda, "device tensors expected"
+    (qt, qh, one), (ot, oh, one2) = q.stride(), o.stride()
+    assert dim == c[6] and o.shape == shape and one == one2 == 1
+    if workspace is None:
+        need = _attention_workspace(tokens, c[13], heads, c[5], dim, max_q, max_kv)
+        if need:
+            workspace = torch.empty(need, dtype=_U8, device=q.device)
+    _check(lib().lcml_fp8_attention(q.data_ptr(), _DTYPE_CODE.get(q.dtype, 0), tokens, heads, qt, qh, o.data_ptr(),
+                                    _DTYPE_CODE.get(o.dtype, 0), ot, oh, *c, max_q, max_kv, scale, causal, window,
+                                    _ptr(workspace), _bytes_of(workspace), _stream(stream)))
     return o
