@@ -81,13 +81,16 @@ __device__ inline float sum_over_quarters(float v) {
     return bits_f32(b[0]) + bits_f32(b[1]);
 }
 
-// The power of two that brings a row's largest finite element to [2^14, 2^15):
-// fp16 then holds a bf16 element exactly down to 2^-31 of that one, and an fp32
-// element in two pieces to 2^-22 of itself.
+// The power of two that brings a row's largest element to [2^14, 2^15): fp16
+// then holds a bf16 element exactly down to 2^-31 of that one, and an fp32
+// element in two pieces to 2^-22 of itself.  (Beside an infinity nothing else
+// matters to a score.)
 __device__ inline float query_factor(float amax) {
     const int e = 127 + 14 + 127 - (int)(f32_bits(amax) >> 23);
     return bits_f32((uint32_t)(e > 253 ? 253 : e) << 23);
 }
+
+__device__ inline float reciprocal(float f) { return bits_f32((254u << 23) - f32_bits(f)); }  // of a power of two
 
 // vs / vref times 2^kVBits, powers of two as their bits
 __device__ inline float v_ratio(uint32_t vs, uint32_t vref) {
@@ -127,6 +130,28 @@ __device__ inline void load_q8(const void *q, int64_t i, float *x) {
     }
 }
 
+// eight elements times f, as one piece or two; zeros where the row has none
+template <int NQ>
+__device__ inline void to_pieces(const float *x, float f, bool in, h8 *hi, h8 *lo) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        const f2 v{x[e] * f, x[e + 1] * f};
+        const h2 p = __builtin_convertvector(v, h2);
+        (*hi)[e] = p[0], (*hi)[e + 1] = p[1];
+        if constexpr (NQ == 2) {
+            const h2 q = __builtin_convertvector(f2{v[0] - (float)p[0], v[1] - (float)p[1]}, h2);
+            (*lo)[e] = q[0], (*lo)[e + 1] = q[1];
+        }
+    }
+    const h8 zero{0, 0, 0, 0, 0, 0, 0, 0};
+    *hi = in ? *hi : zero;
+    if constexpr (NQ == 2) *lo = in ? *lo : zero;
+}
+
+// 16 bytes that this call reads once: non-temporal (32 queries over up to 16384
+// tokens, 619 MB: 134 us without, 123 with)
+__device__ inline u4 load_once(const uint8_t *p) { return __builtin_nontemporal_load(reinterpret_cast<const u4 *>(p)); }
+
 struct __attribute__((packed, aligned(2))) O16 {
     uint16_t v[4];
 };
@@ -164,21 +189,38 @@ __device__ inline Block block_of(const AttentionArgs &a, int32_t head, int32_t t
 }
 __device__ inline uint32_t lane_of(uint32_t v, int i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, i); }
 
+// n / d for n < 2^31, d >= 1, by a multiplication: with 2^(k-1) < d <= 2^k and
+// m = ceil(2^(31+k) / d), n m / 2^(31+k) exceeds n / d by less than 1 / d.  The
+// divisions of a workgroup's start took a third of a short call.
+struct Divider {
+    uint32_t d, m, s;
+    static Divider of(int64_t d) {
+        uint32_t k = 0;
+        while (((int64_t)1 << k) < d) ++k;
+        return Divider{(uint32_t)d, d == 1 ? 0u : (uint32_t)((((unsigned __int128)1 << (31 + k)) + d - 1) / d), k ? k - 1 : 0};
+    }
+    __host__ __device__ uint32_t div(uint32_t n) const {
+        return d == 1 ? n : (uint32_t)(((uint64_t)n * m) >> 32) >> s;
+    }
+};
+
 // How a row's tokens are divided: `splits` parts of `chunk` tokens; with more
 // than one, part results (normalised) and the base-2 logarithms of their
 // weights go to the workspace, [token * q_heads + head][split].
 struct Split {
     int32_t splits, chunk, tiles;  // tiles: row tiles of one sequence and KV head
+    int32_t group;                 // q heads of a KV head
     float *o, *lse;
+    Divider by_splits, by_tiles, by_heads, by_group, by_per;  // by_per: of tiles * splits
 };
 
 // positions that query i of a sequence sees: lo .. hi-1, neither falling with i
 __device__ inline void sees(const AttentionArgs &a, const SeqRows &s, int32_t i, int32_t *lo, int32_t *hi) {
-    const int64_t pos = (int64_t)s.pos0 + i;
-    const int64_t h = a.causal && pos + 1 < s.len ? pos + 1 : s.len;
-    const int64_t l = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
-    *hi = h > 0 ? (int32_t)h : 0;
-    *lo = l < *hi ? (int32_t)l : *hi;
+    const int32_t pos = s.pos0 + i, w = (int32_t)a.window;  // below 2^31; 0: no window
+    const int32_t h = a.causal && pos < s.len ? pos + 1 : s.len;
+    const int32_t l = w > 0 && pos >= w ? pos - w + 1 : 0;
+    *hi = h > 0 ? h : 0;
+    *lo = l < *hi ? l : *hi;
 }
 
 // the part of positions lo .. hi-1 that is this workgroup's, from a multiple of
@@ -207,24 +249,21 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
     __shared__ __attribute__((aligned(16))) float buf[NW][16][kPitch];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int32_t D = a.t.dim, G = a.q_heads / a.t.heads;
-    uint32_t id = blockIdx.x;
-    const int32_t head = id % a.t.heads;
-    id /= a.t.heads;
-    const int32_t split = id % sp.splits;
-    id /= sp.splits;
-    const int32_t tile = id % sp.tiles, b = id / sp.tiles;
+    const int32_t D = a.t.dim, G = sp.group;
+    const uint32_t id0 = blockIdx.x, id1 = sp.by_heads.div(id0), id2 = sp.by_splits.div(id1);
+    const int32_t head = id0 - id1 * a.t.heads, split = id1 - id2 * sp.splits;
+    const int32_t b = sp.by_tiles.div(id2), tile = id2 - b * sp.tiles;
     const SeqRows s = seq_rows(a.t, b);
-    const int64_t rows = (int64_t)s.n * G;
+    const int32_t rows = (s.n < (int32_t)a.max_q ? s.n : (int32_t)a.max_q) * G;
     const int32_t row0 = tile * 16;
     if (row0 >= rows) return;
-    const int32_t last = rows - row0 < 16 ? (int32_t)rows - 1 : row0 + 15;  // of the tile
-    const int32_t row = row0 + r < last ? row0 + r : last;                  // this lane's
-    const int32_t qi = row / G, qh = head * G + row % G;
+    const int32_t last = rows - row0 < 16 ? rows - 1 : row0 + 15;  // of the tile
+    const int32_t row = row0 + r < last ? row0 + r : last;         // this lane's
+    const int32_t qi = sp.by_group.div(row), qh = head * G + row - qi * G;
     int32_t lo, hi, lo_min, hi_min, lo_max, hi_max;
     sees(a, s, qi, &lo, &hi);
-    sees(a, s, row0 / G, &lo_min, &hi_min);
-    sees(a, s, last / G, &lo_max, &hi_max);
+    sees(a, s, sp.by_group.div(row0), &lo_min, &hi_min);
+    sees(a, s, sp.by_group.div(last), &lo_max, &hi_max);
     const Part part = part_of(a, sp, split, lo_min, hi_max);
     const int64_t out_row = ((int64_t)s.row0 + qi) * a.q_heads + qh;
     if (part.steps == 0 && sp.splits > 1) {
@@ -250,7 +289,7 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
             const uint8_t *p = base(a.k, k, sb);
 #pragma unroll
             for (int j = 0; j < DC; ++j)
-                kk[sb][j] = (4 * j + g) * 16 < D ? *reinterpret_cast<const u4 *>(p + (4 * j + g) * 256 + r * 16) : zero;
+                kk[sb][j] = (4 * j + g) * 16 < D ? load_once(p + (4 * j + g) * 256 + r * 16) : zero;
         }
     };
     auto issue_v = [&](int32_t k) {
@@ -259,15 +298,9 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
             const uint8_t *p = base(a.v, k, sb) + g * 4 * D;
 #pragma unroll
             for (int j = 0; j < DC; ++j)
-                vv[sb][j] = 64 * j + 4 * r < D ? *reinterpret_cast<const u4 *>(p + (64 * j + 4 * r) * 4) : zero;
+                vv[sb][j] = 64 * j + 4 * r < D ? load_once(p + (64 * j + 4 * r) * 4) : zero;
         }
     };
-    if (mine > 0) {
-        find(0);
-        issue_k(0);
-        issue_v(0);
-    }
-
     // the row's query in the operand's order: pieces 4 j + g of 16 elements
     h8 qf[NQ][DC][2];
     float cq;
@@ -279,27 +312,26 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int d = 16 * (4 * j + g) + 8 * h;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[j][h][e] = 0.0f;
-                if (d < D) load_q8<NQ == 1>(a.q, at + d, x[j][h]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float v = fabsf(x[j][h][e]);
-                    amax = v > amax && v < kInf ? v : amax;
-                }
+                load_q8<NQ == 1>(a.q, at + (d < D ? d : 0), x[j][h]);
             }
-        const float f = query_factor(max_over_quarters(amax));
-        cq = a.scale * kLog2e * (1.0f / f);
+        if (mine > 0) {
+            find(0);
+            issue_k(0);
+            issue_v(0);
+        }
 #pragma unroll
         for (int j = 0; j < DC; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float v = x[j][h][e] * f;
-                    qf[0][j][h][e] = (_Float16)v;
-                    if constexpr (NQ == 2) qf[NQ - 1][j][h][e] = (_Float16)(v - (float)qf[0][j][h][e]);
-                }
+                for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[j][h][e]));
+        const float f = query_factor(max_over_quarters(amax));
+        cq = a.scale * kLog2e * reciprocal(f);
+#pragma unroll
+        for (int j = 0; j < DC; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                to_pieces<NQ>(x[j][h], f, 16 * (4 * j + g) < D, &qf[0][j][h], &qf[NQ - 1][j][h]);
     }
 
     f4 o[DC][4];  // columns 64 j + 16 g + 4 i + c in o[j][c][i]
@@ -316,21 +348,21 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
             for (int c = 0; c < 4; ++c) o[j][c] *= f;
     };
 
-    for (int32_t k = 0; k < mine; ++k) {
-        const int32_t tok = part.start + ((k * NW + wave) << 6);
-        uint32_t ks[4], vs[4];
-        uint64_t at[4];
+    auto put_o = [&] {  // row by row
 #pragma unroll
-        for (int sb = 0; sb < 4; ++sb) {
-            const int i = (k & 15) * 4 + sb;
-            ks[sb] = lane_of(blk.ks, i);
-            vs[sb] = lane_of(blk.vs, i);
-            at[sb] = (uint64_t)(base(a.v, k, sb) - a.v);
-        }
+        for (int j = 0; j < DC; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f4 *>(&buf[wave][r][64 * j + 16 * g + 4 * i]) = f4{o[j][0][i], o[j][1][i], o[j][2][i], o[j][3][i]};
+    };
+    // one step; MASKED: some rows do not see all of its tokens
+    uint32_t ks[4], vs[4];
+    auto step = [&](int32_t k, int32_t tok, auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
         f4 t[4];
 #pragma unroll
         for (int sb = 0; sb < 4; ++sb) {
-            f4 acc{0.f, 0.f, 0.f, 0.f};
+            t[sb] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < DC; ++j)
 #pragma unroll
@@ -338,43 +370,55 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
                     const h8 kh = widen8(kk[sb][j][2 * h], kk[sb][j][2 * h + 1], 1.0f);
 #pragma unroll
                     for (int q = 0; q < NQ; ++q)
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qf[q][j][h], acc, 0, 0, 0);
+                        t[sb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qf[q][j][h], t[sb], 0, 0, 0);
                 }
-            t[sb] = acc * (cq * bits_f32(ks[sb]));
         }
         if (k + 1 < mine) {
             if (((k + 1) & 15) == 0) find(k + 1);
             issue_k(k + 1);
         }
-        // tokens of this step that some rows do not see
-        const bool masked = !(tok >= lo_max && tok + 64 <= hi_min && vs[0] && vs[1] && vs[2] && vs[3]);
         bool nan = false;
-        if (masked) {
+        if constexpr (MASKED) {
             uint32_t bad = 0;
+            const uint32_t from = tok + 4 * g - lo;
 #pragma unroll
             for (int sb = 0; sb < 4; ++sb) {
-                uint32_t any = 0;  // bytes of a word of V: tokens that a row sees
+                const uint32_t span = vs[sb] ? hi - lo : 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int32_t j = tok + 16 * sb + 4 * g + i;
-                    t[sb][i] = j >= lo && j < hi && vs[sb] ? t[sb][i] : -kInf;
-                    any |= j >= lo_min && j < hi_max && vs[sb] ? 0x80u << (8 * i) : 0u;
-                }
+                for (int i = 0; i < 4; ++i) t[sb][i] = from + 16 * sb + i < span ? t[sb][i] : -kInf;
 #pragma unroll
                 for (int j = 0; j < DC; ++j)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        bad |= nan_bits(vv[sb][j][c]) & any;
-                        vv[sb][j][c] = without_nan(vv[sb][j][c]);
-                    }
+                    for (int c = 0; c < 4; ++c) bad |= nan_bits(vv[sb][j][c]);
             }
-            nan = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+            if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {  // NaN codes: of tokens that a row sees?
+                bad = 0;
+                const uint32_t all = tok + 4 * g - lo_min;
+#pragma unroll
+                for (int sb = 0; sb < 4; ++sb) {
+                    const uint32_t span = vs[sb] ? hi_max - lo_min : 0;
+                    uint32_t seen = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) seen |= all + 16 * sb + i < span ? 0x80u << (8 * i) : 0u;
+#pragma unroll
+                    for (int j = 0; j < DC; ++j)
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            bad |= nan_bits(vv[sb][j][y]) & seen;
+                            vv[sb][j][y] = without_nan(vv[sb][j][y]);
+                        }
+                }
+                nan = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+            }
         }
-        float mx = m;
+        float mx = m, c[4];
 #pragma unroll
-        for (int sb = 0; sb < 4; ++sb)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, t[sb][i]);
+        for (int sb = 0; sb < 4; ++sb) {
+            c[sb] = cq * bits_f32(ks[sb]);
+            const float b = fmaxf(fmaxf(t[sb][0], t[sb][1]), fmaxf(t[sb][2], t[sb][3]));
+            // a factor of 0 (scales below the range) must not make a NaN of a hidden token's -inf
+            mx = fmaxf(mx, MASKED && b == -kInf ? b : b * c[sb]);
+        }
         mx = max_over_quarters(mx);
         if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
             const float f = mx > m ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
@@ -396,8 +440,13 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
         for (int sb = 0; sb < 4; ++sb)
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-                const f2 e{weight_scale<NP>(__builtin_amdgcn_exp2f(t[sb][i] - mm)),
-                           weight_scale<NP>(__builtin_amdgcn_exp2f(t[sb][i + 1] - mm))};
+                f2 e;
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    float v = fmaf(t[sb][i + y], c[sb], -mm);
+                    if (MASKED) v = t[sb][i + y] == -kInf ? -kInf : v;
+                    e[y] = weight_scale<NP>(__builtin_amdgcn_exp2f(v));
+                }
                 l += e[0] + e[1];
                 const h2 eh = __builtin_convertvector(e, h2);
                 const int at0 = (sb & 1) * 4 + i;
@@ -415,33 +464,53 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
 #pragma unroll
             for (int j = 0; j < DC; ++j)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const h8 va = __builtin_shufflevector(widen4(vv[2 * h][j][c], ratio[2 * h]),
-                                                          widen4(vv[2 * h + 1][j][c], ratio[2 * h + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
+                for (int y = 0; y < 4; ++y) {
+                    const h8 va = __builtin_shufflevector(widen4(vv[2 * h][j][y], ratio[2 * h]),
+                                                          widen4(vv[2 * h + 1][j][y], ratio[2 * h + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
                     for (int q = 0; q < NP; ++q)
-                        o[j][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[q][h], o[j][c], 0, 0, 0);
+                        o[j][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[q][h], o[j][y], 0, 0, 0);
                 }
-        if (nan) {  // NaN codes of V reach the rows that see their token, and no others
+        if (nan) {  // NaN codes of V reach the rows that see their token, and no others: by way of LDS
+            put_o();
 #pragma unroll 1
-            for (int e = 0; e < 64; ++e) {
-                const int32_t j = tok + e;
-                const uint64_t blk_at = e < 16 ? at[0] : e < 32 ? at[1] : e < 48 ? at[2] : at[3];
-                const bool on = j >= lo && j < hi && (e < 16 ? vs[0] : e < 32 ? vs[1] : e < 48 ? vs[2] : vs[3]) != 0;
-                if (!on) continue;
-#pragma unroll
-                for (int jj = 0; jj < DC; ++jj)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int d = 64 * jj + 16 * g + 4 * i + c;
-                            const uint32_t w = d < D ? a.v[blk_at + v_place(e & 15, d, D)] : 0u;
-                            if ((w & 0x7fu) == 0x7fu) o[jj][c][i] = __builtin_nanf("");
-                        }
+            for (int32_t j = tok > lo_min ? tok : lo_min; j < tok + 64 && j < hi_max; ++j) {
+                const Block w = block_of(a, head, j, find_page(a, b, j, part.end));
+                if (!w.vs) continue;
+                const uint8_t *p = a.v + (w.lo | (uint64_t)w.hi << 32) * (uint64_t)(16 * D);
+#pragma unroll 1
+                for (int32_t d = lane; d < D; d += 64)
+                    if ((p[v_place(j & 15, d, D)] & 0x7f) == 0x7f)
+#pragma unroll 1
+                        for (int rr = 0; rr < 16; ++rr)
+                            if (j >= (int32_t)lane_of(lo, rr) && j < (int32_t)lane_of(hi, rr))
+                                buf[wave][rr][d] = __builtin_nanf("");
             }
+#pragma unroll
+            for (int j = 0; j < DC; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f4 v = *reinterpret_cast<const f4 *>(&buf[wave][r][64 * j + 16 * g + 4 * i]);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) o[j][y][i] = v[y];
+                }
         }
         if (k + 1 < mine) issue_v(k + 1);
+    };
+    // steps that all rows see whole, in a loop of their own
+    for (int32_t k = 0; k < mine; ++k) {
+        int32_t tok;
+        for (; k < mine; ++k) {
+            tok = part.start + ((k * NW + wave) << 6);
+#pragma unroll
+            for (int sb = 0; sb < 4; ++sb) {
+                ks[sb] = lane_of(blk.ks, (k & 15) * 4 + sb);
+                vs[sb] = lane_of(blk.vs, (k & 15) * 4 + sb);
+            }
+            if (!(tok >= lo_max && tok + 64 <= hi_min && vs[0] && vs[1] && vs[2] && vs[3])) break;
+            step(k, tok, std::false_type{});
+        }
+        if (k < mine) step(k, tok, std::true_type{});
     }
 
     // join the wavefronts
@@ -454,13 +523,8 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
     auto weight = [&](float v) { return v == top ? 1.0f : __builtin_amdgcn_exp2f(v - top); };
 #pragma unroll
     for (int w = 0; w < NW; ++w) sum += red_l[w][r] * weight(red_m[w][r]);
-    const float f = weight(m) / sum * (bits_f32(vref) * (1.0f / (1 << kVBits)));
-#pragma unroll
-    for (int j = 0; j < DC; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<f4 *>(&buf[wave][r][64 * j + 16 * g + 4 * i]) =
-                sum == 0.0f ? f4{0.f, 0.f, 0.f, 0.f} : f4{o[j][0][i], o[j][1][i], o[j][2][i], o[j][3][i]} * f;
+    scale_o(sum == 0.0f ? 0.0f : weight(m) / sum * (bits_f32(vref) * (1.0f / (1 << kVBits))));
+    put_o();
     if (sp.splits > 1 && wave == 0 && g == 0 && row0 + r <= last)
         sp.lse[out_row * sp.splits + split] = sum == 0.0f ? -kInf : top + __builtin_amdgcn_logf(sum);
     __syncthreads();
@@ -492,36 +556,37 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
     constexpr int CPL = DP >= 128 ? 4 : 2;   // columns of V that a lane reads at once
     constexpr int VR = MT / CPL;             // such reads for a group of four tokens
     constexpr int PL = DP / 64;              // 16-byte loads for a lane of a 16-token block
-    constexpr int kHalf = 64 * DP + 4 * DP;  // K's or V's bytes of a step, and room for reads past D
-    __shared__ __attribute__((aligned(16))) uint8_t stage[2][2][kHalf];
+    // K's and V's bytes of a step.  LDS holds DP columns: past D, zeros for K and
+    // anything for V, whose columns there are not stored.
+    __shared__ __attribute__((aligned(16))) uint8_t stage[2][2][64 * DP];
     __shared__ uint32_t has_nan[2][4];  // a block's V
     const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int32_t D = EXACT ? DP : a.t.dim, G = a.q_heads / a.t.heads;
+    const int32_t D = EXACT ? DP : a.t.dim, G = sp.group;
     // workgroups of one sequence and KV head on one XCD (blockIdx modulo 8),
     // whose L2 then holds their K and V; the longest rows first
     const uint32_t pairs = (uint32_t)a.t.seqs * a.t.heads, per = (uint32_t)sp.tiles * sp.splits;
     const bool by_xcd = pairs % 8 == 0;
-    const uint32_t pair = by_xcd ? blockIdx.x % 8 + 8 * (blockIdx.x / (8 * per)) : blockIdx.x / per;
-    const uint32_t rest = by_xcd ? blockIdx.x / 8 % per : blockIdx.x % per;
-    const int32_t head = pair % a.t.heads, b = pair / a.t.heads;
-    const int32_t split = rest % sp.splits, tile = sp.tiles - 1 - (int32_t)(rest / sp.splits);
+    const uint32_t id = by_xcd ? blockIdx.x / 8 : blockIdx.x, over = sp.by_per.div(id), rest = id - over * per;
+    const uint32_t pair = by_xcd ? blockIdx.x % 8 + 8 * over : over;
+    const int32_t b = sp.by_heads.div(pair), head = pair - b * a.t.heads;
+    const int32_t place = sp.by_splits.div(rest), split = rest - place * sp.splits, tile = sp.tiles - 1 - place;
     const SeqRows s = seq_rows(a.t, b);
-    const int64_t rows = (int64_t)s.n * G, row0 = (int64_t)tile * kManyRows;
+    const int32_t rows = (s.n < (int32_t)a.max_q ? s.n : (int32_t)a.max_q) * G, row0 = tile * kManyRows;
     if (row0 >= rows) return;
-    const int64_t last = rows - row0 < kManyRows ? rows - 1 : row0 + kManyRows - 1;
+    const int32_t last = rows - row0 < kManyRows ? rows - 1 : row0 + kManyRows - 1;
     // this wavefront's rows and this lane's
-    const int64_t w0 = row0 + 32 * wave < last ? row0 + 32 * wave : last, w1 = w0 + 31 < last ? w0 + 31 : last;
+    const int32_t w0 = row0 + 32 * wave < last ? row0 + 32 * wave : last, w1 = w0 + 31 < last ? w0 + 31 : last;
     const bool live = row0 + 32 * wave + r <= last;
-    const int64_t row = live ? row0 + 32 * wave + r : w1;
-    const int32_t qi = (int32_t)(row / G), qh = head * G + (int32_t)(row % G);
+    const int32_t row = live ? row0 + 32 * wave + r : w1;
+    const int32_t qi = sp.by_group.div(row), qh = head * G + row - qi * G;
     int32_t lo, hi, lo_min, hi_max, w_lo, w_hi, w_lo_max, w_hi_min, unused;
     sees(a, s, qi, &lo, &hi);
-    sees(a, s, (int32_t)(row0 / G), &lo_min, &unused);
-    sees(a, s, (int32_t)(last / G), &unused, &hi_max);
+    sees(a, s, sp.by_group.div(row0), &lo_min, &unused);
+    sees(a, s, sp.by_group.div(last), &unused, &hi_max);
     // tokens that any row of the wavefront sees, and that all do
-    sees(a, s, __builtin_amdgcn_readfirstlane((int32_t)(w0 / G)), &w_lo, &w_hi_min);
-    sees(a, s, __builtin_amdgcn_readfirstlane((int32_t)(w1 / G)), &w_lo_max, &w_hi);
+    sees(a, s, sp.by_group.div(w0), &w_lo, &w_hi_min);
+    sees(a, s, sp.by_group.div(w1), &w_lo_max, &w_hi);
     const Part part = part_of(a, sp, split, lo_min, hi_max);
     const int64_t out_row = ((int64_t)s.row0 + qi) * a.q_heads + qh;
     if (part.steps == 0 && sp.splits > 1) {
@@ -557,10 +622,9 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
                 const uint32_t keep = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1;
                 vr[x] &= u4{keep, keep, keep, keep};
             }
-            if (EXACT || 64 * x + lane < D) {
-                *reinterpret_cast<u4 *>(&stage[buf][0][wave * 16 * D + (64 * x + lane) * 16]) = kr[x];
-                *reinterpret_cast<u4 *>(&stage[buf][1][wave * 16 * D + (64 * x + lane) * 16]) = vr[x];
-            }
+            const int u = 64 * x + lane, v = EXACT ? u * 16 : u / (D >> 2) * 4 * DP + u % (D >> 2) * 16;
+            *reinterpret_cast<u4 *>(&stage[buf][0][wave * 16 * DP + u * 16]) = kr[x];  // zeros past D
+            if (EXACT || u < D) *reinterpret_cast<u4 *>(&stage[buf][1][wave * 16 * DP + v]) = vr[x];
 #pragma unroll
             for (int c = 0; c < 4; ++c) bad |= nan_bits(vr[x][c]);
         }
@@ -582,27 +646,21 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int d = 32 * j + 16 * h + 8 * u;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[j][u][e] = 0.0f;
-                if (EXACT || d < D) load_q8<NQ == 1>(a.q, at + d, x[j][u]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float v = fabsf(x[j][u][e]);
-                    amax = v > amax && v < kInf ? v : amax;
-                }
+                load_q8<NQ == 1>(a.q, at + (EXACT || d < D ? d : 0), x[j][u]);
             }
-        const float f = query_factor(max_over_halves(amax));
-        cq = a.scale * kLog2e * (1.0f / f);
 #pragma unroll
         for (int j = 0; j < KJ; ++j)
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float v = x[j][u][e] * f;
-                    qf[0][j][u][e] = (_Float16)v;
-                    if constexpr (NQ == 2) qf[NQ - 1][j][u][e] = (_Float16)(v - (float)qf[0][j][u][e]);
-                }
+                for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[j][u][e]));
+        const float f = query_factor(max_over_halves(amax));
+        cq = a.scale * kLog2e * reciprocal(f);
+#pragma unroll
+        for (int j = 0; j < KJ; ++j)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                to_pieces<NQ>(x[j][u], f, EXACT || 32 * j + 16 * h < D, &qf[0][j][u], &qf[NQ - 1][j][u]);
     }
 
     f16v o[MT];  // columns 128 x + CPL (8 a + 4 h + b) + c in o[x * CPL + c][4 a + b]
@@ -627,12 +685,10 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
         for (int q = 0; q < 2; ++q) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) t[q][i] = 0.0f;
-            const uint8_t *p = sk + (2 * q + (r >> 4)) * 16 * D + h * 256 + (r & 15) * 16;
+            const uint8_t *p = sk + (2 * q + (r >> 4)) * 16 * DP + h * 256 + (r & 15) * 16;
 #pragma unroll
             for (int j = 0; j < KJ; ++j) {
-                if (!EXACT && 32 * j >= D) break;
-                u4 w = *reinterpret_cast<const u4 *>(p + j * 512);
-                if (!EXACT && 32 * j + 16 * h >= D) w = u4{0, 0, 0, 0};
+                const u4 w = *reinterpret_cast<const u4 *>(p + j * 512);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const h8 kh = widen8(w[2 * u], w[2 * u + 1], 1.0f);
@@ -646,13 +702,16 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
 #pragma unroll
         for (int q = 0; q < 4; ++q) c[q] = cq * bits_f32(ks[q]);
         if constexpr (MASKED) {
+            const uint32_t from = tok + 4 * h - lo;
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t span = vs[q] ? hi - lo : 0;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int32_t j = tok + 32 * q + 8 * (i >> 2) + 4 * h + (i & 3);
-                    t[q][i] = j >= lo && j < hi && vs[2 * q + (i >> 3)] ? t[q][i] : -kInf;
+                for (int i = 0; i < 8; ++i) {
+                    const int at = (q & 1) * 8 + i;
+                    t[q >> 1][at] = from + 16 * q + 8 * (i >> 2) + (i & 3) < span ? t[q >> 1][at] : -kInf;
                 }
+            }
         }
         float mx = m;
 #pragma unroll
@@ -705,14 +764,14 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
             const float ratio = v_ratio(vs[q], vref);
 #pragma unroll
             for (int x = 0; x < VR; ++x) {
-                const uint8_t *pv = sv + q * 16 * D + h * 4 * D + (128 * x + CPL * r) * 4;
+                const uint8_t *pv = sv + q * 16 * DP + h * 4 * DP + (128 * x + CPL * r) * 4;
                 uint32_t v0[CPL], v1[CPL];  // groups h and h + 2 of four tokens
                 if constexpr (CPL == 4) {
-                    const u4 u0 = *reinterpret_cast<const u4 *>(pv), u1 = *reinterpret_cast<const u4 *>(pv + 8 * D);
+                    const u4 u0 = *reinterpret_cast<const u4 *>(pv), u1 = *reinterpret_cast<const u4 *>(pv + 8 * DP);
 #pragma unroll
                     for (int y = 0; y < CPL; ++y) v0[y] = u0[y], v1[y] = u1[y];
                 } else {
-                    const u2 u0 = *reinterpret_cast<const u2 *>(pv), u1 = *reinterpret_cast<const u2 *>(pv + 8 * D);
+                    const u2 u0 = *reinterpret_cast<const u2 *>(pv), u1 = *reinterpret_cast<const u2 *>(pv + 8 * DP);
 #pragma unroll
                     for (int y = 0; y < CPL; ++y) v0[y] = u0[y], v1[y] = u1[y];
                 }
@@ -736,8 +795,7 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int d = 128 * (y / CPL) + CPL * (8 * (i >> 2) + 4 * h + (i & 3)) + y % CPL;
-                        const uint32_t w = EXACT || d < D ? sv[v_place(e, d, D)] : 0u;
-                        if ((w & 0x7fu) == 0x7fu) o[y][i] = __builtin_nanf("");
+                        if ((sv[v_place(e, d, DP)] & 0x7f) == 0x7f) o[y][i] = __builtin_nanf("");
                     }
             }
         }
@@ -805,31 +863,54 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
             }
 }
 
-// Joins a row's parts: one wavefront a row.
+// Joins a row's parts, a workgroup a row: the weights first, then the parts by
+// as many groups of D / 4 threads as there are, four loads each under way.
+constexpr int kMostSplits = 128;
+
 template <bool BF16>
 __global__ __launch_bounds__(256) void k_attention_join(AttentionArgs a, Split sp) {
-    const int32_t D = a.t.dim, lane = threadIdx.x & 63;
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), per = a.max_q * a.q_heads;
-    const int64_t b = id / per, i = id % per / a.q_heads, h = id % a.q_heads;
-    if (b >= a.t.seqs) return;
-    const SeqRows s = seq_rows(a.t, (int32_t)b);
+    __shared__ float weight[kMostSplits];
+    __shared__ f4 buf[256];
+    const int32_t D = a.t.dim, q4 = D >> 2, lane = threadIdx.x & 63;
+    const int64_t per = a.max_q * a.q_heads;
+    const int32_t b = (int32_t)(blockIdx.x / per), i = (int32_t)(blockIdx.x % per / a.q_heads), h = (int32_t)(blockIdx.x % a.q_heads);
+    const SeqRows s = seq_rows(a.t, b);
     if (i >= s.n) return;
-    const int64_t row = (s.row0 + i) * a.q_heads + h;
+    const int64_t row = ((int64_t)s.row0 + i) * a.q_heads + h;
     const float *lse = sp.lse + row * sp.splits, *po = sp.o + row * sp.splits * D;
-    float top = -kInf;
-    for (int32_t k = 0; k < sp.splits; ++k) top = fmaxf(top, lse[k]);
-    float sum = 0.0f;
+    const float x0 = lane < sp.splits ? lse[lane] : -kInf, x1 = lane + 64 < sp.splits ? lse[lane + 64] : -kInf;
+    float top = fmaxf(x0, x1);
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
+    // a part of weight 0 wrote nothing
+    const float w0 = x0 == -kInf ? 0.0f : x0 == top ? 1.0f : __builtin_amdgcn_exp2f(x0 - top);
+    const float w1 = x1 == -kInf ? 0.0f : x1 == top ? 1.0f : __builtin_amdgcn_exp2f(x1 - top);
+    float sum = w0 + w1;
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m);
+    if (threadIdx.x < 64) weight[lane] = x0 == -kInf ? -1.0f : w0, weight[lane + 64] = x1 == -kInf ? -1.0f : w1;
+    __syncthreads();
+    const int32_t groups = 256 / q4, grp = threadIdx.x / q4, d = threadIdx.x % q4 * 4;
     f4 v{0.f, 0.f, 0.f, 0.f};
-    for (int32_t k = 0; k < sp.splits; ++k) {
-        const float x = lse[k];
-        if (x == -kInf) continue;
-        const float w = x == top ? 1.0f : __builtin_amdgcn_exp2f(x - top);
-        sum += w;
-        if (lane * 4 < D) v += *reinterpret_cast<const f4 *>(po + (int64_t)k * D + lane * 4) * w;
-    }
-    if (lane * 4 < D)
-        store_o4<BF16>(a.o, (s.row0 + i) * a.o_token + h * a.o_head + lane * 4,
-                       sum == 0.0f ? f4{0.f, 0.f, 0.f, 0.f} : v * (1.0f / sum));
+    if (grp < groups)
+        for (int32_t k0 = grp; k0 < sp.splits; k0 += 4 * groups) {
+            f4 p[4];
+            float w[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int32_t k = k0 + u * groups;
+                w[u] = k < sp.splits ? weight[k] : -1.0f;
+                p[u] = w[u] >= 0.0f || w[u] != w[u] ? *reinterpret_cast<const f4 *>(po + (int64_t)k * D + d) : f4{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v += p[u] * (w[u] == -1.0f ? 0.0f : w[u]);
+        }
+    buf[threadIdx.x] = v;
+    __syncthreads();
+    if (grp > 0) return;
+    for (int32_t g = 1; g < groups; ++g) v += buf[g * q4 + threadIdx.x];
+    store_o4<BF16>(a.o, ((int64_t)s.row0 + i) * a.o_token + (int64_t)h * a.o_head + d,
+                   sum == 0.0f ? f4{0.f, 0.f, 0.f, 0.f} : v * (1.0f / sum));
 }
 
 // ------------------------------------------------------------------- plan --
@@ -851,10 +932,26 @@ Plan make_plan(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t max_q, i
     int64_t span = max_kv;
     if (window > 0 && window < span && window + max_q + 64 < span) span = window + max_q + 64;
     const int64_t groups = seqs * kv_heads * p.sp.tiles, steps = (span + 63) / 64;
-    int64_t splits = ((p.few ? 1024 : 512) + groups - 1) / groups;
-    const int64_t most = (steps + 3) / 4;  // a step for each wavefront, or four for the workgroup
-    if (splits > most) splits = most;
-    if (splits > 128) splits = 128;
+    // Few rows: 512 workgroups of a step for each wavefront at least, and up to
+    // 2048 of four steps, so that ragged lengths even out.  Many rows: parts
+    // of 32 steps up to two workgroups a CU, of eight up to one, as joining them
+    // reads and writes every result again in fp32.
+    int64_t splits;
+    if (p.few) {
+        const int64_t fine = (steps + 4 * kFewWaves - 1) / (4 * kFewWaves), coarse = (steps + kFewWaves - 1) / kFewWaves;
+        splits = (2048 + groups - 1) / groups;
+        splits = splits < fine ? splits : fine;
+        const int64_t least = (512 + groups - 1) / groups;
+        splits = splits > least ? splits : least < coarse ? least : coarse;
+        // joining costs a launch: not for two steps of a wavefront, nor four on a full GPU
+        if (steps <= 2 * kFewWaves || (groups >= 256 && steps <= 4 * kFewWaves)) splits = 1;
+    } else {
+        const int64_t two = 512 / groups, one = 256 / groups, coarse = steps / 32, fine = steps / 8;
+        splits = two < coarse ? two : coarse;
+        const int64_t least = one < fine ? one : fine;
+        splits = splits > least ? splits : least;
+    }
+    if (splits > kMostSplits) splits = kMostSplits;
     if (splits < 1) splits = 1;
     p.sp.chunk = (int32_t)(((steps + splits - 1) / splits) * 64);
     p.sp.splits = (int32_t)splits;
@@ -889,7 +986,7 @@ hipError_t launch_t(const AttentionArgs &a, const Plan &p, hipStream_t s) {
                        : start_many<256, NQ, NP>(a, p.sp, grid, s);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess || p.sp.splits == 1) return err;
-    const unsigned rows = (unsigned)(((int64_t)a.t.seqs * a.max_q * a.q_heads + 3) / 4);
+    const unsigned rows = (unsigned)((int64_t)a.t.seqs * a.max_q * a.q_heads);
     hipLaunchKernelGGL((k_attention_join<NP == 1>), dim3(rows), dim3(256), 0, s, a, p.sp);
     return hipGetLastError();
 }
@@ -909,6 +1006,10 @@ int64_t attention_groups(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_
 
 hipError_t launch_attention(const AttentionArgs &a, void *work, hipStream_t s, const char **kernel) {
     Plan p = make_plan(a.t.seqs, a.q_heads, a.t.heads, a.max_q, a.max_kv, a.window);
+    p.sp.group = a.q_heads / a.t.heads;
+    p.sp.by_splits = Divider::of(p.sp.splits), p.sp.by_tiles = Divider::of(p.sp.tiles);
+    p.sp.by_heads = Divider::of(a.t.heads), p.sp.by_group = Divider::of(p.sp.group);
+    p.sp.by_per = Divider::of((int64_t)p.sp.tiles * p.sp.splits);
     p.sp.o = static_cast<float *>(work);
     p.sp.lse = p.sp.o + (int64_t)a.t.tokens * a.q_heads * p.sp.splits * a.t.dim;
     const bool join = p.sp.splits > 1;

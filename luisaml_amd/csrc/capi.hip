@@ -973,7 +973,7 @@ int lcml_fp8_attention(const void *q, int q_dtype, int64_t tokens, int64_t q_hea
     // pass 64 bits are past that by far
     const int64_t most = (int64_t)1 << 24;
     if (max_q * q_heads / kv_heads > most * 16 || seqs * kv_heads > most ||
-        lcml::attention_groups(seqs, q_heads, kv_heads, max_q, max_kv) >= most || seqs * max_q >= most * 4 / q_heads)
+        lcml::attention_groups(seqs, q_heads, kv_heads, max_q, max_kv) >= most || seqs * max_q >= most / q_heads)
         return fail(LCML_ERR_UNSUPPORTED, "%s: seqs=%lld max_q=%lld q_heads=%lld exceeds one launch", fn,
                     (long long)seqs, (long long)max_q, (long long)q_heads);
     const int64_t need = lcml::attention_workspace(tokens, seqs, q_heads, kv_heads, head_dim, max_q, max_kv);
@@ -981,7 +981,7 @@ int lcml_fp8_attention(const void *q, int q_dtype, int64_t tokens, int64_t q_hea
         return fail(LCML_ERR_INVALID_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", fn, (long long)need);
     a.q = q, a.o = o, a.k = k_cache, a.v = v_cache, a.ks = k_scale, a.vs = v_scale;
     a.q_token = q_token_stride, a.q_head = q_head_stride, a.o_token = o_token_stride, a.o_head = o_head_stride;
-    a.max_q = max_q, a.max_kv = max_kv, a.window = window;
+    a.max_q = max_q, a.max_kv = max_kv, a.window = window < (int64_t)1 << 31 ? window : 0;  // a longer one hides nothing
     a.q_heads = (int32_t)q_heads, a.causal = causal != 0;
     a.q_bf16 = q_dtype == LCML_DTYPE_BFLOAT16, a.o_bf16 = o_dtype == LCML_DTYPE_BFLOAT16;
     a.scale = scale;
