@@ -10,9 +10,9 @@
 // fp16 matrix instructions with fp32 sums:
 //   * a query row is brought to [2^14, 2^15) by a power of two; a bf16 row is
 //     then one fp16 operand, an fp32 row two (its rounding and the rest);
-//   * weights are 2^14 exp2(t - m): 11 bits down to 2^-28 of the largest (a
-//     bf16 weight would hold 8).  One piece where the result is bf16, whose
-//     own rounding is eight times as coarse, two where it is fp32;
+//   * weights are fp16 too: 11 bits, where bf16 would hold 8.  One piece where
+//     the result is bf16, whose own rounding is eight times as coarse, two
+//     where it is fp32;
 //   * K's page scale multiplies the scores, V's the codes as they are widened:
 //     a power of two below the largest V scale so far (the widening
 //     instruction takes the factor), which multiplies the end result; where
@@ -39,8 +39,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kPBits = 14;  // weights are held times 2^14
-constexpr int kVBits = 7;   // and V's codes times 2^7
+constexpr int kVBits = 7;  // V's codes are held times 2^7
 
 // ---------------------------------------------------------- operand pieces --
 
@@ -98,16 +97,30 @@ __device__ inline float v_ratio(uint32_t vs, uint32_t vref) {
     return bits_f32((uint32_t)(e < 1 ? 1 : e) << 23);
 }
 
-// 2^kPBits 2^(t - m).  Two pieces take the factor after the exponential: in
-// its argument, the rounding of a sum near 14 would cost three bits.
+// A weight is 2^(t - m) times a power of two that keeps it in fp16's range.
+// One piece: times 2^6 in the exponential's argument, and m may stay up to 8
+// below the maximum (sums are scaled by a rising maximum in one step of two
+// otherwise, and that is a fifth of the vector work); 11 bits down to 2^-20 of
+// the largest weight, an error of 2^-31 of it below.  Two pieces: times 2^14
+// after the exponential (in its argument, the rounding of a sum near 14 would
+// cost three bits), and m is the maximum.
+template <int NP>
+__device__ constexpr float weight_slack() {
+    return NP == 1 ? 8.0f : 0.0f;
+}
 template <int NP>
 __device__ inline float weight_base(float m) {
     m = m == -kInf ? 0.0f : m;
-    return NP == 1 ? m - (float)kPBits : m;
+    return NP == 1 ? m - 6.0f : m;
 }
 template <int NP>
 __device__ inline float weight_scale(float e) {
-    return NP == 1 ? e : e * (float)(1 << kPBits);
+    return NP == 1 ? e : e * 0x1p14f;
+}
+// l plus a pair of weights: as rounded where one piece is all there is
+template <int NP>
+__device__ inline float add_weights(float l, f2 e, h2 eh) {
+    return NP == 1 ? __builtin_amdgcn_fdot2(eh, h2{(_Float16)1.0f, (_Float16)1.0f}, l, false) : l + (e[0] + e[1]);
 }
 
 // eight elements of a query at any element-aligned address, as fp32
@@ -348,14 +361,9 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
             for (int c = 0; c < 4; ++c) o[j][c] *= f;
     };
 
-    auto put_o = [&] {  // row by row
-#pragma unroll
-        for (int j = 0; j < DC; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<f4 *>(&buf[wave][r][64 * j + 16 * g + 4 * i]) = f4{o[j][0][i], o[j][1][i], o[j][2][i], o[j][3][i]};
-    };
-    // one step; MASKED: some rows do not see all of its tokens
+    // one step; MASKED: some rows do not see all of its tokens, and V's NaN codes
+    // count as zeros for now
+    bool nan = false;
     uint32_t ks[4], vs[4];
     auto step = [&](int32_t k, int32_t tok, auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
@@ -377,7 +385,6 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
             if (((k + 1) & 15) == 0) find(k + 1);
             issue_k(k + 1);
         }
-        bool nan = false;
         if constexpr (MASKED) {
             uint32_t bad = 0;
             const uint32_t from = tok + 4 * g - lo;
@@ -408,7 +415,7 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
                             vv[sb][j][y] = without_nan(vv[sb][j][y]);
                         }
                 }
-                nan = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+                nan = nan || __builtin_amdgcn_ballot_w64(bad != 0) != 0;
             }
         }
         float mx = m, c[4];
@@ -420,11 +427,11 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
             mx = fmaxf(mx, MASKED && b == -kInf ? b : b * c[sb]);
         }
         mx = max_over_quarters(mx);
-        if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
+        if (__builtin_amdgcn_ballot_w64(mx > m + weight_slack<NP>()) != 0) {
             const float f = mx > m ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
             l *= f;
             scale_o(f);
-            m = mx;
+            m = mx > m ? mx : m;
         }
         uint32_t top = vs[0] > vs[1] ? vs[0] : vs[1];
         top = vs[2] > top ? vs[2] : top;
@@ -447,8 +454,8 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
                     if (MASKED) v = t[sb][i + y] == -kInf ? -kInf : v;
                     e[y] = weight_scale<NP>(__builtin_amdgcn_exp2f(v));
                 }
-                l += e[0] + e[1];
                 const h2 eh = __builtin_convertvector(e, h2);
+                l = add_weights<NP>(l, e, eh);
                 const int at0 = (sb & 1) * 4 + i;
                 p[0][sb >> 1][at0] = eh[0], p[0][sb >> 1][at0 + 1] = eh[1];
                 if constexpr (NP == 2) {
@@ -471,30 +478,6 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
                     for (int q = 0; q < NP; ++q)
                         o[j][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[q][h], o[j][y], 0, 0, 0);
                 }
-        if (nan) {  // NaN codes of V reach the rows that see their token, and no others: by way of LDS
-            put_o();
-#pragma unroll 1
-            for (int32_t j = tok > lo_min ? tok : lo_min; j < tok + 64 && j < hi_max; ++j) {
-                const Block w = block_of(a, head, j, find_page(a, b, j, part.end));
-                if (!w.vs) continue;
-                const uint8_t *p = a.v + (w.lo | (uint64_t)w.hi << 32) * (uint64_t)(16 * D);
-#pragma unroll 1
-                for (int32_t d = lane; d < D; d += 64)
-                    if ((p[v_place(j & 15, d, D)] & 0x7f) == 0x7f)
-#pragma unroll 1
-                        for (int rr = 0; rr < 16; ++rr)
-                            if (j >= (int32_t)lane_of(lo, rr) && j < (int32_t)lane_of(hi, rr))
-                                buf[wave][rr][d] = __builtin_nanf("");
-            }
-#pragma unroll
-            for (int j = 0; j < DC; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const f4 v = *reinterpret_cast<const f4 *>(&buf[wave][r][64 * j + 16 * g + 4 * i]);
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) o[j][y][i] = v[y];
-                }
-        }
         if (k + 1 < mine) issue_v(k + 1);
     };
     // steps that all rows see whole, in a loop of their own
@@ -524,7 +507,24 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
 #pragma unroll
     for (int w = 0; w < NW; ++w) sum += red_l[w][r] * weight(red_m[w][r]);
     scale_o(sum == 0.0f ? 0.0f : weight(m) / sum * (bits_f32(vref) * (1.0f / (1 << kVBits))));
-    put_o();
+#pragma unroll
+    for (int j = 0; j < DC; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<f4 *>(&buf[wave][r][64 * j + 16 * g + 4 * i]) = f4{o[j][0][i], o[j][1][i], o[j][2][i], o[j][3][i]};
+    if (__builtin_expect(nan, 0))  // V's NaN codes reach the rows that see their token, and no others
+        for (int32_t k = 0; k < mine; ++k) {
+            const int32_t tok = part.start + ((k * NW + wave) << 6);
+            for (int32_t j = tok > lo_min ? tok : lo_min; j < tok + 64 && j < part.end; ++j) {
+                const Block w = block_of(a, head, j, find_page(a, b, j, part.end));
+                if (!w.vs) continue;
+                const uint8_t *p = a.v + (w.lo | (uint64_t)w.hi << 32) * (uint64_t)(16 * D);
+                for (int32_t d = lane; d < D; d += 64)
+                    if ((p[v_place(j & 15, d, D)] & 0x7f) == 0x7f)
+                        for (int rr = 0; rr < 16; ++rr)
+                            if (j >= (int32_t)lane_of(lo, rr) && j < (int32_t)lane_of(hi, rr)) buf[wave][rr][d] = __builtin_nanf("");
+            }
+        }
     if (sp.splits > 1 && wave == 0 && g == 0 && row0 + r <= last)
         sp.lse[out_row * sp.splits + split] = sum == 0.0f ? -kInf : top + __builtin_amdgcn_logf(sum);
     __syncthreads();
@@ -544,22 +544,27 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
 // ---------------------------------------------------------------- many rows --
 //
 // One workgroup: 128 rows (queries x heads of the group) of one sequence and
-// KV head, 32 for each wavefront, over one part of the tokens.  K and V go
-// through LDS as codes, 64 tokens a step and two steps in turn, and are widened
-// in registers.  32x32x16 instructions.
+// KV head, 32 for each wavefront, over one part of the tokens, 64 a step.
+// Each wavefront brings 16 of a step's tokens into LDS, K as codes and V
+// widened: bound by the vector ALU and the matrix cores in turn, the kernel
+// shares the widening of V (64 conversions a wavefront and step would be
+// repeated by each of the four), and reads K's codes in half the bytes, as LDS
+// could not feed two fp16 operands.  32x32x16 instructions.
 constexpr int kManyWaves = 4, kManyRows = 32 * kManyWaves;
 
 template <int DP, bool EXACT, int NQ, int NP>
 __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attention_many(AttentionArgs a, Split sp) {
-    constexpr int KJ = DP / 32;              // pairs of 16-element pieces of K
-    constexpr int MT = DP / 32;              // tiles of 32 columns of V
-    constexpr int CPL = DP >= 128 ? 4 : 2;   // columns of V that a lane reads at once
-    constexpr int VR = MT / CPL;             // such reads for a group of four tokens
-    constexpr int PL = DP / 64;              // 16-byte loads for a lane of a 16-token block
-    // K's and V's bytes of a step.  LDS holds DP columns: past D, zeros for K and
-    // anything for V, whose columns there are not stored.
-    __shared__ __attribute__((aligned(16))) uint8_t stage[2][2][64 * DP];
-    __shared__ uint32_t has_nan[2][4];  // a block's V
+    constexpr int KJ = DP / 32;  // pairs of 16-element pieces of K
+    constexpr int MT = DP / 32;  // tiles of 32 columns of V
+    constexpr int PL = DP / 64;  // 16-byte loads for a lane of a 16-token block
+    // LDS holds DP columns: past D, zeros for K and anything for V, whose
+    // columns there are not stored.  K: [4 blocks][DP / 16][16 tokens][16].  V:
+    // [4 blocks][2][DP][8 tokens], in the halves the groups 0 and 2, 1 and 3 of
+    // four tokens, and column 4 u + e in place e * DP / 4 + u: what the lanes
+    // write and what they read is contiguous.
+    __shared__ __attribute__((aligned(16))) uint8_t stage_k[2][64 * DP];
+    __shared__ __attribute__((aligned(16))) _Float16 stage_v[2][64 * DP];
+    __shared__ uint32_t has_nan;  // V, in steps that some row does not see whole
     const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int32_t D = EXACT ? DP : a.t.dim, G = sp.group;
@@ -580,13 +585,14 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
     const bool live = row0 + 32 * wave + r <= last;
     const int32_t row = live ? row0 + 32 * wave + r : w1;
     const int32_t qi = sp.by_group.div(row), qh = head * G + row - qi * G;
-    int32_t lo, hi, lo_min, hi_max, w_lo, w_hi, w_lo_max, w_hi_min, unused;
+    // tokens that this lane's row sees, that any row sees and that all do, of
+    // the workgroup and (any) of the wavefront
+    int32_t lo, hi, lo_min, hi_min, lo_max, hi_max, w_lo, w_hi, unused;
     sees(a, s, qi, &lo, &hi);
-    sees(a, s, sp.by_group.div(row0), &lo_min, &unused);
-    sees(a, s, sp.by_group.div(last), &unused, &hi_max);
-    // tokens that any row of the wavefront sees, and that all do
-    sees(a, s, sp.by_group.div(w0), &w_lo, &w_hi_min);
-    sees(a, s, sp.by_group.div(w1), &w_lo_max, &w_hi);
+    sees(a, s, sp.by_group.div(row0), &lo_min, &hi_min);
+    sees(a, s, sp.by_group.div(last), &lo_max, &hi_max);
+    sees(a, s, sp.by_group.div(w0), &w_lo, &unused);
+    sees(a, s, sp.by_group.div(w1), &unused, &w_hi);
     const Part part = part_of(a, sp, split, lo_min, hi_max);
     const int64_t out_row = ((int64_t)s.row0 + qi) * a.q_heads + qh;
     if (part.steps == 0 && sp.splits > 1) {
@@ -599,11 +605,20 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
     Block blk, next;
     int32_t next_page = -1;
     auto token_of = [&](int32_t k) { return part.start + ((k + (lane >> 2)) << 6) + (lane & 3) * 16; };
-    // a step's 64 tokens: this wavefront brings block `wave` of them
+    uint32_t ks[4], vs[4], ks_next[4], vs_next[4];
+    bool whole, whole_next = false;  // whether every row sees all of a step's tokens
+    // this wavefront's block of step k
     u4 kr[PL], vr[PL];
     auto fetch = [&](int32_t k) {
-        const int i = (k & 15) * 4 + wave;
-        const uint64_t at = (lane_of(blk.lo, i) | (uint64_t)lane_of(blk.hi, i) << 32) * (uint64_t)(16 * D);
+        const int i = (k & 15) * 4;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ks_next[q] = lane_of(blk.ks, i + q), vs_next[q] = lane_of(blk.vs, i + q);
+        const int32_t tok = part.start + (k << 6);
+        uint32_t least = vs_next[0] < vs_next[1] ? vs_next[0] : vs_next[1];
+        least = vs_next[2] < least ? vs_next[2] : least;
+        least = vs_next[3] < least ? vs_next[3] : least;
+        whole_next = tok >= lo_max && tok + 64 <= hi_min && least;
+        const uint64_t at = (lane_of(blk.lo, i + wave) | (uint64_t)lane_of(blk.hi, i + wave) << 32) * (uint64_t)(16 * D);
         const uint8_t *pk = a.k + at, *pv = a.v + at;
 #pragma unroll
         for (int x = 0; x < PL; ++x) {
@@ -612,24 +627,40 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
             vr[x] = in ? *reinterpret_cast<const u4 *>(pv + (64 * x + lane) * 16) : u4{0, 0, 0, 0};
         }
     };
+    uint32_t vref = 0, vref_next = 0;  // the largest V scale up to a step, the same for all wavefronts
     auto deposit = [&](int32_t k, int buf) {
-        const int32_t left = part.end - (part.start + (k << 6) + 16 * wave);  // tokens of the block that exist
-        uint32_t bad = 0;
 #pragma unroll
-        for (int x = 0; x < PL; ++x) {
-            if (left < 16) {  // what lies past the last token counts as zeros
+        for (int q = 0; q < 4; ++q) vref_next = vs_next[q] > vref_next ? vs_next[q] : vref_next;
+        const uint32_t mine = wave == 0 ? vs_next[0] : wave == 1 ? vs_next[1] : wave == 2 ? vs_next[2] : vs_next[3];
+        const float ratio = v_ratio(mine, vref_next);
+        if (__builtin_expect(!whole_next, 0)) {
+            // what lies past the last token counts as zeros, and so do NaN codes
+            // for now
+            const int32_t left = part.end - (part.start + (k << 6) + 16 * wave);
+            uint32_t bad = 0;
+#pragma unroll
+            for (int x = 0; x < PL; ++x) {
                 const int32_t n = left - (64 * x + lane) / (D >> 2) * 4;
                 const uint32_t keep = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1;
                 vr[x] &= u4{keep, keep, keep, keep};
-            }
-            const int u = 64 * x + lane, v = EXACT ? u * 16 : u / (D >> 2) * 4 * DP + u % (D >> 2) * 16;
-            *reinterpret_cast<u4 *>(&stage[buf][0][wave * 16 * DP + u * 16]) = kr[x];  // zeros past D
-            if (EXACT || u < D) *reinterpret_cast<u4 *>(&stage[buf][1][wave * 16 * DP + v]) = vr[x];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) bad |= nan_bits(vr[x][c]);
+                for (int c = 0; c < 4; ++c) {
+                    bad |= nan_bits(vr[x][c]);
+                    vr[x][c] = without_nan(vr[x][c]);
+                }
+            }
+            if (bad) has_nan = 1;
         }
-        const bool any = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
-        if (lane == 0) has_nan[buf][wave] = any;
+#pragma unroll
+        for (int x = 0; x < PL; ++x) {
+            const int u = 64 * x + lane, g = u / (D >> 2), d4 = u - g * (D >> 2);  // a group of tokens, columns 4 d4 ..
+            *reinterpret_cast<u4 *>(&stage_k[buf][wave * 16 * DP + u * 16]) = kr[x];  // zeros past D
+            if (EXACT || u < D)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    *reinterpret_cast<h4 *>(&stage_v[buf][wave * 16 * DP + (g & 1) * 8 * DP + (e * (DP / 4) + d4) * 8 + (g >> 1) * 4]) =
+                        widen4(vr[x][e], ratio);
+        }
     };
     if (part.steps > 0) {
         blk = block_of(a, head, token_of(0), find_page(a, b, token_of(0), part.end));
@@ -663,23 +694,26 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
                 to_pieces<NQ>(x[j][u], f, EXACT || 32 * j + 16 * h < D, &qf[0][j][u], &qf[NQ - 1][j][u]);
     }
 
-    f16v o[MT];  // columns 128 x + CPL (8 a + 4 h + b) + c in o[x * CPL + c][4 a + b]
+    f16v o[MT];  // tile t, row i: place 32 t + 8 (i / 4) + 4 h + i % 4 of V's columns
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+    auto column = [&](int t, int i) {
+        const int p = 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
+        return 4 * (p % (DP / 4)) + p / (DP / 4);
+    };
     float m = -kInf, l = 0.0f;
-    uint32_t vref = 0;
     auto scale_o = [&](float f) {
 #pragma unroll
         for (int t = 0; t < MT; ++t) o[t] *= f;
     };
 
     // one step's tokens from LDS; MASKED: some rows do not see all of them
-    uint32_t ks[4], vs[4];
     auto step = [&](int32_t tok, int buf, auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
-        const uint8_t *sk = stage[buf][0], *sv = stage[buf][1];
+        const uint8_t *sk = stage_k[buf];
+        const _Float16 *sv = stage_v[buf];
         f16v t[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
@@ -719,23 +753,15 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
             float b = t[q >> 1][(q & 1) * 8];
 #pragma unroll
             for (int i = 1; i < 8; ++i) b = fmaxf(b, t[q >> 1][(q & 1) * 8 + i]);
-            // a factor of 0 (a K scale below the range) must not make a NaN of a hidden token's -inf
+            // a factor of 0 (scales below the range) must not make a NaN of a hidden token's -inf
             mx = fmaxf(mx, MASKED && b == -kInf ? b : b * c[q]);
         }
         mx = max_over_halves(mx);
-        if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
+        if (__builtin_amdgcn_ballot_w64(mx > m + weight_slack<NP>()) != 0) {
             const float f = mx > m ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
             l *= f;
             scale_o(f);
-            m = mx;
-        }
-        uint32_t top = vs[0] > vs[1] ? vs[0] : vs[1];
-        top = vs[2] > top ? vs[2] : top;
-        top = vs[3] > top ? vs[3] : top;
-        if (top > vref) {
-            const int e = (int)(vref >> 23) - (int)(top >> 23) + 127;
-            scale_o(bits_f32((uint32_t)(e < 0 ? 0 : e) << 23));
-            vref = top;
+            m = mx > m ? mx : m;
         }
         const float mm = weight_base<NP>(m);
         h8 p[NP][4];
@@ -751,8 +777,8 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
                     if (MASKED) v = x == -kInf ? x : v;
                     e[y] = weight_scale<NP>(__builtin_amdgcn_exp2f(v));
                 }
-                l += e[0] + e[1];
                 const h2 eh = __builtin_convertvector(e, h2);
+                l = add_weights<NP>(l, e, eh);
                 p[0][q][i] = eh[0], p[0][q][i + 1] = eh[1];
                 if constexpr (NP == 2) {
                     const h2 el = __builtin_convertvector(f2{e[0] - (float)eh[0], e[1] - (float)eh[1]}, h2);
@@ -760,53 +786,24 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
                 }
             }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const float ratio = v_ratio(vs[q], vref);
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
-            for (int x = 0; x < VR; ++x) {
-                const uint8_t *pv = sv + q * 16 * DP + h * 4 * DP + (128 * x + CPL * r) * 4;
-                uint32_t v0[CPL], v1[CPL];  // groups h and h + 2 of four tokens
-                if constexpr (CPL == 4) {
-                    const u4 u0 = *reinterpret_cast<const u4 *>(pv), u1 = *reinterpret_cast<const u4 *>(pv + 8 * DP);
+            for (int y = 0; y < MT; ++y) {
+                const h8 va = *reinterpret_cast<const h8 *>(sv + q * 16 * DP + h * 8 * DP + (32 * y + r) * 8);
 #pragma unroll
-                    for (int y = 0; y < CPL; ++y) v0[y] = u0[y], v1[y] = u1[y];
-                } else {
-                    const u2 u0 = *reinterpret_cast<const u2 *>(pv), u1 = *reinterpret_cast<const u2 *>(pv + 8 * DP);
-#pragma unroll
-                    for (int y = 0; y < CPL; ++y) v0[y] = u0[y], v1[y] = u1[y];
-                }
-#pragma unroll
-                for (int y = 0; y < CPL; ++y) {
-                    if (MASKED) v0[y] = without_nan(v0[y]), v1[y] = without_nan(v1[y]);
-                    const h8 va = widen8(v0[y], v1[y], ratio);
-#pragma unroll
-                    for (int z = 0; z < NP; ++z)
-                        o[x * CPL + y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, p[z][q], o[x * CPL + y], 0, 0, 0);
-                }
+                for (int z = 0; z < NP; ++z) o[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, p[z][q], o[y], 0, 0, 0);
             }
-        }
-        if (MASKED && (has_nan[buf][0] | has_nan[buf][1] | has_nan[buf][2] | has_nan[buf][3])) {  // NaN codes of V reach the rows that see their token, and no others
-#pragma unroll 1
-            for (int e = 0; e < 64; ++e) {
-                const uint32_t there = e < 16 ? vs[0] : e < 32 ? vs[1] : e < 48 ? vs[2] : vs[3];
-                if (!there || tok + e < lo || tok + e >= hi) continue;
-#pragma unroll
-                for (int y = 0; y < MT; ++y)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int d = 128 * (y / CPL) + CPL * (8 * (i >> 2) + 4 * h + (i & 3)) + y % CPL;
-                        if ((sv[v_place(e, d, DP)] & 0x7f) == 0x7f) o[y][i] = __builtin_nanf("");
-                    }
-            }
-        }
     };
 
     // around a step: its scales and the next one's loads, and what they brought
     auto before = [&](int32_t k) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            ks[q] = lane_of(blk.ks, (k & 15) * 4 + q);
-            vs[q] = lane_of(blk.vs, (k & 15) * 4 + q);
+        for (int q = 0; q < 4; ++q) ks[q] = ks_next[q], vs[q] = vs_next[q];
+        whole = whole_next;
+        if (vref_next != vref) {
+            const int e = (int)(vref >> 23) - (int)(vref_next >> 23) + 127;
+            scale_o(bits_f32((uint32_t)(e < 0 ? 0 : e) << 23));
+            vref = vref_next;
         }
         if ((k & 15) == 15) blk = next;
         if (k + 1 < part.steps) fetch(k + 1);
@@ -817,50 +814,88 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
         if (k + 1 < part.steps) deposit(k + 1, (k + 1) & 1);
         __syncthreads();
     };
+    if (threadIdx.x == 0) has_nan = 0;
+    __syncthreads();
     if (part.steps > 0) deposit(0, 0);
     __syncthreads();
-    // steps that all of the wavefront's rows see whole, in a loop of their own
+    // steps that all rows see whole, in a loop of their own
     for (int32_t k = 0; k < part.steps; ++k) {
-        int32_t tok;
         for (; k < part.steps; ++k) {
             before(k);
-            tok = part.start + (k << 6);
-            if (!(tok >= w_lo_max && tok + 64 <= w_hi_min && vs[0] && vs[1] && vs[2] && vs[3])) break;
-            step(tok, k & 1, std::false_type{});
+            if (__builtin_expect(!whole, 0)) break;
+            step(part.start + (k << 6), k & 1, std::false_type{});
             after(k);
         }
         if (k < part.steps) {
+            const int32_t tok = part.start + (k << 6);
             if (tok < w_hi && tok + 64 > w_lo) step(tok, k & 1, std::true_type{});
             after(k);
         }
     }
 
     l = sum_over_halves(l);
+    if (__builtin_expect(has_nan, 0)) {
+        // V's NaN codes reach the rows that see their token, and no others: a
+        // product of "is NaN" and "is seen", over the steps that took them for
+        // zeros
+        f16v hit[MT];
+#pragma unroll
+        for (int y = 0; y < MT; ++y)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) hit[y][i] = 0.0f;
+#pragma unroll 1
+        for (int32_t tok = part.start; tok < part.end; tok += 16) {
+            const Block w = block_of(a, head, tok, find_page(a, b, tok, part.end));
+            if (!w.vs) continue;
+            const uint8_t *p = a.v + (w.lo | (uint64_t)w.hi << 32) * (uint64_t)(16 * D) + h * 4 * D;
+            const uint32_t from = tok + 4 * h - lo, span = hi - lo;
+            h8 on;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) on[e] = from + 8 * (e >> 2) + (e & 3) < span ? (_Float16)1.0f : (_Float16)0.0f;
+#pragma unroll
+            for (int y = 0; y < MT; ++y) {
+                const int place = 32 * y + r, d = 4 * (place % (DP / 4)) + place / (DP / 4);
+                const bool in = EXACT || d < D;
+                const uint32_t n0 = in ? nan_bits(*reinterpret_cast<const uint32_t *>(p + 4 * d)) : 0;
+                const uint32_t n1 = in ? nan_bits(*reinterpret_cast<const uint32_t *>(p + 4 * d + 8 * D)) : 0;
+                h8 is;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    is[e] = ((e < 4 ? n0 : n1) >> (8 * (e & 3) + 7)) & 1 ? (_Float16)1.0f : (_Float16)0.0f;
+                hit[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, on, hit[y], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int y = 0; y < MT; ++y)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[y][i] = hit[y][i] > 0.0f ? __builtin_nanf("") : o[y][i];
+    }
     if (!live) return;
     const float f = bits_f32(vref) * (1.0f / (1 << kVBits)) / l;
-    float *po = nullptr;
-    if (sp.splits > 1) {
-        po = sp.o + (out_row * sp.splits + split) * D;
-        if (h == 0) sp.lse[out_row * sp.splits + split] = l == 0.0f ? -kInf : m + __builtin_amdgcn_logf(l);
-    }
-    const int64_t oo = ((int64_t)s.row0 + qi) * a.o_token + (int64_t)qh * a.o_head;
+    // four columns 4 u .. 4 u + 3: places u, DP / 4 + u, ..
+    auto results = [&](auto put) {
 #pragma unroll
-    for (int x = 0; x < VR; ++x)
+        for (int x = 0; x < (DP + 127) / 128; ++x)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < CPL; ++e) {
-                const int d = 128 * x + CPL * (8 * i + 4 * h) + 4 * e;
+            for (int i = 0; i < (DP < 128 ? DP / 8 : 16); ++i) {
+                const int d = column(x, i);  // e = 0
                 f4 v;
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    v[u] = l == 0.0f ? 0.0f : o[x * CPL + (4 * e + u) % CPL][4 * i + (4 * e + u) / CPL] * f;
-                if (!EXACT && d >= D) continue;
-                if (po)
-                    *reinterpret_cast<f4 *>(po + d) = v;
-                else
-                    store_o4<NP == 1>(a.o, oo + d, v);
+                for (int e = 0; e < 4; ++e) {
+                    const int t = (e * (DP / 4) + 32 * x) / 32, up = (e * (DP / 4) + 32 * x) % 32;  // DP 64: half a tile on
+                    v[e] = l == 0.0f ? 0.0f : o[t][i + up / 2] * f;
+                }
+                if (EXACT || d < D) put(d, v);
             }
+    };
+    if (sp.splits > 1) {
+        float *po = sp.o + (out_row * sp.splits + split) * D;
+        if (h == 0) sp.lse[out_row * sp.splits + split] = l == 0.0f ? -kInf : m + __builtin_amdgcn_logf(l);
+        results([&](int d, f4 v) { *reinterpret_cast<f4 *>(po + d) = v; });
+    } else {
+        const int64_t oo = ((int64_t)s.row0 + qi) * a.o_token + (int64_t)qh * a.o_head;
+        results([&](int d, f4 v) { store_o4<NP == 1>(a.o, oo + d, v); });
+    }
 }
 
 // Joins a row's parts, a workgroup a row: the weights first, then the parts by
