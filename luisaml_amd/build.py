@@ -12,6 +12,9 @@ tree).  Flags:
                                             gemv_valu.hip) the N leading scalar
                                             kernel arguments arrive in SGPRs
                                             at wave start
+csrc/binding.cpp (Python calls of the norm, KV cache and attention entry
+points) becomes the module luisaml_amd/_binding.so, compiled by the host
+compiler against torch's and Python's headers and linked to the library.
 Usage:  python -m luisaml_amd.build   (or luisaml_amd.build.build())
 """
 from __future__ import annotations
@@ -22,11 +25,13 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "liblcml_fp8.so")
+BINDING = os.path.join(HERE, "_binding.so")
 ROOT = os.path.dirname(HERE)
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -61,8 +66,25 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _build_binding() -> None:
+    import torch
+    from torch.utils import cpp_extension
+    tmp = BINDING + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch.compiled_with_cxx11_abi(), "-I" + os.path.join(ROOT, "include"),
+           *("-isystem" + d for d in cpp_extension.include_paths()), "-I" + sysconfig.get_paths()["include"],
+           os.path.join(CSRC, "binding.cpp"), "-o", tmp, "-L" + HERE, "-l:" + os.path.basename(LIB),
+           *("-L" + d for d in cpp_extension.library_paths()), "-ltorch_python", "-ltorch_cpu", "-lc10",
+           "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"binding failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BINDING)
+
+
 def build(verbose: bool = False) -> str:
-    """Compile every csrc/*.hip and link liblcml_fp8.so; returns its path."""
+    """Compile every csrc/*.hip, link liblcml_fp8.so and the Python binding;
+    returns the library's path."""
     os.makedirs(OBJ, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
     workers = min(len(srcs), max(1, min(8, os.cpu_count() or 1)))
@@ -74,15 +96,17 @@ def build(verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    _build_binding()
     if verbose:
-        print("built", LIB)
+        print("built", LIB, "and", os.path.basename(BINDING))
     return LIB
 
 
 def clean() -> None:
     shutil.rmtree(OBJ, ignore_errors=True)
-    if os.path.exists(LIB):
-        os.remove(LIB)
+    for path in (LIB, BINDING):
+        if os.path.exists(path):
+            os.remove(path)
 
 
 if __name__ == "__main__":

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import importlib
 import os
 import re
 
@@ -486,14 +487,22 @@ def binary(op: int, a: torch.Tensor, b: torch.Tensor, dtype: int, out: torch.Ten
 
 # ------------------------------------- norm, KV cache, attention -----------
 #
-# These run once or more for every layer and token, so their checks touch each
-# tensor's attributes once: a decode step's calls are as long as their kernels.
+# These run once or more for every layer and token, so their calls go through
+# the compiled module _binding (csrc/binding.cpp), which checks the tensors.
 
-_F32, _U8, _I32 = torch.float32, torch.uint8, torch.int32
+_native = None
 
 
-def _bytes_of(t):
-    return t.numel() * t.element_size() if t is not None else 0
+def _binding():
+    """Load _binding.so (built by luisaml_amd.build); raise if it is absent."""
+    global _native
+    if _native is None:
+        lib()  # the library that it links to
+        path = os.path.join(HERE, "_binding.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is not built; run `python -m luisaml_amd.build`")
+        _native = importlib.import_module("luisaml_amd._binding")
+    return _native
 
 
 def rms_norm(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual: torch.Tensor | None = None,
@@ -503,75 +512,24 @@ def rms_norm(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual: torch.T
     linear.  x [M,H] fp32/bf16; residual fp32/bf16; gamma [H] fp32.  mode
     SCALE_STATIC takes scale[1]; SCALE_TENSOR gives it; SCALE_ROW gives [M].
     Returns (codes uint8 [M,H], scale, h or None)."""
-    shape = x.shape
-    M, H = shape
-    assert x.is_cuda and gamma.is_cuda, "device tensors expected"
-    assert gamma.dtype is _F32 and gamma.numel() == H and gamma.is_contiguous()
-    ldx, one = x.stride()
-    assert one == 1 or H <= 1
-    rp = rop = None
-    rt = ldr = ldro = 0
-    if residual is not None:
-        if residual_out is None:
-            residual_out = torch.empty((M, H), dtype=residual.dtype, device=x.device)
-        rdt = residual.dtype
-        assert residual.is_cuda and residual_out.is_cuda, "device tensors expected"
-        assert residual.shape == shape == residual_out.shape and residual_out.dtype is rdt
-        (ldr, one), (ldro, one2) = residual.stride(), residual_out.stride()
-        assert one == one2 == 1 or H <= 1
-        rp, rop, rt = residual.data_ptr(), residual_out.data_ptr(), _DTYPE_CODE.get(rdt, 0)
-    elif residual_out is not None:
-        raise ValueError("residual_out without residual")
-    y = out if out is not None else torch.empty((M, H), dtype=_U8, device=x.device)
-    ldy, one = y.stride()
-    assert y.is_cuda and y.dtype is _U8 and y.shape == shape and (one == 1 or H <= 1)
-    n = M if mode == SCALE_ROW else 1
+    if residual is not None and residual_out is None:
+        residual_out = torch.empty(residual.shape, dtype=residual.dtype, device=x.device)
+    if out is None:
+        out = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
     if scale is None:
-        assert mode != SCALE_STATIC, "SCALE_STATIC takes a scale"
-        scale = torch.empty(n, dtype=_F32, device=x.device)
-    assert scale.is_cuda and scale.dtype is _F32 and scale.numel() >= n and scale.is_contiguous()
-    if mode == SCALE_TENSOR and M > 1 and workspace is None:
-        workspace = torch.empty(lib().lcml_fp8_rms_norm_workspace_bytes(M, H, mode), dtype=_U8, device=x.device)
-    _check(lib().lcml_fp8_rms_norm(M, H, x.data_ptr(), _DTYPE_CODE.get(x.dtype, 0), ldx, rp, rop, rt, ldr, ldro,
-                                   gamma.data_ptr(), eps, y.data_ptr(), ldy, mode, scale.data_ptr(), _ptr(workspace),
-                                   _bytes_of(workspace), _stream(stream)))
-    return y, scale, residual_out
-
-
-def _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q):
-    """The checked cache arguments, in the C ABI's order; kv heads and head size."""
-    shape = k_cache.shape
-    pages, heads, page_tokens, dim = shape
-    assert (k_cache.is_cuda and v_cache.is_cuda and k_scale.is_cuda and v_scale.is_cuda and block_table.is_cuda
-            and kv_len.is_cuda and cu_q.is_cuda), "device tensors expected"
-    assert k_cache.dtype is _U8 and v_cache.dtype is _U8 and k_scale.dtype is _F32 and v_scale.dtype is _F32
-    assert block_table.dtype is _I32 and kv_len.dtype is _I32 and cu_q.dtype is _I32
-    assert v_cache.shape == shape and k_scale.shape == shape[:2] == v_scale.shape
-    assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()
-    seqs, cols = block_table.shape
-    pitch, one = block_table.stride()
-    assert kv_len.numel() == seqs and cu_q.numel() == seqs + 1 and kv_len.is_contiguous() and cu_q.is_contiguous()
-    assert one == 1 or cols <= 1
-    return (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, heads, dim,
-            page_tokens, block_table.data_ptr(), pitch if pitch > cols else cols, cols, kv_len.data_ptr(),
-            cu_q.data_ptr(), seqs)
-
-
-def _two_rows(k, v, cache):
-    """Of K's and V's rows: dtype, tokens, strides."""
-    shape = k.shape
-    tokens, heads, dim = shape
-    assert k.is_cuda and v.is_cuda, "device tensors expected"
-    assert heads == cache[5] and dim == cache[6] and v.shape == shape and k.dtype is v.dtype
-    (kt, kh, one), (vt, vh, one2) = k.stride(), v.stride()
-    assert one == one2 == 1
-    return _DTYPE_CODE.get(k.dtype, 0), tokens, kt, kh, vt, vh
+        if mode == SCALE_STATIC:
+            raise ValueError("SCALE_STATIC takes a scale")
+        scale = torch.empty(x.shape[0] if mode == SCALE_ROW else 1, dtype=torch.float32, device=x.device)
+    if mode == SCALE_TENSOR and workspace is None and x.shape[0] > 1:
+        workspace = torch.empty(lib().lcml_fp8_rms_norm_workspace_bytes(*x.shape, mode), dtype=torch.uint8, device=x.device)
+    _check(_binding().rms_norm(x, gamma, eps, residual, residual_out, mode, scale, out, workspace, _stream(stream)))
+    return out, scale, residual_out
 
 
 def kv_cache(pages: int, kv_heads: int, page_tokens: int, head_dim: int, device):
     """An empty E4M3 KV cache: (k_cache, v_cache, k_scale, v_scale)."""
     shape = (pages, kv_heads, page_tokens, head_dim)
-    return (torch.zeros(shape, dtype=_U8, device=device), torch.zeros(shape, dtype=_U8, device=device),
+    return (torch.zeros(shape, dtype=torch.uint8, device=device), torch.zeros(shape, dtype=torch.uint8, device=device),
             torch.ones(shape[:2], device=device), torch.ones(shape[:2], device=device))
 
 
@@ -581,8 +539,8 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     """New tokens' k, v [tokens, kv_heads, head_dim] (fp32/bf16, any token and
     head strides) into the cache [pages, kv_heads, page_tokens, head_dim], as
     the last tokens of their sequences (kv_len counts them)."""
-    c = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q)
-    _check(lib().lcml_fp8_kv_cache_write(k.data_ptr(), v.data_ptr(), *_two_rows(k, v, c), *c, max_q, _stream(stream)))
+    _check(_binding().kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q, max_q,
+                                     _stream(stream)))
 
 
 def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -590,9 +548,8 @@ def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.T
                   v_out: torch.Tensor, stream=None) -> None:
     """The inverse of kv_cache_write: the same rows' tokens into k_out, v_out
     [tokens, kv_heads, head_dim] (fp32 or bf16)."""
-    c = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q)
-    _check(lib().lcml_fp8_kv_cache_read(*c, max_q, k_out.data_ptr(), v_out.data_ptr(), *_two_rows(k_out, v_out, c),
-                                        _stream(stream)))
+    _check(_binding().kv_cache_read(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q, max_q, k_out, v_out,
+                                    _stream(stream)))
 
 
 @functools.lru_cache(maxsize=256)
@@ -607,18 +564,13 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_s
     """softmax(scale * q k^T) v over the E4M3 cache: q [tokens, q_heads,
     head_dim] (fp32/bf16) are the last tokens of their sequences, which the
     cache already holds.  window > 0: only the last `window` positions."""
-    c = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q)
-    shape = q.shape
-    tokens, heads, dim = shape
-    o = out if out is not None else torch.empty(shape, dtype=out_dtype or q.dtype, device=q.device)
-    assert q.is_cuda and o.is_cuda, "device tensors expected"
-    (qt, qh, one), (ot, oh, one2) = q.stride(), o.stride()
-    assert dim == c[6] and o.shape == shape and one == one2 == 1
+    if out is None:
+        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
     if workspace is None:
-        need = _attention_workspace(tokens, c[13], heads, c[5], dim, max_q, max_kv)
+        tokens, heads, dim = q.shape
+        need = _attention_workspace(tokens, kv_len.numel(), heads, k_cache.shape[1], dim, max_q, max_kv)
         if need:
-            workspace = torch.empty(need, dtype=_U8, device=q.device)
-    _check(lib().lcml_fp8_attention(q.data_ptr(), _DTYPE_CODE.get(q.dtype, 0), tokens, heads, qt, qh, o.data_ptr(),
-                                    _DTYPE_CODE.get(o.dtype, 0), ot, oh, *c, max_q, max_kv, scale, causal, window,
-                                    _ptr(workspace), _bytes_of(workspace), _stream(stream)))
-    return o
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _check(_binding().attention(q, out, k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q, max_q, max_kv,
+                                scale, causal, window, workspace, _stream(stream)))
+    return out

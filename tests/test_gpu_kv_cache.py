@@ -177,3 +177,35 @@ def test_cache_past_32_bit_offsets(dev):
         err, s = np.abs(got.float().cpu().numpy() - x), np.abs(x).max() / 448.0 * 2
         assert (err <= np.maximum(np.abs(x) * 2.0 ** -4, s * 2.0 ** -10)).all()
     assert int(c[0][:pages - 2].count_nonzero()) == 0 and int(c[1][:pages - 2].count_nonzero()) == 0
+
+
+def test_binding_checks_shapes_and_types(dev):
+    """Tensors that do not fit each other: ValueError, nothing launched."""
+    c = list(capi.kv_cache(3, 2, 16, 32, dev))
+    idx = [i32([[0, 1]], dev), i32([5], dev), i32([0, 5], dev)]
+    k = torch.zeros(5, 2, 32, device=dev)
+    capi.kernel_trace()
+
+    def bad(what, **kw):
+        a = dict(k=k, v=k, kc=c[0], vc=c[1], ks=c[2], vs=c[3], table=idx[0], kv=idx[1], cu=idx[2])
+        a.update(kw)
+        with pytest.raises(ValueError, match=what):
+            capi.kv_cache_write(*a.values(), 5)
+    bad("k_cache", kc=c[0].int())
+    bad("v_cache", vc=c[1][:2].contiguous())
+    bad("k_cache", kc=c[0].transpose(1, 2))
+    bad("scale", ks=c[2].double())
+    bad("scale", vs=c[3][:, :1].contiguous())
+    bad("block_table", table=idx[0].long())
+    bad("kv_len", kv=i32([5, 5], dev))
+    bad("cu_q", cu=i32([0], dev))
+    bad("k:", k=k[:, :1])
+    bad("v:", v=k.bfloat16())
+    bad("k:", k=k.transpose(1, 2))
+    with pytest.raises(capi.LcmlError):
+        capi.kv_cache_write(k.half(), k.half(), *c, *idx, 5)
+    with pytest.raises(ValueError, match="q:"):
+        capi.attention(torch.zeros(5, 4, 16, device=dev), *c, *idx, 5, 5, 0.1)
+    with pytest.raises(capi.LcmlError):
+        capi.attention(torch.zeros(5, 3, 32, device=dev), *c, *idx, 5, 5, 0.1)
+    assert capi.kernel_trace() == []

@@ -131,3 +131,23 @@ def test_plain_attention_of_one_token_is_its_value():
     o, mass, reach = kc.attention(x.repeat(4, 1), c, np.array([[1]]), [1], [0, 1], 1, 0.25)
     v = c.values(1, np.array([1]), 1)[0][0]
     assert np.allclose(o[0], v.repeat(4, 0)) and np.allclose(mass, np.abs(o))
+
+
+def test_binding_refuses_what_it_cannot_check():
+    """Host tensors, wrong types and shapes: ValueError before any call."""
+    import torch
+    x, g = torch.zeros(2, 8), torch.ones(8)
+    out, s = torch.zeros(2, 8, dtype=torch.uint8), torch.ones(2)
+    with pytest.raises(ValueError, match="device tensor"):
+        capi.rms_norm(x, g, 1e-5, mode=capi.SCALE_ROW, scale=s, out=out, stream=0)
+    with pytest.raises(ValueError, match="tensor is expected"):
+        capi.rms_norm(None, g, 1e-5, mode=capi.SCALE_ROW, scale=s, out=out, stream=0)
+    with pytest.raises(ValueError, match="scale"):
+        capi.rms_norm(x, g, 1e-5, mode=capi.SCALE_STATIC, out=out, stream=0)
+    with pytest.raises(ValueError, match="number of arguments"):
+        capi._binding().attention(x)
+    c = [torch.zeros(1)] * 7
+    for call in (lambda: capi.kv_cache_write(x, x, *c, 1, stream=0), lambda: capi.kv_cache_read(*c, 1, x, x, stream=0),
+                 lambda: capi.attention(torch.zeros(1, 2, 16), *c, 1, 1, 0.1, out=x, workspace=x, stream=0)):
+        with pytest.raises(ValueError, match="device tensor"):
+            call()
