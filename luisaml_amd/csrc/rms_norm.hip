@@ -11,6 +11,12 @@
 // comes first): the first one leaves h, r and one partial maximum for each
 // workgroup, the second reads h again, from the memory-side cache where it
 // fits there.
+//
+// Measured: a row of 4096 takes 3.6 us, a launch with one round trip to memory
+// and two barriers.  4096 x 4096 with x in bf16, an fp32 residual and one scale
+// for the tensor, 185 MB at the least: 29.7 us for the first pass (168 MB, 5.6
+// TB/s) and 22 for the second (84 MB, 3.8 TB/s).  4096 x 6144 in bf16 with a
+// scale a row, 176 MB: 41 us, 4.2 TB/s.
 #include "lcml_internal.hpp"
 
 namespace lcml {
@@ -177,7 +183,9 @@ __device__ inline float abs_max4(float m, f4 v) {
 
 // TPR threads a row (64: four rows of a workgroup side by side, no barriers),
 // NV groups of four elements for each thread in registers.  TAIL: rows longer
-// than TPR * NV * 4, which read the rest again.
+// than TPR * NV * 4, which read the rest again.  Every input's loads are under
+// way before the first is waited for, without a branch (with branches, 52 us
+// where this takes 30).
 template <bool XB, int RES, int CUT, int TPR, int NV, bool TAIL>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm(NormArgs a) {
     constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR;
@@ -263,10 +271,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm(NormArgs a) 
 
 // The second pass of one scale for the tensor: codes of h (the stored one, or
 // x + residual again), from the rows' r and the partial maxima.
-template <bool XB, int RES, int CUT>
+template <bool XB, int RES, int CUT, int NV>
 __global__ __launch_bounds__(256) void k_norm_encode(NormArgs a, int npart) {
     __shared__ float red[4];
-    constexpr int NV = 4;
     const bool stored = RES != kNoRes && a.res_out;
     auto load = [&](int64_t m, int64_t i) {
         if (stored)
@@ -276,7 +283,8 @@ __global__ __launch_bounds__(256) void k_norm_encode(NormArgs a, int npart) {
         raw.load(a, m, i);
         return raw.h();
     };
-    int64_t m = blockIdx.x;
+    // last rows first: the caches hold what the first pass stored last
+    int64_t m = (a.M - 1 - (int64_t)blockIdx.x) / gridDim.x * gridDim.x + blockIdx.x;
     f4 h[NV], gamma[NV];
     float r;
     auto begin = [&](int64_t i0) {
@@ -313,8 +321,8 @@ __global__ __launch_bounds__(256) void k_norm_encode(NormArgs a, int npart) {
                     store_codes<CUT>(a, m, i0 + u * 1024, quantize4_t<decltype(fast)::value>(v[0], v[1], v[2], v[3], d));
                 }
             }
-            m += gridDim.x;
-            if (m >= a.M) break;
+            m -= gridDim.x;
+            if (m < 0) break;
             begin(first);
         }
     };
@@ -335,25 +343,56 @@ hipError_t launch_t(const NormArgs &a, hipStream_t s) {
     };
     const int64_t most = two ? kParts : 1 << 20;
     unsigned n;
-    if constexpr (CUT == kTiny) {
-        hipLaunchKernelGGL((k_rms_norm<XB, RES, CUT, 64, 1, false>), dim3(n = grid(4, most)), dim3(256), 0, s, a);
-    } else {
-        if (a.H <= 1024)
-            hipLaunchKernelGGL((k_rms_norm<XB, RES, CUT, 64, 4, false>), dim3(n = grid(4, most)), dim3(256), 0, s, a);
-        else if (a.H <= 4096 && a.M >= 256)
-            hipLaunchKernelGGL((k_rms_norm<XB, RES, CUT, 256, 4, false>), dim3(n = grid(1, most)), dim3(256), 0, s, a);
-        else if (a.H <= 4096)  // the rows are waited for
-            hipLaunchKernelGGL((k_rms_norm<XB, RES, CUT, 1024, 1, false>), dim3(n = grid(1, most)), dim3(1024), 0, s, a);
-        else if (a.H <= 8192 && a.M >= 256)
-            hipLaunchKernelGGL((k_rms_norm<XB, RES, CUT, 512, 4, false>), dim3(n = grid(1, most)), dim3(512), 0, s, a);
-        else if (a.H <= 8192)
-            hipLaunchKernelGGL((k_rms_norm<XB, RES, CUT, 1024, 2, false>), dim3(n = grid(1, most)), dim3(1024), 0, s, a);
-        else
-            hipLaunchKernelGGL((k_rms_norm<XB, RES, CUT, 1024, 4, true>), dim3(n = grid(1, most)), dim3(1024), 0, s, a);
-    }
+    // Threads by the row's length: as many as hold it in four groups each (a
+    // wavefront a row of 4096 in 16 groups: 39 us for 4096 of them, against 30),
+    // and the number of groups that just holds it: unused ones cost registers
+    // and slots of the loads (4096 rows of 6144 in 3 groups of 512 threads 41
+    // us, in 4 51; of 1536 in 2 of 256 13, in 4 17; of 300 in 2 of 64 5.2, in 4
+    // 6.7).  Fewer than 256 rows do not fill the GPU: a row's own time counts,
+    // which 1024 threads shorten (one row of 4096: 3.6 us, with 256 6.6).
+    auto start = [&](auto tpr, auto nv, auto tail) {
+        constexpr int TPR = decltype(tpr)::value, kThreads = TPR < 256 ? 256 : TPR;
+        n = grid(kThreads / TPR, most);
+        hipLaunchKernelGGL((k_rms_norm<XB, RES, CUT, TPR, decltype(nv)::value, decltype(tail)::value>), dim3(n),
+                           dim3(kThreads), 0, s, a);
+    };
+    const std::integral_constant<int, 64> t64;
+    const std::integral_constant<int, 256> t256;
+    const std::integral_constant<int, 512> t512;
+    const std::integral_constant<int, 1024> t1024;
+    const std::integral_constant<int, 1> n1;
+    const std::integral_constant<int, 2> n2;
+    const std::integral_constant<int, 3> n3;
+    const std::integral_constant<int, 4> n4;
+    const std::false_type whole;
+    const std::true_type tail;
+    const int64_t q = (a.H + 255) / 256;  // groups of a wavefront
+    if constexpr (CUT == kTiny)
+        start(t64, n1, whole);
+    else if (q <= 4)
+        q == 1 ? start(t64, n1, whole) : q == 2 ? start(t64, n2, whole) : q == 3 ? start(t64, n3, whole) : start(t64, n4, whole);
+    else if (q <= 16 && a.M >= 256)
+        q <= 8 ? start(t256, n2, whole) : q <= 12 ? start(t256, n3, whole) : start(t256, n4, whole);
+    else if (q <= 16)
+        start(t1024, n1, whole);
+    else if (q <= 32 && a.M >= 256)
+        q <= 24 ? start(t512, n3, whole) : start(t512, n4, whole);
+    else if (q <= 32)
+        start(t1024, n2, whole);
+    else
+        start(t1024, n4, tail);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess || !two) return err;
-    hipLaunchKernelGGL((k_norm_encode<XB, RES, CUT>), dim3(grid(1, 2048)), dim3(256), 0, s, a, (int)n);
+    auto encode = [&](auto nv) {
+        hipLaunchKernelGGL((k_norm_encode<XB, RES, CUT, decltype(nv)::value>), dim3(grid(1, 2048)), dim3(256), 0, s, a, (int)n);
+    };
+    // a row in rounds of 256 threads x 1 to 4 groups, the fewest rounds and then
+    // the fewest groups (4096 rows of 2048 in 2 27 us with the first pass, in 4 33)
+    const int64_t rounds = (q + 15) / 16, groups = ((q + 3) / 4 + rounds - 1) / rounds;
+    if constexpr (CUT == kTiny)
+        encode(n1);
+    else
+        groups == 1 ? encode(n1) : groups == 2 ? encode(n2) : groups == 3 ? encode(n3) : encode(n4);
     return hipGetLastError();
 }
 

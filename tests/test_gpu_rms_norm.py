@@ -76,6 +76,22 @@ def test_matches_64_bit(dev, M, H, mode, xt, rt):
     check(x, res, gamma, 1e-5, mode, y.cpu().numpy(), s.cpu().numpy(), hn)
 
 
+@pytest.mark.parametrize("H", [256, 257, 511, 514, 768, 771, 1026, 2048, 2049, 2560, 3074, 4095, 4100, 6144, 6146, 8191,
+                               8196])
+@pytest.mark.parametrize("M,mode", [(2, "row"), (257, "tensor"), (300, "row")])
+def test_either_side_of_each_width(dev, H, M, mode):
+    """Rows that just fill the registers of a number of threads, and that just
+    do not, of few rows and of many."""
+    x, res = kc.bf16(synth.normal(M + H, (M, H), std=2.0)), synth.normal(M + 2 * H, (M, H), std=3.0)
+    gamma = 1.0 + synth.normal(H, (H,), std=0.2)
+    y, s, h = capi.rms_norm(torch.from_numpy(x).to(dev).bfloat16(), torch.from_numpy(gamma).to(dev), 1e-5,
+                            residual=torch.from_numpy(res).to(dev), mode=MODES[mode])
+    torch.cuda.synchronize()
+    hn = x + res
+    assert np.array_equal(h.cpu().numpy(), hn)
+    check(x, res, gamma, 1e-5, mode, y.cpu().numpy(), s.cpu().numpy(), hn)
+
+
 @pytest.mark.parametrize("mode", ["static", "tensor", "row"])
 @pytest.mark.parametrize("H", [100, 4200])
 def test_pitches_alignment_in_place_and_other_stream(dev, mode, H):
