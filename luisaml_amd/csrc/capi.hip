@@ -969,14 +969,18 @@ int lcml_fp8_attention(const void *q, int q_dtype, int64_t tokens, int64_t q_hea
     if (tokens == 0 || seqs == 0 || max_q == 0) return LCML_OK;
     if (!q || !o || !elem_aligned(q, q_dtype) || !elem_aligned(o, o_dtype))
         return fail(LCML_ERR_INVALID_ARG, "%s: q or o NULL or not aligned to its elements", fn);
-    // 256 threads each, 2^32 work items a launch; sizes whose products would
-    // pass 64 bits are past that by far
+    // 256 threads each, 2^32 work items a launch, and a workgroup for each row
+    // where parts are joined; sizes whose products would pass 64 bits are past
+    // that by far
     const int64_t most = (int64_t)1 << 24;
     if (max_q * q_heads / kv_heads > most * 16 || seqs * kv_heads > most ||
-        lcml::attention_groups(seqs, q_heads, kv_heads, max_q, max_kv) >= most || seqs * max_q >= most / q_heads)
+        lcml::attention_groups(seqs, q_heads, kv_heads, max_q, max_kv) >= most)
         return fail(LCML_ERR_UNSUPPORTED, "%s: seqs=%lld max_q=%lld q_heads=%lld exceeds one launch", fn,
                     (long long)seqs, (long long)max_q, (long long)q_heads);
     const int64_t need = lcml::attention_workspace(tokens, seqs, q_heads, kv_heads, head_dim, max_q, max_kv);
+    if (need && seqs * max_q >= most / q_heads)
+        return fail(LCML_ERR_UNSUPPORTED, "%s: seqs=%lld max_q=%lld q_heads=%lld exceeds one launch", fn,
+                    (long long)seqs, (long long)max_q, (long long)q_heads);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return fail(LCML_ERR_INVALID_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", fn, (long long)need);
     a.q = q, a.o = o, a.k = k_cache, a.v = v_cache, a.ks = k_scale, a.vs = v_scale;

@@ -153,6 +153,12 @@ def test_bounds_of_the_host_hold(dev):
     run(dev, [100, 40], [1, 1], max_q=50, max_kv=100, seed=4, ot="f")
 
 
+def test_far_larger_max_q(dev):
+    """Sequences times max_q beyond the rows that a join could take, where
+    nothing is split: workgroups without rows end at once."""
+    run(dev, [100, 40], [1, 3], max_q=1 << 22, max_kv=100, seed=4)
+
+
 def test_other_stream_and_graph(dev):
     """Decode captured in a graph, replayed while lengths grow: equal to the
     eager call each time."""
