@@ -12,7 +12,7 @@
 // workgroup, the second reads h again, from the memory-side cache where it
 // fits there.
 //
-// Measured: a row of 4096 takes 3.6 us, a launch with one round trip to memory
+// Measured: a row of 4096 takes 3.7 us, a launch with one round trip to memory
 // and two barriers.  4096 x 4096 with x in bf16, an fp32 residual and one scale
 // for the tensor, 185 MB at the least: 29.7 us for the first pass (168 MB, 5.6
 // TB/s) and 22 for the second (84 MB, 3.8 TB/s).  4096 x 6144 in bf16 with a
@@ -348,8 +348,11 @@ hipError_t launch_t(const NormArgs &a, hipStream_t s) {
     // and the number of groups that just holds it: unused ones cost registers
     // and slots of the loads (4096 rows of 6144 in 3 groups of 512 threads 41
     // us, in 4 51; of 1536 in 2 of 256 13, in 4 17; of 300 in 2 of 64 5.2, in 4
-    // 6.7).  Fewer than 256 rows do not fill the GPU: a row's own time counts,
-    // which 1024 threads shorten (one row of 4096: 3.6 us, with 256 6.6).
+    // 6.7).  Up to 256 rows do not fill the GPU: a row's own time counts, and
+    // twice the threads with half the groups shorten it (256 rows of 4096, 512
+    // threads 4.5 us, 256 threads 5.0; 512 rows 6.2 and 6.5, 4096 rows 29.5 and
+    // 26.9; 64 rows of 8000, 1024 threads 5.2, 512 threads 5.5; from 256 rows on
+    // equal).
     auto start = [&](auto tpr, auto nv, auto tail) {
         constexpr int TPR = decltype(tpr)::value, kThreads = TPR < 256 ? 256 : TPR;
         n = grid(kThreads / TPR, most);
@@ -371,14 +374,14 @@ hipError_t launch_t(const NormArgs &a, hipStream_t s) {
         start(t64, n1, whole);
     else if (q <= 4)
         q == 1 ? start(t64, n1, whole) : q == 2 ? start(t64, n2, whole) : q == 3 ? start(t64, n3, whole) : start(t64, n4, whole);
-    else if (q <= 16 && a.M >= 256)
-        q <= 8 ? start(t256, n2, whole) : q <= 12 ? start(t256, n3, whole) : start(t256, n4, whole);
+    else if (q <= 8)
+        start(t256, n2, whole);
     else if (q <= 16)
-        start(t1024, n1, whole);
-    else if (q <= 32 && a.M >= 256)
-        q <= 24 ? start(t512, n3, whole) : start(t512, n4, whole);
+        a.M <= 256 ? start(t512, n2, whole) : q <= 12 ? start(t256, n3, whole) : start(t256, n4, whole);
+    else if (q <= 24)
+        start(t512, n3, whole);
     else if (q <= 32)
-        start(t1024, n2, whole);
+        a.M <= 256 ? start(t1024, n2, whole) : start(t512, n4, whole);
     else
         start(t1024, n4, tail);
     hipError_t err = hipGetLastError();
