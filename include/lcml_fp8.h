@@ -509,9 +509,9 @@ LCML_API int lcml_fp8_kv_cache_read(const uint8_t *k_cache, const uint8_t *v_cac
  * q, o: [tokens][q_heads][head_dim], FLOAT or BFLOAT16, strides in elements,
  *   elements of a head contiguous; q head h reads KV head
  *   h / (q_heads / kv_heads).
- * Cache and index arguments as above; kv_len[b] <= max_kv and
- * cu_q[b+1] - cu_q[b] <= max_q are the host's bounds (rows and positions past
- * them are left out).  scale > 0.
+ * Cache and index arguments as above; cu_q[b+1] - cu_q[b] <= max_q and
+ * kv_len[b] <= max_kv are the host's bounds (rows past max_q are left out;
+ * max_kv divides the work, and longer sequences only take longer).  scale > 0.
  * workspace: lcml_fp8_attention_workspace_bytes(...) bytes, 16-byte aligned,
  * written before they are read (0: may be NULL).
  * No counterpart in the reference.

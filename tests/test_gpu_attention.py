@@ -159,6 +159,12 @@ def test_far_larger_max_q(dev):
     run(dev, [100, 40], [1, 3], max_q=1 << 22, max_kv=100, seed=4)
 
 
+@pytest.mark.parametrize("kv,n", [([300, 40], [1, 1]), ([3000, 900], [1, 2]), ([700, 300], [100, 80])])
+def test_longer_than_max_kv(dev, kv, n):
+    """A graph that outlives its bound: slower, and still the whole sequence."""
+    run(dev, kv, n, 16, 1, 2, 64, max_kv=64, seed=9)
+
+
 def test_other_stream_and_graph(dev):
     """Decode captured in a graph, replayed while lengths grow: equal to the
     eager call each time."""

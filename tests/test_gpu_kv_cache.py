@@ -87,6 +87,27 @@ def test_empty_sequences_missing_tokens_and_pages(dev):
     run(dev, 3, 16, 64, [0, 20, 3, 0, 40, 20, 90], [0, 0, 5, 2, 40, 20, 60], seed=3, table=holes)
 
 
+@pytest.mark.parametrize("T,D", [(256, 256), (128, 80), (64, 128)])
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_growth_behind_few_new_tokens(dev, T, D, n):
+    """Far larger values at the end of pages that are nearly full: more units
+    of earlier tokens to encode again than the call has threads."""
+    H, L = 2, T - 2
+    rng = np.random.default_rng(T + n)
+    table, pages = kc.tables([L, L - 5], T, rng)
+    cache = kc.Cache(pages, H, T, D, rng)
+    c = cache.to(dev)
+    for lens, cu, by in (([L - n, L - 5 - n], [0, L - n, 2 * (L - n) - 5], 1.0), ([L, L - 5], [0, n, 2 * n], 900.0)):
+        k, v = values(T, (cu[-1], H, D), False) * np.float32(by), values(n, (cu[-1], H, D), False) * np.float32(by)
+        capi.kv_cache_write(torch.from_numpy(k).to(dev), torch.from_numpy(v).to(dev), *c, i32(table, dev), i32(lens, dev),
+                            i32(cu, dev), max(np.diff(cu)))
+        cache.write(k, v, table, np.array(lens), np.array(cu))
+        torch.cuda.synchronize()
+        for w in (0, 1):
+            assert np.array_equal(c[2 + w].cpu().numpy(), cache.scale[w])
+            assert kc.same_codes(c[w].cpu().numpy(), cache.packed(w))
+
+
 def test_tokens_one_by_one_grow_the_scale(dev):
     """A page filled token by token, each larger than the last: the codes that
     stay are encoded again whenever the scale grows."""
