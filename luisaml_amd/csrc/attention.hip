@@ -255,6 +255,13 @@ __device__ inline Part part_of(const AttentionArgs &a, const Split &sp, int32_t 
 // and KV head, over one part of the tokens; its wavefronts take turns of 64
 // tokens, straight from memory into registers, and join at the end.
 // 16x16x32 instructions.
+//
+// Bound by the cache's bytes: 16 KB of loads a wavefront under way (256
+// registers, two wavefronts a SIMD; three spilled and took 213 us where this
+// takes 119, eight in a workgroup 166).  32 queries of 32 heads over up to 16384
+// tokens of 8 KV heads of 128, 619 MB: 119 us, 5.2 TB/s.  One over 500 tokens: 8
+// us, five dependent round trips to memory (lengths, table, scales, codes, the
+// join's LDS).
 template <int DC, int NQ, int NP, int NW>
 __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(AttentionArgs a, Split sp) {
     constexpr int DP = DC * 64, kPitch = DP + 4;
@@ -548,8 +555,15 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
 // Each wavefront brings 16 of a step's tokens into LDS, K as codes and V
 // widened: bound by the vector ALU and the matrix cores in turn, the kernel
 // shares the widening of V (64 conversions a wavefront and step would be
-// repeated by each of the four), and reads K's codes in half the bytes, as LDS
-// could not feed two fp16 operands.  32x32x16 instructions.
+// repeated by each of the four), and reads K's codes in half the bytes (K
+// widened as well: 610 us where this takes 600).  32x32x16 instructions.
+//
+// A prompt of 8192 tokens, 32 heads over 8 of 128, 0.55 TFLOP: 600 us, 917
+// TFLOP/s, where a product of 8192^3 in bf16 reaches 1190.  A step's 32 matrix
+// instructions take 1024 cycles of a SIMD, its 313 vector ones 1250, and two
+// wavefronts a SIMD overlap them to two thirds of the sum.  (Two groups of
+// wavefronts half a step apart: 1075 us, for the registers spilled.)  D > 128
+// has one wavefront a SIMD, and nothing to overlap LDS reads with: 150 TFLOP/s.
 constexpr int kManyWaves = 4, kManyRows = 32 * kManyWaves;
 
 template <int DP, bool EXACT, int NQ, int NP>
@@ -898,9 +912,50 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
     }
 }
 
+constexpr int kMostSplits = 128, kRowsSplits = 16;
+
+// Joins few parts of many rows: D / 4 threads a row, as many rows a workgroup
+// as fit, and no barriers; every thread weighs all of its row's parts.
+template <bool BF16>
+__global__ __launch_bounds__(256) void k_attention_join_rows(AttentionArgs a, Split sp, uint32_t total) {
+    const int32_t D = a.t.dim, q4 = D >> 2, per = 256 / q4;
+    const int32_t grp = threadIdx.x / q4, d = (threadIdx.x - grp * q4) * 4;
+    const uint32_t id = blockIdx.x * (uint32_t)per + grp;
+    if (grp >= per || id >= total) return;
+    const uint32_t per_seq = (uint32_t)(a.max_q * a.q_heads);
+    const int32_t b = id / per_seq, at = id - b * per_seq, i = at / a.q_heads, h = at - i * a.q_heads;
+    const SeqRows s = seq_rows(a.t, b);
+    if (i >= s.n) return;
+    const int64_t row = ((int64_t)s.row0 + i) * a.q_heads + h;
+    const float *lse = sp.lse + row * sp.splits, *po = sp.o + row * sp.splits * D + d;
+    float x[kRowsSplits], top = -kInf, sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kRowsSplits; ++k) x[k] = lse[k < sp.splits ? k : 0];
+#pragma unroll
+    for (int k = 0; k < kRowsSplits; ++k) top = fmaxf(top, x[k]);
+    f4 v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k0 = 0; k0 < kRowsSplits; k0 += 4) {
+        if (k0 >= sp.splits) break;
+        f4 p[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)  // a part of weight 0 wrote nothing
+            p[u] = k0 + u < sp.splits && x[k0 + u] != -kInf ? *reinterpret_cast<const f4 *>(po + (int64_t)(k0 + u) * D)
+                                                            : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float e = x[k0 + u];
+            const float w = k0 + u >= sp.splits || e == -kInf ? 0.0f : e == top ? 1.0f : __builtin_amdgcn_exp2f(e - top);
+            sum += w;
+            v += p[u] * w;
+        }
+    }
+    store_o4<BF16>(a.o, ((int64_t)s.row0 + i) * a.o_token + (int64_t)h * a.o_head + d,
+                   sum == 0.0f ? f4{0.f, 0.f, 0.f, 0.f} : v * (1.0f / sum));
+}
+
 // Joins a row's parts, a workgroup a row: the weights first, then the parts by
 // as many groups of D / 4 threads as there are, four loads each under way.
-constexpr int kMostSplits = 128;
 
 template <bool BF16>
 __global__ __launch_bounds__(256) void k_attention_join(AttentionArgs a, Split sp) {
@@ -954,25 +1009,27 @@ constexpr int kFewWaves = 4;
 
 struct Plan {
     bool few;
+    int64_t groups;  // workgroups
     Split sp;
 };
 
-Plan make_plan(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t max_q, int64_t max_kv, int64_t window) {
+int width_of(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }  // columns that the kernels are built for
+
+// one kernel's division of rows of `pairs` (sequence, KV head), that see `span`
+// tokens at most
+Plan divide(bool few, int64_t pairs, int64_t rows, int64_t span) {
     Plan p{};
-    const int64_t rows = max_q * (q_heads / kv_heads);
-    p.few = rows <= 64;
-    const int64_t tile = p.few ? 16 : kManyRows;
+    p.few = few;
+    const int64_t tile = few ? 16 : kManyRows;
     p.sp.tiles = (int32_t)((rows + tile - 1) / tile);
-    // tokens that a row tile can see
-    int64_t span = max_kv;
-    if (window > 0 && window < span && window + max_q + 64 < span) span = window + max_q + 64;
-    const int64_t groups = seqs * kv_heads * p.sp.tiles, steps = (span + 63) / 64;
+    const int64_t groups = pairs * p.sp.tiles, steps = (span + 63) / 64;
     // Few rows: 512 workgroups of a step for each wavefront at least, and up to
-    // 2048 of four steps, so that ragged lengths even out.  Many rows: parts
-    // of 32 steps up to two workgroups a CU, of eight up to one, as joining them
-    // reads and writes every result again in fp32.
+    // 2048 of four steps, so that ragged lengths even out (4096: 1 x 32000 28 us
+    // against 20).  Many rows: parts of 32 steps up to two workgroups a CU, of
+    // eight up to one, as joining them reads and writes every result again in
+    // fp32.
     int64_t splits;
-    if (p.few) {
+    if (few) {
         const int64_t fine = (steps + 4 * kFewWaves - 1) / (4 * kFewWaves), coarse = (steps + kFewWaves - 1) / kFewWaves;
         splits = (2048 + groups - 1) / groups;
         splits = splits < fine ? splits : fine;
@@ -990,7 +1047,36 @@ Plan make_plan(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t max_q, i
     if (splits < 1) splits = 1;
     p.sp.chunk = (int32_t)(((steps + splits - 1) / splits) * 64);
     p.sp.splits = (int32_t)splits;
+    p.groups = groups * splits;
     return p;
+}
+
+// Up to 64 rows the kernel for few rows is the faster one (64 rows: 8 sequences
+// of 4000 tokens 40.5 us against 46, 32 of 1000 35 against 38).  Above, the sum
+// of what either takes decides, in us by measurement: a start, a step of 64
+// tokens, as many workgroups as run at once, a join.  Of 68 cases of 1 to 32
+// sequences, 16 to 1500 queries and all widths it takes the slower one in two (10
+// us for 8.3, 32 for 30).  Some: 1 x 256 9.0 us in the kernel for few rows, 14 in
+// the one for many; 1 x 512 18 and 21; 1 x 700 28 and 27; 8 x 128 30 and 14; 32
+// after 4000 18 and 28; 4 x 100 after 900 31 and 36; one KV head of 256, 512
+// queries of 8 heads, 15 and 45.
+// max_kv decides, not the window: the workspace then covers any window.
+Plan make_plan(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t max_q, int64_t max_kv,
+               int64_t window) {
+    const int64_t rows = max_q * (q_heads / kv_heads), pairs = seqs * kv_heads;
+    bool few = rows <= 64;
+    if (!few) {
+        const Plan f = divide(true, pairs, rows, max_kv), m = divide(false, pairs, rows, max_kv);
+        const int width = width_of(dim);
+        const double at_once = 65536.0 / width, step = width == 64 ? 1.1 : width == 128 ? 1.65 : 3.3;
+        const double rf = f.groups / at_once, rm = m.groups / 512.0;
+        const int64_t sf = (f.sp.chunk / 64 + kFewWaves - 1) / kFewWaves, sm = m.sp.chunk / 64;
+        few = 3.0 + (rf > 1.0 ? rf : 1.0) * (3.5 + 2.5 * sf) + (f.sp.splits > 1 ? 4.0 : 0.0) <
+              8.0 + (rm > 1.0 ? rm : 1.0) * step * sm + (m.sp.splits > 1 ? 6.0 : 0.0);
+    }
+    int64_t span = max_kv;  // tokens that a row tile can see
+    if (window > 0 && window < span && window + max_q + 64 < span) span = window + max_q + 64;
+    return divide(few, pairs, rows, span);
 }
 
 template <int DC, int NQ, int NP>
@@ -1009,8 +1095,8 @@ void start_many(const AttentionArgs &a, const Split &sp, unsigned grid, hipStrea
 // NQ = 1: q is bf16; NP = 1: o is
 template <int NQ, int NP>
 hipError_t launch_t(const AttentionArgs &a, const Plan &p, hipStream_t s) {
-    const unsigned grid = (unsigned)((int64_t)a.t.seqs * a.t.heads * p.sp.tiles * p.sp.splits);
-    const int width = a.t.dim <= 64 ? 64 : a.t.dim <= 128 ? 128 : 256;
+    const unsigned grid = (unsigned)p.groups;
+    const int width = width_of(a.t.dim);
     if (p.few)
         width == 64    ? start_few<1, NQ, NP>(a, p.sp, grid, s)
         : width == 128 ? start_few<2, NQ, NP>(a, p.sp, grid, s)
@@ -1022,6 +1108,14 @@ hipError_t launch_t(const AttentionArgs &a, const Plan &p, hipStream_t s) {
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess || p.sp.splits == 1) return err;
     const unsigned rows = (unsigned)((int64_t)a.t.seqs * a.max_q * a.q_heads);
+    const unsigned per = 1024u / a.t.dim;
+    // from 512 rows on many rows a workgroup (8 x 16 x 32 rows of 4 parts 40.5 us
+    // with attention, a workgroup a row 44; 16384 rows of 2 22 and 43; 128 rows of
+    // 16 15.7 and 15.0)
+    if (rows >= 512 && p.sp.splits <= kRowsSplits) {
+        hipLaunchKernelGGL((k_attention_join_rows<NP == 1>), dim3((rows + per - 1) / per), dim3(256), 0, s, a, p.sp, rows);
+        return hipGetLastError();
+    }
     hipLaunchKernelGGL((k_attention_join<NP == 1>), dim3(rows), dim3(256), 0, s, a, p.sp);
     return hipGetLastError();
 }
@@ -1030,17 +1124,16 @@ hipError_t launch_t(const AttentionArgs &a, const Plan &p, hipStream_t s) {
 
 int64_t attention_workspace(int64_t tokens, int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim,
                             int64_t max_q, int64_t max_kv) {
-    const Plan p = make_plan(seqs, q_heads, kv_heads, max_q, max_kv, 0);  // a window only takes parts away
+    const Plan p = make_plan(seqs, q_heads, kv_heads, dim, max_q, max_kv, 0);  // a window only takes parts away
     return p.sp.splits > 1 ? tokens * q_heads * p.sp.splits * (dim + 1) * 4 : 0;
 }
 
-int64_t attention_groups(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t max_q, int64_t max_kv) {
-    const Plan p = make_plan(seqs, q_heads, kv_heads, max_q, max_kv, 0);
-    return seqs * kv_heads * p.sp.tiles * p.sp.splits;
+int64_t attention_groups(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t max_q, int64_t max_kv) {
+    return make_plan(seqs, q_heads, kv_heads, dim, max_q, max_kv, 0).groups;
 }
 
 hipError_t launch_attention(const AttentionArgs &a, void *work, hipStream_t s, const char **kernel) {
-    Plan p = make_plan(a.t.seqs, a.q_heads, a.t.heads, a.max_q, a.max_kv, a.window);
+    Plan p = make_plan(a.t.seqs, a.q_heads, a.t.heads, a.t.dim, a.max_q, a.max_kv, a.window);
     p.sp.group = a.q_heads / a.t.heads;
     p.sp.by_splits = Divider::of(p.sp.splits), p.sp.by_tiles = Divider::of(p.sp.tiles);
     p.sp.by_heads = Divider::of(a.t.heads), p.sp.by_group = Divider::of(p.sp.group);

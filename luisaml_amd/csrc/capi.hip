@@ -974,7 +974,7 @@ int lcml_fp8_attention(const void *q, int q_dtype, int64_t tokens, int64_t q_hea
     // that by far
     const int64_t most = (int64_t)1 << 24;
     if (max_q * q_heads / kv_heads > most * 16 || seqs * kv_heads > most ||
-        lcml::attention_groups(seqs, q_heads, kv_heads, max_q, max_kv) >= most)
+        lcml::attention_groups(seqs, q_heads, kv_heads, head_dim, max_q, max_kv) >= most)
         return fail(LCML_ERR_UNSUPPORTED, "%s: seqs=%lld max_q=%lld q_heads=%lld exceeds one launch", fn,
                     (long long)seqs, (long long)max_q, (long long)q_heads);
     const int64_t need = lcml::attention_workspace(tokens, seqs, q_heads, kv_heads, head_dim, max_q, max_kv);

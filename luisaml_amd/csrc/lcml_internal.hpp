@@ -145,7 +145,7 @@ hipError_t launch_kv_read(const KvTokens &t, int64_t max_q, void *k, void *v, bo
 // workspace bytes, workgroups, and a call (work: that many bytes)
 int64_t attention_workspace(int64_t tokens, int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim,
                             int64_t max_q, int64_t max_kv);
-int64_t attention_groups(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t max_q, int64_t max_kv);
+int64_t attention_groups(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t max_q, int64_t max_kv);
 hipError_t launch_attention(const AttentionArgs &a, void *work, hipStream_t s, const char **kernel);
 
 // A kernel's dynamic-LDS limit (hipFuncSetAttribute) is per device: set it

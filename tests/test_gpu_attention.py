@@ -212,3 +212,67 @@ def test_cache_past_32_bit_offsets(dev):
         outs.append(capi.attention(q[-1:], *c, *one, 1, n, D ** -0.5))
     torch.cuda.synchronize()
     assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3]) and outs[0].abs().sum() > 0
+
+
+# A max_q far above the true one takes the kernel for many rows.
+MANY = 1 << 15
+
+
+def many(dev, *args, **kw):
+    capi.kernel_trace()
+    got = run(dev, *args, max_q=MANY, **kw)
+    assert any("attention_many" in k for k in capi.kernel_trace())
+    return got
+
+
+@pytest.mark.parametrize("T,H,G,D", [(16, 2, 4, 128), (32, 1, 1, 64), (64, 2, 7, 128), (16, 1, 2, 80), (128, 1, 16, 64),
+                                     (256, 1, 8, 256), (16, 1, 4, 192), (32, 2, 4, 16)])
+@pytest.mark.parametrize("qt,ot", [("b", "b"), ("b", "f"), ("f", "f"), ("f", "b")])
+def test_many_rows(dev, T, H, G, D, qt, ot):
+    many(dev, [1, 17, 64, 70, 130, 150], [1, 17, 64, 35, 130, 7], T, H, G, D, qt, ot, seed=T + D + G)
+
+
+@pytest.mark.parametrize("window,causal", [(1, True), (5, True), (40, True), (64, True), (1000, True), (0, False), (20, False)])
+def test_many_rows_window_and_not_causal(dev, window, causal):
+    many(dev, [90, 133, 200, 1], [90, 6, 101, 1], 32, 1, 4, 64, window=window, causal=causal, seed=window)
+
+
+def test_many_rows_that_see_nothing(dev):
+    def holes(q, cache, table):
+        t = table.copy()
+        t[4, :], t[5, 1], t[6, 0] = -1, 10 ** 6, -5
+        return t[:, :4]
+    got = many(dev, [0, 3, 0, 20, 30, 60, 90], [1, 8, 4, 0, 2, 3, 33], 16, 2, 2, 64, seed=1, change=holes)
+    assert (got[:1] == 0).all() and (got[1:6] == 0).all() and not (got[6:9] == 0).any()
+
+
+@pytest.mark.parametrize("ot", ["b", "f"])
+def test_many_rows_scales_far_apart_and_large_scores(dev, ot):
+    many(dev, [100, 300], [50, 50], 16, 1, 4, 64, "b", ot, seed=9, spread=1e8)
+    many(dev, [100, 300], [50, 50], 16, 1, 4, 64, "b", ot, seed=9, q_scale=40.0)
+    many(dev, [100, 300], [50, 50], 16, 1, 4, 64, "b", ot, seed=9, q_scale=1e-6)
+
+
+@pytest.mark.parametrize("D", [64, 80, 256])
+def test_many_rows_infinite_and_nan_queries_and_codes(dev, D):
+    def change(q, cache, table):
+        q[0, 0, 3] = np.nan
+        q[0, 1, :] = 0.0
+        cache.codes[1][table[1, 1], :, 2, 5] = kc.NAN_CODE  # position 18 of sequence 1
+        return table
+    got = many(dev, [60, 60], [40, 40], 16, 1, 4, D, seed=2, change=change, window=0)
+    assert np.isnan(got[0, 0]).all() and not np.isnan(got[0, 1]).any()
+    assert np.isnan(got[-1, :, 5]).all() and not np.isnan(got[-1, :, 6]).any()
+    got = many(dev, [60, 60], [40, 40], 16, 1, 4, D, seed=2, change=change, window=20)
+    assert not np.isnan(got[-1]).any()
+
+
+@pytest.mark.parametrize("ot", ["b", "f"])
+@pytest.mark.parametrize("n,D,kernel", [(700, 64, "attention_few, attention_join"), (130, 64, "attention_few, attention_join"),
+                                        (9, 64, "attention_few, attention_join"), (700, 128, "attention_many, attention_join")])
+def test_long_axis_split_and_joined(dev, n, D, kernel, ot):
+    """Parts of many rows and of few, joined a workgroup a row and many rows a
+    workgroup."""
+    capi.kernel_trace()
+    run(dev, [3000, 1000], [n, min(n, 100)], 64, 1, 4, D, "b", ot, seed=n)
+    assert kernel in ", ".join(capi.kernel_trace())
