@@ -1025,9 +1025,10 @@ Plan divide(bool few, int64_t pairs, int64_t rows, int64_t span) {
     const int64_t groups = pairs * p.sp.tiles, steps = (span + 63) / 64;
     // Few rows: 512 workgroups of a step for each wavefront at least, and up to
     // 2048 of four steps, so that ragged lengths even out (4096: 1 x 32000 28 us
-    // against 20).  Many rows: parts of 32 steps up to two workgroups a CU, of
+    // against 20).  Many rows: parts of 15 steps up to two workgroups a CU, of
     // eight up to one, as joining them reads and writes every result again in
-    // fp32.
+    // fp32 (3 x 383 x 5292 in three parts 97 us, in two 135; 1 x 400 x 4000 in four
+    // 60, in two 73; 1 x 1500 x 1500, 24 steps, in two 66, in one 51).
     int64_t splits;
     if (few) {
         const int64_t fine = (steps + 4 * kFewWaves - 1) / (4 * kFewWaves), coarse = (steps + kFewWaves - 1) / kFewWaves;
@@ -1038,7 +1039,7 @@ Plan divide(bool few, int64_t pairs, int64_t rows, int64_t span) {
         // joining costs a launch: not for two steps of a wavefront, nor four on a full GPU
         if (steps <= 2 * kFewWaves || (groups >= 256 && steps <= 4 * kFewWaves)) splits = 1;
     } else {
-        const int64_t two = 512 / groups, one = 256 / groups, coarse = steps / 32, fine = steps / 8;
+        const int64_t two = (512 + groups / 2) / groups, one = 256 / groups, coarse = steps / 15, fine = steps / 8;
         splits = two < coarse ? two : coarse;
         const int64_t least = one < fine ? one : fine;
         splits = splits > least ? splits : least;
