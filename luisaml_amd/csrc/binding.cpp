@@ -130,6 +130,7 @@ Cache cache(Args a) {
     need(table.scalar_type() == at::kInt && table.dim() == 2 && (table.stride(1) == 1 || table.size(1) <= 1),
          "block_table: int32 [seqs, columns] with contiguous rows is expected");
     const int64_t seqs = table.size(0), cols = table.size(1);
+    need(seqs <= 1 || table.stride(0) >= cols, "block_table: rows that do not overlap are expected (an expanded table's do)");
     need(len.scalar_type() == at::kInt && len.numel() == seqs && len.is_contiguous(), "kv_len: contiguous int32 [seqs] is expected");
     need(cu.scalar_type() == at::kInt && cu.numel() == seqs + 1 && cu.is_contiguous(), "cu_q: contiguous int32 [seqs + 1] is expected");
     return Cache{static_cast<uint8_t *>(k.data_ptr()), static_cast<uint8_t *>(v.data_ptr()), static_cast<float *>(ks.data_ptr()),
