@@ -3,6 +3,11 @@
 torch supplies device memory and the current HIP stream; every call goes
 straight to the gfx950 kernels of liblcml_fp8.so.  There is no fallback:
 if the library is missing or a call fails, an exception is raised.
+
+A call with `stream=` (a torch stream or a raw handle) runs there, and what it
+allocates itself comes from that stream's pool, as under
+torch.cuda.stream(stream); ordering it after the inputs' producers and before
+the results' readers is the caller's.
 """
 from __future__ import annotations
 
@@ -151,6 +156,22 @@ def _stream(stream=None):
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else stream
 
 
+def _empty(shape, dtype, device, stream):
+    """A new tensor for a call on `stream`.  On a stream other than the current
+    one it comes from that stream's pool, as under torch.cuda.stream(stream):
+    memory of the current stream's pool may still be in use there, and would be
+    handed out there again while the call's kernels run.  The current stream,
+    whose program takes the result, is recorded."""
+    if stream is None or device.type != "cuda" or _stream(stream) == _stream():
+        return torch.empty(shape, dtype=dtype, device=device)
+    s = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(_stream(stream), device=device)
+    here = torch.cuda.current_stream(device)
+    with torch.cuda.stream(s):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    t.record_stream(here)
+    return t
+
+
 # ----------------------------------------------------------- Q / DQ ---------
 
 def _axis_view(shape, axis, nscale):
@@ -175,7 +196,7 @@ def quantize(x: torch.Tensor, scale: torch.Tensor, axis: int = 1, out: torch.Ten
     """QuantizeLinear fp32 -> E4M3 (uint8 tensor)."""
     assert x.dtype == torch.float32 and x.is_contiguous()
     scale = scale.reshape(-1)
-    y = out if out is not None else torch.empty(x.shape, dtype=torch.uint8, device=x.device)
+    y = out if out is not None else _empty(x.shape, torch.uint8, x.device, stream)
     o, a, i = _axis_view(tuple(x.shape), axis, scale.numel())
     _check(lib().lcml_fp8_quantize(_ptr(x), _ptr(y), o, a, i, _ptr(scale), _stream(stream)))
     return y
@@ -186,7 +207,7 @@ def dequantize(q: torch.Tensor, scale: torch.Tensor, axis: int = 1, out: torch.T
     """DequantizeLinear E4M3 (uint8) -> fp32."""
     assert q.dtype == torch.uint8 and q.is_contiguous()
     scale = scale.reshape(-1)
-    y = out if out is not None else torch.empty(q.shape, dtype=torch.float32, device=q.device)
+    y = out if out is not None else _empty(q.shape, torch.float32, q.device, stream)
     o, a, i = _axis_view(tuple(q.shape), axis, scale.numel())
     _check(lib().lcml_fp8_dequantize(_ptr(q), _ptr(y), o, a, i, _ptr(scale), _stream(stream)))
     return y
@@ -197,10 +218,10 @@ def quantize_dynamic(x: torch.Tensor, out: torch.Tensor | None = None,
                      stream=None):
     """Dynamic per-tensor quantisation; returns (codes, scale[1])."""
     assert x.dtype == torch.float32 and x.is_contiguous()
-    y = out if out is not None else torch.empty(x.shape, dtype=torch.uint8, device=x.device)
-    s = scale_out if scale_out is not None else torch.empty(1, dtype=torch.float32, device=x.device)
+    y = out if out is not None else _empty(x.shape, torch.uint8, x.device, stream)
+    s = scale_out if scale_out is not None else _empty(1, torch.float32, x.device, stream)
     if workspace is None and x.numel() > DYNAMIC_SMALL_MAX:
-        workspace = torch.empty(DYNAMIC_WORKSPACE_BYTES, dtype=torch.uint8, device=x.device)
+        workspace = _empty(DYNAMIC_WORKSPACE_BYTES, torch.uint8, x.device, stream)
     _check(lib().lcml_fp8_quantize_dynamic(_ptr(x), _ptr(y), x.numel(), _ptr(s), _ptr(workspace),
                                            _stream(stream)))
     return y, s
@@ -208,7 +229,7 @@ def quantize_dynamic(x: torch.Tensor, out: torch.Tensor | None = None,
 
 def amax(x: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     assert x.dtype == torch.float32 and x.is_contiguous()
-    o = out if out is not None else torch.empty(1, dtype=torch.float32, device=x.device)
+    o = out if out is not None else _empty(1, torch.float32, x.device, stream)
     _check(lib().lcml_fp8_amax(_ptr(x), x.numel(), _ptr(o), _stream(stream)))
     return o
 
@@ -223,14 +244,14 @@ def pack_weight(w: torch.Tensor, w_is_nk: bool, stream=None) -> torch.Tensor:
     """Pack an E4M3 weight ([K,N], or [N,K] when w_is_nk) into MFMA panels."""
     assert w.dtype == torch.uint8 and w.is_contiguous() and w.dim() == 2
     N, K = (w.shape[0], w.shape[1]) if w_is_nk else (w.shape[1], w.shape[0])
-    p = torch.empty(packed_weight_bytes(K, N), dtype=torch.uint8, device=w.device)
+    p = _empty(packed_weight_bytes(K, N), torch.uint8, w.device, stream)
     _check(lib().lcml_fp8_pack_weight(_ptr(w), K, N, int(w_is_nk), _ptr(p), _stream(stream)))
     return p
 
 
 def unpack_weight(p: torch.Tensor, K: int, N: int, w_is_nk: bool, stream=None) -> torch.Tensor:
     shape = (N, K) if w_is_nk else (K, N)
-    w = torch.empty(shape, dtype=torch.uint8, device=p.device)
+    w = _empty(shape, torch.uint8, p.device, stream)
     _check(lib().lcml_fp8_unpack_weight(_ptr(p), K, N, int(w_is_nk), _ptr(w), _stream(stream)))
     return w
 
@@ -254,7 +275,7 @@ def gemm(a: torch.Tensor, a_scale: torch.Tensor, b_packed: torch.Tensor, b_scale
     """W8A8 GEMM: a [M,K] E4M3 (uint8) x packed E4M3 weight -> [M,N] fp32/bf16."""
     assert a.dtype == torch.uint8 and a.dim() == 2 and a.stride(1) == 1
     M = a.shape[0]
-    y = out if out is not None else torch.empty((M, N), dtype=out_dtype, device=a.device)
+    y = out if out is not None else _empty((M, N), out_dtype, a.device, stream)
     ydt = _DTYPE_CODE.get(y.dtype, 0)
     cc, nd, c0, c1 = _c_args(c)
     per_ch = int(b_scale.numel() > 1)
@@ -275,7 +296,7 @@ def gemm_dynamic(x: torch.Tensor, b_packed: torch.Tensor, b_scale: torch.Tensor,
     used when the fused small-M kernel does not apply."""
     assert x.dtype == torch.float32 and x.dim() == 2 and x.stride(1) == 1
     M = x.shape[0]
-    y = out if out is not None else torch.empty((M, N), dtype=out_dtype, device=x.device)
+    y = out if out is not None else _empty((M, N), out_dtype, x.device, stream)
     ydt = _DTYPE_CODE.get(y.dtype, 0)
     cc, nd, c0, c1 = _c_args(c)
     per_ch = int(b_scale.numel() > 1)
@@ -283,7 +304,7 @@ def gemm_dynamic(x: torch.Tensor, b_packed: torch.Tensor, b_scale: torch.Tensor,
     # two-step path, whose size the (never fusing) MFMA kernel's query gives
     need = lib().lcml_fp8_gemm_dynamic_workspace_bytes(M, K, int(kernel) if x.data_ptr() % 16 == 0 else KERNEL_MFMA)
     if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+        workspace = _empty(need, torch.uint8, x.device, stream)
     ws_bytes = workspace.numel() if workspace is not None else 0
     _check(lib().lcml_fp8_gemm_dynamic(M, N, K, _ptr(x), x.stride(0), _ptr(b_packed), _ptr(b_scale), per_ch,
                                        float(alpha), _ptr(cc), nd, c0, c1, float(beta), int(act), _ptr(y), ydt,
@@ -308,13 +329,13 @@ def gemm_dynamic_ex(x: torch.Tensor, b_packed: torch.Tensor, b_scale: torch.Tens
     (y, count of y partials written, or 0)."""
     assert x.dtype == torch.float32 and x.dim() == 2 and x.stride(1) == 1
     M = x.shape[0]
-    y = out if out is not None else torch.empty((M, N), dtype=out_dtype, device=x.device)
+    y = out if out is not None else _empty((M, N), out_dtype, x.device, stream)
     ydt = _DTYPE_CODE.get(y.dtype, 0)
     cc, nd, c0, c1 = _c_args(c)
     per_ch = int(b_scale.numel() > 1)
     need = lib().lcml_fp8_gemm_dynamic_workspace_bytes(M, K, int(kernel) if x.data_ptr() % 16 == 0 else KERNEL_MFMA)
     if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+        workspace = _empty(need, torch.uint8, x.device, stream)
     ws_bytes = workspace.numel() if workspace is not None else 0
     xp, xn = (x_amax[0], int(x_amax[1])) if x_amax is not None else (None, 0)
     npart = C.c_int(0)
@@ -334,11 +355,10 @@ def quantize_nhwc(x: torch.Tensor, scale: torch.Tensor | None = None, out: torch
     Returns (codes [n, h, w, c], scale[1])."""
     assert x.dtype == torch.float32 and x.is_contiguous() and x.dim() == 4
     n, c, h, w = x.shape
-    y = out if out is not None else torch.empty((n, h, w, c), dtype=torch.uint8, device=x.device)
+    y = out if out is not None else _empty((n, h, w, c), torch.uint8, x.device, stream)
     if scale is None:
-        s = scale_out if scale_out is not None else torch.empty(1, dtype=torch.float32, device=x.device)
-        ws = workspace if workspace is not None else torch.empty(DYNAMIC_WORKSPACE_BYTES, dtype=torch.uint8,
-                                                                 device=x.device)
+        s = scale_out if scale_out is not None else _empty(1, torch.float32, x.device, stream)
+        ws = workspace if workspace is not None else _empty(DYNAMIC_WORKSPACE_BYTES, torch.uint8, x.device, stream)
         _check(lib().lcml_fp8_quantize_nhwc(_ptr(x), _ptr(y), n, c, h, w, None, _ptr(s), _ptr(ws), _stream(stream)))
         return y, s
     _check(lib().lcml_fp8_quantize_nhwc(_ptr(x), _ptr(y), n, c, h, w, _ptr(scale), None, None, _stream(stream)))
@@ -349,8 +369,7 @@ def pack_conv_weight(w: torch.Tensor, group: int = 1, stream=None) -> torch.Tens
     """Pack E4M3 conv weights [cout, cin/group, kh, kw] for conv2d."""
     assert w.dtype == torch.uint8 and w.is_contiguous() and w.dim() == 4
     cout, cin_g, kh, kw = w.shape
-    p = torch.empty(lib().lcml_fp8_packed_conv_weight_bytes(cout, cin_g, kh, kw, group), dtype=torch.uint8,
-                    device=w.device)
+    p = _empty(lib().lcml_fp8_packed_conv_weight_bytes(cout, cin_g, kh, kw, group), torch.uint8, w.device, stream)
     _check(lib().lcml_fp8_pack_conv_weight(_ptr(w), cout, cin_g, kh, kw, group, _ptr(p), _stream(stream)))
     return p
 
@@ -368,7 +387,7 @@ def conv2d(x_nhwc: torch.Tensor, x_scale: torch.Tensor, w_packed: torch.Tensor, 
         out_hw = ((h + 2 * pads[0] - dilations[0] * (kh - 1) - 1) // strides[0] + 1,
                   (w + 2 * pads[1] - dilations[1] * (kw - 1) - 1) // strides[1] + 1)
     oh, ow = out_hw
-    y = out if out is not None else torch.empty((n, cout, oh, ow), dtype=out_dtype, device=x_nhwc.device)
+    y = out if out is not None else _empty((n, cout, oh, ow), out_dtype, x_nhwc.device, stream)
     per_ch = int(w_scale.numel() > 1)
     _check(lib().lcml_fp8_conv2d(_ptr(x_nhwc), _ptr(x_scale), n, c, h, w, _ptr(w_packed), _ptr(w_scale), per_ch,
                                  cout, kh, kw, strides[0], strides[1], pads[0], pads[1], dilations[0], dilations[1],
@@ -386,7 +405,7 @@ def conv2d_f32(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
     if out_hw is None:
         out_hw = ((h + 2 * pads[0] - dilations[0] * (kh - 1) - 1) // strides[0] + 1,
                   (wd + 2 * pads[1] - dilations[1] * (kw - 1) - 1) // strides[1] + 1)
-    y = torch.empty((n, cout, *out_hw), dtype=torch.float32, device=x.device)
+    y = _empty((n, cout, *out_hw), torch.float32, x.device, stream)
     _check(lib().lcml_fp8_conv2d_f32(_ptr(x), _ptr(w), _ptr(bias), _ptr(y), n, c, h, wd, cout, kh, kw, strides[0],
                                      strides[1], pads[0], pads[1], dilations[0], dilations[1], group, out_hw[0],
                                      out_hw[1], int(act), _stream(stream)))
@@ -400,7 +419,7 @@ def gemm_w8a32(a: torch.Tensor, b_packed: torch.Tensor, b_scale: torch.Tensor, N
     """W8A32 linear: a [M,K] fp32 x packed E4M3 weight -> [M,N]."""
     assert a.dtype == torch.float32 and a.dim() == 2 and a.stride(1) == 1
     M = a.shape[0]
-    y = out if out is not None else torch.empty((M, N), dtype=out_dtype, device=a.device)
+    y = out if out is not None else _empty((M, N), out_dtype, a.device, stream)
     ydt = _DTYPE_CODE.get(y.dtype, 0)
     cc, nd, c0, c1 = _c_args(c)
     per_ch = int(b_scale.numel() > 1)
@@ -416,7 +435,7 @@ def sgemm(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor | None = None, alpha
     assert a.dtype == torch.float32 and b.dtype == torch.float32 and a.is_contiguous() and b.is_contiguous()
     M, K = (a.shape[1], a.shape[0]) if trans_a else (a.shape[0], a.shape[1])
     N = b.shape[0] if trans_b else b.shape[1]
-    y = torch.empty((M, N), dtype=torch.float32, device=a.device)
+    y = _empty((M, N), torch.float32, a.device, stream)
     cc, nd, c0, c1 = _c_args(c)
     _check(lib().lcml_fp8_sgemm(M, N, K, _ptr(a), a.shape[1], int(trans_a), _ptr(b), b.shape[1], int(trans_b),
                                 float(alpha), _ptr(cc), nd, c0, c1, float(beta), int(act), _ptr(y), DTYPE_FLOAT,
@@ -426,7 +445,7 @@ def sgemm(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor | None = None, alpha
 
 def activation(x: torch.Tensor, act: int, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     assert x.dtype == torch.float32 and x.is_contiguous()
-    y = out if out is not None else torch.empty_like(x)
+    y = out if out is not None else _empty(x.shape, x.dtype, x.device, stream)
     _check(lib().lcml_fp8_activation(_ptr(x), _ptr(y), x.numel(), int(act), _stream(stream)))
     return y
 
@@ -446,7 +465,7 @@ def cast(x: torch.Tensor, x_dtype: int, y_dtype: int, out: torch.Tensor | None =
     DTYPE_FLOAT8E5M2 (uint8 code tensors)."""
     assert x.is_contiguous()
     tdt = torch.float32 if y_dtype == DTYPE_FLOAT else torch.uint8
-    y = out if out is not None else torch.empty(x.shape, dtype=tdt, device=x.device)
+    y = out if out is not None else _empty(x.shape, tdt, x.device, stream)
     _check(lib().lcml_fp8_cast(_ptr(x), int(x_dtype), _ptr(y), int(y_dtype), x.numel(), _stream(stream)))
     return y
 
@@ -456,7 +475,7 @@ def quantize_e5m2(x: torch.Tensor, scale: torch.Tensor, axis: int = 1, saturate:
     """QuantizeLinear fp32 -> E5M2 codes (uint8)."""
     assert x.dtype == torch.float32 and x.is_contiguous()
     scale = scale.reshape(-1)
-    y = out if out is not None else torch.empty(x.shape, dtype=torch.uint8, device=x.device)
+    y = out if out is not None else _empty(x.shape, torch.uint8, x.device, stream)
     o, a, i = _axis_view(tuple(x.shape), axis, scale.numel())
     _check(lib().lcml_fp8_quantize_e5m2(_ptr(x), _ptr(y), o, a, i, _ptr(scale), int(saturate), _stream(stream)))
     return y
@@ -466,7 +485,7 @@ def dequantize_e5m2(q: torch.Tensor, scale: torch.Tensor, axis: int = 1, out: to
                     stream=None) -> torch.Tensor:
     assert q.dtype == torch.uint8 and q.is_contiguous()
     scale = scale.reshape(-1)
-    y = out if out is not None else torch.empty(q.shape, dtype=torch.float32, device=q.device)
+    y = out if out is not None else _empty(q.shape, torch.float32, q.device, stream)
     o, a, i = _axis_view(tuple(q.shape), axis, scale.numel())
     _check(lib().lcml_fp8_dequantize_e5m2(_ptr(q), _ptr(y), o, a, i, _ptr(scale), _stream(stream)))
     return y
@@ -478,7 +497,7 @@ def binary(op: int, a: torch.Tensor, b: torch.Tensor, dtype: int, out: torch.Ten
     or DTYPE_FLOAT8E4M3FN / DTYPE_FLOAT8E5M2 (uint8 code tensors)."""
     assert a.is_contiguous() and b.is_contiguous()
     ys = tuple(torch.broadcast_shapes(a.shape, b.shape))
-    y = out if out is not None else torch.empty(ys, dtype=a.dtype, device=a.device)
+    y = out if out is not None else _empty(ys, a.dtype, a.device, stream)
     sh = lambda t: (C.c_int64 * max(1, len(t)))(*t)
     _check(lib().lcml_fp8_binary(int(op), int(dtype), _ptr(a), sh(tuple(a.shape)), a.dim(), _ptr(b),
                                  sh(tuple(b.shape)), b.dim(), _ptr(y), sh(tuple(y.shape)), y.dim(), _stream(stream)))
@@ -513,15 +532,15 @@ def rms_norm(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual: torch.T
     SCALE_STATIC takes scale[1]; SCALE_TENSOR gives it; SCALE_ROW gives [M].
     Returns (codes uint8 [M,H], scale, h or None)."""
     if residual is not None and residual_out is None:
-        residual_out = torch.empty(residual.shape, dtype=residual.dtype, device=x.device)
+        residual_out = _empty(residual.shape, residual.dtype, x.device, stream)
     if out is None:
-        out = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
+        out = _empty(x.shape, torch.uint8, x.device, stream)
     if scale is None:
         if mode == SCALE_STATIC:
             raise ValueError("SCALE_STATIC takes a scale")
-        scale = torch.empty(x.shape[0] if mode == SCALE_ROW else 1, dtype=torch.float32, device=x.device)
+        scale = _empty(x.shape[0] if mode == SCALE_ROW else 1, torch.float32, x.device, stream)
     if mode == SCALE_TENSOR and workspace is None and x.shape[0] > 1:
-        workspace = torch.empty(lib().lcml_fp8_rms_norm_workspace_bytes(*x.shape, mode), dtype=torch.uint8, device=x.device)
+        workspace = _empty(lib().lcml_fp8_rms_norm_workspace_bytes(*x.shape, mode), torch.uint8, x.device, stream)
     _check(_binding().rms_norm(x, gamma, eps, residual, residual_out, mode, scale, out, workspace, _stream(stream)))
     return out, scale, residual_out
 
@@ -565,12 +584,12 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_s
     head_dim] (fp32/bf16) are the last tokens of their sequences, which the
     cache already holds.  window > 0: only the last `window` positions."""
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
+        out = _empty(q.shape, out_dtype or q.dtype, q.device, stream)
     if workspace is None:
         tokens, heads, dim = q.shape
         need = _attention_workspace(tokens, kv_len.numel(), heads, k_cache.shape[1], dim, max_q, max_kv)
         if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            workspace = _empty(need, torch.uint8, q.device, stream)
     _check(_binding().attention(q, out, k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q, max_q, max_kv,
                                 scale, causal, window, workspace, _stream(stream)))
     return out
