@@ -16,7 +16,10 @@
 //   * K's page scale multiplies the scores, V's the codes as they are widened:
 //     a power of two below the largest V scale so far (the widening
 //     instruction takes the factor), which multiplies the end result; where
-//     that largest one grows, the sums are scaled down.
+//     that largest one grows, the sums are scaled down.  All of that is exact
+//     while the V scales are within 2^kSpread of each other; from the step on
+//     that goes beyond, each 16-token block (which has one scale) is weighted
+//     by its own maximum, multiplied by itself and added in fp32.
 // Both kernels compute S^T = K Q^T and O^T = V^T P^T, so that a query row is a
 // lane's column in all of S, P and O: maximum, sum and scaling are a lane's own
 // but for one exchange between lanes, and S^T's accumulators are P^T's operand
@@ -90,6 +93,38 @@ __device__ inline float query_factor(float amax) {
 }
 
 __device__ inline float reciprocal(float f) { return bits_f32((254u << 23) - f32_bits(f)); }  // of a power of two
+
+// The V scales of the steps so far, as their bits: the largest, and the
+// smallest.  With codes down to 2^-9 relative to the largest scale, fp16 would
+// hold all of them up to a spread of 2^22; 2^10 also keeps what the weights'
+// own fp16 loses (2^-31 of the largest weight, times the largest values) below
+// a bf16 result's rounding where only values of the smallest scale count.
+// Pages of one head are seldom further apart than 2^4.
+constexpr int kSpread = 10;
+struct Scales {
+    uint32_t top = 0, low = 0x7f800000u;
+    __device__ inline void take(const uint32_t (&vs)[4]) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            top = vs[q] > top ? vs[q] : top;
+            low = vs[q] && vs[q] < low ? vs[q] : low;
+        }
+    }
+    __device__ inline bool apart() const { return (int)(top >> 23) - (int)(low >> 23) > kSpread; }
+};
+
+// How a block of maximum mb and sum lb joins a row of maximum m and sum l whose
+// result is already divided by l: the factors of the row's result and of the
+// block's products.
+__device__ inline void join_block(float &m, float &l, float mb, float lb, float *keep, float *add) {
+    const float top = fmaxf(m, mb);
+    const float fa = m == top ? l : l * __builtin_amdgcn_exp2f(m - top);
+    const float wb = mb == top ? 1.0f : __builtin_amdgcn_exp2f(mb - top), fb = lb * wb;
+    m = top, l = fa + fb;
+    const float inv = 1.0f / l;
+    *keep = fb == 0.0f ? 1.0f : fa * inv;  // nothing to add: the row as it is
+    *add = fb == 0.0f ? 0.0f : wb * inv;
+}
 
 // vs / vref times 2^kVBits, powers of two as their bits
 __device__ inline float v_ratio(uint32_t vs, uint32_t vref) {
@@ -368,13 +403,11 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
             for (int c = 0; c < 4; ++c) o[j][c] *= f;
     };
 
-    // one step; MASKED: some rows do not see all of its tokens, and V's NaN codes
-    // count as zeros for now
     bool nan = false;
     uint32_t ks[4], vs[4];
-    auto step = [&](int32_t k, int32_t tok, auto masked) {
-        constexpr bool MASKED = decltype(masked)::value;
-        f4 t[4];
+    Scales scales;
+    // one step's scores; then the next one's K is on its way
+    auto products = [&](int32_t k, f4 (&t)[4]) {
 #pragma unroll
         for (int sb = 0; sb < 4; ++sb) {
             t[sb] = f4{0.f, 0.f, 0.f, 0.f};
@@ -392,39 +425,47 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
             if (((k + 1) & 15) == 0) find(k + 1);
             issue_k(k + 1);
         }
-        if constexpr (MASKED) {
-            uint32_t bad = 0;
-            const uint32_t from = tok + 4 * g - lo;
+    };
+    // hides what the lane's row does not see; V's NaN codes count as zeros for now
+    auto mask = [&](int32_t tok, f4 (&t)[4]) {
+        uint32_t bad = 0;
+        const uint32_t from = tok + 4 * g - lo;
+#pragma unroll
+        for (int sb = 0; sb < 4; ++sb) {
+            const uint32_t span = vs[sb] ? hi - lo : 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[sb][i] = from + 16 * sb + i < span ? t[sb][i] : -kInf;
+#pragma unroll
+            for (int j = 0; j < DC; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) bad |= nan_bits(vv[sb][j][c]);
+        }
+        if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {  // NaN codes: of tokens that a row sees?
+            bad = 0;
+            const uint32_t all = tok + 4 * g - lo_min;
 #pragma unroll
             for (int sb = 0; sb < 4; ++sb) {
-                const uint32_t span = vs[sb] ? hi - lo : 0;
+                const uint32_t span = vs[sb] ? hi_max - lo_min : 0;
+                uint32_t seen = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) t[sb][i] = from + 16 * sb + i < span ? t[sb][i] : -kInf;
+                for (int i = 0; i < 4; ++i) seen |= all + 16 * sb + i < span ? 0x80u << (8 * i) : 0u;
 #pragma unroll
                 for (int j = 0; j < DC; ++j)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) bad |= nan_bits(vv[sb][j][c]);
+                    for (int y = 0; y < 4; ++y) {
+                        bad |= nan_bits(vv[sb][j][y]) & seen;
+                        vv[sb][j][y] = without_nan(vv[sb][j][y]);
+                    }
             }
-            if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {  // NaN codes: of tokens that a row sees?
-                bad = 0;
-                const uint32_t all = tok + 4 * g - lo_min;
-#pragma unroll
-                for (int sb = 0; sb < 4; ++sb) {
-                    const uint32_t span = vs[sb] ? hi_max - lo_min : 0;
-                    uint32_t seen = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) seen |= all + 16 * sb + i < span ? 0x80u << (8 * i) : 0u;
-#pragma unroll
-                    for (int j = 0; j < DC; ++j)
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            bad |= nan_bits(vv[sb][j][y]) & seen;
-                            vv[sb][j][y] = without_nan(vv[sb][j][y]);
-                        }
-                }
-                nan = nan || __builtin_amdgcn_ballot_w64(bad != 0) != 0;
-            }
+            nan = nan || __builtin_amdgcn_ballot_w64(bad != 0) != 0;
         }
+    };
+    // one step; MASKED: some rows do not see all of its tokens
+    auto step = [&](int32_t k, int32_t tok, auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+        f4 t[4];
+        products(k, t);
+        if constexpr (MASKED) mask(tok, t);
         float mx = m, c[4];
 #pragma unroll
         for (int sb = 0; sb < 4; ++sb) {
@@ -440,13 +481,10 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
             scale_o(f);
             m = mx > m ? mx : m;
         }
-        uint32_t top = vs[0] > vs[1] ? vs[0] : vs[1];
-        top = vs[2] > top ? vs[2] : top;
-        top = vs[3] > top ? vs[3] : top;
-        if (top > vref) {
-            const int e = (int)(vref >> 23) - (int)(top >> 23) + 127;
+        if (scales.top > vref) {
+            const int e = (int)(vref >> 23) - (int)(scales.top >> 23) + 127;  // vref 0: sums of 0
             scale_o(bits_f32((uint32_t)(e < 0 ? 0 : e) << 23));
-            vref = top;
+            vref = scales.top;
         }
         const float mm = weight_base<NP>(m);
         h8 p[NP][2];
@@ -487,24 +525,85 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
                 }
         if (k + 1 < mine) issue_v(k + 1);
     };
+    // one step where V's scales are far apart; o is the result so far, divided
+    // by l, and l the row's whole sum
+    auto step_apart = [&](int32_t k, int32_t tok) {
+        f4 t[4];
+        products(k, t);
+        mask(tok, t);
+#pragma unroll
+        for (int sb = 0; sb < 4; ++sb) {
+            if (!vs[sb]) continue;
+            const float c = cq * bits_f32(ks[sb]), s = bits_f32(vs[sb]);
+            const float b = fmaxf(fmaxf(t[sb][0], t[sb][1]), fmaxf(t[sb][2], t[sb][3]));
+            const float mb = max_over_quarters(b == -kInf ? b : b * c), mm = weight_base<NP>(mb);
+            float lb = 0.0f, keep, add;
+            h8 p[NP];  // this block's weights, and zeros for the operand's other four
+#pragma unroll
+            for (int q = 0; q < NP; ++q) p[q] = h8{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                f2 e;
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const float x = t[sb][i + y];
+                    e[y] = weight_scale<NP>(__builtin_amdgcn_exp2f(x == -kInf ? x : fmaf(x, c, -mm)));
+                }
+                const h2 eh = __builtin_convertvector(e, h2);
+                lb = add_weights<NP>(lb, e, eh);
+                p[0][i] = eh[0], p[0][i + 1] = eh[1];
+                if constexpr (NP == 2) {
+                    const h2 el = __builtin_convertvector(f2{e[0] - (float)eh[0], e[1] - (float)eh[1]}, h2);
+                    p[NP - 1][i] = el[0], p[NP - 1][i + 1] = el[1];
+                }
+            }
+            join_block(m, l, mb, sum_over_quarters(lb), &keep, &add);
+#pragma unroll
+            for (int j = 0; j < DC; ++j)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const h8 va = __builtin_shufflevector(widen4(vv[sb][j][y], 1.0f), h4{0, 0, 0, 0}, 0, 1, 2, 3, 4, 5, 6, 7);
+                    f4 x{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int q = 0; q < NP; ++q) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[q], x, 0, 0, 0);
+                    o[j][y] = o[j][y] * keep + x * add * s;
+                }
+        }
+        if (k + 1 < mine) issue_v(k + 1);
+    };
+    auto scales_of = [&](int32_t k) {
+#pragma unroll
+        for (int sb = 0; sb < 4; ++sb) {
+            ks[sb] = lane_of(blk.ks, (k & 15) * 4 + sb);
+            vs[sb] = lane_of(blk.vs, (k & 15) * 4 + sb);
+        }
+        scales.take(vs);
+    };
     // steps that all rows see whole, in a loop of their own
-    for (int32_t k = 0; k < mine; ++k) {
+    int32_t k = 0;
+    for (; k < mine; ++k) {
         int32_t tok;
         for (; k < mine; ++k) {
             tok = part.start + ((k * NW + wave) << 6);
-#pragma unroll
-            for (int sb = 0; sb < 4; ++sb) {
-                ks[sb] = lane_of(blk.ks, (k & 15) * 4 + sb);
-                vs[sb] = lane_of(blk.vs, (k & 15) * 4 + sb);
-            }
-            if (!(tok >= lo_max && tok + 64 <= hi_min && vs[0] && vs[1] && vs[2] && vs[3])) break;
+            scales_of(k);
+            if (!(tok >= lo_max && tok + 64 <= hi_min && vs[0] && vs[1] && vs[2] && vs[3]) || scales.apart()) break;
             step(k, tok, std::false_type{});
         }
-        if (k < mine) step(k, tok, std::true_type{});
+        if (k >= mine || scales.apart()) break;
+        step(k, tok, std::true_type{});
+    }
+    l = sum_over_quarters(l);
+    const bool apart = k < mine;
+    if (__builtin_expect(apart, 0)) {
+        scale_o(l == 0.0f ? 0.0f : 1.0f / (1 << kVBits) / l);
+        scale_o(bits_f32(vref));
+        for (; k < mine; ++k) {
+            scales_of(k);
+            step_apart(k, part.start + ((k * NW + wave) << 6));
+        }
     }
 
     // join the wavefronts
-    l = sum_over_quarters(l);
     if (g == 0) red_m[wave][r] = m, red_l[wave][r] = l;
     __syncthreads();
     float top = -kInf, sum = 0.0f;
@@ -513,7 +612,9 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
     auto weight = [&](float v) { return v == top ? 1.0f : __builtin_amdgcn_exp2f(v - top); };
 #pragma unroll
     for (int w = 0; w < NW; ++w) sum += red_l[w][r] * weight(red_m[w][r]);
-    scale_o(sum == 0.0f ? 0.0f : weight(m) / sum * (bits_f32(vref) * (1.0f / (1 << kVBits))));
+    // (the scale last: with a factor of the other two it could leave fp32's range)
+    scale_o(sum == 0.0f ? 0.0f : weight(m) / sum * (apart ? l : 1.0f / (1 << kVBits)));
+    if (!apart) scale_o(bits_f32(vref));
 #pragma unroll
     for (int j = 0; j < DC; ++j)
 #pragma unroll
@@ -621,9 +722,10 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
     auto token_of = [&](int32_t k) { return part.start + ((k + (lane >> 2)) << 6) + (lane & 3) * 16; };
     uint32_t ks[4], vs[4], ks_next[4], vs_next[4];
     bool whole, whole_next = false;  // whether every row sees all of a step's tokens
+    Scales scales;                   // of the steps fetched so far, the same for all wavefronts
     // this wavefront's block of step k
     u4 kr[PL], vr[PL];
-    auto fetch = [&](int32_t k) {
+    auto fetch = [&](int32_t k) __attribute__((always_inline)) {
         const int i = (k & 15) * 4;
 #pragma unroll
         for (int q = 0; q < 4; ++q) ks_next[q] = lane_of(blk.ks, i + q), vs_next[q] = lane_of(blk.vs, i + q);
@@ -632,6 +734,7 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
         least = vs_next[2] < least ? vs_next[2] : least;
         least = vs_next[3] < least ? vs_next[3] : least;
         whole_next = tok >= lo_max && tok + 64 <= hi_min && least;
+        scales.take(vs_next);
         const uint64_t at = (lane_of(blk.lo, i + wave) | (uint64_t)lane_of(blk.hi, i + wave) << 32) * (uint64_t)(16 * D);
         const uint8_t *pk = a.k + at, *pv = a.v + at;
 #pragma unroll
@@ -641,12 +744,10 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
             vr[x] = in ? *reinterpret_cast<const u4 *>(pv + (64 * x + lane) * 16) : u4{0, 0, 0, 0};
         }
     };
-    uint32_t vref = 0, vref_next = 0;  // the largest V scale up to a step, the same for all wavefronts
-    auto deposit = [&](int32_t k, int buf) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) vref_next = vs_next[q] > vref_next ? vs_next[q] : vref_next;
+    uint32_t vref = 0;  // the largest V scale up to the step that is worked on
+    auto deposit = [&](int32_t k, int buf) __attribute__((always_inline)) {
         const uint32_t mine = wave == 0 ? vs_next[0] : wave == 1 ? vs_next[1] : wave == 2 ? vs_next[2] : vs_next[3];
-        const float ratio = v_ratio(mine, vref_next);
+        const float ratio = scales.apart() ? 1.0f : v_ratio(mine, scales.top);
         if (__builtin_expect(!whole_next, 0)) {
             // what lies past the last token counts as zeros, and so do NaN codes
             // for now
@@ -723,12 +824,9 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
         for (int t = 0; t < MT; ++t) o[t] *= f;
     };
 
-    // one step's tokens from LDS; MASKED: some rows do not see all of them
-    auto step = [&](int32_t tok, int buf, auto masked) {
-        constexpr bool MASKED = decltype(masked)::value;
+    // one step's scores from LDS; MASKED: some rows do not see all of its tokens
+    auto scores = [&](int32_t tok, int buf, f16v (&t)[2], float (&c)[4], auto masked) __attribute__((always_inline)) {
         const uint8_t *sk = stage_k[buf];
-        const _Float16 *sv = stage_v[buf];
-        f16v t[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
 #pragma unroll
@@ -746,10 +844,9 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
                 }
             }
         }
-        float c[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) c[q] = cq * bits_f32(ks[q]);
-        if constexpr (MASKED) {
+        if constexpr (decltype(masked)::value) {
             const uint32_t from = tok + 4 * h - lo;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -761,6 +858,13 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
                 }
             }
         }
+    };
+    auto step = [&](int32_t tok, int buf, auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+        const _Float16 *sv = stage_v[buf];
+        f16v t[2];
+        float c[4];
+        scores(tok, buf, t, c, masked);
         float mx = m;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -808,23 +912,62 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
                 for (int z = 0; z < NP; ++z) o[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, p[z][q], o[y], 0, 0, 0);
             }
     };
+    // one step where V's scales are far apart (its codes lie in LDS as they are);
+    // o is the result so far, divided by l, and l the row's whole sum
+    auto step_apart = [&](int32_t tok, int buf) __attribute__((always_inline)) {
+        const _Float16 *sv = stage_v[buf];
+        f16v t[2];
+        float c[4];
+        scores(tok, buf, t, c, std::true_type{});
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (!vs[q]) continue;
+            float b = t[q >> 1][(q & 1) * 8], lb = 0.0f, keep, add;
+#pragma unroll
+            for (int i = 1; i < 8; ++i) b = fmaxf(b, t[q >> 1][(q & 1) * 8 + i]);
+            const float mb = max_over_halves(b == -kInf ? b : b * c[q]), mm = weight_base<NP>(mb), s = bits_f32(vs[q]);
+            h8 p[NP];
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                f2 e;
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const float x = t[q >> 1][(q & 1) * 8 + i + y];
+                    e[y] = weight_scale<NP>(__builtin_amdgcn_exp2f(x == -kInf ? x : fmaf(x, c[q], -mm)));
+                }
+                const h2 eh = __builtin_convertvector(e, h2);
+                lb = add_weights<NP>(lb, e, eh);
+                p[0][i] = eh[0], p[0][i + 1] = eh[1];
+                if constexpr (NP == 2) {
+                    const h2 el = __builtin_convertvector(f2{e[0] - (float)eh[0], e[1] - (float)eh[1]}, h2);
+                    p[NP - 1][i] = el[0], p[NP - 1][i + 1] = el[1];
+                }
+            }
+            join_block(m, l, mb, sum_over_halves(lb), &keep, &add);
+#pragma unroll
+            for (int y = 0; y < MT; ++y) {
+                const h8 va = *reinterpret_cast<const h8 *>(sv + q * 16 * DP + h * 8 * DP + (32 * y + r) * 8);
+                f16v x;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+#pragma unroll
+                for (int z = 0; z < NP; ++z) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, p[z], x, 0, 0, 0);
+                o[y] = o[y] * keep + x * add * s;
+            }
+        }
+    };
 
     // around a step: its scales and the next one's loads, and what they brought
-    auto before = [&](int32_t k) {
+    auto before = [&](int32_t k) __attribute__((always_inline)) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) ks[q] = ks_next[q], vs[q] = vs_next[q];
         whole = whole_next;
-        if (vref_next != vref) {
-            const int e = (int)(vref >> 23) - (int)(vref_next >> 23) + 127;
-            scale_o(bits_f32((uint32_t)(e < 0 ? 0 : e) << 23));
-            vref = vref_next;
-        }
         if ((k & 15) == 15) blk = next;
         if (k + 1 < part.steps) fetch(k + 1);
         if ((k & 15) == 0) next_page = find_page(a, b, token_of(k + 16), part.end);
         if ((k & 15) == 4) next = block_of(a, head, token_of(k + 12), next_page);
     };
-    auto after = [&](int32_t k) {
+    auto after = [&](int32_t k) __attribute__((always_inline)) {
         if (k + 1 < part.steps) deposit(k + 1, (k + 1) & 1);
         __syncthreads();
     };
@@ -833,21 +976,39 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
     if (part.steps > 0) deposit(0, 0);
     __syncthreads();
     // steps that all rows see whole, in a loop of their own
-    for (int32_t k = 0; k < part.steps; ++k) {
+    int32_t k = 0;
+    bool apart = false;
+    for (; k < part.steps; ++k) {
         for (; k < part.steps; ++k) {
+            apart = scales.apart();
+            if (__builtin_expect(apart, 0)) break;
+            if (scales.top != vref) {
+                const int e = (int)(vref >> 23) - (int)(scales.top >> 23) + 127;  // vref 0: sums of 0
+                scale_o(bits_f32((uint32_t)(e < 0 ? 0 : e) << 23));
+                vref = scales.top;
+            }
             before(k);
             if (__builtin_expect(!whole, 0)) break;
             step(part.start + (k << 6), k & 1, std::false_type{});
             after(k);
         }
-        if (k < part.steps) {
+        if (k >= part.steps || apart) break;
+        const int32_t tok = part.start + (k << 6);
+        if (tok < w_hi && tok + 64 > w_lo) step(tok, k & 1, std::true_type{});
+        after(k);
+    }
+    l = sum_over_halves(l);
+    if (__builtin_expect(apart, 0)) {
+        scale_o(l == 0.0f ? 0.0f : 1.0f / (1 << kVBits) / l);
+        scale_o(bits_f32(vref));
+        for (; k < part.steps; ++k) {
+            before(k);
             const int32_t tok = part.start + (k << 6);
-            if (tok < w_hi && tok + 64 > w_lo) step(tok, k & 1, std::true_type{});
+            if (tok < w_hi && tok + 64 > w_lo) step_apart(tok, k & 1);
             after(k);
         }
     }
 
-    l = sum_over_halves(l);
     if (__builtin_expect(has_nan, 0)) {
         // V's NaN codes reach the rows that see their token, and no others: a
         // product of "is NaN" and "is seen", over the steps that took them for
@@ -885,7 +1046,8 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
             for (int i = 0; i < 16; ++i) o[y][i] = hit[y][i] > 0.0f ? __builtin_nanf("") : o[y][i];
     }
     if (!live) return;
-    const float f = bits_f32(vref) * (1.0f / (1 << kVBits)) / l;
+    // (the scale last: with the other factor it could leave fp32's range)
+    const float f = apart ? 1.0f : 1.0f / (1 << kVBits) / l, scale = apart ? 1.0f : bits_f32(vref);
     // four columns 4 u .. 4 u + 3: places u, DP / 4 + u, ..
     auto results = [&](auto put) {
 #pragma unroll
@@ -897,7 +1059,7 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int t = (e * (DP / 4) + 32 * x) / 32, up = (e * (DP / 4) + 32 * x) % 32;  // DP 64: half a tile on
-                    v[e] = l == 0.0f ? 0.0f : o[t][i + up / 2] * f;
+                    v[e] = l == 0.0f ? 0.0f : o[t][i + up / 2] * f * scale;
                 }
                 if (EXACT || d < D) put(d, v);
             }
