@@ -187,7 +187,9 @@ __device__ inline void to_pieces(const float *x, float f, bool in, h8 *hi, h8 *l
         const h2 p = __builtin_convertvector(v, h2);
         (*hi)[e] = p[0], (*hi)[e + 1] = p[1];
         if constexpr (NQ == 2) {
-            const h2 q = __builtin_convertvector(f2{v[0] - (float)p[0], v[1] - (float)p[1]}, h2);
+            // an infinity is all in its first piece: the rest of it is no NaN
+            const f2 rest{fabsf(v[0]) == kInf ? 0.0f : v[0] - (float)p[0], fabsf(v[1]) == kInf ? 0.0f : v[1] - (float)p[1]};
+            const h2 q = __builtin_convertvector(rest, h2);
             (*lo)[e] = q[0], (*lo)[e + 1] = q[1];
         }
     }
