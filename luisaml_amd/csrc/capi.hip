@@ -881,11 +881,9 @@ int make_tokens(lcml::KvTokens &t, const char *fn, int64_t tokens, const void *k
     return LCML_OK;
 }
 
-// 2^32 work items a launch: at most 256 threads for a page and head, or a
-// thread for 4 tokens x 8 elements of it
-int check_kv_grid(const char *fn, const lcml::KvTokens &t, int64_t max_q) {
+// 2^32 work items a launch, with `threads` for a page and head of K or of V
+int check_kv_grid(const char *fn, const lcml::KvTokens &t, int64_t max_q, int64_t threads) {
     const int64_t per_seq = lcml::kv_pages_per_seq(max_q, t.tshift) * 2 * t.heads;
-    const int64_t units = (int64_t)(t.dim >> 3) << (t.tshift - 2), threads = units > 256 ? units : 256;
     if (per_seq > (((int64_t)1 << 32) - 256) / threads / t.seqs)
         return fail(LCML_ERR_UNSUPPORTED, "%s: seqs=%lld max_q=%lld exceeds one launch", fn, (long long)t.seqs,
                     (long long)max_q);
@@ -908,7 +906,7 @@ int lcml_fp8_kv_cache_write(const void *k, const void *v, int dtype, int64_t tok
     if (tokens == 0 || seqs == 0 || max_q == 0 || pages == 0) return LCML_OK;
     if (!k || !v || !elem_aligned(k, dtype) || !elem_aligned(v, dtype))
         return fail(LCML_ERR_INVALID_ARG, "%s: k or v NULL or not aligned to its elements", fn);
-    if (int rc = check_kv_grid(fn, t, max_q)) return rc;
+    if (int rc = check_kv_grid(fn, t, max_q, lcml::kv_write_threads(max_q, t.dim, t.tshift))) return rc;
     return hip_status(lcml::launch_kv_write(t, max_q, k, v, dtype == LCML_DTYPE_BFLOAT16, k_token_stride, k_head_stride,
                                             v_token_stride, v_head_stride, k_cache, v_cache, k_scale, v_scale,
                                             (hipStream_t)stream),
@@ -930,7 +928,8 @@ int lcml_fp8_kv_cache_read(const uint8_t *k_cache, const uint8_t *v_cache, const
     if (tokens == 0 || seqs == 0 || max_q == 0 || pages == 0) return LCML_OK;
     if (!k || !v || !elem_aligned(k, dtype) || !elem_aligned(v, dtype))
         return fail(LCML_ERR_INVALID_ARG, "%s: k or v NULL or not aligned to its elements", fn);
-    if (int rc = check_kv_grid(fn, t, max_q)) return rc;
+    const int64_t units = (int64_t)(t.dim >> 3) << (t.tshift - 2);  // of 4 tokens x 8 elements, a thread each
+    if (int rc = check_kv_grid(fn, t, max_q, units)) return rc;
     return hip_status(lcml::launch_kv_read(t, max_q, k, v, dtype == LCML_DTYPE_BFLOAT16, k_token_stride, k_head_stride,
                                            v_token_stride, v_head_stride, k_cache, v_cache, k_scale, v_scale,
                                            (hipStream_t)stream),

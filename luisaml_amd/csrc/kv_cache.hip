@@ -288,32 +288,33 @@ __global__ __launch_bounds__(kThreads) void k_kv_read(KvTokens t, Rows rows, con
 // pages that max_q tokens of one sequence can touch
 int64_t kv_pages_per_seq(int64_t max_q, int tshift) { return ((max_q - 2 + ((int64_t)1 << tshift)) >> tshift) + 1; }
 
+// Threads of a write's workgroup, which has a page of one head: one for each
+// unit that can hold a new token.  8 x 512 tokens of 8 heads of 128: 10.3 to
+// 10.6 us whatever the page, where 64 and 256 threads alone took 13.7 at pages
+// of 32 and 13.4 at pages of 128 tokens (four units a thread there); one token
+// in pages of 128 4.7, with threads for the whole page 9.
+int kv_write_threads(int64_t max_q, int32_t dim, int tshift) {
+    const int64_t groups = (max_q + 2) / 4 + 1, all = (int64_t)1 << (tshift - 2);
+    const int64_t units = (groups < all ? groups : all) * (dim >> 3);
+    return units <= 64 ? 64 : units <= 128 ? 128 : units <= 256 ? 256 : units <= 512 ? 512 : 1024;
+}
+
 template <bool BF16>
 static void start_kv_write(const KvTokens &t, const Rows &r, uint8_t *kc, uint8_t *vc, float *ks, float *vs, int64_t max_q,
                            hipStream_t s) {
     const int32_t pp = (int32_t)kv_pages_per_seq(max_q, t.tshift);
-    const dim3 grid((unsigned)(2 * t.heads * pp * t.seqs));
-    // A thread for each unit that can hold a new token.  8 x 512 tokens of 8
-    // heads of 128: 10.3 to 10.6 us whatever the page, where 64 and 256 threads
-    // alone took 13.7 at pages of 32 and 13.4 at pages of 128 tokens (four units
-    // a thread there); one token in pages of 128 4.7, with threads for the whole
-    // page 9.
-    const int64_t groups = (max_q + 2) / 4 + 1, all = (int64_t)1 << (t.tshift - 2);
-    const int64_t units = (groups < all ? groups : all) * (t.dim >> 3);
+    const dim3 grid((unsigned)(2 * (int64_t)t.heads * pp * t.seqs));
     auto start = [&](auto nt) {
         constexpr int NT = decltype(nt)::value;
         hipLaunchKernelGGL((k_kv_write<BF16, NT>), grid, dim3(NT), 0, s, t, r, kc, vc, ks, vs, pp);
     };
-    if (units <= 64)
-        start(std::integral_constant<int, 64>{});
-    else if (units <= 128)
-        start(std::integral_constant<int, 128>{});
-    else if (units <= 256)
-        start(std::integral_constant<int, 256>{});
-    else if (units <= 512)
-        start(std::integral_constant<int, 512>{});
-    else
-        start(std::integral_constant<int, 1024>{});
+    switch (kv_write_threads(max_q, t.dim, t.tshift)) {
+        case 64: return start(std::integral_constant<int, 64>{});
+        case 128: return start(std::integral_constant<int, 128>{});
+        case 256: return start(std::integral_constant<int, 256>{});
+        case 512: return start(std::integral_constant<int, 512>{});
+        default: return start(std::integral_constant<int, 1024>{});
+    }
 }
 
 hipError_t launch_kv_write(const KvTokens &t, int64_t max_q, const void *k, const void *v, bool bf16, int64_t kt,

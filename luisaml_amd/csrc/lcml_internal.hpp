@@ -136,6 +136,7 @@ hipError_t launch_rms_norm(int64_t M, int64_t H, const void *x, bool x_bf16, int
 struct KvTokens;
 struct AttentionArgs;
 int64_t kv_pages_per_seq(int64_t max_q, int tshift);
+int kv_write_threads(int64_t max_q, int32_t dim, int tshift);  // of a workgroup: a page of one head, of K or of V
 hipError_t launch_kv_write(const KvTokens &t, int64_t max_q, const void *k, const void *v, bool bf16, int64_t kt,
                            int64_t kh, int64_t vt, int64_t vh, uint8_t *kc, uint8_t *vc, float *ks, float *vs,
                            hipStream_t s);
