@@ -25,12 +25,19 @@ void need(bool ok, const char *what) {
 
 using Args = PyObject *const *;
 
-const at::Tensor &tensor(PyObject *o, const char *name) {
-    if (!THPVariable_Check(o)) throw Bad{std::string(name) + ": a tensor is expected"};
-    const at::Tensor &t = THPVariable_Unpack(o);
-    if (!t.is_cuda()) throw Bad{std::string(name) + ": a device tensor is expected"};
-    return t;
-}
+// the tensors of one call, all on one device
+struct Tensors {
+    int device = -1;
+    const at::Tensor &operator()(PyObject *o, const char *name) {
+        if (!THPVariable_Check(o)) throw Bad{std::string(name) + ": a tensor is expected"};
+        const at::Tensor &t = THPVariable_Unpack(o);
+        if (!t.is_cuda()) throw Bad{std::string(name) + ": a device tensor is expected"};
+        const int at = t.get_device();
+        if (device >= 0 && at != device) throw Bad{std::string(name) + ": the other tensors' device is expected"};
+        device = at;
+        return t;
+    }
+};
 int64_t integer(PyObject *o, const char *name) {
     const long long v = PyLong_AsLongLong(o);
     if (v == -1 && PyErr_Occurred()) {
@@ -74,6 +81,7 @@ PyObject *guarded(Py_ssize_t n, Py_ssize_t want, F f) {
 // x, gamma, eps, residual, residual_out, mode, scale, out, workspace, stream
 PyObject *rms_norm(PyObject *, Args a, Py_ssize_t n) {
     return guarded(n, 10, [&] {
+        Tensors tensor;
         const at::Tensor &x = tensor(a[0], "x"), &gamma = tensor(a[1], "gamma"), &scale = tensor(a[6], "scale"),
                          &y = tensor(a[7], "out");
         need(x.dim() == 2, "x: a matrix is expected");
@@ -117,7 +125,7 @@ struct Cache {
     int64_t pages, heads, dim, page, stride, cols, seqs;
 };
 // k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q
-Cache cache(Args a) {
+Cache cache(Tensors &tensor, Args a) {
     const at::Tensor &k = tensor(a[0], "k_cache"), &v = tensor(a[1], "v_cache"), &ks = tensor(a[2], "k_scale"),
                      &vs = tensor(a[3], "v_scale"), &table = tensor(a[4], "block_table"), &len = tensor(a[5], "kv_len"),
                      &cu = tensor(a[6], "cu_q");
@@ -146,8 +154,9 @@ void heads_of(const at::Tensor &t, int64_t heads, int64_t dim, const char *what)
 // k, v, the cache's seven, max_q, stream
 PyObject *kv_cache_write(PyObject *, Args a, Py_ssize_t n) {
     return guarded(n, 11, [&] {
+        Tensors tensor;
         const at::Tensor &k = tensor(a[0], "k"), &v = tensor(a[1], "v");
-        const Cache c = cache(a + 2);
+        const Cache c = cache(tensor, a + 2);
         heads_of(k, c.heads, c.dim, "k: [tokens, kv_heads, head_dim] is expected");
         heads_of(v, c.heads, c.dim, "v: [tokens, kv_heads, head_dim] is expected");
         need(k.size(0) == v.size(0) && k.scalar_type() == v.scalar_type(), "v: k's tokens and type are expected");
@@ -161,7 +170,8 @@ PyObject *kv_cache_write(PyObject *, Args a, Py_ssize_t n) {
 // the cache's seven, max_q, k_out, v_out, stream
 PyObject *kv_cache_read(PyObject *, Args a, Py_ssize_t n) {
     return guarded(n, 11, [&] {
-        const Cache c = cache(a);
+        Tensors tensor;
+        const Cache c = cache(tensor, a);
         const at::Tensor &k = tensor(a[8], "k_out"), &v = tensor(a[9], "v_out");
         heads_of(k, c.heads, c.dim, "k_out: [tokens, kv_heads, head_dim] is expected");
         heads_of(v, c.heads, c.dim, "v_out: [tokens, kv_heads, head_dim] is expected");
@@ -176,8 +186,9 @@ PyObject *kv_cache_read(PyObject *, Args a, Py_ssize_t n) {
 // q, out, the cache's seven, max_q, max_kv, scale, causal, window, workspace, stream
 PyObject *attention(PyObject *, Args a, Py_ssize_t n) {
     return guarded(n, 16, [&] {
+        Tensors tensor;
         const at::Tensor &q = tensor(a[0], "q"), &o = tensor(a[1], "out");
-        const Cache c = cache(a + 2);
+        const Cache c = cache(tensor, a + 2);
         heads_of(q, -1, c.dim, "q: [tokens, q_heads, head_dim] is expected");
         heads_of(o, q.size(1), c.dim, "out: q's shape is expected");
         need(o.size(0) == q.size(0), "out: q's shape is expected");

@@ -45,3 +45,39 @@ def test_block_tables_whose_rows_overlap(fake):
               cache(fake, seqs=1) | dict(table=fake(4, dt=I32).as_strided((1, 4), (1, 1)))):
         for call in calls(fake, c):
             reaches_the_library(call)
+
+
+@pytest.mark.skipif(torch.cuda.is_available() and torch.cuda.device_count() < 2, reason="cuda:1 cannot be named beside one GPU")
+def test_tensors_of_two_devices(fake):
+    """One tensor of another device among a call's: refused by its name."""
+    other = dict(kc=(8, 2, 16, 64), vc=(8, 2, 16, 64), ks=(8, 2), vs=(8, 2), table=(2, 4), kv=(2,), cu=(3,))
+    for name, shape in other.items():
+        c = cache(fake)
+        c[name] = fake(*shape, dt=c[name].dtype, dev="cuda:1")
+        for call in calls(fake, c):
+            with pytest.raises(ValueError, match="device is expected"):
+                call()
+    x, far = fake(3, 8), fake(3, 8, dev="cuda:1")
+    a = dict(x=x, gamma=fake(8), eps=1e-5, residual=x, residual_out=x, mode=capi.SCALE_ROW, scale=fake(3), out=fake(3, 8, dt=U8))
+    reaches_the_library(lambda: capi.rms_norm(**a, stream=0))
+    for name in ("gamma", "residual", "residual_out", "scale", "out"):
+        with pytest.raises(ValueError, match="device is expected"):
+            capi.rms_norm(**(a | {name: fake(*a[name].shape, dt=a[name].dtype, dev="cuda:1")}), stream=0)
+    with pytest.raises(ValueError, match="workspace: the other"):
+        capi.rms_norm(**a | dict(mode=capi.SCALE_TENSOR), workspace=far, stream=0)
+    q = fake(2, 4, 64)
+    with pytest.raises(ValueError, match="workspace: the other"):
+        capi.attention(q, *cache(fake).values(), 1, 64, 0.1, out=q, workspace=far, stream=0)
+
+
+def test_current_stream_is_of_the_tensors_device(fake, monkeypatch):
+    """Without a stream, a call goes to the current device's: tensors of another
+    one are refused."""
+    monkeypatch.setattr(capi, "_device", lambda: 1)
+    c = cache(fake).values()
+    k, x, y = fake(2, 2, 64), fake(3, 8), fake(3, 8, dt=U8)
+    for call in (lambda: capi.kv_cache_write(k, k, *c, 1), lambda: capi.kv_cache_read(*c, 1, k, k),
+                 lambda: capi.attention(k, *c, 1, 64, 0.1, out=k, workspace=k),
+                 lambda: capi.rms_norm(x, fake(8), 1e-5, mode=capi.SCALE_ROW, scale=fake(3), out=y)):
+        with pytest.raises(ValueError, match="current device cuda:1"):
+            call()
