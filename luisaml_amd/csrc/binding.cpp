@@ -62,6 +62,8 @@ int dtype_code(const at::Tensor &t) {
 void rows(const at::Tensor &t, int64_t M, int64_t H, const char *what) {
     need(t.dim() == 2 && t.size(0) == M && t.size(1) == H && (t.stride(1) == 1 || H <= 1), what);
 }
+// from row to row, which a single row's stride does not say
+int64_t pitch(const at::Tensor &t) { return t.size(0) > 1 || t.stride(0) > t.size(1) ? t.stride(0) : t.size(1); }
 
 template <class F>
 PyObject *guarded(Py_ssize_t n, Py_ssize_t want, F f) {
@@ -101,7 +103,7 @@ PyObject *rms_norm(PyObject *, Args a, Py_ssize_t n) {
             rows(res, M, H, "residual: x's shape and contiguous rows are expected");
             rows(out, M, H, "residual_out: x's shape and contiguous rows are expected");
             need(res.scalar_type() == out.scalar_type(), "residual_out: the residual's type is expected");
-            r = res.data_ptr(), ro = out.data_ptr(), ldr = res.stride(0), ldro = out.stride(0), rt = dtype_code(res);
+            r = res.data_ptr(), ro = out.data_ptr(), ldr = pitch(res), ldro = pitch(out), rt = dtype_code(res);
         } else {
             need(a[4] == Py_None, "residual_out without residual");
         }
@@ -111,9 +113,9 @@ PyObject *rms_norm(PyObject *, Args a, Py_ssize_t n) {
             const at::Tensor &w = tensor(a[8], "workspace");
             ws = w.data_ptr(), bytes = (int64_t)w.nbytes();
         }
-        return lcml_fp8_rms_norm(M, H, x.data_ptr(), dtype_code(x), x.stride(0), r, ro, rt, ldr, ldro,
+        return lcml_fp8_rms_norm(M, H, x.data_ptr(), dtype_code(x), pitch(x), r, ro, rt, ldr, ldro,
                                  static_cast<const float *>(gamma.data_ptr()), number(a[2], "eps"),
-                                 static_cast<uint8_t *>(y.data_ptr()), y.stride(0), (int)mode,
+                                 static_cast<uint8_t *>(y.data_ptr()), pitch(y), (int)mode,
                                  static_cast<float *>(scale.data_ptr()), ws, bytes, reinterpret_cast<void *>(integer(a[9], "stream")));
     });
 }

@@ -81,3 +81,15 @@ def test_current_stream_is_of_the_tensors_device(fake, monkeypatch):
                  lambda: capi.rms_norm(x, fake(8), 1e-5, mode=capi.SCALE_ROW, scale=fake(3), out=y)):
         with pytest.raises(ValueError, match="current device cuda:1"):
             call()
+
+
+def test_one_row_of_any_stride(fake):
+    """The row stride of a matrix of one row means nothing (an expanded vector's
+    is 0); that of more rows does."""
+    def norm(x, res, y, s):
+        return lambda: capi.rms_norm(x, fake(8), 1e-5, residual=res, residual_out=res, mode=capi.SCALE_ROW, scale=s, out=y, stream=0)
+    row = fake(8).expand(1, 8)
+    reaches_the_library(norm(row, row, fake(8, dt=U8).expand(1, 8), fake(1)))
+    for x, res in ((fake(8).expand(2, 8), fake(2, 8)), (fake(2, 8), fake(8).expand(2, 8))):
+        with pytest.raises(capi.LcmlError, match="pitch"):
+            norm(x, res, fake(2, 8, dt=U8), fake(2))()
