@@ -90,6 +90,6 @@ def test_one_row_of_any_stride(fake):
         return lambda: capi.rms_norm(x, fake(8), 1e-5, residual=res, residual_out=res, mode=capi.SCALE_ROW, scale=s, out=y, stream=0)
     row = fake(8).expand(1, 8)
     reaches_the_library(norm(row, row, fake(8, dt=U8).expand(1, 8), fake(1)))
-    for x, res in ((fake(8).expand(2, 8), fake(2, 8)), (fake(2, 8), fake(8).expand(2, 8))):
+    for x, y in ((fake(8).expand(2, 8), fake(2, 8, dt=U8)), (fake(2, 8), fake(8, dt=U8).expand(2, 8))):
         with pytest.raises(capi.LcmlError, match="pitch"):
-            norm(x, res, fake(2, 8, dt=U8), fake(2))()
+            norm(x, fake(2, 8), y, fake(2))()
