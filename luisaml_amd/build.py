@@ -14,7 +14,9 @@ tree).  Flags:
                                             at wave start
 csrc/binding.cpp (Python calls of the norm, KV cache and attention entry
 points) becomes the module luisaml_amd/_binding.so, compiled by the host
-compiler against torch's and Python's headers and linked to the library.
+compiler (g++, or hipcc without it) against torch's and Python's headers and
+linked to the library; where those are not installed the library is all that is
+built.
 Usage:  python -m luisaml_amd.build   (or luisaml_amd.build.build())
 """
 from __future__ import annotations
@@ -66,11 +68,37 @@ def _compile(src: str) -> str:
     return obj
 
 
-def _build_binding() -> None:
+def _binding_lacks() -> str:
+    """What the binding needs beside the library and is not installed, or ''."""
+    try:
+        import torch  # noqa: F401
+        from torch.utils import cpp_extension
+    except ImportError:
+        return "torch"
+    if not any(os.path.exists(os.path.join(d, "torch", "csrc", "autograd", "python_variable.h"))
+               for d in cpp_extension.include_paths()):
+        return "torch's headers"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "Python's headers"
+    return ""
+
+
+def _build_binding() -> bool:
+    """The Python binding, which users of the C ABI do not need: without torch
+    or the headers it is left out (and an older one taken away), and capi's
+    calls that go through it say so."""
+    lacks = _binding_lacks()
+    if lacks:
+        if os.path.exists(BINDING):
+            os.remove(BINDING)
+        print(f"{os.path.basename(BINDING)} (norm, KV cache and attention from Python) is left out: {lacks} not found",
+              file=sys.stderr)
+        return False
     import torch
     from torch.utils import cpp_extension
     tmp = BINDING + ".tmp"
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+    cxx = os.environ.get("CXX") or shutil.which("g++") or HIPCC
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
            "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch.compiled_with_cxx11_abi(), "-I" + os.path.join(ROOT, "include"),
            *("-isystem" + d for d in cpp_extension.include_paths()), "-I" + sysconfig.get_paths()["include"],
            os.path.join(CSRC, "binding.cpp"), "-o", tmp, "-L" + HERE, "-l:" + os.path.basename(LIB),
@@ -80,6 +108,7 @@ def _build_binding() -> None:
     if r.returncode != 0:
         raise RuntimeError(f"binding failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, BINDING)
+    return True
 
 
 def build(verbose: bool = False) -> str:
@@ -96,9 +125,9 @@ def build(verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
-    _build_binding()
+    bound = _build_binding()
     if verbose:
-        print("built", LIB, "and", os.path.basename(BINDING))
+        print("built", LIB, *(("and", os.path.basename(BINDING)) if bound else ()))
     return LIB
 
 
