@@ -1092,11 +1092,18 @@ __global__ __launch_bounds__(256) void k_attention_join_rows(AttentionArgs a, Sp
     if (i >= s.n) return;
     const int64_t row = ((int64_t)s.row0 + i) * a.q_heads + h;
     const float *lse = sp.lse + row * sp.splits, *po = sp.o + row * sp.splits * D + d;
-    float x[kRowsSplits], top = -kInf, sum = 0.0f;
+    float x[kRowsSplits], w[kRowsSplits], top = -kInf, sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < kRowsSplits; ++k) x[k] = lse[k < sp.splits ? k : 0];
 #pragma unroll
     for (int k = 0; k < kRowsSplits; ++k) top = fmaxf(top, x[k]);
+#pragma unroll
+    for (int k = 0; k < kRowsSplits; ++k) {
+        w[k] = k >= sp.splits || x[k] == -kInf ? 0.0f : x[k] == top ? 1.0f : __builtin_amdgcn_exp2f(x[k] - top);
+        sum += w[k];
+    }
+    // weights divided by their sum: the parts' own could leave fp32's range
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     f4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k0 = 0; k0 < kRowsSplits; k0 += 4) {
@@ -1107,15 +1114,9 @@ __global__ __launch_bounds__(256) void k_attention_join_rows(AttentionArgs a, Sp
             p[u] = k0 + u < sp.splits && x[k0 + u] != -kInf ? *reinterpret_cast<const f4 *>(po + (int64_t)(k0 + u) * D)
                                                             : f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const float e = x[k0 + u];
-            const float w = k0 + u >= sp.splits || e == -kInf ? 0.0f : e == top ? 1.0f : __builtin_amdgcn_exp2f(e - top);
-            sum += w;
-            v += p[u] * w;
-        }
+        for (int u = 0; u < 4; ++u) v += p[u] * (w[k0 + u] * inv);
     }
-    store_o4<BF16>(a.o, ((int64_t)s.row0 + i) * a.o_token + (int64_t)h * a.o_head + d,
-                   sum == 0.0f ? f4{0.f, 0.f, 0.f, 0.f} : v * (1.0f / sum));
+    store_o4<BF16>(a.o, ((int64_t)s.row0 + i) * a.o_token + (int64_t)h * a.o_head + d, v);
 }
 
 // Joins a row's parts, a workgroup a row: the weights first, then the parts by
@@ -1142,7 +1143,9 @@ __global__ __launch_bounds__(256) void k_attention_join(AttentionArgs a, Split s
     float sum = w0 + w1;
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m);
-    if (threadIdx.x < 64) weight[lane] = x0 == -kInf ? -1.0f : w0, weight[lane + 64] = x1 == -kInf ? -1.0f : w1;
+    // weights divided by their sum: the parts' own could leave fp32's range
+    const float inv = 1.0f / sum;
+    if (threadIdx.x < 64) weight[lane] = x0 == -kInf ? -1.0f : w0 * inv, weight[lane + 64] = x1 == -kInf ? -1.0f : w1 * inv;
     __syncthreads();
     const int32_t groups = 256 / q4, grp = threadIdx.x / q4, d = threadIdx.x % q4 * 4;
     f4 v{0.f, 0.f, 0.f, 0.f};
@@ -1163,8 +1166,7 @@ __global__ __launch_bounds__(256) void k_attention_join(AttentionArgs a, Split s
     __syncthreads();
     if (grp > 0) return;
     for (int32_t g = 1; g < groups; ++g) v += buf[g * q4 + threadIdx.x];
-    store_o4<BF16>(a.o, ((int64_t)s.row0 + i) * a.o_token + (int64_t)h * a.o_head + d,
-                   sum == 0.0f ? f4{0.f, 0.f, 0.f, 0.f} : v * (1.0f / sum));
+    store_o4<BF16>(a.o, ((int64_t)s.row0 + i) * a.o_token + (int64_t)h * a.o_head + d, v);
 }
 
 // ------------------------------------------------------------------- plan --

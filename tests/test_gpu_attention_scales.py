@@ -146,3 +146,16 @@ def test_split_over_long_sequences(dev, n, D, ot):
     size = 10.0 ** r.uniform(-20, 10, 400)
     run(dev, [5000, 3000], [n, n], steps(*size, every=64), T=64, H=1, G=4, D=D, ot=ot, many=n == 300, seed=n)
     run(dev, [5000, 3000], [n, n], steps(1.0, 1e-10, every=2500), T=64, H=1, G=4, D=D, ot=ot, many=n == 300, seed=n)
+
+
+@pytest.mark.parametrize("ot", ["b", "f"])
+@pytest.mark.parametrize("kv,n,D,many", [([20000], 1, 64, False), ([5000, 3000], 300, 128, True), ([700], 3, 64, False),
+                                         ([3000, 2000], 150, 64, False)])
+def test_parts_near_the_largest_number_joined(dev, kv, n, D, many, ot):
+    """Every value is 448 times 2^119, 7/8 of fp32's range: so is the result,
+    however many parts it is joined from."""
+    def change(cache, table):
+        cache.codes[1][:] = 0x7E
+        cache.scale[1][:] = 2.0 ** 119
+    got = run(dev, kv, [n] * len(kv), steps(1.0), T=64, H=1, G=4, D=D, ot=ot, many=many, change=change)
+    assert (np.abs(got / (448.0 * 2.0 ** 119) - 1.0) < 1e-5).all()
