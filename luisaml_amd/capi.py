@@ -156,14 +156,15 @@ def _stream(stream=None):
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else stream
 
 
-def _stream_of(t, stream):
-    """The stream of a call of the compiled binding: the given one, or the
-    current one, which has to be of t's device."""
-    if stream is None and isinstance(t, torch.Tensor) and t.is_cuda:
-        current = _device() if _device is not None else torch.cuda.current_device()
-        if t.get_device() != current:
-            raise ValueError(f"tensors on {t.device}, current device cuda:{current}")
-    return _stream(stream)
+def _where(stream):
+    """The stream of a call of the compiled binding and the device that its
+    tensors have to be on (-1 with a given stream: any one)."""
+    if stream is not None:
+        return _stream(stream), -1
+    if _raw_stream is not None and _device is not None and torch.cuda.is_initialized():
+        device = _device()
+        return _raw_stream(device), device
+    return torch.cuda.current_stream().cuda_stream, torch.cuda.current_device()
 
 
 def _empty(shape, dtype, device, stream):
@@ -551,7 +552,7 @@ def rms_norm(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual: torch.T
         scale = _empty(x.shape[0] if mode == SCALE_ROW else 1, torch.float32, x.device, stream)
     if mode == SCALE_TENSOR and workspace is None and x.shape[0] > 1:
         workspace = _empty(lib().lcml_fp8_rms_norm_workspace_bytes(*x.shape, mode), torch.uint8, x.device, stream)
-    _check(_binding().rms_norm(x, gamma, eps, residual, residual_out, mode, scale, out, workspace, _stream_of(x, stream)))
+    _check(_binding().rms_norm(x, gamma, eps, residual, residual_out, mode, scale, out, workspace, *_where(stream)))
     return out, scale, residual_out
 
 
@@ -569,7 +570,7 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     head strides) into the cache [pages, kv_heads, page_tokens, head_dim], as
     the last tokens of their sequences (kv_len counts them)."""
     _check(_binding().kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q, max_q,
-                                     _stream_of(k, stream)))
+                                     *_where(stream)))
 
 
 def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -578,7 +579,7 @@ def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.T
     """The inverse of kv_cache_write: the same rows' tokens into k_out, v_out
     [tokens, kv_heads, head_dim] (fp32 or bf16)."""
     _check(_binding().kv_cache_read(k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q, max_q, k_out, v_out,
-                                    _stream_of(k_out, stream)))
+                                    *_where(stream)))
 
 
 @functools.lru_cache(maxsize=256)
@@ -601,5 +602,5 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_s
         if need:
             workspace = _empty(need, torch.uint8, q.device, stream)
     _check(_binding().attention(q, out, k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q, max_q, max_kv,
-                                scale, causal, window, workspace, _stream_of(q, stream)))
+                                scale, causal, window, workspace, *_where(stream)))
     return out

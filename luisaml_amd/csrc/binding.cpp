@@ -65,6 +65,15 @@ void rows(const at::Tensor &t, int64_t M, int64_t H, const char *what) {
 // from row to row, which a single row's stride does not say
 int64_t pitch(const at::Tensor &t) { return t.size(0) > 1 || t.stride(0) > t.size(1) ? t.stride(0) : t.size(1); }
 
+// the call's stream, at the end of its checks: the handle and the device that
+// are its last two arguments
+void *stream_of(const Tensors &t, Args a) {
+    const int64_t current = integer(a[1], "device");
+    if (current >= 0 && t.device != current)
+        throw Bad{"tensors on cuda:" + std::to_string(t.device) + ", current device cuda:" + std::to_string(current)};
+    return reinterpret_cast<void *>(integer(a[0], "stream"));
+}
+
 template <class F>
 PyObject *guarded(Py_ssize_t n, Py_ssize_t want, F f) {
     try {
@@ -80,9 +89,9 @@ PyObject *guarded(Py_ssize_t n, Py_ssize_t want, F f) {
     return nullptr;
 }
 
-// x, gamma, eps, residual, residual_out, mode, scale, out, workspace, stream
+// x, gamma, eps, residual, residual_out, mode, scale, out, workspace, stream, device
 PyObject *rms_norm(PyObject *, Args a, Py_ssize_t n) {
-    return guarded(n, 10, [&] {
+    return guarded(n, 11, [&] {
         Tensors tensor;
         const at::Tensor &x = tensor(a[0], "x"), &gamma = tensor(a[1], "gamma"), &scale = tensor(a[6], "scale"),
                          &y = tensor(a[7], "out");
@@ -116,7 +125,7 @@ PyObject *rms_norm(PyObject *, Args a, Py_ssize_t n) {
         return lcml_fp8_rms_norm(M, H, x.data_ptr(), dtype_code(x), pitch(x), r, ro, rt, ldr, ldro,
                                  static_cast<const float *>(gamma.data_ptr()), number(a[2], "eps"),
                                  static_cast<uint8_t *>(y.data_ptr()), pitch(y), (int)mode,
-                                 static_cast<float *>(scale.data_ptr()), ws, bytes, reinterpret_cast<void *>(integer(a[9], "stream")));
+                                 static_cast<float *>(scale.data_ptr()), ws, bytes, stream_of(tensor, a + 9));
     });
 }
 
@@ -153,9 +162,9 @@ void heads_of(const at::Tensor &t, int64_t heads, int64_t dim, const char *what)
     need(t.dim() == 3 && (heads < 0 || t.size(1) == heads) && t.size(2) == dim && t.stride(2) == 1, what);
 }
 
-// k, v, the cache's seven, max_q, stream
+// k, v, the cache's seven, max_q, stream, device
 PyObject *kv_cache_write(PyObject *, Args a, Py_ssize_t n) {
-    return guarded(n, 11, [&] {
+    return guarded(n, 12, [&] {
         Tensors tensor;
         const at::Tensor &k = tensor(a[0], "k"), &v = tensor(a[1], "v");
         const Cache c = cache(tensor, a + 2);
@@ -165,13 +174,13 @@ PyObject *kv_cache_write(PyObject *, Args a, Py_ssize_t n) {
         return lcml_fp8_kv_cache_write(k.data_ptr(), v.data_ptr(), dtype_code(k), k.size(0), k.stride(0), k.stride(1), v.stride(0),
                                        v.stride(1), c.k, c.v, c.ks, c.vs, c.pages, c.heads, c.dim, c.page, c.table, c.stride,
                                        c.cols, c.kv_len, c.cu_q, c.seqs, integer(a[9], "max_q"),
-                                       reinterpret_cast<void *>(integer(a[10], "stream")));
+                                       stream_of(tensor, a + 10));
     });
 }
 
-// the cache's seven, max_q, k_out, v_out, stream
+// the cache's seven, max_q, k_out, v_out, stream, device
 PyObject *kv_cache_read(PyObject *, Args a, Py_ssize_t n) {
-    return guarded(n, 11, [&] {
+    return guarded(n, 12, [&] {
         Tensors tensor;
         const Cache c = cache(tensor, a);
         const at::Tensor &k = tensor(a[8], "k_out"), &v = tensor(a[9], "v_out");
@@ -181,13 +190,13 @@ PyObject *kv_cache_read(PyObject *, Args a, Py_ssize_t n) {
         return lcml_fp8_kv_cache_read(c.k, c.v, c.ks, c.vs, c.pages, c.heads, c.dim, c.page, c.table, c.stride, c.cols, c.kv_len,
                                       c.cu_q, c.seqs, integer(a[7], "max_q"), k.data_ptr(), v.data_ptr(), dtype_code(k), k.size(0),
                                       k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                                      reinterpret_cast<void *>(integer(a[10], "stream")));
+                                      stream_of(tensor, a + 10));
     });
 }
 
-// q, out, the cache's seven, max_q, max_kv, scale, causal, window, workspace, stream
+// q, out, the cache's seven, max_q, max_kv, scale, causal, window, workspace, stream, device
 PyObject *attention(PyObject *, Args a, Py_ssize_t n) {
-    return guarded(n, 16, [&] {
+    return guarded(n, 17, [&] {
         Tensors tensor;
         const at::Tensor &q = tensor(a[0], "q"), &o = tensor(a[1], "out");
         const Cache c = cache(tensor, a + 2);
@@ -204,7 +213,7 @@ PyObject *attention(PyObject *, Args a, Py_ssize_t n) {
                                   dtype_code(o), o.stride(0), o.stride(1), c.k, c.v, c.ks, c.vs, c.pages, c.heads, c.dim, c.page,
                                   c.table, c.stride, c.cols, c.kv_len, c.cu_q, c.seqs, integer(a[9], "max_q"),
                                   integer(a[10], "max_kv"), number(a[11], "scale"), (int)integer(a[12], "causal"),
-                                  integer(a[13], "window"), ws, bytes, reinterpret_cast<void *>(integer(a[15], "stream")));
+                                  integer(a[13], "window"), ws, bytes, stream_of(tensor, a + 15));
     });
 }
 

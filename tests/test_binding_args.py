@@ -74,6 +74,8 @@ def test_current_stream_is_of_the_tensors_device(fake, monkeypatch):
     """Without a stream, a call goes to the current device's: tensors of another
     one are refused."""
     monkeypatch.setattr(capi, "_device", lambda: 1)
+    monkeypatch.setattr(capi, "_raw_stream", lambda device: 0)
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
     c = cache(fake).values()
     k, x, y = fake(2, 2, 64), fake(3, 8), fake(3, 8, dt=U8)
     for call in (lambda: capi.kv_cache_write(k, k, *c, 1), lambda: capi.kv_cache_read(*c, 1, k, k),
