@@ -429,7 +429,9 @@ LCML_API int lcml_fp8_binary(int op, int dtype, const void *a, const int64_t *a_
  * mode: LCML_SCALE_STATIC  s = scale[0], an input;
  *       LCML_SCALE_TENSOR  s = max |v| / 448 of the tensor, written to
  *                          scale[0]: lcml_fp8_gemm's a_scale;
- *       LCML_SCALE_ROW     s = max |v| / 448 of row m, written to scale[m];
+ *       LCML_SCALE_ROW     s = max |v| / 448 of row m, written to scale[m]
+ *                          (no linear here takes more than one a_scale: for
+ *                          M > 1 it is for the caller's own use);
  *   NaN is left out of the maximum, and s is 1 where that is not a positive
  *   finite number.
  * x: M rows of H, FLOAT or BFLOAT16, row pitch ldx elements; residual (may be
@@ -512,6 +514,12 @@ LCML_API int lcml_fp8_kv_cache_read(const uint8_t *k_cache, const uint8_t *v_cac
  * Cache and index arguments as above; cu_q[b+1] - cu_q[b] <= max_q and
  * kv_len[b] <= max_kv are the host's bounds (rows past max_q are left out;
  * max_kv divides the work, and longer sequences only take longer).  scale > 0.
+ * Numbers: scores, maximum and sums are fp32, and the cache's codes and scales
+ * enter exactly; the elements of a query do down to 2^-31 (bf16) of the row's
+ * largest, or to 2^-22 of themselves (fp32).  A weight is rounded to fp16 before
+ * it meets v: for bf16 results once, which leaves an error of 2^-11 of it, or of
+ * 2^-31 of the largest weight where that is more; for fp32 results in two pieces,
+ * 2^-22 and 2^-39.
  * workspace: lcml_fp8_attention_workspace_bytes(...) bytes, 16-byte aligned,
  * written before they are read (0: may be NULL).
  * No counterpart in the reference.

@@ -540,7 +540,8 @@ def rms_norm(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual: torch.T
              out: torch.Tensor | None = None, workspace: torch.Tensor | None = None, stream=None):
     """h = x + residual, RMS norm of h, E4M3 codes of it: the input of an FP8
     linear.  x [M,H] fp32/bf16; residual fp32/bf16; gamma [H] fp32.  mode
-    SCALE_STATIC takes scale[1]; SCALE_TENSOR gives it; SCALE_ROW gives [M].
+    SCALE_STATIC takes scale[1]; SCALE_TENSOR gives it, as gemm takes it;
+    SCALE_ROW gives [M], which no linear here takes for M > 1.
     Returns (codes uint8 [M,H], scale, h or None)."""
     if residual is not None and residual_out is None:
         residual_out = _empty(residual.shape, residual.dtype, x.device, stream)
@@ -593,7 +594,9 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_s
               out_dtype=None, workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """softmax(scale * q k^T) v over the E4M3 cache: q [tokens, q_heads,
     head_dim] (fp32/bf16) are the last tokens of their sequences, which the
-    cache already holds.  window > 0: only the last `window` positions."""
+    cache already holds.  window > 0: only the last `window` positions.
+    Weights are rounded to fp16 before they meet v: to 11 bits for bf16 results,
+    to 22 for fp32 ones."""
     if out is None:
         out = _empty(q.shape, out_dtype or q.dtype, q.device, stream)
     if workspace is None:

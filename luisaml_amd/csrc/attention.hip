@@ -11,8 +11,8 @@
 //   * a query row is brought to [2^14, 2^15) by a power of two; a bf16 row is
 //     then one fp16 operand, an fp32 row two (its rounding and the rest);
 //   * weights are fp16 too: 11 bits, where bf16 would hold 8.  One piece where
-//     the result is bf16, whose own rounding is eight times as coarse, two
-//     where it is fp32;
+//     the result is bf16, whose own rounding is eight times as coarse, also for
+//     fp32 queries; two where it is fp32;
 //   * K's page scale multiplies the scores, V's the codes as they are widened:
 //     a power of two below the largest V scale so far (the widening
 //     instruction takes the factor), which multiplies the end result; where
@@ -293,12 +293,12 @@ __device__ inline Part part_of(const AttentionArgs &a, const Split &sp, int32_t 
 // tokens, straight from memory into registers, and join at the end.
 // 16x16x32 instructions.
 //
-// Bound by the cache's bytes: 16 KB of loads a wavefront under way (256
+// Bound by the cache's bytes: 16 KB of loads a wavefront under way (212
 // registers, two wavefronts a SIMD; three spilled and took 213 us where this
-// takes 119, eight in a workgroup 166).  32 queries of 32 heads over up to 16384
-// tokens of 8 KV heads of 128, 619 MB: 119 us, 5.2 TB/s.  One over 500 tokens: 8
-// us, five dependent round trips to memory (lengths, table, scales, codes, the
-// join's LDS).
+// takes 120, eight in a workgroup 166).  32 queries of 32 heads over up to 16384
+// tokens of 8 KV heads of 128, 619 MB: 120 us, 5.2 TB/s; fp32 queries and
+// results 130.  One over 500 tokens: 8.4 us, five dependent round trips to
+// memory (lengths, table, scales, codes, the join's LDS); fp32 10.
 template <int DC, int NQ, int NP, int NW>
 __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(AttentionArgs a, Split sp) {
     constexpr int DP = DC * 64, kPitch = DP + 4;
@@ -659,14 +659,16 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
 // widened: bound by the vector ALU and the matrix cores in turn, the kernel
 // shares the widening of V (64 conversions a wavefront and step would be
 // repeated by each of the four), and reads K's codes in half the bytes (K
-// widened as well: 610 us where this takes 600).  32x32x16 instructions.
+// widened as well: 2% slower).  32x32x16 instructions.
 //
-// A prompt of 8192 tokens, 32 heads over 8 of 128, 0.55 TFLOP: 600 us, 917
+// A prompt of 8192 tokens, 32 heads over 8 of 128, 0.55 TFLOP: 610 us, 900
 // TFLOP/s, where a product of 8192^3 in bf16 reaches 1190.  A step's 32 matrix
-// instructions take 1024 cycles of a SIMD, its 313 vector ones 1250, and two
+// instructions take 1024 cycles of a SIMD, its 320 vector ones 1280, and two
 // wavefronts a SIMD overlap them to two thirds of the sum.  (Two groups of
 // wavefronts half a step apart: 1075 us, for the registers spilled.)  D > 128
-// has one wavefront a SIMD, and nothing to overlap LDS reads with: 150 TFLOP/s.
+// has one wavefront a SIMD, and nothing to overlap LDS reads with: 220 TFLOP/s
+// on a prompt of 2048 tokens, 260 on one of 4000.  What happens around a step is
+// in three loops, always inlined: out of line, its registers lie in scratch.
 constexpr int kManyWaves = 4, kManyRows = 32 * kManyWaves;
 
 template <int DP, bool EXACT, int NQ, int NP>
@@ -1193,8 +1195,8 @@ Plan divide(bool few, int64_t pairs, int64_t rows, int64_t span) {
     // 2048 of four steps, so that ragged lengths even out (4096: 1 x 32000 28 us
     // against 20).  Many rows: parts of 15 steps up to two workgroups a CU, of
     // eight up to one, as joining them reads and writes every result again in
-    // fp32 (3 x 383 x 5292 in three parts 97 us, in two 135; 1 x 400 x 4000 in four
-    // 60, in two 73; 1 x 1500 x 1500, 24 steps, in two 66, in one 51).
+    // fp32 (3 x 383 x 5292 in three parts 102 us, in two 135; 1 x 400 x 4000 in
+    // four 61, in two 73; 1 x 1500 x 1500, 24 steps, in two 66, in one 52).
     int64_t splits;
     if (few) {
         const int64_t fine = (steps + 4 * kFewWaves - 1) / (4 * kFewWaves), coarse = (steps + kFewWaves - 1) / kFewWaves;
@@ -1219,14 +1221,17 @@ Plan divide(bool few, int64_t pairs, int64_t rows, int64_t span) {
 }
 
 // Up to 64 rows the kernel for few rows is the faster one (64 rows: 8 sequences
-// of 4000 tokens 40.5 us against 46, 32 of 1000 35 against 38).  Above, the sum
-// of what either takes decides, in us by measurement: a start, a step of 64
-// tokens, as many workgroups as run at once, a join.  Of 68 cases of 1 to 32
-// sequences, 16 to 1500 queries and all widths it takes the slower one in two (10
-// us for 8.3, 32 for 30).  Some: 1 x 256 9.0 us in the kernel for few rows, 14 in
-// the one for many; 1 x 512 18 and 21; 1 x 700 28 and 27; 8 x 128 30 and 14; 32
-// after 4000 18 and 28; 4 x 100 after 900 31 and 36; one KV head of 256, 512
-// queries of 8 heads, 15 and 45.
+// of 4000 tokens 43.2 us against 44.6, 32 of 1000 36.2 against 39.0, one of 4000
+// 16 against 25).  Above, the sum of what either takes decides, in us by
+// measurement: a start, a step of 64 tokens, as many workgroups as run at once, a
+// join.  Of 91 cases of 1 to 32 sequences, 16 to 4000 queries and all widths,
+// bf16 but for nine, it takes one that is more than 5% slower in three (10.5 us
+// for 8.5, 44 for 37, 65 for 53).  Some: 1 x 256 9.2 us in the kernel for few
+// rows, 14 in the one for many; 1 x 512 19 and 21; 1 x 700 28 and 27; 8 x 128 30
+// and 14; 32 after 4000 18 and 29; 4 x 100 after 900 31 and 36; one KV head of
+// 256, 512 queries of 8 heads, 15 and 37.  Types do not enter: fp32's two pieces
+// cost both kernels twice the products (2 x 200 19.1 and 18.6, 4 x 333 over 4000
+// 59 and 56).
 // max_kv decides, not the window: the workspace then covers any window.
 Plan make_plan(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t max_q, int64_t max_kv,
                int64_t window) {
@@ -1277,8 +1282,8 @@ hipError_t launch_t(const AttentionArgs &a, const Plan &p, hipStream_t s) {
     const unsigned rows = (unsigned)((int64_t)a.t.seqs * a.max_q * a.q_heads);
     const unsigned per = 1024u / a.t.dim;
     // from 512 rows on many rows a workgroup (8 x 16 x 32 rows of 4 parts 40.5 us
-    // with attention, a workgroup a row 44; 16384 rows of 2 22 and 43; 128 rows of
-    // 16 15.7 and 15.0)
+    // with attention, a workgroup a row 44; 16384 rows of 2 parts 22 and 43; 128
+    // rows of 16 parts 15.7 and 15.0, before the parts' weights were divided)
     if (rows >= 512 && p.sp.splits <= kRowsSplits) {
         hipLaunchKernelGGL((k_attention_join_rows<NP == 1>), dim3((rows + per - 1) / per), dim3(256), 0, s, a, p.sp, rows);
         return hipGetLastError();

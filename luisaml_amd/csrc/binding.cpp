@@ -4,8 +4,9 @@
 // A decode step makes these calls for every layer and token, and their kernels
 // take 4 to 10 us; through ctypes a call's argument handling alone took as
 // long (cache write 8.4 us, attention 9.4 us).  Each function checks its
-// tensors (ValueError), calls the C ABI on the stream handle given, and
-// returns its status; allocation and status handling stay in capi.py.
+// tensors (ValueError), their device among it, calls the C ABI on the stream
+// handle given, and returns its status; allocation and status handling stay in
+// capi.py.
 #include <Python.h>
 
 #include <torch/csrc/autograd/python_variable.h>

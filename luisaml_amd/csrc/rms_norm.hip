@@ -352,7 +352,9 @@ hipError_t launch_t(const NormArgs &a, hipStream_t s) {
     // twice the threads with half the groups shorten it (256 rows of 4096, 512
     // threads 4.5 us, 256 threads 5.0; 512 rows 6.2 and 6.5, 4096 rows 29.5 and
     // 26.9; 64 rows of 8000, 1024 threads 5.2, 512 threads 5.5; from 256 rows on
-    // equal).
+    // equal).  Rows past 8192 take four groups of 1024 threads whatever their
+    // length, and read what is past 16384 once more (4096 rows of 12288 in bf16
+    // 120 us, 2.9 TB/s); fewer groups were not measured there.
     auto start = [&](auto tpr, auto nv, auto tail) {
         constexpr int TPR = decltype(tpr)::value, kThreads = TPR < 256 ? 256 : TPR;
         n = grid(kThreads / TPR, most);
