@@ -4,13 +4,13 @@
     a  = attention(norm(h) Wqkv, cache) Wo
     h' = h + a;  y = gelu(norm(h') Wup) Wdown
 
-Every step is a call of luisaml_amd.capi: the norms add the residual and emit
-the E4M3 codes and the scale that the QKV and up projections take, K and V go
-from columns of the QKV projection's output into a paged E4M3 cache, attention
-reads them there, and the output and down projections quantise their fp32
-inputs as they run.  Sequences of any lengths share the pages; a step of single
-tokens needs no host value that changes, so that it can be captured in a HIP
-graph and replayed while the sequences grow.
+No positions are encoded.  Every step is a call of luisaml_amd.capi: the norms
+add the residual and emit the E4M3 codes and the scale that the QKV and up
+projections take, K and V go from columns of the QKV projection's output into a
+paged E4M3 cache, attention reads them there, and the output and down
+projections quantise their fp32 inputs as they run.  Sequences of any lengths
+share the pages; a step of single tokens needs no host value that changes, so
+that it can be captured in a HIP graph and replayed while the sequences grow.
 
     python examples/decoder_layer.py [--graph]
 """
