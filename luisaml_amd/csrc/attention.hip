@@ -99,7 +99,8 @@ __device__ inline float reciprocal(float f) { return bits_f32((254u << 23) - f32
 // hold all of them up to a spread of 2^22; 2^10 also keeps what the weights'
 // own fp16 loses (2^-31 of the largest weight, times the largest values) below
 // a bf16 result's rounding where only values of the smallest scale count.
-// Pages of one head are seldom further apart than 2^4.
+// Beyond, a step takes longer (every other page 2^20 smaller: 32 queries over up
+// to 16384 tokens 165 us for 124, a prompt of 8192 1372 for 610).
 constexpr int kSpread = 10;
 struct Scales {
     uint32_t top = 0, low = 0x7f800000u;
