@@ -502,6 +502,69 @@ LCML_API int lcml_fp8_kv_cache_read(const uint8_t *k_cache, const uint8_t *v_cac
                                     int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, void *stream);
 
 /*
+ * A step's page table, lengths and row indexes from the tokens that each
+ * request brings, so that a step needs nothing from the host:
+ *   old = ended[b] ? 0 : kv_len_in[b],   kv_len[b] = old + new_tokens[b],
+ *   cu_q = the sums of new_tokens before each sequence
+ * (negative entries count as 0).  free_pages holds free_count[0] free pages at
+ * its beginning, a stack.  First the pages of sequences with ended[b] != 0
+ * (columns first_own[b] .. ceil(kv_len_in[b] / page_tokens) - 1 of their rows;
+ * the earlier ones belong to others too) go onto it, in order of sequence and
+ * column; entries outside [0, pages) are skipped, and there is room for `pages`
+ * in all.  Then every column ceil(old / page_tokens) .. ceil(kv_len[b] /
+ * page_tokens) - 1 below table_cols takes the page on its top, in the same
+ * order, or -1 when there is none; other entries of block_table stay, and so do
+ * entries of free_pages that nothing was put on.  left[0]: free pages that
+ * remain, negative if as many were lacking (a later call's free_count; negative
+ * counts as 0).  A page must not be in the stack twice, nor be its sequence's.
+ * Row cu_q[b] + i: positions = old + i, slots = page * page_tokens + position %
+ * page_tokens, -1 where it has no page; rows from cu_q[seqs] up to `tokens` have
+ * -1 in both.
+ * ended and first_own (all 0), positions and slots may be NULL; kv_len may be
+ * kv_len_in, and left free_count: a captured step then runs on by itself.
+ * workspace: lcml_fp8_kv_cache_plan_workspace_bytes(seqs, tokens) bytes, 8-byte
+ * aligned, written before they are read (0: may be NULL).
+ * No counterpart in the reference.
+ */
+LCML_API int64_t lcml_fp8_kv_cache_plan_workspace_bytes(int64_t seqs, int64_t tokens);
+LCML_API int lcml_fp8_kv_cache_plan(const int32_t *new_tokens, const int32_t *kv_len_in, const int32_t *ended,
+                                    const int32_t *first_own, int64_t seqs, int32_t *free_pages,
+                                    const int32_t *free_count, int64_t pages, int64_t page_tokens, int32_t *block_table,
+                                    int64_t table_stride, int64_t table_cols, int32_t *kv_len, int32_t *cu_q,
+                                    int32_t *left, int32_t *positions, int64_t *slots, int64_t tokens, void *workspace,
+                                    int64_t workspace_bytes, void *stream);
+
+/*
+ * RMS norms of the heads of queries and keys, and the rotation by position, in
+ * one pass: for every head x of D elements
+ *   v = x / sqrt(mean(x^2) + eps) * gamma            (x itself where gamma is NULL)
+ *   (v_a, v_b) -> (v_a c - v_b s, v_b c + v_a s)
+ * for the pairs i < rot_dim / 2, (a, b) = (i, i + rot_dim / 2), or (2 i, 2 i + 1)
+ * if `interleaved`; elements from rot_dim on stay as they are.  fp32 throughout,
+ * rounded once to out_dtype.
+ *   q, k: [tokens][heads][head_dim], FLOAT or BFLOAT16 (`dtype`), strides in
+ *     elements, elements of a head contiguous (columns of a QKV projection are);
+ *     the outputs likewise (`out_dtype`), each may be its input with the same
+ *     strides and type.  k_heads (or q_heads) 0: no k (q).
+ *   q_gamma, k_gamma: head_dim floats each, or NULL.
+ *   table: [table_rows][rot_dim] floats, row p the rot_dim / 2 cosines of
+ *     position p and then its sines.
+ *   positions: [tokens] int32.  A row whose position is negative or not below
+ *     table_rows is left as it was.  (rot_dim 0: any position, and NULL takes
+ *     every row.)
+ * head_dim 16 to 256 in steps of 16, rot_dim even.  A head whose sum of squares
+ * overflows fp32 gives zeros, as the formula does.
+ * No counterpart in the reference.
+ */
+LCML_API int lcml_fp8_qk_norm_rope(const void *q, const void *k, int dtype, int64_t tokens, int64_t q_heads,
+                                   int64_t k_heads, int64_t head_dim, int64_t q_token_stride, int64_t q_head_stride,
+                                   int64_t k_token_stride, int64_t k_head_stride, const float *q_gamma,
+                                   const float *k_gamma, float eps, const int32_t *positions, const float *table,
+                                   int64_t table_rows, int64_t rot_dim, int interleaved, void *q_out, void *k_out,
+                                   int out_dtype, int64_t qo_token_stride, int64_t qo_head_stride,
+                                   int64_t ko_token_stride, int64_t ko_head_stride, void *stream);
+
+/*
  * Attention over the E4M3 KV cache, for prompts, chunks of prompts and single
  * tokens alike: for row cu_q[b] + i at position p = kv_len[b] - n + i,
  *   o = sum_j w_j v_j / sum_j w_j,   w_j = exp(scale * q.k_j)
@@ -534,6 +597,57 @@ LCML_API int lcml_fp8_attention(const void *q, int q_dtype, int64_t tokens, int6
                                 int64_t table_stride, int64_t table_cols, const int32_t *kv_len, const int32_t *cu_q,
                                 int64_t seqs, int64_t max_q, int64_t max_kv, float scale, int causal, int64_t window,
                                 void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * lcml_fp8_attention with first positions that the window does not hide: a row
+ * at position p sees j < kv_len[b], j <= p if `causal`, and j > p - window or
+ * j < sinks (window > 0; without one, or with sinks 0, it is lcml_fp8_attention).
+ * Arguments, numbers and workspace are lcml_fp8_attention's.
+ */
+LCML_API int lcml_fp8_attention_sinks(const void *q, int q_dtype, int64_t tokens, int64_t q_heads,
+                                      int64_t q_token_stride, int64_t q_head_stride, void *o, int o_dtype,
+                                      int64_t o_token_stride, int64_t o_head_stride, const uint8_t *k_cache,
+                                      const uint8_t *v_cache, const float *k_scale, const float *v_scale, int64_t pages,
+                                      int64_t kv_heads, int64_t head_dim, int64_t page_tokens,
+                                      const int32_t *block_table, int64_t table_stride, int64_t table_cols,
+                                      const int32_t *kv_len, const int32_t *cu_q, int64_t seqs, int64_t max_q,
+                                      int64_t max_kv, float scale, int causal, int64_t window, int64_t sinks,
+                                      void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * lcml_fp8_attention (without a window) for groups of sequences that share
+ * their first tokens' pages, which are read once for a group:
+ *   group g is the sequences group_seq[g] .. group_seq[g+1]-1 (group_seq[0] = 0,
+ *   rising; sequences from group_seq[groups] on share nothing); its first
+ *   prefix_len[g] tokens (0: none) lie in the pages prefix_table[g][..]
+ *   ([groups] rows of prefix_cols pages, row pitch prefix_stride), in tokens'
+ *   order as in block_table.
+ * A sequence whose rows all lie behind its group's prefix (kv_len[b] - n >=
+ * prefix_len[g]) reads the prefix there and the other tokens through its own row
+ * of block_table; any other one reads all of them through its own row.  Where a
+ * group's rows of block_table begin with the prefix's pages, as they do when its
+ * sequences were started behind it, the result is lcml_fp8_attention's but for
+ * the order of sums.
+ * group_seq, prefix_table and prefix_len are int32 on the device.  Host's
+ * bounds, which divide the work (longer ones only take longer): max_own, of a
+ * sequence's tokens behind its prefix, and max_prefix; max_q as ever.
+ * workspace: lcml_fp8_attention_shared_workspace_bytes(...) bytes, 16-byte
+ * aligned, written before they are read.
+ */
+LCML_API int64_t lcml_fp8_attention_shared_workspace_bytes(int64_t tokens, int64_t seqs, int64_t groups, int64_t q_heads,
+                                                           int64_t kv_heads, int64_t head_dim, int64_t max_q,
+                                                           int64_t max_own, int64_t max_prefix);
+LCML_API int lcml_fp8_attention_shared(const void *q, int q_dtype, int64_t tokens, int64_t q_heads,
+                                       int64_t q_token_stride, int64_t q_head_stride, void *o, int o_dtype,
+                                       int64_t o_token_stride, int64_t o_head_stride, const uint8_t *k_cache,
+                                       const uint8_t *v_cache, const float *k_scale, const float *v_scale,
+                                       int64_t pages, int64_t kv_heads, int64_t head_dim, int64_t page_tokens,
+                                       const int32_t *block_table, int64_t table_stride, int64_t table_cols,
+                                       const int32_t *kv_len, const int32_t *cu_q, int64_t seqs,
+                                       const int32_t *group_seq, const int32_t *prefix_table, int64_t prefix_stride,
+                                       int64_t prefix_cols, const int32_t *prefix_len, int64_t groups, int64_t max_q,
+                                       int64_t max_own, int64_t max_prefix, float scale, int causal, void *workspace,
+                                       int64_t workspace_bytes, void *stream);
 
 /*
  * Measurement aid, no counterpart in the reference: reads `bytes` bytes

@@ -95,6 +95,18 @@ _SIGS = {
     "lcml_fp8_attention": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _vp, _int, _i64, _i64, _vp, _vp, _vp, _vp, _i64,
                                   _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _f32, _int, _i64,
                                   _vp, _i64, _vp]),
+    "lcml_fp8_attention_sinks": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _vp, _int, _i64, _i64, _vp, _vp, _vp, _vp,
+                                        _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _f32, _int,
+                                        _i64, _i64, _vp, _i64, _vp]),
+    "lcml_fp8_attention_shared_workspace_bytes": (_i64, [_i64] * 9),
+    "lcml_fp8_attention_shared": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _vp, _int, _i64, _i64, _vp, _vp, _vp, _vp,
+                                         _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64,
+                                         _vp, _i64, _i64, _i64, _i64, _f32, _int, _vp, _i64, _vp]),
+    "lcml_fp8_kv_cache_plan_workspace_bytes": (_i64, [_i64, _i64]),
+    "lcml_fp8_kv_cache_plan": (_int, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
+                                      _vp, _vp, _i64, _vp, _i64, _vp]),
+    "lcml_fp8_qk_norm_rope": (_int, [_vp, _vp, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _f32, _vp,
+                                     _vp, _i64, _i64, _int, _vp, _vp, _int, _i64, _i64, _i64, _i64, _vp]),
     "lcml_fp8_stream_read": (_int, [_vp, _i64, _int, _vp, _vp]),
 }
 
@@ -515,7 +527,7 @@ def binary(op: int, a: torch.Tensor, b: torch.Tensor, dtype: int, out: torch.Ten
     return y
 
 
-# ------------------------------------- norm, KV cache, attention -----------
+# ------------------------- norm, rotation, KV cache, attention -------------
 #
 # These run once or more for every layer and token, so their calls go through
 # the compiled module _binding (csrc/binding.cpp), which checks the tensors.
@@ -583,6 +595,65 @@ def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.T
                                     *_where(stream)))
 
 
+def kv_cache_plan(new_tokens: torch.Tensor, kv_len: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+                  free_count: torch.Tensor, page_tokens: int, tokens: int | None = None, ended: torch.Tensor | None = None,
+                  first_own: torch.Tensor | None = None, kv_len_out: torch.Tensor | None = None,
+                  cu_q: torch.Tensor | None = None, left: torch.Tensor | None = None,
+                  positions: torch.Tensor | None = None, slots: torch.Tensor | None = None,
+                  workspace: torch.Tensor | None = None, stream=None):
+    """A step's lengths, row offsets, pages and row indexes on the device, from
+    the tokens that each sequence brings (all int32 but slots, int64).
+    free_pages [pages] is a stack of free_count[0] pages: those of sequences that
+    `ended` (from column first_own on) go onto it, new columns of block_table
+    take them from its top, -1 when it is empty.  positions, slots [tokens]: of
+    the rows, -1 past the last (new tensors for `tokens` rows if they are not
+    given; without either they are left out).  kv_len_out may be kv_len, left
+    may be free_count.
+    Returns (kv_len_out, cu_q, left, positions, slots)."""
+    dev, i32 = new_tokens.device, torch.int32
+    kv_len_out = _empty(kv_len.shape, i32, dev, stream) if kv_len_out is None else kv_len_out
+    cu_q = _empty((kv_len.numel() + 1,), i32, dev, stream) if cu_q is None else cu_q
+    left = _empty((1,), i32, dev, stream) if left is None else left
+    if tokens is not None:
+        positions = _empty((tokens,), i32, dev, stream) if positions is None else positions
+        slots = _empty((tokens,), torch.int64, dev, stream) if slots is None else slots
+    if workspace is None:
+        rows = next((t.numel() for t in (positions, slots) if t is not None), 0)
+        need = lib().lcml_fp8_kv_cache_plan_workspace_bytes(kv_len.numel(), rows)
+        if need:
+            workspace = _empty((need,), torch.uint8, dev, stream)
+    _check(_binding().kv_cache_plan(new_tokens, kv_len, block_table, free_pages, free_count, page_tokens, ended, first_own,
+                                    kv_len_out, cu_q, left, positions, slots, workspace, *_where(stream)))
+    return kv_len_out, cu_q, left, positions, slots
+
+
+def rope_table(positions: int, rot_dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """[positions, rot_dim] fp32 for qk_norm_rope: of every position the cosines
+    and then the sines of position * base^(-2 i / rot_dim), from 64-bit angles."""
+    half = rot_dim // 2
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * \
+        base ** (-torch.arange(half, dtype=torch.float64) / max(half, 1))
+    return torch.cat([angle.cos(), angle.sin()], dim=1).float().to(device)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor | None, table: torch.Tensor | None,
+                 q_gamma: torch.Tensor | None = None, k_gamma: torch.Tensor | None = None, eps: float = 1e-6,
+                 interleaved: bool = False, q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None,
+                 out_dtype=None, stream=None):
+    """RMS norms of the heads of q [tokens, q_heads, head_dim] and k [tokens,
+    k_heads, head_dim] (fp32/bf16, any token and head strides; no norm without a
+    gamma) and the rotation of their first rot_dim elements by position, table
+    [rows, rot_dim] as from rope_table (None: no rotation).  Rows whose position is not in the
+    table are left as they were.  q_out may be q, k_out k.  Returns (q_out, k_out)."""
+    if q_out is None:
+        q_out = _empty(q.shape, out_dtype or q.dtype, q.device, stream)
+    if k is not None and k_out is None:
+        k_out = _empty(k.shape, q_out.dtype, q.device, stream)
+    _check(_binding().qk_norm_rope(q, k, positions, table, q_gamma, k_gamma, eps, int(interleaved), q_out, k_out,
+                                   *_where(stream)))
+    return q_out, k_out
+
+
 @functools.lru_cache(maxsize=256)
 def _attention_workspace(tokens, seqs, q_heads, kv_heads, dim, max_q, max_kv):
     return lib().lcml_fp8_attention_workspace_bytes(tokens, seqs, q_heads, kv_heads, dim, max_q, max_kv)
@@ -591,10 +662,11 @@ def _attention_workspace(tokens, seqs, q_heads, kv_heads, dim, max_q, max_kv):
 def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
               v_scale: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor, cu_q: torch.Tensor, max_q: int,
               max_kv: int, scale: float, causal: bool = True, window: int = 0, out: torch.Tensor | None = None,
-              out_dtype=None, workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+              out_dtype=None, workspace: torch.Tensor | None = None, stream=None, sinks: int = 0) -> torch.Tensor:
     """softmax(scale * q k^T) v over the E4M3 cache: q [tokens, q_heads,
     head_dim] (fp32/bf16) are the last tokens of their sequences, which the
-    cache already holds.  window > 0: only the last `window` positions.
+    cache already holds.  window > 0: only the last `window` positions, and the
+    first `sinks` ones.
     Weights are rounded to fp16 before they meet v: to 11 bits for bf16 results,
     to 22 for fp32 ones."""
     if out is None:
@@ -605,5 +677,34 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_s
         if need:
             workspace = _empty(need, torch.uint8, q.device, stream)
     _check(_binding().attention(q, out, k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q, max_q, max_kv,
-                                scale, causal, window, workspace, *_where(stream)))
+                                scale, causal, window, sinks, workspace, *_where(stream)))
+    return out
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_shared_workspace(*sizes):
+    return lib().lcml_fp8_attention_shared_workspace_bytes(*sizes)
+
+
+def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                     v_scale: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor, cu_q: torch.Tensor,
+                     group_seq: torch.Tensor, prefix_table: torch.Tensor, prefix_len: torch.Tensor, max_q: int,
+                     max_own: int, max_prefix: int, scale: float, causal: bool = True, out: torch.Tensor | None = None,
+                     out_dtype=None, workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """attention() for groups of sequences that share their first tokens: group g
+    is the sequences group_seq[g] .. group_seq[g+1]-1, and its first
+    prefix_len[g] tokens are read once for all of them, from the pages
+    prefix_table[g] (block_table's rows begin with the same ones).  max_own:
+    the most tokens that a sequence has behind them."""
+    if out is None:
+        out = _empty(q.shape, out_dtype or q.dtype, q.device, stream)
+    if workspace is None:
+        tokens, heads, dim = q.shape
+        need = _attention_shared_workspace(tokens, kv_len.numel(), prefix_len.numel(), heads, k_cache.shape[1], dim, max_q,
+                                           max_own, max_prefix)
+        if need:
+            workspace = _empty((need,), torch.uint8, q.device, stream)
+    _check(_binding().attention_shared(q, out, k_cache, v_cache, k_scale, v_scale, block_table, kv_len, cu_q, group_seq,
+                                       prefix_table, prefix_len, max_q, max_own, max_prefix, scale, causal, workspace,
+                                       *_where(stream)))
     return out

@@ -1,4 +1,6 @@
-// attention.hip -- attention over the E4M3 KV cache (gfx950).
+// attention_kernels.hpp -- attention over the E4M3 KV cache (gfx950): the
+// kernels and their plans, for attention.hip, attention_sinks.hip and
+// attention_shared.hip, which build them for their calls.
 //
 //   o = sum_j w_j v_j / sum_j w_j,   w_j = exp(scale q.k_j)
 // over the tokens j that a query sees: j < kv_len, j <= its own position
@@ -25,6 +27,8 @@
 // but for one exchange between lanes, and S^T's accumulators are P^T's operand
 // as they stand, because a reduction may run over the tokens in any order and
 // V lies in the cache in just this one.
+#pragma once
+
 #include "kv_cache.hpp"
 #include "lcml_internal.hpp"
 
@@ -263,28 +267,154 @@ struct Split {
     int32_t group;                 // q heads of a KV head
     float *o, *lse;
     Divider by_splits, by_tiles, by_heads, by_group, by_per;  // by_per: of tiles * splits
+    int32_t parts, first;  // kPrefix, kOwn: a row's parts of both, and where this one's begin
 };
 
-// positions that query i of a sequence sees: lo .. hi-1, neither falling with i
-__device__ inline void sees(const AttentionArgs &a, const SeqRows &s, int32_t i, int32_t *lo, int32_t *hi) {
+// Which tokens a call reads of a sequence:
+//   kPlain   one range, as causality and the window bound it
+//   kSinks   also the first `sinks` positions, wherever the window has gone.
+//            Steps run over an axis that leaves out whole steps between the two.
+//   kPrefix  for all rows of a group of sequences, the tokens that these share
+//   kOwn     the tokens from there on, or all where a sequence's rows do not
+//            lie behind what it shares
+// The last two leave parts in the workspace, which one join puts together.
+enum Form { kPlain, kSinks, kPrefix, kOwn };
+template <Form F>
+constexpr bool kShares = F == kPrefix || F == kOwn;
+
+template <Form F>
+__device__ inline bool in_parts(const Split &sp) {
+    return kShares<F> || sp.splits > 1;
+}
+// a row's part in the workspace
+template <Form F>
+__device__ inline int64_t part_at(const Split &sp, int64_t row, int32_t split) {
+    return kShares<F> ? row * sp.parts + sp.first + split : row * sp.splits + split;
+}
+
+// the rows of group g, and the tokens that it shares; n 0: none
+__device__ inline SeqRows group_rows(const AttentionArgs &a, int32_t g) {
+    SeqRows s{0, 0, 0, 0};
+    if (g >= a.groups) return s;
+    const int32_t b0 = a.group_seq[g], b1 = a.group_seq[g + 1], len = a.prefix_len[g];
+    if (b0 < 0 || b1 < b0 || b1 > a.t.seqs || len <= 0) return s;
+    const int32_t row0 = a.t.cu[b0], end = a.t.cu[b1];
+    if (row0 < 0 || end > a.t.tokens || end < row0) return s;
+    return SeqRows{row0, end - row0, len, len};
+}
+
+// the tokens that sequence b reads with its group; 0: none, also where its rows
+// do not all lie behind them (b the same in all lanes, and all lanes active)
+__device__ inline int32_t shared_tokens(const AttentionArgs &a, int32_t b, const SeqRows &s) {
+    const int32_t lane = threadIdx.x & 63;
+    int32_t len = 0;
+    for (int32_t g0 = 0; g0 < a.groups; g0 += 64) {
+        const int32_t g = g0 + lane;
+        const bool in = g < a.groups;
+        const int32_t end = in ? a.group_seq[g + 1] : 0x7fffffff, own = in ? a.prefix_len[g] : 0;
+        const uint64_t over = __builtin_amdgcn_ballot_w64(end > b);  // b's group, and those after it
+        if (!over) continue;
+        len = __builtin_amdgcn_readlane(own, __builtin_ctzll(over));
+        break;
+    }
+    return len > 0 && s.pos0 >= len ? len : 0;
+}
+
+// the same, for a sequence of a lane's own
+__device__ inline int32_t shared_tokens_of_lane(const AttentionArgs &a, int32_t b, const SeqRows &s) {
+    int32_t lo = 0, hi = a.groups;  // the first group that ends behind b
+    while (lo < hi) {
+        const int32_t m = (lo + hi) >> 1;
+        if (a.group_seq[m + 1] > b)
+            hi = m;
+        else
+            lo = m + 1;
+    }
+    const int32_t len = lo < a.groups ? a.prefix_len[lo] : 0;
+    return len > 0 && s.pos0 >= len ? len : 0;
+}
+
+// A workgroup's rows: of which sequence (kPrefix: group), which tile of them,
+// and the first position that they may see.
+struct Work {
+    SeqRows s;
+    int32_t b, tile, from;
+};
+// tile `id` of sequence b; kPrefix: among the tiles that the groups have, one
+// group's after the other's
+template <Form F, int ROWS>
+__device__ inline Work work_of(const AttentionArgs &a, const Split &sp, int32_t b, uint32_t id) {
+    if constexpr (F == kPrefix) {
+        const int32_t lane = threadIdx.x & 63;
+        uint32_t before = 0;
+        for (int32_t g0 = 0; g0 < a.groups; g0 += 64) {
+            const SeqRows s = group_rows(a, g0 + lane);
+            const uint32_t tiles = ((uint32_t)s.n * sp.group + ROWS - 1) / ROWS;
+            uint32_t sum = tiles;  // of the lanes up to this one
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) {
+                const uint32_t v = __shfl_up(sum, m);
+                sum += lane >= m ? v : 0;
+            }
+            const uint64_t over = __builtin_amdgcn_ballot_w64(before + sum > id);
+            if (over) {
+                const int at = __builtin_ctzll(over);
+                const auto of = [&](int32_t v) { return __builtin_amdgcn_readlane(v, at); };
+                const uint32_t tile = id - before - of((int32_t)(sum - tiles));
+                if (tile >= (uint32_t)of((int32_t)tiles)) break;  // groups that overlap
+                return Work{SeqRows{of(s.row0), of(s.n), of(s.pos0), of(s.len)}, g0 + at, (int32_t)tile, 0};
+            }
+            before += __builtin_amdgcn_readlane((int32_t)sum, 63);
+        }
+        return Work{SeqRows{0, 0, 0, 0}, 0, 0, 0};
+    } else {
+        const SeqRows s = seq_rows(a.t, b);
+        return Work{s, b, (int32_t)id, F == kOwn ? shared_tokens(a, b, s) : 0};
+    }
+}
+
+// positions that query i of a sequence sees: lo .. hi-1, neither falling with
+// i; kSinks: and 0 .. sinks-1 below hi; kOwn: from `from` on
+template <Form F>
+__device__ inline void sees(const AttentionArgs &a, const SeqRows &s, int32_t from, int32_t i, int32_t *lo, int32_t *hi) {
     const int32_t pos = s.pos0 + i, w = (int32_t)a.window;  // below 2^31; 0: no window
     const int32_t h = a.causal && pos < s.len ? pos + 1 : s.len;
-    const int32_t l = w > 0 && pos >= w ? pos - w + 1 : 0;
+    int32_t l = w > 0 && pos >= w ? pos - w + 1 : 0;
+    if (F == kOwn) l = l > from ? l : from;
     *hi = h > 0 ? h : 0;
     *lo = l < *hi ? l : *hi;
 }
+// whether position j is seen by a row of lo, hi
+template <Form F>
+__device__ inline bool seen(const AttentionArgs &a, int32_t j, int32_t lo, int32_t hi) {
+    return j < hi && (j >= lo || (F == kSinks && j < a.sinks));
+}
 
 // the part of positions lo .. hi-1 that is this workgroup's, from a multiple of
-// 64 on, in steps of 64
+// 64 on, in steps of 64; kSinks: start lies on the axis that leaves out `gap`
+// positions (whole steps) after the first `edge` ones, which hold the sinks
 struct Part {
-    int32_t start, end, steps;
+    int32_t start, end, steps, edge, gap;
 };
+template <Form F>
 __device__ inline Part part_of(const AttentionArgs &a, const Split &sp, int32_t split, int32_t lo, int32_t hi) {
+    int32_t edge = 0, gap = 0;
+    if (F == kSinks) {
+        const int64_t up = ((int64_t)(a.sinks < hi ? a.sinks : hi) + 63) & ~63;
+        edge = (int32_t)(up < 0x7fffffc0 ? up : 0x7fffffc0), gap = (lo & ~63) > edge ? (lo & ~63) - edge : 0;
+        lo = 0, hi -= gap;
+    }
     const int64_t from = (lo & ~63) + (int64_t)split * sp.chunk;
     int64_t to = split + 1 < sp.splits ? from + sp.chunk : hi;
     to = to < hi ? to : hi;
-    if (from >= to || a.t.pages == 0) return Part{0, 0, 0};
-    return Part{(int32_t)from, (int32_t)to, (int32_t)((to - from + 63) >> 6)};
+    if (from >= to || a.t.pages == 0) return Part{0, 0, 0, 0, 0};
+    return Part{(int32_t)from, (int32_t)(F == kSinks && to > edge ? to + gap : to), (int32_t)((to - from + 63) >> 6), edge, gap};
+}
+// the first token of the part's step k
+template <Form F>
+__device__ inline int32_t step_token(const Part &p, int32_t k) {
+    const int32_t at = p.start + (k << 6);
+    return F == kSinks && at >= p.edge ? at + p.gap : at;
 }
 
 // ----------------------------------------------- few rows for each KV head --
@@ -300,7 +430,7 @@ __device__ inline Part part_of(const AttentionArgs &a, const Split &sp, int32_t 
 // tokens of 8 KV heads of 128, 619 MB: 120 us, 5.2 TB/s; fp32 queries and
 // results 130.  One over 500 tokens: 8.4 us, five dependent round trips to
 // memory (lengths, table, scales, codes, the join's LDS); fp32 10.
-template <int DC, int NQ, int NP, int NW>
+template <int DC, int NQ, int NP, int NW, Form F>
 __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(AttentionArgs a, Split sp) {
     constexpr int DP = DC * 64, kPitch = DP + 4;
     __shared__ float red_m[NW][16], red_l[NW][16];
@@ -310,29 +440,31 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
     const int32_t D = a.t.dim, G = sp.group;
     const uint32_t id0 = blockIdx.x, id1 = sp.by_heads.div(id0), id2 = sp.by_splits.div(id1);
     const int32_t head = id0 - id1 * a.t.heads, split = id1 - id2 * sp.splits;
-    const int32_t b = sp.by_tiles.div(id2), tile = id2 - b * sp.tiles;
-    const SeqRows s = seq_rows(a.t, b);
+    const int32_t seq = F == kPrefix ? 0 : sp.by_tiles.div(id2);
+    const Work work = work_of<F, 16>(a, sp, seq, id2 - seq * sp.tiles);
+    const SeqRows s = work.s;
+    const int32_t b = work.b;
     const int32_t rows = (s.n < (int32_t)a.max_q ? s.n : (int32_t)a.max_q) * G;
-    const int32_t row0 = tile * 16;
+    const int32_t row0 = work.tile * 16;
     if (row0 >= rows) return;
     const int32_t last = rows - row0 < 16 ? rows - 1 : row0 + 15;  // of the tile
     const int32_t row = row0 + r < last ? row0 + r : last;         // this lane's
     const int32_t qi = sp.by_group.div(row), qh = head * G + row - qi * G;
     int32_t lo, hi, lo_min, hi_min, lo_max, hi_max;
-    sees(a, s, qi, &lo, &hi);
-    sees(a, s, sp.by_group.div(row0), &lo_min, &hi_min);
-    sees(a, s, sp.by_group.div(last), &lo_max, &hi_max);
-    const Part part = part_of(a, sp, split, lo_min, hi_max);
+    sees<F>(a, s, work.from, qi, &lo, &hi);
+    sees<F>(a, s, work.from, sp.by_group.div(row0), &lo_min, &hi_min);
+    sees<F>(a, s, work.from, sp.by_group.div(last), &lo_max, &hi_max);
+    const Part part = part_of<F>(a, sp, split, lo_min, hi_max);
     const int64_t out_row = ((int64_t)s.row0 + qi) * a.q_heads + qh;
-    if (part.steps == 0 && sp.splits > 1) {
-        if (threadIdx.x < 16 && row0 + r <= last) sp.lse[out_row * sp.splits + split] = -kInf;
+    if (part.steps == 0 && in_parts<F>(sp)) {
+        if (threadIdx.x < 16 && row0 + r <= last) sp.lse[part_at<F>(sp, out_row, split)] = -kInf;
         return;
     }
     const int32_t mine = (part.steps - wave + NW - 1) / NW;
 
     Block blk;
     auto find = [&](int32_t k) {  // lane i: block i of the wavefront's next 16 steps
-        const int32_t tok = part.start + (((k + (lane >> 2)) * NW + wave) << 6) + (lane & 3) * 16;
+        const int32_t tok = step_token<F>(part, (k + (lane >> 2)) * NW + wave) + (lane & 3) * 16;
         blk = block_of(a, head, tok, find_page(a, b, tok, part.end));
     };
     u4 kk[4][DC], vv[4][DC];
@@ -409,6 +541,9 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
     bool nan = false;
     uint32_t ks[4], vs[4];
     Scales scales;
+    // kSinks: positions below these are seen by the lane's row, by any row, by all
+    const uint32_t sinks = a.sinks < hi ? a.sinks : hi, sinks_max = a.sinks < hi_max ? a.sinks : hi_max,
+                   sinks_min = a.sinks < hi_min ? a.sinks : hi_min;
     // one step's scores; then the next one's K is on its way
     auto products = [&](int32_t k, f4 (&t)[4]) {
 #pragma unroll
@@ -435,9 +570,12 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
         const uint32_t from = tok + 4 * g - lo;
 #pragma unroll
         for (int sb = 0; sb < 4; ++sb) {
-            const uint32_t span = vs[sb] ? hi - lo : 0;
+            const uint32_t span = vs[sb] ? hi - lo : 0, first = F == kSinks && vs[sb] ? sinks : 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) t[sb][i] = from + 16 * sb + i < span ? t[sb][i] : -kInf;
+            for (int i = 0; i < 4; ++i) {
+                const bool in = from + 16 * sb + i < span || (F == kSinks && (uint32_t)(tok + 4 * g + 16 * sb + i) < first);
+                t[sb][i] = in ? t[sb][i] : -kInf;
+            }
 #pragma unroll
             for (int j = 0; j < DC; ++j)
 #pragma unroll
@@ -448,10 +586,13 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
             const uint32_t all = tok + 4 * g - lo_min;
 #pragma unroll
             for (int sb = 0; sb < 4; ++sb) {
-                const uint32_t span = vs[sb] ? hi_max - lo_min : 0;
+                const uint32_t span = vs[sb] ? hi_max - lo_min : 0, first = F == kSinks && vs[sb] ? sinks_max : 0;
                 uint32_t seen = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) seen |= all + 16 * sb + i < span ? 0x80u << (8 * i) : 0u;
+                for (int i = 0; i < 4; ++i) {
+                    const bool in = all + 16 * sb + i < span || (F == kSinks && (uint32_t)(tok + 4 * g + 16 * sb + i) < first);
+                    seen |= in ? 0x80u << (8 * i) : 0u;
+                }
 #pragma unroll
                 for (int j = 0; j < DC; ++j)
 #pragma unroll
@@ -587,9 +728,10 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
     for (; k < mine; ++k) {
         int32_t tok;
         for (; k < mine; ++k) {
-            tok = part.start + ((k * NW + wave) << 6);
+            tok = step_token<F>(part, k * NW + wave);
             scales_of(k);
-            if (!(tok >= lo_max && tok + 64 <= hi_min && vs[0] && vs[1] && vs[2] && vs[3]) || scales.apart()) break;
+            const bool all = (tok >= lo_max && tok + 64 <= hi_min) || (F == kSinks && (uint32_t)tok + 64 <= sinks_min);
+            if (!(all && vs[0] && vs[1] && vs[2] && vs[3]) || scales.apart()) break;
             step(k, tok, std::false_type{});
         }
         if (k >= mine || scales.apart()) break;
@@ -602,7 +744,7 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
         scale_o(bits_f32(vref));
         for (; k < mine; ++k) {
             scales_of(k);
-            step_apart(k, part.start + ((k * NW + wave) << 6));
+            step_apart(k, step_token<F>(part, k * NW + wave));
         }
     }
 
@@ -625,19 +767,19 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
             *reinterpret_cast<f4 *>(&buf[wave][r][64 * j + 16 * g + 4 * i]) = f4{o[j][0][i], o[j][1][i], o[j][2][i], o[j][3][i]};
     if (__builtin_expect(nan, 0))  // V's NaN codes reach the rows that see their token, and no others
         for (int32_t k = 0; k < mine; ++k) {
-            const int32_t tok = part.start + ((k * NW + wave) << 6);
-            for (int32_t j = tok > lo_min ? tok : lo_min; j < tok + 64 && j < part.end; ++j) {
+            const int32_t tok = step_token<F>(part, k * NW + wave);
+            for (int32_t j = F == kSinks || tok > lo_min ? tok : lo_min; j < tok + 64 && j < part.end; ++j) {
                 const Block w = block_of(a, head, j, find_page(a, b, j, part.end));
                 if (!w.vs) continue;
                 const uint8_t *p = a.v + (w.lo | (uint64_t)w.hi << 32) * (uint64_t)(16 * D);
                 for (int32_t d = lane; d < D; d += 64)
                     if ((p[v_place(j & 15, d, D)] & 0x7f) == 0x7f)
                         for (int rr = 0; rr < 16; ++rr)
-                            if (j >= (int32_t)lane_of(lo, rr) && j < (int32_t)lane_of(hi, rr)) buf[wave][rr][d] = __builtin_nanf("");
+                            if (seen<F>(a, j, (int32_t)lane_of(lo, rr), (int32_t)lane_of(hi, rr))) buf[wave][rr][d] = __builtin_nanf("");
             }
         }
-    if (sp.splits > 1 && wave == 0 && g == 0 && row0 + r <= last)
-        sp.lse[out_row * sp.splits + split] = sum == 0.0f ? -kInf : top + __builtin_amdgcn_logf(sum);
+    if (in_parts<F>(sp) && wave == 0 && g == 0 && row0 + r <= last)
+        sp.lse[part_at<F>(sp, out_row, split)] = sum == 0.0f ? -kInf : top + __builtin_amdgcn_logf(sum);
     __syncthreads();
     const int32_t q4 = D >> 2;
     for (int32_t e = threadIdx.x; e < (last - row0 + 1) * q4; e += NW * 64) {
@@ -645,8 +787,8 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
         f4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < NW; ++w) v += *reinterpret_cast<const f4 *>(&buf[w][rr][d]);
-        if (sp.splits > 1)
-            *reinterpret_cast<f4 *>(sp.o + ((((int64_t)s.row0 + i) * a.q_heads + h) * sp.splits + split) * D + d) = v;
+        if (in_parts<F>(sp))
+            *reinterpret_cast<f4 *>(sp.o + part_at<F>(sp, ((int64_t)s.row0 + i) * a.q_heads + h, split) * D + d) = v;
         else
             store_o4<NP == 1>(a.o, ((int64_t)s.row0 + i) * a.o_token + (int64_t)h * a.o_head + d, v);
     }
@@ -672,7 +814,7 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
 // in three loops, always inlined: out of line, its registers lie in scratch.
 constexpr int kManyWaves = 4, kManyRows = 32 * kManyWaves;
 
-template <int DP, bool EXACT, int NQ, int NP>
+template <int DP, bool EXACT, int NQ, int NP, Form F>
 __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attention_many(AttentionArgs a, Split sp) {
     constexpr int KJ = DP / 32;  // pairs of 16-element pieces of K
     constexpr int MT = DP / 32;  // tiles of 32 columns of V
@@ -690,14 +832,16 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
     const int32_t D = EXACT ? DP : a.t.dim, G = sp.group;
     // workgroups of one sequence and KV head on one XCD (blockIdx modulo 8),
     // whose L2 then holds their K and V; the longest rows first
-    const uint32_t pairs = (uint32_t)a.t.seqs * a.t.heads, per = (uint32_t)sp.tiles * sp.splits;
+    const uint32_t pairs = F == kPrefix ? a.t.heads : (uint32_t)a.t.seqs * a.t.heads, per = (uint32_t)sp.tiles * sp.splits;
     const bool by_xcd = pairs % 8 == 0;
     const uint32_t id = by_xcd ? blockIdx.x / 8 : blockIdx.x, over = sp.by_per.div(id), rest = id - over * per;
     const uint32_t pair = by_xcd ? blockIdx.x % 8 + 8 * over : over;
-    const int32_t b = sp.by_heads.div(pair), head = pair - b * a.t.heads;
-    const int32_t place = sp.by_splits.div(rest), split = rest - place * sp.splits, tile = sp.tiles - 1 - place;
-    const SeqRows s = seq_rows(a.t, b);
-    const int32_t rows = (s.n < (int32_t)a.max_q ? s.n : (int32_t)a.max_q) * G, row0 = tile * kManyRows;
+    const int32_t place = sp.by_splits.div(rest), split = rest - place * sp.splits;
+    const int32_t seq = F == kPrefix ? 0 : sp.by_heads.div(pair), head = pair - seq * a.t.heads;
+    const Work work = work_of<F, kManyRows>(a, sp, seq, F == kPrefix ? place : sp.tiles - 1 - place);
+    const SeqRows s = work.s;
+    const int32_t b = work.b;
+    const int32_t rows = (s.n < (int32_t)a.max_q ? s.n : (int32_t)a.max_q) * G, row0 = work.tile * kManyRows;
     if (row0 >= rows) return;
     const int32_t last = rows - row0 < kManyRows ? rows - 1 : row0 + kManyRows - 1;
     // this wavefront's rows and this lane's
@@ -708,23 +852,29 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
     // tokens that this lane's row sees, that any row sees and that all do, of
     // the workgroup and (any) of the wavefront
     int32_t lo, hi, lo_min, hi_min, lo_max, hi_max, w_lo, w_hi, unused;
-    sees(a, s, qi, &lo, &hi);
-    sees(a, s, sp.by_group.div(row0), &lo_min, &hi_min);
-    sees(a, s, sp.by_group.div(last), &lo_max, &hi_max);
-    sees(a, s, sp.by_group.div(w0), &w_lo, &unused);
-    sees(a, s, sp.by_group.div(w1), &unused, &w_hi);
-    const Part part = part_of(a, sp, split, lo_min, hi_max);
+    sees<F>(a, s, work.from, qi, &lo, &hi);
+    sees<F>(a, s, work.from, sp.by_group.div(row0), &lo_min, &hi_min);
+    sees<F>(a, s, work.from, sp.by_group.div(last), &lo_max, &hi_max);
+    sees<F>(a, s, work.from, sp.by_group.div(w0), &w_lo, &unused);
+    sees<F>(a, s, work.from, sp.by_group.div(w1), &unused, &w_hi);
+    const Part part = part_of<F>(a, sp, split, lo_min, hi_max);
     const int64_t out_row = ((int64_t)s.row0 + qi) * a.q_heads + qh;
-    if (part.steps == 0 && sp.splits > 1) {
-        if (h == 0 && live) sp.lse[out_row * sp.splits + split] = -kInf;
+    if (part.steps == 0 && in_parts<F>(sp)) {
+        if (h == 0 && live) sp.lse[part_at<F>(sp, out_row, split)] = -kInf;
         return;
     }
+    // kSinks: positions below these are seen by the lane's row, by any row of
+    // the wavefront, by all rows
+    const uint32_t sinks = a.sinks < hi ? a.sinks : hi, sinks_wave = a.sinks < w_hi ? a.sinks : w_hi,
+                   sinks_min = a.sinks < hi_min ? a.sinks : hi_min;
+    // whether any row of the wavefront sees one of the step's tokens
+    auto touches = [&](int32_t tok) { return (tok < w_hi && tok + 64 > w_lo) || (F == kSinks && (uint32_t)tok < sinks_wave); };
 
     // lane i: block i of 16 steps; the next 16 steps' pages and blocks are
     // looked up while these are worked on
     Block blk, next;
     int32_t next_page = -1;
-    auto token_of = [&](int32_t k) { return part.start + ((k + (lane >> 2)) << 6) + (lane & 3) * 16; };
+    auto token_of = [&](int32_t k) { return step_token<F>(part, k + (lane >> 2)) + (lane & 3) * 16; };
     uint32_t ks[4], vs[4], ks_next[4], vs_next[4];
     bool whole, whole_next = false;  // whether every row sees all of a step's tokens
     Scales scales;                   // of the steps fetched so far, the same for all wavefronts
@@ -734,11 +884,11 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
         const int i = (k & 15) * 4;
 #pragma unroll
         for (int q = 0; q < 4; ++q) ks_next[q] = lane_of(blk.ks, i + q), vs_next[q] = lane_of(blk.vs, i + q);
-        const int32_t tok = part.start + (k << 6);
+        const int32_t tok = step_token<F>(part, k);
         uint32_t least = vs_next[0] < vs_next[1] ? vs_next[0] : vs_next[1];
         least = vs_next[2] < least ? vs_next[2] : least;
         least = vs_next[3] < least ? vs_next[3] : least;
-        whole_next = tok >= lo_max && tok + 64 <= hi_min && least;
+        whole_next = ((tok >= lo_max && tok + 64 <= hi_min) || (F == kSinks && (uint32_t)tok + 64 <= sinks_min)) && least;
         scales.take(vs_next);
         const uint64_t at = (lane_of(blk.lo, i + wave) | (uint64_t)lane_of(blk.hi, i + wave) << 32) * (uint64_t)(16 * D);
         const uint8_t *pk = a.k + at, *pv = a.v + at;
@@ -756,7 +906,7 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
         if (__builtin_expect(!whole_next, 0)) {
             // what lies past the last token counts as zeros, and so do NaN codes
             // for now
-            const int32_t left = part.end - (part.start + (k << 6) + 16 * wave);
+            const int32_t left = part.end - (step_token<F>(part, k) + 16 * wave);
             uint32_t bad = 0;
 #pragma unroll
             for (int x = 0; x < PL; ++x) {
@@ -855,11 +1005,12 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
             const uint32_t from = tok + 4 * h - lo;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const uint32_t span = vs[q] ? hi - lo : 0;
+                const uint32_t span = vs[q] ? hi - lo : 0, first = F == kSinks && vs[q] ? sinks : 0;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const int at = (q & 1) * 8 + i;
-                    t[q >> 1][at] = from + 16 * q + 8 * (i >> 2) + (i & 3) < span ? t[q >> 1][at] : -kInf;
+                    const int at = (q & 1) * 8 + i, off = 16 * q + 8 * (i >> 2) + (i & 3);
+                    const bool in = from + off < span || (F == kSinks && (uint32_t)(tok + 4 * h + off) < first);
+                    t[q >> 1][at] = in ? t[q >> 1][at] : -kInf;
                 }
             }
         }
@@ -994,12 +1145,12 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
             }
             before(k);
             if (__builtin_expect(!whole, 0)) break;
-            step(part.start + (k << 6), k & 1, std::false_type{});
+            step(step_token<F>(part, k), k & 1, std::false_type{});
             after(k);
         }
         if (k >= part.steps || apart) break;
-        const int32_t tok = part.start + (k << 6);
-        if (tok < w_hi && tok + 64 > w_lo) step(tok, k & 1, std::true_type{});
+        const int32_t tok = step_token<F>(part, k);
+        if (touches(tok)) step(tok, k & 1, std::true_type{});
         after(k);
     }
     l = sum_over_halves(l);
@@ -1008,8 +1159,8 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
         scale_o(bits_f32(vref));
         for (; k < part.steps; ++k) {
             before(k);
-            const int32_t tok = part.start + (k << 6);
-            if (tok < w_hi && tok + 64 > w_lo) step_apart(tok, k & 1);
+            const int32_t tok = step_token<F>(part, k);
+            if (touches(tok)) step_apart(tok, k & 1);
             after(k);
         }
     }
@@ -1024,14 +1175,20 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
 #pragma unroll
             for (int i = 0; i < 16; ++i) hit[y][i] = 0.0f;
 #pragma unroll 1
-        for (int32_t tok = part.start; tok < part.end; tok += 16) {
+        for (int32_t at = part.start; at < part.start + part.steps * 64; at += 16) {
+            const int32_t tok = F == kSinks && at >= part.edge ? at + part.gap : at;
+            if (tok >= part.end) break;
             const Block w = block_of(a, head, tok, find_page(a, b, tok, part.end));
             if (!w.vs) continue;
             const uint8_t *p = a.v + (w.lo | (uint64_t)w.hi << 32) * (uint64_t)(16 * D) + h * 4 * D;
             const uint32_t from = tok + 4 * h - lo, span = hi - lo;
             h8 on;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) on[e] = from + 8 * (e >> 2) + (e & 3) < span ? (_Float16)1.0f : (_Float16)0.0f;
+            for (int e = 0; e < 8; ++e) {
+                const int off = 8 * (e >> 2) + (e & 3);
+                const bool in = from + off < span || (F == kSinks && (uint32_t)(tok + 4 * h + off) < sinks);
+                on[e] = in ? (_Float16)1.0f : (_Float16)0.0f;
+            }
 #pragma unroll
             for (int y = 0; y < MT; ++y) {
                 const int place = 32 * y + r, d = 4 * (place % (DP / 4)) + place / (DP / 4);
@@ -1069,9 +1226,9 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
                 if (EXACT || d < D) put(d, v);
             }
     };
-    if (sp.splits > 1) {
-        float *po = sp.o + (out_row * sp.splits + split) * D;
-        if (h == 0) sp.lse[out_row * sp.splits + split] = l == 0.0f ? -kInf : m + __builtin_amdgcn_logf(l);
+    if (in_parts<F>(sp)) {
+        float *po = sp.o + part_at<F>(sp, out_row, split) * D;
+        if (h == 0) sp.lse[part_at<F>(sp, out_row, split)] = l == 0.0f ? -kInf : m + __builtin_amdgcn_logf(l);
         results([&](int d, f4 v) { *reinterpret_cast<f4 *>(po + d) = v; });
     } else {
         const int64_t oo = ((int64_t)s.row0 + qi) * a.o_token + (int64_t)qh * a.o_head;
@@ -1081,9 +1238,21 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
 
 constexpr int kMostSplits = 128, kRowsSplits = 16;
 
+// how many parts a row has, and how many of the first ones do not count: the
+// prefix's, for rows that read it with their own tokens
+template <Form F>
+__device__ inline int32_t parts_of(const Split &sp) {
+    return kShares<F> ? sp.parts : sp.splits;
+}
+template <Form F, bool PER_LANE>
+__device__ inline int32_t skipped(const AttentionArgs &a, const Split &sp, int32_t b, const SeqRows &s) {
+    if constexpr (kShares<F>) return (PER_LANE ? shared_tokens_of_lane(a, b, s) : shared_tokens(a, b, s)) > 0 ? 0 : sp.first;
+    return 0;
+}
+
 // Joins few parts of many rows: D / 4 threads a row, as many rows a workgroup
 // as fit, and no barriers; every thread weighs all of its row's parts.
-template <bool BF16>
+template <bool BF16, Form F>
 __global__ __launch_bounds__(256) void k_attention_join_rows(AttentionArgs a, Split sp, uint32_t total) {
     const int32_t D = a.t.dim, q4 = D >> 2, per = 256 / q4;
     const int32_t grp = threadIdx.x / q4, d = (threadIdx.x - grp * q4) * 4;
@@ -1094,15 +1263,19 @@ __global__ __launch_bounds__(256) void k_attention_join_rows(AttentionArgs a, Sp
     const SeqRows s = seq_rows(a.t, b);
     if (i >= s.n) return;
     const int64_t row = ((int64_t)s.row0 + i) * a.q_heads + h;
-    const float *lse = sp.lse + row * sp.splits, *po = sp.o + row * sp.splits * D + d;
+    const int32_t parts = parts_of<F>(sp), skip = skipped<F, true>(a, sp, b, s);
+    const float *lse = sp.lse + row * parts, *po = sp.o + row * parts * D + d;
     float x[kRowsSplits], w[kRowsSplits], top = -kInf, sum = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kRowsSplits; ++k) x[k] = lse[k < sp.splits ? k : 0];
+    for (int k = 0; k < kRowsSplits; ++k) x[k] = lse[k < parts ? k : 0];
+    if (kShares<F>)
+#pragma unroll
+        for (int k = 0; k < kRowsSplits; ++k) x[k] = k < skip || k >= parts ? -kInf : x[k];
 #pragma unroll
     for (int k = 0; k < kRowsSplits; ++k) top = fmaxf(top, x[k]);
 #pragma unroll
     for (int k = 0; k < kRowsSplits; ++k) {
-        w[k] = k >= sp.splits || x[k] == -kInf ? 0.0f : x[k] == top ? 1.0f : __builtin_amdgcn_exp2f(x[k] - top);
+        w[k] = k >= parts || x[k] == -kInf ? 0.0f : x[k] == top ? 1.0f : __builtin_amdgcn_exp2f(x[k] - top);
         sum += w[k];
     }
     // weights divided by their sum: the parts' own could leave fp32's range
@@ -1110,11 +1283,11 @@ __global__ __launch_bounds__(256) void k_attention_join_rows(AttentionArgs a, Sp
     f4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k0 = 0; k0 < kRowsSplits; k0 += 4) {
-        if (k0 >= sp.splits) break;
+        if (k0 >= parts) break;
         f4 p[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u)  // a part of weight 0 wrote nothing
-            p[u] = k0 + u < sp.splits && x[k0 + u] != -kInf ? *reinterpret_cast<const f4 *>(po + (int64_t)(k0 + u) * D)
+            p[u] = k0 + u < parts && x[k0 + u] != -kInf ? *reinterpret_cast<const f4 *>(po + (int64_t)(k0 + u) * D)
                                                             : f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < 4; ++u) v += p[u] * (w[k0 + u] * inv);
@@ -1125,7 +1298,7 @@ __global__ __launch_bounds__(256) void k_attention_join_rows(AttentionArgs a, Sp
 // Joins a row's parts, a workgroup a row: the weights first, then the parts by
 // as many groups of D / 4 threads as there are, four loads each under way.
 
-template <bool BF16>
+template <bool BF16, Form F>
 __global__ __launch_bounds__(256) void k_attention_join(AttentionArgs a, Split sp) {
     __shared__ float weight[kMostSplits];
     __shared__ f4 buf[256];
@@ -1135,8 +1308,10 @@ __global__ __launch_bounds__(256) void k_attention_join(AttentionArgs a, Split s
     const SeqRows s = seq_rows(a.t, b);
     if (i >= s.n) return;
     const int64_t row = ((int64_t)s.row0 + i) * a.q_heads + h;
-    const float *lse = sp.lse + row * sp.splits, *po = sp.o + row * sp.splits * D;
-    const float x0 = lane < sp.splits ? lse[lane] : -kInf, x1 = lane + 64 < sp.splits ? lse[lane + 64] : -kInf;
+    const int32_t parts = parts_of<F>(sp), skip = skipped<F, false>(a, sp, b, s);
+    const float *lse = sp.lse + row * parts, *po = sp.o + row * parts * D;
+    const float x0 = lane < parts && lane >= skip ? lse[lane] : -kInf;
+    const float x1 = lane + 64 < parts && lane + 64 >= skip ? lse[lane + 64] : -kInf;
     float top = fmaxf(x0, x1);
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
@@ -1147,19 +1322,19 @@ __global__ __launch_bounds__(256) void k_attention_join(AttentionArgs a, Split s
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m);
     // weights divided by their sum: the parts' own could leave fp32's range
-    const float inv = 1.0f / sum;
+    const float inv = kShares<F> && sum == 0.0f ? 0.0f : 1.0f / sum;
     if (threadIdx.x < 64) weight[lane] = x0 == -kInf ? -1.0f : w0 * inv, weight[lane + 64] = x1 == -kInf ? -1.0f : w1 * inv;
     __syncthreads();
     const int32_t groups = 256 / q4, grp = threadIdx.x / q4, d = threadIdx.x % q4 * 4;
     f4 v{0.f, 0.f, 0.f, 0.f};
     if (grp < groups)
-        for (int32_t k0 = grp; k0 < sp.splits; k0 += 4 * groups) {
+        for (int32_t k0 = grp; k0 < parts; k0 += 4 * groups) {
             f4 p[4];
             float w[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int32_t k = k0 + u * groups;
-                w[u] = k < sp.splits ? weight[k] : -1.0f;
+                w[u] = k < parts ? weight[k] : -1.0f;
                 p[u] = w[u] >= 0.0f || w[u] != w[u] ? *reinterpret_cast<const f4 *>(po + (int64_t)k * D + d) : f4{0.f, 0.f, 0.f, 0.f};
             }
 #pragma unroll
@@ -1182,11 +1357,11 @@ struct Plan {
     Split sp;
 };
 
-int width_of(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }  // columns that the kernels are built for
+inline int width_of(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }  // columns that the kernels are built for
 
 // one kernel's division of rows of `pairs` (sequence, KV head), that see `span`
 // tokens at most
-Plan divide(bool few, int64_t pairs, int64_t rows, int64_t span) {
+inline Plan divide(bool few, int64_t pairs, int64_t rows, int64_t span) {
     Plan p{};
     p.few = few;
     const int64_t tile = few ? 16 : kManyRows;
@@ -1234,9 +1409,7 @@ Plan divide(bool few, int64_t pairs, int64_t rows, int64_t span) {
 // cost both kernels twice the products (2 x 200 19.1 and 18.6, 4 x 333 over 4000
 // 59 and 56).
 // max_kv decides, not the window: the workspace then covers any window.
-Plan make_plan(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t max_q, int64_t max_kv,
-               int64_t window) {
-    const int64_t rows = max_q * (q_heads / kv_heads), pairs = seqs * kv_heads;
+inline bool few_rows(int64_t pairs, int64_t dim, int64_t rows, int64_t max_kv) {
     bool few = rows <= 64;
     if (!few) {
         const Plan f = divide(true, pairs, rows, max_kv), m = divide(false, pairs, rows, max_kv);
@@ -1247,77 +1420,85 @@ Plan make_plan(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, int
         few = 3.0 + (rf > 1.0 ? rf : 1.0) * (3.5 + 2.5 * sf) + (f.sp.splits > 1 ? 4.0 : 0.0) <
               8.0 + (rm > 1.0 ? rm : 1.0) * step * sm + (m.sp.splits > 1 ? 6.0 : 0.0);
     }
+    return few;
+}
+inline Plan make_plan(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t max_q, int64_t max_kv,
+                      int64_t window, int64_t sinks) {
+    const int64_t rows = max_q * (q_heads / kv_heads), pairs = seqs * kv_heads;
     int64_t span = max_kv;  // tokens that a row tile can see
-    if (window > 0 && window < span && window + max_q + 64 < span) span = window + max_q + 64;
-    return divide(few, pairs, rows, span);
+    if (window > 0 && window < span && window + sinks + max_q + 128 < span)
+        span = window + max_q + 64 + (sinks + 63) / 64 * 64;
+    return divide(few_rows(pairs, dim, rows, max_kv), pairs, rows, span);
 }
 
-template <int DC, int NQ, int NP>
+template <Form F, int DC, int NQ, int NP>
 void start_few(const AttentionArgs &a, const Split &sp, unsigned grid, hipStream_t s) {
-    hipLaunchKernelGGL((k_attention_few<DC, NQ, NP, kFewWaves>), dim3(grid), dim3(kFewWaves * 64), 0, s, a, sp);
+    hipLaunchKernelGGL((k_attention_few<DC, NQ, NP, kFewWaves, F>), dim3(grid), dim3(kFewWaves * 64), 0, s, a, sp);
 }
 
-template <int DP, int NQ, int NP>
+template <Form F, int DP, int NQ, int NP>
 void start_many(const AttentionArgs &a, const Split &sp, unsigned grid, hipStream_t s) {
     if (a.t.dim == DP)
-        hipLaunchKernelGGL((k_attention_many<DP, true, NQ, NP>), dim3(grid), dim3(kManyWaves * 64), 0, s, a, sp);
+        hipLaunchKernelGGL((k_attention_many<DP, true, NQ, NP, F>), dim3(grid), dim3(kManyWaves * 64), 0, s, a, sp);
     else
-        hipLaunchKernelGGL((k_attention_many<DP, false, NQ, NP>), dim3(grid), dim3(kManyWaves * 64), 0, s, a, sp);
+        hipLaunchKernelGGL((k_attention_many<DP, false, NQ, NP, F>), dim3(grid), dim3(kManyWaves * 64), 0, s, a, sp);
 }
 
 // NQ = 1: q is bf16; NP = 1: o is
-template <int NQ, int NP>
-hipError_t launch_t(const AttentionArgs &a, const Plan &p, hipStream_t s) {
+template <Form F, int NQ, int NP>
+hipError_t start_attention(const AttentionArgs &a, const Plan &p, hipStream_t s) {
     const unsigned grid = (unsigned)p.groups;
     const int width = width_of(a.t.dim);
     if (p.few)
-        width == 64    ? start_few<1, NQ, NP>(a, p.sp, grid, s)
-        : width == 128 ? start_few<2, NQ, NP>(a, p.sp, grid, s)
-                       : start_few<4, NQ, NP>(a, p.sp, grid, s);
+        width == 64    ? start_few<F, 1, NQ, NP>(a, p.sp, grid, s)
+        : width == 128 ? start_few<F, 2, NQ, NP>(a, p.sp, grid, s)
+                       : start_few<F, 4, NQ, NP>(a, p.sp, grid, s);
     else
-        width == 64    ? start_many<64, NQ, NP>(a, p.sp, grid, s)
-        : width == 128 ? start_many<128, NQ, NP>(a, p.sp, grid, s)
-                       : start_many<256, NQ, NP>(a, p.sp, grid, s);
-    const hipError_t err = hipGetLastError();
-    if (err != hipSuccess || p.sp.splits == 1) return err;
+        width == 64    ? start_many<F, 64, NQ, NP>(a, p.sp, grid, s)
+        : width == 128 ? start_many<F, 128, NQ, NP>(a, p.sp, grid, s)
+                       : start_many<F, 256, NQ, NP>(a, p.sp, grid, s);
+    return hipGetLastError();
+}
+
+template <Form F, int NP>
+hipError_t start_join(const AttentionArgs &a, const Split &sp, int32_t parts, hipStream_t s) {
     const unsigned rows = (unsigned)((int64_t)a.t.seqs * a.max_q * a.q_heads);
     const unsigned per = 1024u / a.t.dim;
     // from 512 rows on many rows a workgroup (8 x 16 x 32 rows of 4 parts 40.5 us
     // with attention, a workgroup a row 44; 16384 rows of 2 parts 22 and 43; 128
     // rows of 16 parts 15.7 and 15.0, before the parts' weights were divided)
-    if (rows >= 512 && p.sp.splits <= kRowsSplits) {
-        hipLaunchKernelGGL((k_attention_join_rows<NP == 1>), dim3((rows + per - 1) / per), dim3(256), 0, s, a, p.sp, rows);
-        return hipGetLastError();
-    }
-    hipLaunchKernelGGL((k_attention_join<NP == 1>), dim3(rows), dim3(256), 0, s, a, p.sp);
+    if (rows >= 512 && parts <= kRowsSplits)
+        hipLaunchKernelGGL((k_attention_join_rows<NP == 1, F>), dim3((rows + per - 1) / per), dim3(256), 0, s, a, sp, rows);
+    else
+        hipLaunchKernelGGL((k_attention_join<NP == 1, F>), dim3(rows), dim3(256), 0, s, a, sp);
     return hipGetLastError();
 }
 
-}  // namespace
-
-int64_t attention_workspace(int64_t tokens, int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim,
-                            int64_t max_q, int64_t max_kv) {
-    const Plan p = make_plan(seqs, q_heads, kv_heads, dim, max_q, max_kv, 0);  // a window only takes parts away
-    return p.sp.splits > 1 ? tokens * q_heads * p.sp.splits * (dim + 1) * 4 : 0;
+// the divisors of a plan's indexes
+inline void set_divisors(Split &sp, const AttentionArgs &a) {
+    sp.group = a.q_heads / a.t.heads;
+    sp.by_splits = Divider::of(sp.splits), sp.by_tiles = Divider::of(sp.tiles);
+    sp.by_heads = Divider::of(a.t.heads), sp.by_group = Divider::of(sp.group);
+    sp.by_per = Divider::of((int64_t)sp.tiles * sp.splits);
 }
 
-int64_t attention_groups(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t max_q, int64_t max_kv) {
-    return make_plan(seqs, q_heads, kv_heads, dim, max_q, max_kv, 0).groups;
+// a call over one plan: attention, and the join where its rows are in parts
+template <Form F, int NQ, int NP>
+hipError_t launch_t(const AttentionArgs &a, const Plan &p, hipStream_t s) {
+    const hipError_t err = start_attention<F, NQ, NP>(a, p, s);
+    return err != hipSuccess || p.sp.splits == 1 ? err : start_join<F, NP>(a, p.sp, p.sp.splits, s);
 }
-
-hipError_t launch_attention(const AttentionArgs &a, void *work, hipStream_t s, const char **kernel) {
-    Plan p = make_plan(a.t.seqs, a.q_heads, a.t.heads, a.t.dim, a.max_q, a.max_kv, a.window);
-    p.sp.group = a.q_heads / a.t.heads;
-    p.sp.by_splits = Divider::of(p.sp.splits), p.sp.by_tiles = Divider::of(p.sp.tiles);
-    p.sp.by_heads = Divider::of(a.t.heads), p.sp.by_group = Divider::of(p.sp.group);
-    p.sp.by_per = Divider::of((int64_t)p.sp.tiles * p.sp.splits);
+template <Form F>
+hipError_t launch_form(const AttentionArgs &a, Plan &p, void *work, hipStream_t s, const char **kernel) {
+    set_divisors(p.sp, a);
     p.sp.o = static_cast<float *>(work);
     p.sp.lse = p.sp.o + (int64_t)a.t.tokens * a.q_heads * p.sp.splits * a.t.dim;
     const bool join = p.sp.splits > 1;
     *kernel = p.few ? (join ? "attention_few, attention_join" : "attention_few")
                     : (join ? "attention_many, attention_join" : "attention_many");
-    if (a.q_bf16) return a.o_bf16 ? launch_t<1, 1>(a, p, s) : launch_t<1, 2>(a, p, s);
-    return a.o_bf16 ? launch_t<2, 1>(a, p, s) : launch_t<2, 2>(a, p, s);
+    if (a.q_bf16) return a.o_bf16 ? launch_t<F, 1, 1>(a, p, s) : launch_t<F, 1, 2>(a, p, s);
+    return a.o_bf16 ? launch_t<F, 2, 1>(a, p, s) : launch_t<F, 2, 2>(a, p, s);
 }
 
+}  // namespace
 }  // namespace lcml

@@ -1,4 +1,4 @@
-// binding.cpp -- Python calls of the norm, KV cache and attention entry points
+// binding.cpp -- Python calls of the norm, rotation, KV cache and attention entry points
 // (module luisaml_amd._binding, host code only).
 //
 // A decode step makes these calls for every layer and token, and their kernels
@@ -195,31 +195,180 @@ PyObject *kv_cache_read(PyObject *, Args a, Py_ssize_t n) {
     });
 }
 
-// q, out, the cache's seven, max_q, max_kv, scale, causal, window, workspace, stream, device
+struct Workspace {
+    void *p = nullptr;
+    int64_t bytes = 0;
+};
+Workspace workspace(Tensors &tensor, PyObject *o) {
+    if (o == Py_None) return {};
+    const at::Tensor &w = tensor(o, "workspace");
+    need(w.is_contiguous(), "workspace: a contiguous tensor is expected");
+    return {w.data_ptr(), (int64_t)w.nbytes()};
+}
+
+// q, out, the cache's seven, max_q, max_kv, scale, causal, window, sinks, workspace, stream, device
 PyObject *attention(PyObject *, Args a, Py_ssize_t n) {
-    return guarded(n, 17, [&] {
+    return guarded(n, 18, [&] {
         Tensors tensor;
         const at::Tensor &q = tensor(a[0], "q"), &o = tensor(a[1], "out");
         const Cache c = cache(tensor, a + 2);
         heads_of(q, -1, c.dim, "q: [tokens, q_heads, head_dim] is expected");
         heads_of(o, q.size(1), c.dim, "out: q's shape is expected");
         need(o.size(0) == q.size(0), "out: q's shape is expected");
+        const int64_t sinks = integer(a[14], "sinks");
         void *ws = nullptr;
         int64_t bytes = 0;
-        if (a[14] != Py_None) {
-            const at::Tensor &w = tensor(a[14], "workspace");
+        if (a[15] != Py_None) {
+            const at::Tensor &w = tensor(a[15], "workspace");
             ws = w.data_ptr(), bytes = (int64_t)w.nbytes();
         }
+        if (sinks != 0)
+            return lcml_fp8_attention_sinks(q.data_ptr(), dtype_code(q), q.size(0), q.size(1), q.stride(0), q.stride(1),
+                                            o.data_ptr(), dtype_code(o), o.stride(0), o.stride(1), c.k, c.v, c.ks, c.vs, c.pages,
+                                            c.heads, c.dim, c.page, c.table, c.stride, c.cols, c.kv_len, c.cu_q, c.seqs,
+                                            integer(a[9], "max_q"), integer(a[10], "max_kv"), number(a[11], "scale"),
+                                            (int)integer(a[12], "causal"), integer(a[13], "window"), sinks, ws, bytes,
+                                            stream_of(tensor, a + 16));
         return lcml_fp8_attention(q.data_ptr(), dtype_code(q), q.size(0), q.size(1), q.stride(0), q.stride(1), o.data_ptr(),
                                   dtype_code(o), o.stride(0), o.stride(1), c.k, c.v, c.ks, c.vs, c.pages, c.heads, c.dim, c.page,
                                   c.table, c.stride, c.cols, c.kv_len, c.cu_q, c.seqs, integer(a[9], "max_q"),
                                   integer(a[10], "max_kv"), number(a[11], "scale"), (int)integer(a[12], "causal"),
-                                  integer(a[13], "window"), ws, bytes, stream_of(tensor, a + 15));
+                                  integer(a[13], "window"), ws, bytes, stream_of(tensor, a + 16));
+    });
+}
+
+// `count` contiguous int32, for any count if it is negative
+int32_t *ints(const at::Tensor &t, int64_t count, const char *what) {
+    need(t.scalar_type() == at::kInt && t.is_contiguous() && (count < 0 || t.numel() == count), what);
+    return static_cast<int32_t *>(t.data_ptr());
+}
+
+// rows of an int32 table that do not overlap
+struct Table {
+    int32_t *p;
+    int64_t stride, cols;
+};
+Table table_of(const at::Tensor &t, int64_t rows, const char *what) {
+    need(t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) == rows && (t.stride(1) == 1 || t.size(1) <= 1), what);
+    need(rows <= 1 || t.stride(0) >= t.size(1), what);
+    return {static_cast<int32_t *>(t.data_ptr()), t.stride(0) > t.size(1) ? t.stride(0) : t.size(1), t.size(1)};
+}
+
+// q, out, the cache's seven, group_seq, prefix_table, prefix_len, max_q, max_own, max_prefix, scale, causal, workspace,
+// stream, device
+PyObject *attention_shared(PyObject *, Args a, Py_ssize_t n) {
+    return guarded(n, 20, [&] {
+        Tensors tensor;
+        const at::Tensor &q = tensor(a[0], "q"), &o = tensor(a[1], "out");
+        const Cache c = cache(tensor, a + 2);
+        heads_of(q, -1, c.dim, "q: [tokens, q_heads, head_dim] is expected");
+        heads_of(o, q.size(1), c.dim, "out: q's shape is expected");
+        need(o.size(0) == q.size(0), "out: q's shape is expected");
+        const at::Tensor &len = tensor(a[11], "prefix_len");
+        const int64_t groups = len.numel();
+        const int32_t *prefix_len = ints(len, groups, "prefix_len: contiguous int32 [groups] is expected");
+        const int32_t *group_seq = ints(tensor(a[9], "group_seq"), groups + 1, "group_seq: contiguous int32 [groups + 1] is expected");
+        const Table t = table_of(tensor(a[10], "prefix_table"), groups,
+                                 "prefix_table: int32 [groups, columns] with contiguous rows that do not overlap is expected");
+        const Workspace w = workspace(tensor, a[17]);
+        return lcml_fp8_attention_shared(q.data_ptr(), dtype_code(q), q.size(0), q.size(1), q.stride(0), q.stride(1),
+                                         o.data_ptr(), dtype_code(o), o.stride(0), o.stride(1), c.k, c.v, c.ks, c.vs, c.pages,
+                                         c.heads, c.dim, c.page, c.table, c.stride, c.cols, c.kv_len, c.cu_q, c.seqs, group_seq,
+                                         t.p, t.stride, t.cols, prefix_len, groups, integer(a[12], "max_q"),
+                                         integer(a[13], "max_own"), integer(a[14], "max_prefix"), number(a[15], "scale"),
+                                         (int)integer(a[16], "causal"), w.p, w.bytes, stream_of(tensor, a + 18));
+    });
+}
+
+// new_tokens, kv_len, block_table, free_pages, free_count, page_tokens, ended, first_own, kv_len_out, cu_q, left, positions,
+// slots, workspace, stream, device
+PyObject *kv_cache_plan(PyObject *, Args a, Py_ssize_t n) {
+    return guarded(n, 16, [&] {
+        Tensors tensor;
+        const at::Tensor &len = tensor(a[1], "kv_len"), &free = tensor(a[3], "free_pages");
+        const int64_t seqs = len.numel(), pages = free.numel();
+        const Table t = table_of(tensor(a[2], "block_table"), seqs,
+                                 "block_table: int32 [seqs, columns] with contiguous rows that do not overlap is expected");
+        const auto some = [&](int i, const char *name, const char *what) -> int32_t * {
+            return a[i] == Py_None ? nullptr : ints(tensor(a[i], name), seqs, what);
+        };
+        int64_t rows = -1;
+        int32_t *positions = nullptr;
+        int64_t *slots = nullptr;
+        if (a[11] != Py_None) {
+            const at::Tensor &p = tensor(a[11], "positions");
+            positions = ints(p, -1, "positions: contiguous int32 is expected"), rows = p.numel();
+        }
+        if (a[12] != Py_None) {
+            const at::Tensor &s = tensor(a[12], "slots");
+            need(s.scalar_type() == at::kLong && s.is_contiguous() && (rows < 0 || s.numel() == rows),
+                 "slots: contiguous int64, as many as positions, is expected");
+            slots = static_cast<int64_t *>(s.data_ptr()), rows = s.numel();
+        }
+        const Workspace w = workspace(tensor, a[13]);
+        return lcml_fp8_kv_cache_plan(
+            ints(tensor(a[0], "new_tokens"), seqs, "new_tokens: contiguous int32 [seqs] is expected"),
+            ints(len, seqs, "kv_len: contiguous int32 [seqs] is expected"),
+            some(6, "ended", "ended: contiguous int32 [seqs] is expected"),
+            some(7, "first_own", "first_own: contiguous int32 [seqs] is expected"), seqs,
+            ints(free, pages, "free_pages: contiguous int32 [pages] is expected"),
+            ints(tensor(a[4], "free_count"), 1, "free_count: int32 [1] is expected"), pages, integer(a[5], "page_tokens"), t.p,
+            t.stride, t.cols, ints(tensor(a[8], "kv_len_out"), seqs, "kv_len_out: contiguous int32 [seqs] is expected"),
+            ints(tensor(a[9], "cu_q"), seqs + 1, "cu_q: contiguous int32 [seqs + 1] is expected"),
+            ints(tensor(a[10], "left"), 1, "left: int32 [1] is expected"), positions, slots, rows < 0 ? 0 : rows, w.p, w.bytes,
+            stream_of(tensor, a + 14));
+    });
+}
+
+// q, k, positions, table, q_gamma, k_gamma, eps, interleaved, q_out, k_out, stream, device
+PyObject *qk_norm_rope(PyObject *, Args a, Py_ssize_t n) {
+    return guarded(n, 12, [&] {
+        Tensors tensor;
+        const at::Tensor &q = tensor(a[0], "q"), &qo = tensor(a[8], "q_out");
+        need(q.dim() == 3, "q: [tokens, q_heads, head_dim] is expected");
+        const int64_t tokens = q.size(0), dim = q.size(2);
+        heads_of(q, -1, dim, "q: [tokens, q_heads, head_dim] is expected");
+        heads_of(qo, q.size(1), dim, "q_out: q's shape is expected");
+        need(qo.size(0) == tokens, "q_out: q's shape is expected");
+        const void *k = nullptr;
+        void *ko = nullptr;
+        int64_t k_heads = 0, kt = 0, kh = 0, kot = 0, koh = 0;
+        if (a[1] != Py_None) {
+            const at::Tensor &x = tensor(a[1], "k"), &y = tensor(a[9], "k_out");
+            heads_of(x, -1, dim, "k: [tokens, k_heads, head_dim] is expected");
+            heads_of(y, x.size(1), dim, "k_out: k's shape is expected");
+            need(x.size(0) == tokens && x.scalar_type() == q.scalar_type(), "k: q's tokens and type are expected");
+            need(y.size(0) == tokens && y.scalar_type() == qo.scalar_type(), "k_out: k's shape and q_out's type are expected");
+            k = x.data_ptr(), ko = y.data_ptr(), k_heads = x.size(1);
+            kt = x.stride(0), kh = x.stride(1), kot = y.stride(0), koh = y.stride(1);
+        } else {
+            need(a[9] == Py_None, "k_out without k");
+        }
+        const auto gamma = [&](int i, const char *name, const char *what) -> const float * {
+            if (a[i] == Py_None) return nullptr;
+            const at::Tensor &g = tensor(a[i], name);
+            need(g.scalar_type() == at::kFloat && g.numel() == dim && g.is_contiguous(), what);
+            return static_cast<const float *>(g.data_ptr());
+        };
+        const float *table = nullptr;
+        int64_t table_rows = 0, rot = 0;
+        if (a[3] != Py_None) {
+            const at::Tensor &t = tensor(a[3], "table");
+            need(t.scalar_type() == at::kFloat && t.dim() == 2 && t.is_contiguous(), "table: contiguous float [rows, rot_dim] is expected");
+            table = static_cast<const float *>(t.data_ptr()), table_rows = t.size(0), rot = t.size(1);
+        }
+        const int32_t *positions = a[2] == Py_None ? nullptr : ints(tensor(a[2], "positions"), tokens, "positions: contiguous int32 [tokens] is expected");
+        return lcml_fp8_qk_norm_rope(q.data_ptr(), k, dtype_code(q), tokens, q.size(1), k_heads, dim, q.stride(0), q.stride(1), kt,
+                                     kh, gamma(4, "q_gamma", "q_gamma: head_dim floats are expected"),
+                                     gamma(5, "k_gamma", "k_gamma: head_dim floats are expected"), number(a[6], "eps"), positions,
+                                     table, table_rows, rot, (int)integer(a[7], "interleaved"), qo.data_ptr(), ko, dtype_code(qo),
+                                     qo.stride(0), qo.stride(1), kot, koh, stream_of(tensor, a + 10));
     });
 }
 
 #define METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(f)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(rms_norm), METHOD(kv_cache_write), METHOD(kv_cache_read), METHOD(attention), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {METHOD(rms_norm), METHOD(kv_cache_write), METHOD(kv_cache_read), METHOD(attention), METHOD(attention_shared),
+                         METHOD(kv_cache_plan), METHOD(qk_norm_rope), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

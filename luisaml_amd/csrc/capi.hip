@@ -936,12 +936,177 @@ int lcml_fp8_kv_cache_read(const uint8_t *k_cache, const uint8_t *v_cache, const
                       fn);
 }
 
+int64_t lcml_fp8_kv_cache_plan_workspace_bytes(int64_t seqs, int64_t tokens) {
+    return seqs < 0 || tokens < 0 ? 0 : lcml::kv_plan_workspace(seqs, tokens);
+}
+
+int lcml_fp8_kv_cache_plan(const int32_t *new_tokens, const int32_t *kv_len_in, const int32_t *ended,
+                           const int32_t *first_own, int64_t seqs, int32_t *free_pages, const int32_t *free_count,
+                           int64_t pages, int64_t page_tokens, int32_t *block_table, int64_t table_stride,
+                           int64_t table_cols, int32_t *kv_len, int32_t *cu_q, int32_t *left, int32_t *positions,
+                           int64_t *slots, int64_t tokens, void *workspace, int64_t workspace_bytes, void *stream) {
+    const char *fn = "lcml_fp8_kv_cache_plan";
+    if (seqs < 0 || pages < 0 || table_cols < 0 || tokens < 0)
+        return fail(LCML_ERR_INVALID_ARG, "%s: seqs=%lld pages=%lld table_cols=%lld tokens=%lld", fn, (long long)seqs,
+                    (long long)pages, (long long)table_cols, (long long)tokens);
+    if (page_tokens < 16 || page_tokens > 256 || (page_tokens & (page_tokens - 1)))
+        return fail(LCML_ERR_UNSUPPORTED, "%s: page_tokens=%lld (16, 32, 64, 128 or 256)", fn, (long long)page_tokens);
+    const int64_t most = ((int64_t)1 << 31) - 1;
+    if (seqs >= most || pages > most || table_cols > most || tokens > most)
+        return fail(LCML_ERR_UNSUPPORTED, "%s: a size of 2^31 or more", fn);
+    if (table_stride < table_cols)
+        return fail(LCML_ERR_INVALID_ARG, "%s: table_stride=%lld < table_cols=%lld", fn, (long long)table_stride,
+                    (long long)table_cols);
+    if ((seqs && (!new_tokens || !kv_len_in || !kv_len || (table_cols && !block_table))) || (pages && !free_pages) ||
+        !free_count || !cu_q || !left)
+        return fail(LCML_ERR_INVALID_ARG, "%s: NULL index array", fn);
+    for (const void *p : {(const void *)new_tokens, (const void *)kv_len_in, (const void *)ended, (const void *)first_own,
+                          (const void *)free_pages, (const void *)free_count, (const void *)block_table,
+                          (const void *)kv_len, (const void *)cu_q, (const void *)left, (const void *)positions})
+        if (!aligned(p, 4)) return fail(LCML_ERR_INVALID_ARG, "%s: index arrays not 4-byte aligned", fn);
+    if (!aligned(slots, 8)) return fail(LCML_ERR_INVALID_ARG, "%s: slots not 8-byte aligned", fn);
+    if (const int64_t need = lcml::kv_plan_workspace(seqs, tokens);
+        need && (!workspace || workspace_bytes < need || !aligned(workspace, 8)))
+        return fail(LCML_ERR_INVALID_ARG, "%s: needs an 8-byte aligned workspace of %lld bytes", fn, (long long)need);
+    const lcml::KvPlan p{new_tokens, ended, first_own, kv_len_in, free_count, free_pages, block_table, table_stride,
+                         (int32_t)table_cols, (int32_t)seqs, (int32_t)pages,
+                         __builtin_ctzll((unsigned long long)page_tokens), kv_len, cu_q, left, positions, slots, tokens,
+                         static_cast<int64_t *>(workspace)};
+    const char *label = nullptr;
+    const hipError_t err = lcml::launch_kv_plan(p, (hipStream_t)stream, &label);
+    return hip_status(err, fn, label);
+}
+
+int lcml_fp8_qk_norm_rope(const void *q, const void *k, int dtype, int64_t tokens, int64_t q_heads, int64_t k_heads,
+                          int64_t head_dim, int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
+                          int64_t k_head_stride, const float *q_gamma, const float *k_gamma, float eps,
+                          const int32_t *positions, const float *table, int64_t table_rows, int64_t rot_dim,
+                          int interleaved, void *q_out, void *k_out, int out_dtype, int64_t qo_token_stride,
+                          int64_t qo_head_stride, int64_t ko_token_stride, int64_t ko_head_stride, void *stream) {
+    const char *fn = "lcml_fp8_qk_norm_rope";
+    if (!float_or_bf16(dtype) || !float_or_bf16(out_dtype))
+        return fail(LCML_ERR_UNSUPPORTED, "%s: dtypes %d, out %d", fn, dtype, out_dtype);
+    if (tokens < 0 || q_heads < 0 || k_heads < 0 || table_rows < 0)
+        return fail(LCML_ERR_INVALID_ARG, "%s: tokens=%lld q_heads=%lld k_heads=%lld table_rows=%lld", fn,
+                    (long long)tokens, (long long)q_heads, (long long)k_heads, (long long)table_rows);
+    if (head_dim < 16 || head_dim > 256 || head_dim % 16)
+        return fail(LCML_ERR_UNSUPPORTED, "%s: head_dim=%lld (16 to 256, in steps of 16)", fn, (long long)head_dim);
+    if (rot_dim < 0 || rot_dim > head_dim || rot_dim % 2)
+        return fail(LCML_ERR_INVALID_ARG, "%s: rot_dim=%lld (even, up to head_dim=%lld)", fn, (long long)rot_dim,
+                    (long long)head_dim);
+    if (!(eps >= 0.0f)) return fail(LCML_ERR_INVALID_ARG, "%s: eps %g", fn, (double)eps);
+    if (q_heads > 65535 || k_heads > 65535 || tokens >= (int64_t)1 << 31 || table_rows >= (int64_t)1 << 31)
+        return fail(LCML_ERR_UNSUPPORTED, "%s: tokens=%lld q_heads=%lld k_heads=%lld table_rows=%lld", fn,
+                    (long long)tokens, (long long)q_heads, (long long)k_heads, (long long)table_rows);
+    if (tokens == 0 || q_heads + k_heads == 0) return LCML_OK;
+    if ((q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out)) ||
+        (q_heads && (!elem_aligned(q, dtype) || !elem_aligned(q_out, out_dtype))) ||
+        (k_heads && (!elem_aligned(k, dtype) || !elem_aligned(k_out, out_dtype))))
+        return fail(LCML_ERR_INVALID_ARG, "%s: q, k or an output NULL or not aligned to its elements", fn);
+    if (rot_dim && (!positions || (table_rows && !table)))
+        return fail(LCML_ERR_INVALID_ARG, "%s: a rotation takes positions and a table", fn);
+    if (!aligned(q_gamma, 4) || !aligned(k_gamma, 4) || !aligned(positions, 4) || !aligned(table, 4))
+        return fail(LCML_ERR_INVALID_ARG, "%s: gammas, positions or table not 4-byte aligned", fn);
+    // 64 threads each, 2^32 work items a launch
+    if (tokens * lcml::qk_norm_rope_parts(tokens, (int32_t)q_heads, (int32_t)k_heads, (int32_t)head_dim) >= ((int64_t)1 << 26) - 4)
+        return fail(LCML_ERR_UNSUPPORTED, "%s: tokens=%lld exceeds one launch", fn, (long long)tokens);
+    const lcml::RopeArgs a{q, k, q_out, k_out, q_gamma, k_gamma, table, positions, q_token_stride,
+                           q_head_stride, k_token_stride, k_head_stride, qo_token_stride, qo_head_stride,
+                           ko_token_stride, ko_head_stride, tokens, (int32_t)q_heads, (int32_t)k_heads,
+                           (int32_t)head_dim, (int32_t)rot_dim,
+                           rot_dim ? (int32_t)table_rows : 0x7fffffff, interleaved != 0, eps,
+                           1.0f / (float)head_dim, 0};
+    return hip_status(lcml::launch_qk_norm_rope(a, dtype == LCML_DTYPE_BFLOAT16, out_dtype == LCML_DTYPE_BFLOAT16,
+                                                (hipStream_t)stream),
+                      fn);
+}
+
 int64_t lcml_fp8_attention_workspace_bytes(int64_t tokens, int64_t seqs, int64_t q_heads, int64_t kv_heads,
                                            int64_t head_dim, int64_t max_q, int64_t max_kv) {
     if (tokens <= 0 || seqs <= 0 || kv_heads <= 0 || q_heads < kv_heads || head_dim <= 0 || max_q <= 0 || max_kv <= 0)
         return 0;
     return lcml::attention_workspace(tokens, seqs, q_heads, kv_heads, head_dim, max_q, max_kv);
 }
+
+namespace {
+// what the attention entry points are given alike
+struct AttentionCall {
+    const void *q;
+    int q_dtype;
+    int64_t tokens, q_heads, q_token_stride, q_head_stride;
+    void *o;
+    int o_dtype;
+    int64_t o_token_stride, o_head_stride;
+    const uint8_t *k_cache, *v_cache;
+    const float *k_scale, *v_scale;
+    int64_t pages, kv_heads, head_dim, page_tokens;
+    const int32_t *block_table;
+    int64_t table_stride, table_cols;
+    const int32_t *kv_len, *cu_q;
+    int64_t seqs, max_q, max_kv;
+    float scale;
+    int causal;
+    int64_t window;
+};
+// 256 threads each, 2^32 work items a launch, and a workgroup for each row
+// where parts are joined; sizes whose products would pass 64 bits are past
+// that by far
+constexpr int64_t kMostGroups = (int64_t)1 << 24;
+
+int too_large(const char *fn, const AttentionCall &c) {
+    return fail(LCML_ERR_UNSUPPORTED, "%s: seqs=%lld max_q=%lld q_heads=%lld exceeds one launch", fn, (long long)c.seqs,
+                (long long)c.max_q, (long long)c.q_heads);
+}
+// Checks c and fills a; *rows false: a call without rows.
+int make_attention(lcml::AttentionArgs &a, const char *fn, const AttentionCall &c, bool *rows) {
+    if (!float_or_bf16(c.q_dtype) || !float_or_bf16(c.o_dtype))
+        return fail(LCML_ERR_UNSUPPORTED, "%s: dtypes q %d, o %d", fn, c.q_dtype, c.o_dtype);
+    if (!(c.scale > 0.0f) || c.scale > 3.0e38f) return fail(LCML_ERR_INVALID_ARG, "%s: scale %g", fn, (double)c.scale);
+    if (c.window < 0 || c.max_kv < 0)
+        return fail(LCML_ERR_INVALID_ARG, "%s: window=%lld max_kv=%lld", fn, (long long)c.window, (long long)c.max_kv);
+    if (int rc = make_tokens(a.t, fn, c.tokens, c.k_cache, c.v_cache, c.k_scale, c.v_scale, c.pages, c.kv_heads,
+                             c.head_dim, c.page_tokens, c.block_table, c.table_stride, c.table_cols, c.kv_len, c.cu_q,
+                             c.seqs, c.max_q))
+        return rc;
+    if (c.q_heads <= 0 || c.q_heads % c.kv_heads)
+        return fail(LCML_ERR_INVALID_ARG, "%s: q_heads=%lld is not a multiple of kv_heads=%lld", fn,
+                    (long long)c.q_heads, (long long)c.kv_heads);
+    if (c.q_heads > 65535 || c.max_kv >= (int64_t)1 << 31)
+        return fail(LCML_ERR_UNSUPPORTED, "%s: q_heads=%lld max_kv=%lld", fn, (long long)c.q_heads, (long long)c.max_kv);
+    *rows = c.tokens > 0 && c.seqs > 0 && c.max_q > 0;
+    if (!*rows) return LCML_OK;
+    if (!c.q || !c.o || !elem_aligned(c.q, c.q_dtype) || !elem_aligned(c.o, c.o_dtype))
+        return fail(LCML_ERR_INVALID_ARG, "%s: q or o NULL or not aligned to its elements", fn);
+    if (c.max_q * c.q_heads / c.kv_heads > kMostGroups * 16 || c.seqs * c.kv_heads > kMostGroups) return too_large(fn, c);
+    a.q = c.q, a.o = c.o, a.k = c.k_cache, a.v = c.v_cache, a.ks = c.k_scale, a.vs = c.v_scale;
+    a.q_token = c.q_token_stride, a.q_head = c.q_head_stride, a.o_token = c.o_token_stride, a.o_head = c.o_head_stride;
+    a.max_q = c.max_q, a.max_kv = c.max_kv;
+    a.window = c.window < (int64_t)1 << 31 ? c.window : 0;  // a longer one hides nothing
+    a.q_heads = (int32_t)c.q_heads, a.causal = c.causal != 0;
+    a.q_bf16 = c.q_dtype == LCML_DTYPE_BFLOAT16, a.o_bf16 = c.o_dtype == LCML_DTYPE_BFLOAT16;
+    a.scale = c.scale;
+    return LCML_OK;
+}
+
+// lcml_fp8_attention, and with sinks > 0 lcml_fp8_attention_sinks
+int attend(const char *fn, const AttentionCall &c, int64_t sinks, void *workspace, int64_t workspace_bytes, void *stream) {
+    lcml::AttentionArgs a{};
+    bool rows = false;
+    if (int rc = make_attention(a, fn, c, &rows)) return rc;
+    if (!rows) return LCML_OK;
+    if (lcml::attention_groups(c.seqs, c.q_heads, c.kv_heads, c.head_dim, c.max_q, c.max_kv) >= kMostGroups)
+        return too_large(fn, c);
+    const int64_t need = lcml::attention_workspace(c.tokens, c.seqs, c.q_heads, c.kv_heads, c.head_dim, c.max_q, c.max_kv);
+    if (need && c.seqs * c.max_q >= kMostGroups / c.q_heads) return too_large(fn, c);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+        return fail(LCML_ERR_INVALID_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", fn, (long long)need);
+    a.sinks = sinks < (int64_t)1 << 31 ? (uint32_t)sinks : 0x7fffffffu;
+    const char *label = nullptr;
+    const hipError_t err = a.window > 0 && sinks > 0 ? lcml::launch_attention_sinks(a, workspace, (hipStream_t)stream, &label)
+                                                     : lcml::launch_attention(a, workspace, (hipStream_t)stream, &label);
+    return hip_status(err, fn, label);
+}
+}  // namespace
 
 int lcml_fp8_attention(const void *q, int q_dtype, int64_t tokens, int64_t q_heads, int64_t q_token_stride,
                        int64_t q_head_stride, void *o, int o_dtype, int64_t o_token_stride, int64_t o_head_stride,
@@ -950,46 +1115,83 @@ int lcml_fp8_attention(const void *q, int q_dtype, int64_t tokens, int64_t q_hea
                        const int32_t *block_table, int64_t table_stride, int64_t table_cols, const int32_t *kv_len,
                        const int32_t *cu_q, int64_t seqs, int64_t max_q, int64_t max_kv, float scale, int causal,
                        int64_t window, void *workspace, int64_t workspace_bytes, void *stream) {
-    const char *fn = "lcml_fp8_attention";
-    if (!float_or_bf16(q_dtype) || !float_or_bf16(o_dtype))
-        return fail(LCML_ERR_UNSUPPORTED, "%s: dtypes q %d, o %d", fn, q_dtype, o_dtype);
-    if (!(scale > 0.0f) || scale > 3.0e38f) return fail(LCML_ERR_INVALID_ARG, "%s: scale %g", fn, (double)scale);
-    if (window < 0 || max_kv < 0)
-        return fail(LCML_ERR_INVALID_ARG, "%s: window=%lld max_kv=%lld", fn, (long long)window, (long long)max_kv);
+    return attend("lcml_fp8_attention",
+                  AttentionCall{q, q_dtype, tokens, q_heads, q_token_stride, q_head_stride, o, o_dtype, o_token_stride,
+                                o_head_stride, k_cache, v_cache, k_scale, v_scale, pages, kv_heads, head_dim, page_tokens,
+                                block_table, table_stride, table_cols, kv_len, cu_q, seqs, max_q, max_kv, scale, causal,
+                                window},
+                  0, workspace, workspace_bytes, stream);
+}
+
+int lcml_fp8_attention_sinks(const void *q, int q_dtype, int64_t tokens, int64_t q_heads, int64_t q_token_stride,
+                             int64_t q_head_stride, void *o, int o_dtype, int64_t o_token_stride, int64_t o_head_stride,
+                             const uint8_t *k_cache, const uint8_t *v_cache, const float *k_scale, const float *v_scale,
+                             int64_t pages, int64_t kv_heads, int64_t head_dim, int64_t page_tokens,
+                             const int32_t *block_table, int64_t table_stride, int64_t table_cols, const int32_t *kv_len,
+                             const int32_t *cu_q, int64_t seqs, int64_t max_q, int64_t max_kv, float scale, int causal,
+                             int64_t window, int64_t sinks, void *workspace, int64_t workspace_bytes, void *stream) {
+    const char *fn = "lcml_fp8_attention_sinks";
+    if (sinks < 0) return fail(LCML_ERR_INVALID_ARG, "%s: sinks=%lld", fn, (long long)sinks);
+    return attend(fn,
+                  AttentionCall{q, q_dtype, tokens, q_heads, q_token_stride, q_head_stride, o, o_dtype, o_token_stride,
+                                o_head_stride, k_cache, v_cache, k_scale, v_scale, pages, kv_heads, head_dim, page_tokens,
+                                block_table, table_stride, table_cols, kv_len, cu_q, seqs, max_q, max_kv, scale, causal,
+                                window},
+                  sinks, workspace, workspace_bytes, stream);
+}
+
+int64_t lcml_fp8_attention_shared_workspace_bytes(int64_t tokens, int64_t seqs, int64_t groups, int64_t q_heads,
+                                                  int64_t kv_heads, int64_t head_dim, int64_t max_q, int64_t max_own,
+                                                  int64_t max_prefix) {
+    if (tokens <= 0 || seqs <= 0 || groups < 0 || kv_heads <= 0 || q_heads < kv_heads || head_dim <= 0 || max_q <= 0 ||
+        max_own < 0 || max_prefix < 0)
+        return 0;
+    int64_t workgroups = 0;
+    return lcml::attention_shared_workspace(tokens, seqs, groups, q_heads, kv_heads, head_dim, max_q, max_own, max_prefix,
+                                            &workgroups);
+}
+
+int lcml_fp8_attention_shared(const void *q, int q_dtype, int64_t tokens, int64_t q_heads, int64_t q_token_stride,
+                              int64_t q_head_stride, void *o, int o_dtype, int64_t o_token_stride, int64_t o_head_stride,
+                              const uint8_t *k_cache, const uint8_t *v_cache, const float *k_scale, const float *v_scale,
+                              int64_t pages, int64_t kv_heads, int64_t head_dim, int64_t page_tokens,
+                              const int32_t *block_table, int64_t table_stride, int64_t table_cols, const int32_t *kv_len,
+                              const int32_t *cu_q, int64_t seqs, const int32_t *group_seq, const int32_t *prefix_table,
+                              int64_t prefix_stride, int64_t prefix_cols, const int32_t *prefix_len, int64_t groups,
+                              int64_t max_q, int64_t max_own, int64_t max_prefix, float scale, int causal,
+                              void *workspace, int64_t workspace_bytes, void *stream) {
+    const char *fn = "lcml_fp8_attention_shared";
+    const AttentionCall c{q, q_dtype, tokens, q_heads, q_token_stride, q_head_stride, o, o_dtype, o_token_stride,
+                          o_head_stride, k_cache, v_cache, k_scale, v_scale, pages, kv_heads, head_dim, page_tokens,
+                          block_table, table_stride, table_cols, kv_len, cu_q, seqs, max_q, max_own, scale, causal, 0};
     lcml::AttentionArgs a{};
-    if (int rc = make_tokens(a.t, fn, tokens, k_cache, v_cache, k_scale, v_scale, pages, kv_heads, head_dim, page_tokens,
-                             block_table, table_stride, table_cols, kv_len, cu_q, seqs, max_q))
-        return rc;
-    if (q_heads <= 0 || q_heads % kv_heads)
-        return fail(LCML_ERR_INVALID_ARG, "%s: q_heads=%lld is not a multiple of kv_heads=%lld", fn, (long long)q_heads,
-                    (long long)kv_heads);
-    if (q_heads > 65535 || max_kv >= (int64_t)1 << 31)
-        return fail(LCML_ERR_UNSUPPORTED, "%s: q_heads=%lld max_kv=%lld", fn, (long long)q_heads, (long long)max_kv);
-    if (tokens == 0 || seqs == 0 || max_q == 0) return LCML_OK;
-    if (!q || !o || !elem_aligned(q, q_dtype) || !elem_aligned(o, o_dtype))
-        return fail(LCML_ERR_INVALID_ARG, "%s: q or o NULL or not aligned to its elements", fn);
-    // 256 threads each, 2^32 work items a launch, and a workgroup for each row
-    // where parts are joined; sizes whose products would pass 64 bits are past
-    // that by far
-    const int64_t most = (int64_t)1 << 24;
-    if (max_q * q_heads / kv_heads > most * 16 || seqs * kv_heads > most ||
-        lcml::attention_groups(seqs, q_heads, kv_heads, head_dim, max_q, max_kv) >= most)
-        return fail(LCML_ERR_UNSUPPORTED, "%s: seqs=%lld max_q=%lld q_heads=%lld exceeds one launch", fn,
-                    (long long)seqs, (long long)max_q, (long long)q_heads);
-    const int64_t need = lcml::attention_workspace(tokens, seqs, q_heads, kv_heads, head_dim, max_q, max_kv);
-    if (need && seqs * max_q >= most / q_heads)
-        return fail(LCML_ERR_UNSUPPORTED, "%s: seqs=%lld max_q=%lld q_heads=%lld exceeds one launch", fn,
-                    (long long)seqs, (long long)max_q, (long long)q_heads);
-    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    bool rows = false;
+    if (int rc = make_attention(a, fn, c, &rows)) return rc;
+    if (groups < 0 || prefix_cols < 0 || max_prefix < 0)
+        return fail(LCML_ERR_INVALID_ARG, "%s: groups=%lld prefix_cols=%lld max_prefix=%lld", fn, (long long)groups,
+                    (long long)prefix_cols, (long long)max_prefix);
+    if (prefix_stride < prefix_cols)
+        return fail(LCML_ERR_INVALID_ARG, "%s: prefix_stride=%lld < prefix_cols=%lld", fn, (long long)prefix_stride,
+                    (long long)prefix_cols);
+    if (groups > kMostGroups || prefix_cols >= (int64_t)1 << 31 || max_prefix >= (int64_t)1 << 31)
+        return fail(LCML_ERR_UNSUPPORTED, "%s: groups=%lld prefix_cols=%lld max_prefix=%lld", fn, (long long)groups,
+                    (long long)prefix_cols, (long long)max_prefix);
+    if (!rows) return LCML_OK;
+    if (groups && (!group_seq || !prefix_len || (prefix_cols && !prefix_table)))
+        return fail(LCML_ERR_INVALID_ARG, "%s: NULL index array", fn);
+    if (!aligned(group_seq, 4) || !aligned(prefix_len, 4) || !aligned(prefix_table, 4))
+        return fail(LCML_ERR_INVALID_ARG, "%s: index arrays not 4-byte aligned", fn);
+    if (tokens * (q_heads / kv_heads) > kMostGroups * 16 || seqs * max_q >= kMostGroups / q_heads) return too_large(fn, c);
+    int64_t workgroups = 0;
+    const int64_t need = lcml::attention_shared_workspace(tokens, seqs, groups, q_heads, kv_heads, head_dim, max_q, max_own,
+                                                          max_prefix, &workgroups);
+    if (workgroups >= kMostGroups) return too_large(fn, c);
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
         return fail(LCML_ERR_INVALID_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", fn, (long long)need);
-    a.q = q, a.o = o, a.k = k_cache, a.v = v_cache, a.ks = k_scale, a.vs = v_scale;
-    a.q_token = q_token_stride, a.q_head = q_head_stride, a.o_token = o_token_stride, a.o_head = o_head_stride;
-    a.max_q = max_q, a.max_kv = max_kv, a.window = window < (int64_t)1 << 31 ? window : 0;  // a longer one hides nothing
-    a.q_heads = (int32_t)q_heads, a.causal = causal != 0;
-    a.q_bf16 = q_dtype == LCML_DTYPE_BFLOAT16, a.o_bf16 = o_dtype == LCML_DTYPE_BFLOAT16;
-    a.scale = scale;
+    a.group_seq = group_seq, a.prefix_len = prefix_len, a.groups = (int32_t)groups;
     const char *label = nullptr;
-    const hipError_t err = lcml::launch_attention(a, workspace, (hipStream_t)stream, &label);
+    const hipError_t err = lcml::launch_attention_shared(a, prefix_table, prefix_stride, prefix_cols, max_prefix, workspace,
+                                                         (hipStream_t)stream, &label);
     return hip_status(err, fn, label);
 }
 

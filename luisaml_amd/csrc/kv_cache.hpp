@@ -72,6 +72,25 @@ struct AttentionArgs {
     int64_t max_q, max_kv, window;             // window 0: none
     int32_t q_heads, causal, q_bf16, o_bf16;
     float scale;
+    uint32_t sinks;  // first positions that the window does not hide
+    // groups of sequences that share their first tokens (none: groups 0)
+    const int32_t *group_seq, *prefix_len;  // [groups + 1] first sequences, [groups] shared tokens
+    int32_t groups;
+};
+
+// One call that plans a step (kv_plan.hip).
+struct KvPlan {
+    const int32_t *new_tokens, *ended, *first_own;  // [seqs]; the last two may be NULL
+    const int32_t *kv_len_in, *free_in;             // [seqs], [1]
+    int32_t *free_pages;                            // [pages], the first free_in[0] are free
+    int32_t *table;
+    int64_t table_stride;
+    int32_t table_cols, seqs, pages, tshift;
+    int32_t *kv_len, *cu_q, *left;  // [seqs], [seqs + 1], [1]
+    int32_t *positions;             // [tokens] or NULL
+    int64_t *slots;                 // [tokens] or NULL
+    int64_t tokens;
+    int64_t *work;  // [seqs + 2]: new columns before each sequence, all of them, the stack's height
 };
 
 // the smallest power of two s >= 2^-126 with a <= 448 s, for finite a >= 0:

@@ -143,11 +143,41 @@ hipError_t launch_kv_write(const KvTokens &t, int64_t max_q, const void *k, cons
 hipError_t launch_kv_read(const KvTokens &t, int64_t max_q, void *k, void *v, bool bf16, int64_t kt, int64_t kh,
                           int64_t vt, int64_t vh, const uint8_t *kc, const uint8_t *vc, const float *ks,
                           const float *vs, hipStream_t s);
+// a step's pages, lengths and row indexes; p.work: kv_plan_workspace bytes
+struct KvPlan;
+int64_t kv_plan_workspace(int64_t seqs, int64_t tokens);
+hipError_t launch_kv_plan(const KvPlan &p, hipStream_t s, const char **kernel);
+
+// norms and rotation of queries and keys; strides in elements
+struct RopeArgs {
+    const void *q, *k;
+    void *q_out, *k_out;
+    const float *q_gamma, *k_gamma;  // NULL: no norm
+    const float *table;              // [table_rows][rot]: cosines, then sines
+    const int32_t *positions;        // NULL: every row, where rot is 0
+    int64_t q_token, q_head, k_token, k_head, qo_token, qo_head, ko_token, ko_head;
+    int64_t tokens;
+    int32_t q_heads, k_heads, dim, rot, table_rows, interleaved;
+    float eps, inv_dim;
+    int32_t parts;  // wavefronts of a token
+};
+hipError_t launch_qk_norm_rope(RopeArgs p, bool in_bf16, bool out_bf16, hipStream_t s);
+// wavefronts of a token
+int64_t qk_norm_rope_parts(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t dim);
+
 // workspace bytes, workgroups, and a call (work: that many bytes)
 int64_t attention_workspace(int64_t tokens, int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim,
                             int64_t max_q, int64_t max_kv);
 int64_t attention_groups(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t max_q, int64_t max_kv);
 hipError_t launch_attention(const AttentionArgs &a, void *work, hipStream_t s, const char **kernel);
+// window > 0 and sinks > 0
+hipError_t launch_attention_sinks(const AttentionArgs &a, void *work, hipStream_t s, const char **kernel);
+// a.max_kv: of a sequence's own tokens
+int64_t attention_shared_workspace(int64_t tokens, int64_t seqs, int64_t groups, int64_t q_heads, int64_t kv_heads,
+                                   int64_t dim, int64_t max_q, int64_t max_own, int64_t max_prefix, int64_t *workgroups);
+hipError_t launch_attention_shared(const AttentionArgs &a, const int32_t *prefix_table, int64_t prefix_stride,
+                                   int64_t prefix_cols, int64_t max_prefix, void *work, hipStream_t s,
+                                   const char **kernel);
 
 // A kernel's dynamic-LDS limit (hipFuncSetAttribute) is per device: set it
 // once per (kernel, device), tracked in `done` (bit d = device d; devices past
