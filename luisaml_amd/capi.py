@@ -595,6 +595,11 @@ def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.T
                                     *_where(stream)))
 
 
+@functools.lru_cache(maxsize=256)
+def _plan_workspace(seqs, rows):
+    return lib().lcml_fp8_kv_cache_plan_workspace_bytes(seqs, rows)
+
+
 def kv_cache_plan(new_tokens: torch.Tensor, kv_len: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
                   free_count: torch.Tensor, page_tokens: int, tokens: int | None = None, ended: torch.Tensor | None = None,
                   first_own: torch.Tensor | None = None, kv_len_out: torch.Tensor | None = None,
@@ -618,10 +623,10 @@ def kv_cache_plan(new_tokens: torch.Tensor, kv_len: torch.Tensor, block_table: t
         positions = _empty((tokens,), i32, dev, stream) if positions is None else positions
         slots = _empty((tokens,), torch.int64, dev, stream) if slots is None else slots
     if workspace is None:
-        rows = next((t.numel() for t in (positions, slots) if t is not None), 0)
-        need = lib().lcml_fp8_kv_cache_plan_workspace_bytes(kv_len.numel(), rows)
+        rows = positions.numel() if positions is not None else slots.numel() if slots is not None else 0
+        need = _plan_workspace(kv_len.numel(), rows)
         if need:
-            workspace = _empty((need,), torch.uint8, dev, stream)
+            workspace = _empty(need, torch.uint8, dev, stream)
     _check(_binding().kv_cache_plan(new_tokens, kv_len, block_table, free_pages, free_count, page_tokens, ended, first_own,
                                     kv_len_out, cu_q, left, positions, slots, workspace, *_where(stream)))
     return kv_len_out, cu_q, left, positions, slots

@@ -17,35 +17,49 @@
 namespace lcml {
 namespace {
 
-constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
-constexpr int kLdsSeqs = 2048;    // sequences whose sums fit a workgroup's LDS
+constexpr int kMostThreads = 1024;
+constexpr int kLdsSeqs = 2048;  // sequences whose sums fit a workgroup's LDS
 constexpr int kEmitThreads = 256;
 
-// inclusive sum over the lanes of a wavefront
-__device__ inline int64_t wave_scan(int64_t v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const int64_t u = __shfl_up((long long)v, m);
-        v += (threadIdx.x & 63) >= (unsigned)m ? u : 0;
-    }
-    return v;
+// v plus the value that the DPP control brings, where it brings one
+template <int CTRL, int ROWS>
+__device__ inline int64_t add_dpp(int64_t v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+    return v + (int64_t)((uint64_t)hi << 32 | lo);
 }
-// exclusive sum over the workgroup; *total: of all
-__device__ inline int64_t block_scan(int64_t v, int64_t *red, int64_t *total) {
+// inclusive sum over the lanes of a wavefront: 1, 2, 4, 8 to the right within
+// sixteen lanes, then each sixteen's last lane to the next, then 32's
+__device__ inline int64_t wave_scan(int64_t v) {
+    v = add_dpp<0x111, 0xf>(v);
+    v = add_dpp<0x112, 0xf>(v);
+    v = add_dpp<0x114, 0xf>(v);
+    v = add_dpp<0x118, 0xf>(v);
+    v = add_dpp<0x142, 0xa>(v);
+    return add_dpp<0x143, 0xc>(v);
+}
+// v[x]: exclusive sum over the workgroup, total[x]: of all; red alternates
+// between two calls, so that one barrier does
+template <int NT, int N>
+__device__ inline void block_scan(int64_t (&v)[N], int64_t (&total)[N], int64_t (*red)[NT / 64]) {
     const int wave = threadIdx.x >> 6;
-    const int64_t in = wave_scan(v);
-    if ((threadIdx.x & 63) == 63) red[wave] = in;
-    __syncthreads();
-    int64_t before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < kPlanWaves; ++w) {
-        const int64_t u = red[w];
-        before += w < wave ? u : 0;
-        all += u;
+    for (int x = 0; x < N; ++x) {
+        const int64_t in = wave_scan(v[x]);
+        if ((threadIdx.x & 63) == 63) red[x][wave] = in;
+        v[x] = in - v[x];
     }
     __syncthreads();
-    *total = all;
-    return before + in - v;
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+        total[x] = 0;
+#pragma unroll
+        for (int w = 0; w < NT / 64; ++w) {
+            const int64_t u = red[x][w];
+            v[x] += w < wave ? u : 0;
+            total[x] += u;
+        }
+    }
 }
 
 // the last of at[0 .. n] (rising, at[0] <= i < at[n]) that is not above i
@@ -70,143 +84,159 @@ __device__ inline int32_t columns(const KvPlan &p, int32_t n) {
     return c < p.table_cols ? c : p.table_cols;
 }
 
-// a sequence before and after
-struct Seq {
-    int32_t old, kv;
-};
-__device__ inline Seq seq_of(const KvPlan &p, int32_t b) {
-    const int32_t held = p.kv_len_in[b], n = p.new_tokens[b];
-    Seq s;
-    s.old = (p.ended && p.ended[b] != 0) || held < 0 ? 0 : held;
-    s.kv = clamp32((int64_t)s.old + (n > 0 ? n : 0));
-    return s;
-}
-
 // What is left to write once the sums are there: the new columns' pages, and
 // the rows' positions and slots.  cu: row offsets; need: new columns before
-// each sequence; both [seqs + 1].
-template <class Need>
-__device__ inline void emit(const KvPlan &p, const int32_t *cu, const Need *need, int32_t top, int64_t first, int64_t step) {
-    const int64_t pages = (int64_t)need[p.seqs];
-    for (int64_t i = first; i < pages; i += step) {
-        const int32_t b = find(need, p.seqs, i), kv = p.kv_len[b];
-        const int64_t at = top - 1 - i;
-        // the last of a sequence's new columns is its last column
-        const int32_t c = columns(p, kv) - (int32_t)((int64_t)need[b + 1] - i);
-        p.table[(int64_t)b * p.table_stride + c] = at >= 0 ? p.free_pages[at] : -1;
-    }
-    if (!p.positions && !p.slots) return;
-    for (int64_t r = first; r < p.tokens; r += step) {
-        int32_t pos = -1;
-        int64_t slot = -1;
-        if (r < cu[p.seqs]) {
-            const int32_t b = find(cu, p.seqs, r), kv = p.kv_len[b];
-            pos = kv - (cu[b + 1] - (int32_t)r);
-            const int32_t c = pos >> p.tshift, fresh = columns(p, kv) - (int32_t)((int64_t)need[b + 1] - (int64_t)need[b]);
+// each sequence; both [seqs + 1]; kv: lengths.
+__device__ inline void emit(const KvPlan &p, const int32_t *cu, const int64_t *need, const int32_t *kv, int32_t top,
+                            int64_t first, int64_t step) {
+    const int64_t fresh = need[p.seqs], rows = p.positions || p.slots ? p.tokens : 0;
+    const int64_t most = fresh > rows ? fresh : rows;
+    for (int64_t i = first; i < most; i += step) {
+        // loads of both before the stores
+        int32_t page = -1, pos = -1, of = -1;
+        int64_t column = -1;
+        if (i < fresh) {
+            const int32_t b = find(need, p.seqs, i);
+            // the last of a sequence's new columns is its last column
+            column = (int64_t)b * p.table_stride + (columns(p, kv[b]) - (int32_t)(need[b + 1] - i));
+            if (top - 1 - i >= 0) page = p.free_pages[top - 1 - i];
+        }
+        if (i < rows && i < cu[p.seqs]) {
+            const int32_t b = find(cu, p.seqs, i);
+            pos = kv[b] - (cu[b + 1] - (int32_t)i);
+            const int32_t c = pos >> p.tshift, old = columns(p, kv[b]) - (int32_t)(need[b + 1] - need[b]);
             if (p.slots && c < p.table_cols) {
-                const int64_t at = top - 1 - ((int64_t)need[b] + c - fresh);
-                const int32_t page = c < fresh ? p.table[(int64_t)b * p.table_stride + c] : at >= 0 ? p.free_pages[at] : -1;
-                if (page >= 0 && page < p.pages) slot = ((int64_t)page << p.tshift) + (pos & ((1 << p.tshift) - 1));
+                const int64_t at = top - 1 - (need[b] + c - old);
+                if (c < old)
+                    of = p.table[(int64_t)b * p.table_stride + c];
+                else if (at >= 0)
+                    of = p.free_pages[at];
             }
         }
-        if (p.positions) p.positions[r] = pos;
-        if (p.slots) p.slots[r] = slot;
+        if (column >= 0) p.table[column] = page;
+        if (i >= rows) continue;
+        if (p.positions) p.positions[i] = pos;
+        if (p.slots)
+            p.slots[i] = of >= 0 && of < p.pages ? ((int64_t)of << p.tshift) + (pos & ((1 << p.tshift) - 1)) : -1;
     }
 }
 
-// One workgroup: returned pages, lengths and sums; ALL: and the rest.  (Every
-// input that an output may be the same array as is read before the barrier
-// that the output is written after.)
-template <bool ALL>
-__global__ __launch_bounds__(kPlanThreads) void k_kv_plan(KvPlan p) {
-    __shared__ int64_t red[kPlanWaves];
-    __shared__ int64_t lens[kPlanThreads + 1];
-    __shared__ int32_t s_cu[ALL ? kPlanThreads + 1 : 1];
-    const int tid = threadIdx.x;
+// One workgroup: returned pages, lengths and sums; ALL (seqs <= NT): and the
+// rest.  Each input that an output may share memory with is read by the thread
+// that writes there, or before a barrier.
+template <int NT, bool ALL>
+__global__ __launch_bounds__(NT) void k_kv_plan(KvPlan p) {
+    // table entries of a thread at a time; one count for each of them and each
+    // wavefront, a lane of which scans them
+    constexpr int kEach = 4, kCounts = kEach * NT / 64;
+    static_assert(kCounts <= 64, "one lane each");
+    __shared__ int64_t red[2][3][NT / 64];
+    __shared__ int64_t lens[NT + 1];
+    __shared__ int32_t firsts[NT], counts[2][kCounts];
+    __shared__ int64_t s_need[ALL ? NT + 1 : 1];
+    __shared__ int32_t s_cu[ALL ? NT + 1 : 1], s_kv[ALL ? NT : 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int turn = 0;
     int32_t top = p.free_in[0];
-    top = top < 0 ? 0 : top > p.pages ? p.pages : top;
-    __syncthreads();  // `left` may be the same word
-    if (p.ended) {
-        for (int32_t b0 = 0; b0 < p.seqs; b0 += kPlanThreads) {
-            const int32_t b = b0 + tid;
-            int32_t from = 0, n = 0;
-            if (b < p.seqs && p.ended[b] != 0) {
-                const int32_t held = p.kv_len_in[b];
-                from = p.first_own ? p.first_own[b] : 0;
-                from = from > 0 ? from : 0;
-                n = columns(p, held > 0 ? held : 0) - from;
-            }
-            int64_t total, got;
-            const int64_t at = block_scan(n > 0 ? n : 0, red, &total);
-            lens[tid] = at;
-            if (tid == 0) lens[kPlanThreads] = total;
-            __syncthreads();
-            for (int64_t i0 = 0; i0 < total; i0 += kPlanThreads) {
-                const int64_t i = i0 + tid;
-                int32_t page = -1;
-                if (i < total) {
-                    const int32_t k = find(lens, kPlanThreads, i), bb = b0 + k;
-                    int32_t c = p.first_own ? p.first_own[bb] : 0;
-                    c = (c > 0 ? c : 0) + (int32_t)(i - lens[k]);
-                    page = p.table[(int64_t)bb * p.table_stride + c];
-                }
-                const bool back = page >= 0 && page < p.pages;
-                const int64_t place = top + block_scan(back, red, &got);
-                if (back && place < p.pages) p.free_pages[place] = page;
-                top = clamp32(top + got < p.pages ? top + got : p.pages);
-            }
-            __syncthreads();
-        }
-    }
     int64_t rows = 0, fresh = 0;
-    for (int32_t b0 = 0; b0 < p.seqs; b0 += kPlanThreads) {
+    for (int32_t b0 = 0; b0 < p.seqs; b0 += NT) {
         const int32_t b = b0 + tid;
-        Seq s{0, 0};
-        if (b < p.seqs) s = seq_of(p, b);
-        int64_t n, f;
-        const int32_t want = columns(p, s.kv) - columns(p, s.old);
-        const int64_t row = rows + block_scan(s.kv - s.old, red, &n);
-        const int64_t need = fresh + block_scan(want, red, &f);
-        if (b < p.seqs) {
-            p.kv_len[b] = s.kv;
-            p.cu_q[b] = clamp32(row);
-            if (ALL)
-                lens[tid] = need, s_cu[tid] = clamp32(row);
-            else
-                p.work[b] = need;
+        const bool in = b < p.seqs;
+        const int32_t held0 = in ? p.kv_len_in[b] : 0, n = in ? p.new_tokens[b] : 0;
+        const bool ended = p.ended && in && p.ended[b] != 0;
+        int32_t own = p.first_own && in ? p.first_own[b] : 0;
+        own = own > 0 ? own : 0;
+        const int32_t held = held0 > 0 ? held0 : 0, old = ended ? 0 : held, kv = clamp32((int64_t)old + (n > 0 ? n : 0));
+        const int32_t back = ended ? columns(p, held) - own : 0;
+        // rows, new columns, returned columns
+        int64_t at[3] = {kv - old, columns(p, kv) - columns(p, old), back > 0 ? back : 0}, total[3];
+        block_scan<NT>(at, total, red[turn]);
+        turn ^= 1;
+        if (b0 == 0) top = top < 0 ? 0 : top > p.pages ? p.pages : top;
+        if (total[2] > 0) {
+            const int32_t there = p.seqs - b0 < NT ? p.seqs - b0 : NT;
+            lens[tid] = at[2], firsts[tid] = own;
+            if (tid == 0) lens[NT] = total[2];
+            __syncthreads();
+            for (int64_t i0 = 0; i0 < total[2]; i0 += (int64_t)NT * kEach) {
+                int32_t page[kEach];
+                uint64_t back[kEach];
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const int64_t i = i0 + e * NT + tid;
+                    page[e] = -1;
+                    if (i < total[2]) {
+                        const int32_t k = find(lens, there, i);
+                        page[e] = p.table[(int64_t)(b0 + k) * p.table_stride + firsts[k] + (int32_t)(i - lens[k])];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    back[e] = __builtin_amdgcn_ballot_w64(page[e] >= 0 && page[e] < p.pages);
+                    if (lane == 0) counts[turn][e * (NT / 64) + wave] = __builtin_popcountll(back[e]);
+                }
+                __syncthreads();
+                const int64_t mine = lane < kCounts ? counts[turn][lane] : 0, sums = wave_scan(mine);
+                turn ^= 1;
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const int32_t before = __builtin_amdgcn_readlane((int32_t)(sums - mine), e * (NT / 64) + wave);
+                    const int64_t place = top + before + (int32_t)__builtin_popcountll(back[e] & ((1ull << lane) - 1));
+                    if ((back[e] >> lane & 1) && place < p.pages) p.free_pages[place] = page[e];
+                }
+                const int64_t all = top + (int64_t)__builtin_amdgcn_readlane((int32_t)sums, 63);
+                top = (int32_t)(all < p.pages ? all : p.pages);
+            }
+            if (b0 + NT < p.seqs) __syncthreads();  // lens is written again
         }
-        rows += n, fresh += f;
+        if (in) {
+            const int32_t row = clamp32(rows + at[0]);
+            p.kv_len[b] = kv;
+            p.cu_q[b] = row;
+            if (ALL)
+                s_need[tid] = at[1], s_cu[tid] = row, s_kv[tid] = kv;
+            else
+                p.work[b] = fresh + at[1];
+        }
+        rows += total[0], fresh += total[1];
+    }
+    if (p.seqs == 0) {
+        __syncthreads();  // `left` may be free_in
+        top = top < 0 ? 0 : top > p.pages ? p.pages : top;
     }
     if (tid == 0) {
         p.cu_q[p.seqs] = clamp32(rows);
         p.left[0] = (int32_t)(top - fresh > -0x7fffffff ? top - fresh : -0x7fffffff);
         if (ALL)
-            lens[p.seqs] = fresh, s_cu[p.seqs] = clamp32(rows);
+            s_need[p.seqs] = fresh, s_cu[p.seqs] = clamp32(rows);
         else
             p.work[p.seqs] = fresh, p.work[p.seqs + 1] = top;
     }
     if constexpr (ALL) {
-        __syncthreads();  // and the returned pages, and kv_len
-        emit(p, s_cu, lens, top, tid, kPlanThreads);
+        __syncthreads();  // and the returned pages
+        emit(p, s_cu, s_need, s_kv, top, tid, NT);
     }
 }
 
 template <bool LDS>
 __global__ __launch_bounds__(kEmitThreads) void k_kv_plan_emit(KvPlan p) {
-    __shared__ int32_t cu[LDS ? kLdsSeqs + 1 : 1];
+    __shared__ int32_t cu[LDS ? kLdsSeqs + 1 : 1], kv[LDS ? kLdsSeqs : 1];
     __shared__ int64_t need[LDS ? kLdsSeqs + 1 : 1];
     const int32_t top = (int32_t)p.work[p.seqs + 1];
     const int64_t first = (int64_t)blockIdx.x * kEmitThreads + threadIdx.x, step = (int64_t)gridDim.x * kEmitThreads;
     if constexpr (LDS) {
-        for (int32_t b = threadIdx.x; b <= p.seqs; b += kEmitThreads) cu[b] = p.cu_q[b], need[b] = p.work[b];
+        for (int32_t b = threadIdx.x; b <= p.seqs; b += kEmitThreads) {
+            cu[b] = p.cu_q[b], need[b] = p.work[b];
+            if (b < p.seqs) kv[b] = p.kv_len[b];
+        }
         __syncthreads();
-        emit(p, cu, need, top, first, step);
+        emit(p, cu, need, kv, top, first, step);
     } else {
-        emit(p, p.cu_q, p.work, top, first, step);
+        emit(p, p.cu_q, p.work, p.kv_len, top, first, step);
     }
 }
 
-bool at_once(int64_t seqs, int64_t tokens) { return seqs <= kPlanThreads && tokens <= 2048; }
+bool at_once(int64_t seqs, int64_t tokens) { return seqs <= kMostThreads && tokens <= 2 * kMostThreads; }
 
 }  // namespace
 
@@ -215,11 +245,14 @@ int64_t kv_plan_workspace(int64_t seqs, int64_t tokens) { return at_once(seqs, t
 hipError_t launch_kv_plan(const KvPlan &p, hipStream_t s, const char **kernel) {
     if (at_once(p.seqs, p.tokens)) {
         *kernel = "kv_plan";
-        hipLaunchKernelGGL(k_kv_plan<true>, dim3(1), dim3(kPlanThreads), 0, s, p);
+        if (p.seqs <= 256 && p.tokens <= 512)
+            hipLaunchKernelGGL((k_kv_plan<256, true>), dim3(1), dim3(256), 0, s, p);
+        else
+            hipLaunchKernelGGL((k_kv_plan<kMostThreads, true>), dim3(1), dim3(kMostThreads), 0, s, p);
         return hipGetLastError();
     }
     *kernel = "kv_plan, kv_plan_emit";
-    hipLaunchKernelGGL(k_kv_plan<false>, dim3(1), dim3(kPlanThreads), 0, s, p);
+    hipLaunchKernelGGL((k_kv_plan<kMostThreads, false>), dim3(1), dim3(kMostThreads), 0, s, p);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     const int64_t most = p.tokens > p.seqs ? p.tokens : p.seqs, groups = (most + kEmitThreads - 1) / kEmitThreads;
