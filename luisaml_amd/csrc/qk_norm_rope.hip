@@ -16,50 +16,49 @@ namespace {
 
 constexpr int kThreads = 256;
 
-struct __attribute__((packed, aligned(2))) H8 {
-    uint16_t v[8];
-};
-struct __attribute__((packed, aligned(4))) F8 {
-    float v[8];
-};
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));  // converted to nearest even, in hardware
 
-template <bool BF16>
-__device__ inline void load8(const void *p, int64_t i, float *x) {
+// N elements from or to any element-aligned address
+template <int N>
+struct __attribute__((packed, aligned(2))) Halfs {
+    uint16_t v[N];
+};
+template <int N>
+struct __attribute__((packed, aligned(2))) Words {
+    uint32_t v[N];
+};
+template <int N>
+struct __attribute__((packed, aligned(4))) Floats {
+    float v[N];
+};
+template <bool BF16, int N>
+__device__ inline void load(const void *p, int64_t i, float *x) {
     if constexpr (BF16) {
-        const H8 q = *reinterpret_cast<const H8 *>(static_cast<const uint16_t *>(p) + i);
+        const Halfs<N> q = *reinterpret_cast<const Halfs<N> *>(static_cast<const uint16_t *>(p) + i);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = bits_f32((uint32_t)q.v[e] << 16);
+        for (int e = 0; e < N; ++e) x[e] = bits_f32((uint32_t)q.v[e] << 16);
     } else {
-        const F8 q = *reinterpret_cast<const F8 *>(static_cast<const float *>(p) + i);
+        const Floats<N> q = *reinterpret_cast<const Floats<N> *>(static_cast<const float *>(p) + i);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = q.v[e];
+        for (int e = 0; e < N; ++e) x[e] = q.v[e];
     }
 }
-template <bool BF16>
-__device__ inline float load1(const void *p, int64_t i) {
-    if constexpr (BF16) return bits_f32((uint32_t)static_cast<const uint16_t *>(p)[i] << 16);
-    return static_cast<const float *>(p)[i];
-}
-template <bool BF16>
-__device__ inline void store8(void *p, int64_t i, const float *x) {
-    if constexpr (BF16) {
-        H8 q;
+template <bool BF16, int N>
+__device__ inline void store(void *p, int64_t i, const float *x) {
+    if constexpr (BF16 && N == 1) {
+        static_cast<uint16_t *>(p)[i] = bf16_rne(x[0]);
+    } else if constexpr (BF16) {
+        Words<N / 2> q;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q.v[e] = bf16_rne(x[e]);
-        *reinterpret_cast<H8 *>(static_cast<uint16_t *>(p) + i) = q;
+        for (int e = 0; e < N; e += 2) q.v[e / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x[e], x[e + 1]}, bf2));
+        *reinterpret_cast<Words<N / 2> *>(static_cast<uint16_t *>(p) + i) = q;
     } else {
-        F8 q;
+        Floats<N> q;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q.v[e] = x[e];
-        *reinterpret_cast<F8 *>(static_cast<float *>(p) + i) = q;
+        for (int e = 0; e < N; ++e) q.v[e] = x[e];
+        *reinterpret_cast<Floats<N> *>(static_cast<float *>(p) + i) = q;
     }
-}
-template <bool BF16>
-__device__ inline void store1(void *p, int64_t i, float x) {
-    if constexpr (BF16)
-        static_cast<uint16_t *>(p)[i] = bf16_rne(x);
-    else
-        static_cast<float *>(p)[i] = x;
 }
 
 // sum over the LANES neighbours of a lane
@@ -75,14 +74,20 @@ __device__ inline float group_sum(float v) {
     return v;
 }
 
-// how a lane's eight pairs lie in memory: two runs of eight elements, one run
-// of sixteen, or anywhere (rot not a multiple of 16)
+// how a pair lies in memory: halves of the rotated part, neighbours, or halves
+// that a lane's runs would straddle
 enum { kHalves = 0, kNeighbours = 1, kScattered = 2 };
+
+// A lane's eight pairs are runs of RUN, of 16 bytes of input where the pairs
+// allow it: run g of lane u starts at pair g * D / 2 / RUNS + RUN * u, so that
+// every load of a wavefront is contiguous.
+template <int PAIRS, bool IB>
+constexpr int kRun = PAIRS == kScattered ? 1 : PAIRS == kNeighbours ? (IB ? 4 : 2) : (IB ? 8 : 4);
 
 // LANES for each head; IB, OB: bf16 in and out
 template <int LANES, int PAIRS, bool IB, bool OB>
 __global__ __launch_bounds__(kThreads) void k_qk_norm_rope(RopeArgs p) {
-    constexpr int ROWS = 64 / LANES;
+    constexpr int ROWS = 64 / LANES, RUN = kRun<PAIRS, IB>, RUNS = 8 / RUN;
     const int lane = threadIdx.x & 63, u = lane % LANES, r = lane / LANES;
     const int32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t id = blockIdx.x * (kThreads / 64) + wave;
@@ -93,42 +98,38 @@ __global__ __launch_bounds__(kThreads) void k_qk_norm_rope(RopeArgs p) {
         pos = p.positions[token];
         if (pos < 0 || pos >= p.table_rows) return;
     }
-    const int32_t D = p.dim, half = p.rot >> 1, rest = (D - p.rot) >> 1, pair0 = 8 * u;
-    const bool in = pair0 < D >> 1;
+    const int32_t D = p.dim, half = p.rot >> 1, rest = (D - p.rot) >> 1;
+    const bool in = 16 * u < D;
+    const auto pair = [&](int e) { return (e / RUN) * (D / 2 / RUNS) + RUN * (in ? u : 0) + e % RUN; };
     // element of the first and second of pair i
     const auto first = [&](int32_t i) { return PAIRS == kNeighbours ? 2 * i : i < half ? i : p.rot + i - half; };
     const auto second = [&](int32_t i) { return PAIRS == kNeighbours ? 2 * i + 1 : i < half ? i + half : p.rot + i - half + rest; };
     float cs[8], sn[8];
-    {
-        const float *t = p.table + (int64_t)pos * p.rot;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) cs[e] = 1.0f, sn[e] = 0.0f;
-        if (in && pair0 + 8 <= half) {
-            const F8 c = *reinterpret_cast<const F8 *>(t + pair0), s = *reinterpret_cast<const F8 *>(t + half + pair0);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) cs[e] = c.v[e], sn[e] = s.v[e];
-        } else if (in) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (pair0 + e < half) cs[e] = t[pair0 + e], sn[e] = t[half + pair0 + e];
-        }
-    }
-    const int32_t fa = first(in ? pair0 : 0), fb = second(in ? pair0 : 0);
-    // x: a lane's firsts, then its seconds
-    const auto load = [&](const void *base, int64_t at, float *x, auto bf16) {
-        constexpr bool B = decltype(bf16)::value;
-        if constexpr (PAIRS == kHalves) {
-            load8<B>(base, at + fa, x), load8<B>(base, at + fb, x + 8);
-        } else if constexpr (PAIRS == kNeighbours) {
-            float y[16];
-            load8<B>(base, at + fa, y), load8<B>(base, at + fa + 8, y + 8);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = y[2 * e], x[8 + e] = y[2 * e + 1];
+    for (int g = 0; g < 8; g += RUN) {
+        const float *t = p.table + (int64_t)pos * p.rot + pair(g);
+        if (pair(g) + RUN <= half) {
+            load<false, RUN>(t, 0, cs + g), load<false, RUN>(t, half, sn + g);
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int32_t i = in ? pair0 + e : 0;
-                x[e] = load1<B>(base, at + first(i)), x[8 + e] = load1<B>(base, at + second(i));
+            for (int e = g; e < g + RUN; ++e) {
+                const bool turn = pair(e) < half;
+                cs[e] = turn ? t[e - g] : 1.0f, sn[e] = turn ? t[half + e - g] : 0.0f;
+            }
+        }
+    }
+    // x: a lane's firsts, then its seconds
+    const auto take = [&](const void *base, int64_t at, float *x, auto bf16) {
+        constexpr bool B = decltype(bf16)::value;
+#pragma unroll
+        for (int g = 0; g < 8; g += RUN) {
+            if constexpr (PAIRS != kNeighbours) {
+                load<B, RUN>(base, at + first(pair(g)), x + g), load<B, RUN>(base, at + second(pair(g)), x + 8 + g);
+            } else {
+                float y[2 * RUN];
+                load<B, 2 * RUN>(base, at + first(pair(g)), y);
+#pragma unroll
+                for (int e = 0; e < RUN; ++e) x[g + e] = y[2 * e], x[8 + g + e] = y[2 * e + 1];
             }
         }
     };
@@ -139,18 +140,15 @@ __global__ __launch_bounds__(kThreads) void k_qk_norm_rope(RopeArgs p) {
         const bool is_k = i >= q_steps;
         const int32_t head = (is_k ? i - q_steps : i) * ROWS + r, heads = is_k ? p.k_heads : p.q_heads;
         const bool live = in && head < heads;
-        const void *src = is_k ? p.k : p.q;
         void *dst = is_k ? p.k_out : p.q_out;
         const float *g = is_k ? p.k_gamma : p.q_gamma;
         const int64_t row = head < heads ? head : 0;
-        const int64_t at = (is_k ? token * p.k_token + row * p.k_head : token * p.q_token + row * p.q_head);
         float x[16];
-        load(src, at, x, std::integral_constant<bool, IB>{});
-        if (g && have != (int32_t)is_k) {
-            load(g, 0, gamma, std::false_type{});
-            have = is_k;
-        }
+        take(is_k ? p.k : p.q, is_k ? token * p.k_token + row * p.k_head : token * p.q_token + row * p.q_head, x,
+             std::integral_constant<bool, IB>{});
         if (g) {
+            if (have != (int32_t)is_k) take(g, 0, gamma, std::false_type{});
+            have = is_k;
             float sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) sum = fmaf(x[e], x[e], sum);
@@ -162,21 +160,22 @@ __global__ __launch_bounds__(kThreads) void k_qk_norm_rope(RopeArgs p) {
         float y[16];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const bool turn = PAIRS == kHalves ? pair0 < half : pair0 + e < half;
+            // (a product with a sine of 0 would make a NaN of a partner's infinity)
+            const bool turn = pair(PAIRS == kNeighbours ? e : e / RUN * RUN) < half;
             const float a = fmaf(x[e], cs[e], -(x[8 + e] * sn[e])), b = fmaf(x[8 + e], cs[e], x[e] * sn[e]);
             y[e] = turn ? a : x[e], y[8 + e] = turn ? b : x[8 + e];
         }
-        const int64_t to = (is_k ? token * p.ko_token + row * p.ko_head : token * p.qo_token + row * p.qo_head);
-        if constexpr (PAIRS == kHalves) {
-            store8<OB>(dst, to + fa, y), store8<OB>(dst, to + fb, y + 8);
-        } else if constexpr (PAIRS == kNeighbours) {
-            float z[16];
+        const int64_t to = is_k ? token * p.ko_token + row * p.ko_head : token * p.qo_token + row * p.qo_head;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) z[2 * e] = y[e], z[2 * e + 1] = y[8 + e];
-            store8<OB>(dst, to + fa, z), store8<OB>(dst, to + fa + 8, z + 8);
-        } else {
+        for (int g = 0; g < 8; g += RUN) {
+            if constexpr (PAIRS != kNeighbours) {
+                store<OB, RUN>(dst, to + first(pair(g)), y + g), store<OB, RUN>(dst, to + second(pair(g)), y + 8 + g);
+            } else {
+                float z[2 * RUN];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) store1<OB>(dst, to + first(pair0 + e), y[e]), store1<OB>(dst, to + second(pair0 + e), y[8 + e]);
+                for (int e = 0; e < RUN; ++e) z[2 * e] = y[g + e], z[2 * e + 1] = y[8 + g + e];
+                store<OB, 2 * RUN>(dst, to + first(pair(g)), z);
+            }
         }
     }
 }
@@ -198,7 +197,7 @@ template <int LANES>
 void start_lanes(const RopeArgs &p, bool ib, bool ob, dim3 grid, hipStream_t s) {
     if (p.interleaved)
         start<LANES, kNeighbours>(p, ib, ob, grid, s);
-    else if (p.rot % 16 == 0)
+    else if (p.rot % (ib ? 16 : 8) == 0)
         start<LANES, kHalves>(p, ib, ob, grid, s);
     else
         start<LANES, kScattered>(p, ib, ob, grid, s);
