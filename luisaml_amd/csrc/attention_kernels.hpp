@@ -430,15 +430,20 @@ __device__ inline int32_t step_token(const Part &p, int32_t k) {
 // tokens of 8 KV heads of 128, 619 MB: 120 us, 5.2 TB/s; fp32 queries and
 // results 130.  One over 500 tokens: 8.4 us, five dependent round trips to
 // memory (lengths, table, scales, codes, the join's LDS); fp32 10.
+template <int DC, int NW>
+struct FewLds {
+    float red_m[NW][16], red_l[NW][16];
+    __attribute__((aligned(16))) float buf[NW][16][DC * 64 + 4];
+};
 template <int DC, int NQ, int NP, int NW, Form F>
-__global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(AttentionArgs a, Split sp) {
-    constexpr int DP = DC * 64, kPitch = DP + 4;
-    __shared__ float red_m[NW][16], red_l[NW][16];
-    __shared__ __attribute__((aligned(16))) float buf[NW][16][kPitch];
+__device__ __attribute__((always_inline)) inline void few_rows(const AttentionArgs &a, const Split &sp, uint32_t id0,
+                                                               FewLds<DC, NW> &lds) {
+    auto &red_m = lds.red_m, &red_l = lds.red_l;
+    auto &buf = lds.buf;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int32_t D = a.t.dim, G = sp.group;
-    const uint32_t id0 = blockIdx.x, id1 = sp.by_heads.div(id0), id2 = sp.by_splits.div(id1);
+    const uint32_t id1 = sp.by_heads.div(id0), id2 = sp.by_splits.div(id1);
     const int32_t head = id0 - id1 * a.t.heads, split = id1 - id2 * sp.splits;
     const int32_t seq = F == kPrefix ? 0 : sp.by_tiles.div(id2);
     const Work work = work_of<F, 16>(a, sp, seq, id2 - seq * sp.tiles);
@@ -794,6 +799,12 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
     }
 }
 
+template <int DC, int NQ, int NP, int NW, Form F>
+__global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(AttentionArgs a, Split sp) {
+    __shared__ FewLds<DC, NW> lds;
+    few_rows<DC, NQ, NP, NW, F>(a, sp, blockIdx.x, lds);
+}
+
 // ---------------------------------------------------------------- many rows --
 //
 // One workgroup: 128 rows (queries x heads of the group) of one sequence and
@@ -814,28 +825,35 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
 // in three loops, always inlined: out of line, its registers lie in scratch.
 constexpr int kManyWaves = 4, kManyRows = 32 * kManyWaves;
 
+// LDS holds DP columns: past D, zeros for K and anything for V, whose columns
+// there are not stored.  K: [4 blocks][DP / 16][16 tokens][16].  V: [4
+// blocks][2][DP][8 tokens], in the halves the groups 0 and 2, 1 and 3 of four
+// tokens, and column 4 u + e in place e * DP / 4 + u: what the lanes write and
+// what they read is contiguous.
+template <int DP>
+struct ManyLds {
+    __attribute__((aligned(16))) uint8_t k[2][64 * DP];
+    __attribute__((aligned(16))) _Float16 v[2][64 * DP];
+    uint32_t has_nan;  // V, in steps that some row does not see whole
+};
 template <int DP, bool EXACT, int NQ, int NP, Form F>
-__global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attention_many(AttentionArgs a, Split sp) {
+__device__ __attribute__((always_inline)) inline void many_rows(const AttentionArgs &a, const Split &sp, uint32_t id0,
+                                                                ManyLds<DP> &lds) {
     constexpr int KJ = DP / 32;  // pairs of 16-element pieces of K
     constexpr int MT = DP / 32;  // tiles of 32 columns of V
     constexpr int PL = DP / 64;  // 16-byte loads for a lane of a 16-token block
-    // LDS holds DP columns: past D, zeros for K and anything for V, whose
-    // columns there are not stored.  K: [4 blocks][DP / 16][16 tokens][16].  V:
-    // [4 blocks][2][DP][8 tokens], in the halves the groups 0 and 2, 1 and 3 of
-    // four tokens, and column 4 u + e in place e * DP / 4 + u: what the lanes
-    // write and what they read is contiguous.
-    __shared__ __attribute__((aligned(16))) uint8_t stage_k[2][64 * DP];
-    __shared__ __attribute__((aligned(16))) _Float16 stage_v[2][64 * DP];
-    __shared__ uint32_t has_nan;  // V, in steps that some row does not see whole
+    auto &stage_k = lds.k;
+    auto &stage_v = lds.v;
+    uint32_t &has_nan = lds.has_nan;
     const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int32_t D = EXACT ? DP : a.t.dim, G = sp.group;
-    // workgroups of one sequence and KV head on one XCD (blockIdx modulo 8),
+    // workgroups of one sequence and KV head on one XCD (id0 modulo 8),
     // whose L2 then holds their K and V; the longest rows first
     const uint32_t pairs = F == kPrefix ? a.t.heads : (uint32_t)a.t.seqs * a.t.heads, per = (uint32_t)sp.tiles * sp.splits;
     const bool by_xcd = pairs % 8 == 0;
-    const uint32_t id = by_xcd ? blockIdx.x / 8 : blockIdx.x, over = sp.by_per.div(id), rest = id - over * per;
-    const uint32_t pair = by_xcd ? blockIdx.x % 8 + 8 * over : over;
+    const uint32_t id = by_xcd ? id0 / 8 : id0, over = sp.by_per.div(id), rest = id - over * per;
+    const uint32_t pair = by_xcd ? id0 % 8 + 8 * over : over;
     const int32_t place = sp.by_splits.div(rest), split = rest - place * sp.splits;
     const int32_t seq = F == kPrefix ? 0 : sp.by_heads.div(pair), head = pair - seq * a.t.heads;
     const Work work = work_of<F, kManyRows>(a, sp, seq, F == kPrefix ? place : sp.tiles - 1 - place);
@@ -1236,6 +1254,12 @@ __global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attentio
     }
 }
 
+template <int DP, bool EXACT, int NQ, int NP, Form F>
+__global__ __launch_bounds__(kManyWaves * 64, DP <= 128 ? 2 : 1) void k_attention_many(AttentionArgs a, Split sp) {
+    __shared__ ManyLds<DP> lds;
+    many_rows<DP, EXACT, NQ, NP, F>(a, sp, blockIdx.x, lds);
+}
+
 constexpr int kMostSplits = 128, kRowsSplits = 16;
 
 // how many parts a row has, and how many of the first ones do not count: the
@@ -1446,17 +1470,21 @@ void start_many(const AttentionArgs &a, const Split &sp, unsigned grid, hipStrea
 
 // NQ = 1: q is bf16; NP = 1: o is
 template <Form F, int NQ, int NP>
-hipError_t start_attention(const AttentionArgs &a, const Plan &p, hipStream_t s) {
+hipError_t start_attention_few(const AttentionArgs &a, const Plan &p, hipStream_t s) {
     const unsigned grid = (unsigned)p.groups;
     const int width = width_of(a.t.dim);
-    if (p.few)
-        width == 64    ? start_few<F, 1, NQ, NP>(a, p.sp, grid, s)
-        : width == 128 ? start_few<F, 2, NQ, NP>(a, p.sp, grid, s)
-                       : start_few<F, 4, NQ, NP>(a, p.sp, grid, s);
-    else
-        width == 64    ? start_many<F, 64, NQ, NP>(a, p.sp, grid, s)
-        : width == 128 ? start_many<F, 128, NQ, NP>(a, p.sp, grid, s)
-                       : start_many<F, 256, NQ, NP>(a, p.sp, grid, s);
+    width == 64    ? start_few<F, 1, NQ, NP>(a, p.sp, grid, s)
+    : width == 128 ? start_few<F, 2, NQ, NP>(a, p.sp, grid, s)
+                   : start_few<F, 4, NQ, NP>(a, p.sp, grid, s);
+    return hipGetLastError();
+}
+template <Form F, int NQ, int NP>
+hipError_t start_attention_many(const AttentionArgs &a, const Plan &p, hipStream_t s) {
+    const unsigned grid = (unsigned)p.groups;
+    const int width = width_of(a.t.dim);
+    width == 64    ? start_many<F, 64, NQ, NP>(a, p.sp, grid, s)
+    : width == 128 ? start_many<F, 128, NQ, NP>(a, p.sp, grid, s)
+                   : start_many<F, 256, NQ, NP>(a, p.sp, grid, s);
     return hipGetLastError();
 }
 
@@ -1485,7 +1513,7 @@ inline void set_divisors(Split &sp, const AttentionArgs &a) {
 // a call over one plan: attention, and the join where its rows are in parts
 template <Form F, int NQ, int NP>
 hipError_t launch_t(const AttentionArgs &a, const Plan &p, hipStream_t s) {
-    const hipError_t err = start_attention<F, NQ, NP>(a, p, s);
+    const hipError_t err = p.few ? start_attention_few<F, NQ, NP>(a, p, s) : start_attention_many<F, NQ, NP>(a, p, s);
     return err != hipSuccess || p.sp.splits == 1 ? err : start_join<F, NP>(a, p.sp, p.sp.splits, s);
 }
 template <Form F>
