@@ -4,8 +4,8 @@
     a  = attention(norm(h) Wqkv, cache) Wo
     h' = h + a;  y = gelu(norm(h') Wup) Wdown
 
-No positions are encoded.  Every step is a call of luisaml_amd.capi: the norms
-add the residual and emit the E4M3 codes and the scale that the QKV and up
+No positions are encoded here (decode_loop.py does).  Every step is a call of
+luisaml_amd.capi: the norms add the residual and emit the E4M3 codes and the scale that the QKV and up
 projections take, K and V go from columns of the QKV projection's output into a
 paged E4M3 cache, attention reads them there, and the output and down
 projections quantise their fp32 inputs as they run.  Sequences of any lengths
@@ -76,12 +76,20 @@ class DecoderLayer:
         before adds to it (bf16).  The rows are the last tokens of the cache's
         sequences, whose lengths count them.  Returns the same two for the next
         layer."""
-        a, s, h = capi.rms_norm(add, self.gamma1, self.eps, residual=x)
-        qkv = self.qkv.codes(a, s, torch.bfloat16).view(len(a), -1, self.dim)
-        q, k, v = qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=1)
+        (q, k, v), h = self.project(x, add)
         capi.kv_cache_write(k, v, *cache.args(cu_q), max_q)
         o = capi.attention(q, *cache.args(cu_q), max_q, cache.most, self.dim ** -0.5, out_dtype=torch.float32)
-        o = self.o.dynamic(o.view(len(a), -1), torch.bfloat16)
+        return self.finish(o, h)
+
+    def project(self, x, add):
+        """Queries, keys and values of a norm's output, and the residual stream."""
+        a, s, h = capi.rms_norm(add, self.gamma1, self.eps, residual=x)
+        qkv = self.qkv.codes(a, s, torch.bfloat16).view(len(a), -1, self.dim)
+        return qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=1), h
+
+    def finish(self, o, h):
+        """What follows attention."""
+        o = self.o.dynamic(o.view(len(o), -1), torch.bfloat16)
         a, s, h = capi.rms_norm(o, self.gamma2, self.eps, residual=h)
         y = self.up.codes(a, s, torch.float32, act=capi.ACT_GELU_ERF)
         return h, self.down.dynamic(y, torch.bfloat16)
@@ -89,11 +97,7 @@ class DecoderLayer:
     def plain(self, x, add, lengths, history):
         """The layer in fp64 on the same weights, nothing else rounded; history:
         the K and V of each sequence's earlier tokens, which it extends."""
-        def norm(h, gamma):
-            return h / (h.square().mean(dim=1, keepdim=True) + self.eps).sqrt() * gamma.double()
-        h = x.double() + add.double()
-        qkv = (norm(h, self.gamma1) @ self.qkv.values.double()).view(len(x), -1, self.dim)
-        q, k, v = qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=1)
+        (q, k, v), h = self.plain_project(x, add)
         out, at = [], 0
         for b, n in enumerate(lengths):
             K = torch.cat([history[b][0], k[at:at + n]]) if history[b] else k[at:at + n]
@@ -105,8 +109,19 @@ class DecoderLayer:
             w = torch.softmax(sc.masked_fill(hidden, -math.inf), dim=2)
             out.append(torch.einsum("hij,jhd->ihd", w, V.repeat_interleave(grp, 1).cpu()).reshape(n, -1).to(x.device))
             at += n
-        h = h + torch.cat(out) @ self.o.values.double()
-        y = norm(h, self.gamma2) @ self.up.values.double() + self.up.bias.double()
+        return self.plain_finish(torch.cat(out), h)
+
+    def plain_norm(self, h, gamma):
+        return h / (h.square().mean(dim=-1, keepdim=True) + self.eps).sqrt() * gamma.double()
+
+    def plain_project(self, x, add):
+        h = x.double() + add.double()
+        qkv = (self.plain_norm(h, self.gamma1) @ self.qkv.values.double()).view(len(x), -1, self.dim)
+        return qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=1), h
+
+    def plain_finish(self, o, h):
+        h = h + o @ self.o.values.double()
+        y = self.plain_norm(h, self.gamma2) @ self.up.values.double() + self.up.bias.double()
         y = 0.5 * y * (1 + torch.erf(y * 0.5 ** 0.5))
         return h, y @ self.down.values.double() + self.down.bias.double()
 
