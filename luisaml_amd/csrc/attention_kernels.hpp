@@ -900,14 +900,6 @@ __device__ __attribute__((always_inline)) inline void many_rows(const AttentionA
     u4 kr[PL], vr[PL];
     auto fetch = [&](int32_t k) __attribute__((always_inline)) {
         const int i = (k & 15) * 4;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) ks_next[q] = lane_of(blk.ks, i + q), vs_next[q] = lane_of(blk.vs, i + q);
-        const int32_t tok = step_token<F>(part, k);
-        uint32_t least = vs_next[0] < vs_next[1] ? vs_next[0] : vs_next[1];
-        least = vs_next[2] < least ? vs_next[2] : least;
-        least = vs_next[3] < least ? vs_next[3] : least;
-        whole_next = ((tok >= lo_max && tok + 64 <= hi_min) || (F == kSinks && (uint32_t)tok + 64 <= sinks_min)) && least;
-        scales.take(vs_next);
         const uint64_t at = (lane_of(blk.lo, i + wave) | (uint64_t)lane_of(blk.hi, i + wave) << 32) * (uint64_t)(16 * D);
         const uint8_t *pk = a.k + at, *pv = a.v + at;
 #pragma unroll
@@ -916,6 +908,15 @@ __device__ __attribute__((always_inline)) inline void many_rows(const AttentionA
             kr[x] = in ? *reinterpret_cast<const u4 *>(pk + (64 * x + lane) * 16) : u4{0, 0, 0, 0};
             vr[x] = in ? *reinterpret_cast<const u4 *>(pv + (64 * x + lane) * 16) : u4{0, 0, 0, 0};
         }
+        // (the scales after them: they were asked for last)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ks_next[q] = lane_of(blk.ks, i + q), vs_next[q] = lane_of(blk.vs, i + q);
+        const int32_t tok = step_token<F>(part, k);
+        uint32_t least = vs_next[0] < vs_next[1] ? vs_next[0] : vs_next[1];
+        least = vs_next[2] < least ? vs_next[2] : least;
+        least = vs_next[3] < least ? vs_next[3] : least;
+        whole_next = ((tok >= lo_max && tok + 64 <= hi_min) || (F == kSinks && (uint32_t)tok + 64 <= sinks_min)) && least;
+        scales.take(vs_next);
     };
     uint32_t vref = 0;  // the largest V scale up to the step that is worked on
     auto deposit = [&](int32_t k, int buf) __attribute__((always_inline)) {

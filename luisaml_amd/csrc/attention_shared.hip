@@ -47,8 +47,8 @@ void cap_parts(Plan &p) {
 // alone and 2.3 beside another.  64 queries behind 16384 tokens: 16 parts 51 us,
 // 17 (272 workgroups) 56, 24 55, 32 62; 560 rows of 3 groups behind 6000: 3 parts
 // 70 us, 6 53, 8 64.
-void beside_few(Plan &p, const Plan &own) {
-    const int64_t groups = p.groups / p.sp.splits, steps = ((int64_t)p.sp.chunk * p.sp.splits) >> 6;
+void beside_few(Plan &p, const Plan &own, int64_t span) {
+    const int64_t groups = p.groups / p.sp.splits, steps = (span + 63) / 64;
     const auto parts = [&](int64_t each) {
         const int64_t n = each / groups, most = steps / 4;
         return n > most ? (most > 1 ? most : 1) : n > 1 ? n : 1;
@@ -73,7 +73,7 @@ SharedPlan make_shared_plan(int64_t tokens, int64_t seqs, int64_t groups, int64_
     // the tiles of all groups' rows, and one more for each group that ends inside a tile
     const int64_t rows = tokens * (q_heads / kv_heads);
     s.prefix = divide(s.own.few && few_rows(kv_heads, dim, rows, max_prefix), kv_heads, rows, max_prefix);
-    if (s.own.few && !s.prefix.few) beside_few(s.prefix, s.own);
+    if (s.own.few && !s.prefix.few) beside_few(s.prefix, s.own, max_prefix);
     cap_parts(s.prefix);
     s.prefix.sp.tiles += (int32_t)(groups - 1);
     s.prefix.groups = kv_heads * s.prefix.sp.tiles * s.prefix.sp.splits;
