@@ -841,7 +841,7 @@ __device__ __attribute__((always_inline)) inline void many_rows(const AttentionA
                                                                 ManyLds<DP> &lds) {
     constexpr int KJ = DP / 32;  // pairs of 16-element pieces of K
     constexpr int MT = DP / 32;  // tiles of 32 columns of V
-    constexpr int PL = DP / 64;  // 16-byte loads for a lane of a 16-token block
+    constexpr int PL = (DP + 63) / 64;  // 16-byte loads for a lane of a 16-token block
     auto &stage_k = lds.k;
     auto &stage_v = lds.v;
     uint32_t &has_nan = lds.has_nan;
@@ -904,7 +904,7 @@ __device__ __attribute__((always_inline)) inline void many_rows(const AttentionA
         const uint8_t *pk = a.k + at, *pv = a.v + at;
 #pragma unroll
         for (int x = 0; x < PL; ++x) {
-            const bool in = EXACT || 64 * x + lane < D;
+            const bool in = (EXACT && DP % 64 == 0) || 64 * x + lane < D;
             kr[x] = in ? *reinterpret_cast<const u4 *>(pk + (64 * x + lane) * 16) : u4{0, 0, 0, 0};
             vr[x] = in ? *reinterpret_cast<const u4 *>(pv + (64 * x + lane) * 16) : u4{0, 0, 0, 0};
         }
@@ -943,8 +943,8 @@ __device__ __attribute__((always_inline)) inline void many_rows(const AttentionA
 #pragma unroll
         for (int x = 0; x < PL; ++x) {
             const int u = 64 * x + lane, g = u / (D >> 2), d4 = u - g * (D >> 2);  // a group of tokens, columns 4 d4 ..
-            *reinterpret_cast<u4 *>(&stage_k[buf][wave * 16 * DP + u * 16]) = kr[x];  // zeros past D
-            if (EXACT || u < D)
+            if (DP % 64 == 0 || u < DP) *reinterpret_cast<u4 *>(&stage_k[buf][wave * 16 * DP + u * 16]) = kr[x];  // zeros past D
+            if ((EXACT && DP % 64 == 0) || u < D)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     *reinterpret_cast<h4 *>(&stage_v[buf][wave * 16 * DP + (g & 1) * 8 * DP + (e * (DP / 4) + d4) * 8 + (g >> 1) * 4]) =
@@ -988,10 +988,6 @@ __device__ __attribute__((always_inline)) inline void many_rows(const AttentionA
     for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
-    auto column = [&](int t, int i) {
-        const int p = 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
-        return 4 * (p % (DP / 4)) + p / (DP / 4);
-    };
     float m = -kInf, l = 0.0f;
     auto scale_o = [&](float f) {
 #pragma unroll
@@ -1229,18 +1225,19 @@ __device__ __attribute__((always_inline)) inline void many_rows(const AttentionA
     if (!live) return;
     // (the scale last: with the other factor it could leave fp32's range)
     const float f = apart ? 1.0f : 1.0f / (1 << kVBits) / l, scale = apart ? 1.0f : bits_f32(vref);
-    // four columns 4 u .. 4 u + 3: places u, DP / 4 + u, ..
+    // four columns 4 u .. 4 u + 3: places u, DP / 4 + u, .., eight places a group
+    // of four rows of o
     auto results = [&](auto put) {
 #pragma unroll
-        for (int x = 0; x < (DP + 127) / 128; ++x)
+        for (int c = 0; c < DP / 32; ++c)
 #pragma unroll
-            for (int i = 0; i < (DP < 128 ? DP / 8 : 16); ++i) {
-                const int d = column(x, i);  // e = 0
+            for (int i = 0; i < 4; ++i) {
+                const int d = 4 * (8 * c + 4 * h + i);
                 f4 v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int t = (e * (DP / 4) + 32 * x) / 32, up = (e * (DP / 4) + 32 * x) % 32;  // DP 64: half a tile on
-                    v[e] = l == 0.0f ? 0.0f : o[t][i + up / 2] * f * scale;
+                    const int at = e * (DP / 32) + c;
+                    v[e] = l == 0.0f ? 0.0f : o[at / 4][at % 4 * 4 + i] * f * scale;
                 }
                 if (EXACT || d < D) put(d, v);
             }
@@ -1382,7 +1379,11 @@ struct Plan {
     Split sp;
 };
 
-inline int width_of(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }  // columns that the kernels are built for
+// columns that the kernels are built for; the one for many rows also for 96,
+// whose products are three quarters of 128's (4 x 300 queries of heads of 96 in
+// fp32 behind a window TIME96)
+inline int width_of(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+inline int many_width_of(int64_t dim) { return dim > 64 && dim <= 96 ? 96 : width_of(dim); }
 
 // one kernel's division of rows of `pairs` (sequence, KV head), that see `span`
 // tokens at most
@@ -1482,8 +1483,9 @@ hipError_t start_attention_few(const AttentionArgs &a, const Plan &p, hipStream_
 template <Form F, int NQ, int NP>
 hipError_t start_attention_many(const AttentionArgs &a, const Plan &p, hipStream_t s) {
     const unsigned grid = (unsigned)p.groups;
-    const int width = width_of(a.t.dim);
+    const int width = many_width_of(a.t.dim);
     width == 64    ? start_many<F, 64, NQ, NP>(a, p.sp, grid, s)
+    : width == 96  ? start_many<F, 96, NQ, NP>(a, p.sp, grid, s)
     : width == 128 ? start_many<F, 128, NQ, NP>(a, p.sp, grid, s)
                    : start_many<F, 256, NQ, NP>(a, p.sp, grid, s);
     return hipGetLastError();

@@ -1,116 +1,8 @@
-// attention_shared.hip -- attention for groups of sequences that share their
-// first tokens (attention_kernels.hpp, kPrefix and kOwn).
-//
-// What a group shares is read once, for the rows of all its sequences
-// together, which then also fill the matrix instructions' columns; each
-// sequence's own tokens as ever.  Both leave parts (results divided by their
-// sums, and the sums' logarithms), and one join puts a row's together:
-//   o = sum_p o_p 2^(L_p) / sum_p 2^(L_p),   L_p = log2 sum_(j in p) w_j
-#include "attention_kernels.hpp"
+// attention_shared.hip -- calls of attention behind shared prefixes
+// (attention_shared.hpp), and its kernels for bf16 queries.
+#include "attention_shared.hpp"
 
 namespace lcml {
-namespace {
-
-constexpr int kMostParts = kMostSplits / 2;  // of the prefix, and of the own tokens
-
-// The prefix's workgroups, and then the own tokens' where few rows have them,
-// in one launch: the former wait for the matrix cores and the latter for
-// memory, and short calls save a launch.
-template <int DP, bool EXACT, int NQ, int NP, bool MANY>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_shared(AttentionArgs prefix, Split psp,
-                                                                             AttentionArgs own, Split osp, uint32_t first) {
-    using Few = FewLds<DP / 64, kFewWaves>;
-    using Prefix = std::conditional_t<MANY, ManyLds<DP>, Few>;
-    __shared__ __attribute__((aligned(16))) char lds[sizeof(Prefix) > sizeof(Few) ? sizeof(Prefix) : sizeof(Few)];
-    if (blockIdx.x < first) {
-        if constexpr (MANY)
-            many_rows<DP, EXACT, NQ, NP, kPrefix>(prefix, psp, blockIdx.x, *reinterpret_cast<ManyLds<DP> *>(lds));
-        else
-            few_rows<DP / 64, NQ, NP, kFewWaves, kPrefix>(prefix, psp, blockIdx.x, *reinterpret_cast<Few *>(lds));
-    } else {
-        few_rows<DP / 64, NQ, NP, kFewWaves, kOwn>(own, osp, blockIdx.x - first, *reinterpret_cast<Few *>(lds));
-    }
-}
-static_assert(kManyWaves == 4 && kFewWaves == 4, "both in workgroups of 256");
-
-// fewer parts where there are too many for the join
-void cap_parts(Plan &p) {
-    if (p.sp.splits <= kMostParts) return;
-    p.groups = p.groups / p.sp.splits * kMostParts;
-    p.sp.chunk = (int32_t)((((int64_t)p.sp.chunk * p.sp.splits + kMostParts - 1) / kMostParts + 63) & ~63);
-    p.sp.splits = kMostParts;
-}
-
-// The parts of a prefix that many rows read, beside workgroups of few rows: as
-// many as make one workgroup a CU, which leaves the rest of it to those, or two,
-// which they follow; of four steps at least.  By measurement a step takes 1.8 us
-// alone and 2.3 beside another.  64 queries behind 16384 tokens: 16 parts 51 us,
-// 17 (272 workgroups) 56, 24 55, 32 62; 560 rows of 3 groups behind 6000: 3 parts
-// 70 us, 6 53, 8 64.
-void beside_few(Plan &p, const Plan &own, int64_t span) {
-    const int64_t groups = p.groups / p.sp.splits, steps = (span + 63) / 64;
-    const auto parts = [&](int64_t each) {
-        const int64_t n = each / groups, most = steps / 4;
-        return n > most ? (most > 1 ? most : 1) : n > 1 ? n : 1;
-    };
-    const auto length = [&](int64_t n) { return (steps + n - 1) / n; };
-    const double own_us = 3.5 + 2.5 * ((own.sp.chunk / 64 + kFewWaves - 1) / kFewWaves);
-    const int64_t one = parts(256), two = parts(512);
-    const int64_t n = 1.8 * length(one) < 2.3 * length(two) + own_us ? one : two;
-    p.sp.splits = (int32_t)n, p.sp.chunk = (int32_t)(length(n) * 64), p.groups = groups * n;
-}
-
-struct SharedPlan {
-    Plan prefix, own;
-};
-SharedPlan make_shared_plan(int64_t tokens, int64_t seqs, int64_t groups, int64_t q_heads, int64_t kv_heads, int64_t dim,
-                            int64_t max_q, int64_t max_own, int64_t max_prefix) {
-    SharedPlan s{};
-    s.own = make_plan(seqs, q_heads, kv_heads, dim, max_q, max_own + 63, 0, 0);  // from a multiple of 64 on
-    cap_parts(s.own);
-    s.own.sp.parts = s.own.sp.splits;
-    if (groups == 0) return s;
-    // the tiles of all groups' rows, and one more for each group that ends inside a tile
-    const int64_t rows = tokens * (q_heads / kv_heads);
-    s.prefix = divide(s.own.few && few_rows(kv_heads, dim, rows, max_prefix), kv_heads, rows, max_prefix);
-    if (s.own.few && !s.prefix.few) beside_few(s.prefix, s.own, max_prefix);
-    cap_parts(s.prefix);
-    s.prefix.sp.tiles += (int32_t)(groups - 1);
-    s.prefix.groups = kv_heads * s.prefix.sp.tiles * s.prefix.sp.splits;
-    s.own.sp.first = s.prefix.sp.splits;
-    s.prefix.sp.parts = s.own.sp.parts = s.prefix.sp.splits + s.own.sp.splits;
-    return s;
-}
-
-template <int DP, int NQ, int NP>
-void start_shared(const AttentionArgs &prefix, const AttentionArgs &own, const SharedPlan &p, hipStream_t s) {
-    const dim3 grid((unsigned)(p.prefix.groups + p.own.groups)), block(256);
-    const uint32_t first = (uint32_t)p.prefix.groups;
-    if (p.prefix.few)
-        hipLaunchKernelGGL((k_attention_shared<DP, false, NQ, NP, false>), grid, block, 0, s, prefix, p.prefix.sp, own, p.own.sp, first);
-    else if (own.t.dim == DP)
-        hipLaunchKernelGGL((k_attention_shared<DP, true, NQ, NP, true>), grid, block, 0, s, prefix, p.prefix.sp, own, p.own.sp, first);
-    else
-        hipLaunchKernelGGL((k_attention_shared<DP, false, NQ, NP, true>), grid, block, 0, s, prefix, p.prefix.sp, own, p.own.sp, first);
-}
-
-template <int NQ, int NP>
-hipError_t launch_shared_t(const AttentionArgs &prefix, const AttentionArgs &own, const SharedPlan &p, hipStream_t s) {
-    hipError_t err = hipSuccess;
-    if (p.own.few) {
-        const int width = width_of(own.t.dim);
-        width == 64    ? start_shared<64, NQ, NP>(prefix, own, p, s)
-        : width == 128 ? start_shared<128, NQ, NP>(prefix, own, p, s)
-                       : start_shared<256, NQ, NP>(prefix, own, p, s);
-        err = hipGetLastError();
-    } else {
-        if (p.prefix.groups) err = start_attention_many<kPrefix, NQ, NP>(prefix, p.prefix, s);
-        if (err == hipSuccess) err = start_attention_many<kOwn, NQ, NP>(own, p.own, s);
-    }
-    return err == hipSuccess ? start_join<kOwn, NP>(own, p.own.sp, p.own.sp.parts, s) : err;
-}
-
-}  // namespace
 
 int64_t attention_shared_workspace(int64_t tokens, int64_t seqs, int64_t groups, int64_t q_heads, int64_t kv_heads,
                                    int64_t dim, int64_t max_q, int64_t max_own, int64_t max_prefix, int64_t *workgroups) {
@@ -122,23 +14,8 @@ int64_t attention_shared_workspace(int64_t tokens, int64_t seqs, int64_t groups,
 hipError_t launch_attention_shared(const AttentionArgs &own, const int32_t *prefix_table, int64_t prefix_stride,
                                    int64_t prefix_cols, int64_t max_prefix, void *work, hipStream_t s,
                                    const char **kernel) {
-    AttentionArgs prefix = own;
-    prefix.t.table = prefix_table, prefix.t.table_stride = prefix_stride, prefix.t.table_cols = (int32_t)prefix_cols;
-    prefix.max_q = own.t.tokens, prefix.max_kv = max_prefix, prefix.causal = 0;  // all rows lie behind it
-    SharedPlan p = make_shared_plan(own.t.tokens, own.t.seqs, own.groups, own.q_heads, own.t.heads, own.t.dim, own.max_q,
-                                    own.max_kv, max_prefix);
-    if (p.prefix.groups)
-        set_divisors(p.prefix.sp, prefix);
-    else
-        p.prefix.few = true;
-    set_divisors(p.own.sp, own);
-    p.prefix.sp.o = p.own.sp.o = static_cast<float *>(work);
-    p.prefix.sp.lse = p.own.sp.lse = p.own.sp.o + (int64_t)own.t.tokens * own.q_heads * p.own.sp.parts * own.t.dim;
-    *kernel = !p.own.few                         ? "attention_many, attention_many, attention_join"
-              : !p.prefix.few && p.prefix.groups ? "attention_shared_many, attention_join"
-                                                 : "attention_shared_few, attention_join";
-    if (own.q_bf16) return own.o_bf16 ? launch_shared_t<1, 1>(prefix, own, p, s) : launch_shared_t<1, 2>(prefix, own, p, s);
-    return own.o_bf16 ? launch_shared_t<2, 1>(prefix, own, p, s) : launch_shared_t<2, 2>(prefix, own, p, s);
+    return own.q_bf16 ? launch_shared<1>(own, prefix_table, prefix_stride, prefix_cols, max_prefix, work, s, kernel)
+                      : launch_attention_shared_f32(own, prefix_table, prefix_stride, prefix_cols, max_prefix, work, s, kernel);
 }
 
 }  // namespace lcml

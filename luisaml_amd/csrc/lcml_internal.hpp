@@ -178,6 +178,9 @@ int64_t attention_shared_workspace(int64_t tokens, int64_t seqs, int64_t groups,
 hipError_t launch_attention_shared(const AttentionArgs &a, const int32_t *prefix_table, int64_t prefix_stride,
                                    int64_t prefix_cols, int64_t max_prefix, void *work, hipStream_t s,
                                    const char **kernel);
+hipError_t launch_attention_shared_f32(const AttentionArgs &a, const int32_t *prefix_table, int64_t prefix_stride,
+                                       int64_t prefix_cols, int64_t max_prefix, void *work, hipStream_t s,
+                                       const char **kernel);
 
 // A kernel's dynamic-LDS limit (hipFuncSetAttribute) is per device: set it
 // once per (kernel, device), tracked in `done` (bit d = device d; devices past
