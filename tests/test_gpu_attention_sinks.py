@@ -119,12 +119,23 @@ def test_scales_far_apart(dev, max_q, ot):
 def test_long_sequences(dev, n, L, window, sinks, ot):
     """Windows at which the work of a row is split and joined, sinks that fill
     whole parts, and holes of a few tokens."""
-    run(dev, [L, L // 3, 7], [n, n, min(n, 7)], window, sinks, 64, 1, 4, 64, "b", ot, seed=n)
+    run(dev, [L, L // 3, 7], [n, n, min(n, 7)], window, sinks, 64, 1, 4, 64, "b", ot, seed=n,
+        kernel="attention_few, attention_join" if n < 40 else None)
 
 
-@pytest.mark.parametrize("D", [64, 128])
-def test_many_rows_split_and_joined(dev, D):
-    run(dev, [3000, 1000], [700, 100], 1500, 100, 64, 1, 4, D, seed=D, kernel="attention_join")
+@pytest.mark.parametrize("D,kernel", [(64, "attention_few"), (128, "attention_many, attention_join")])
+def test_many_queries_over_a_long_window(dev, D, kernel):
+    run(dev, [3000, 1000], [700, 100], 1500, 100, 64, 1, 4, D, seed=D, kernel=kernel)
+
+
+@pytest.mark.parametrize("qt,ot", [("b", "b"), ("b", "f"), ("f", "f"), ("f", "b")])
+@pytest.mark.parametrize("D", [32, 64, 80, 128])
+def test_eight_wavefronts_and_none_of_their_steps(dev, D, qt, ot):
+    """One workgroup a row tile: 9 to 20 steps, of which most wavefronts have two
+    or three, some one and in short sequences none."""
+    run(dev, [1200, 1, 70, 700, 0, 1130], [1, 1, 1, 1, 1, 1], 900, 130, 16, 2, 4, D, qt, ot, seed=D, max_kv=1200, kernel="attention_few")
+    run(dev, [1200, 300], [3, 2], 900, 130, 32, 1, 4, D, qt, ot, seed=D)
+    assert "attention_join" not in ", ".join(capi.kernel_trace())
 
 
 @pytest.mark.parametrize("kv,n", [([300, 40], [1, 1]), ([3000, 900], [1, 2]), ([700, 300], [100, 80])])
