@@ -617,8 +617,8 @@ LCML_API int lcml_fp8_attention_sinks(const void *q, int q_dtype, int64_t tokens
 /*
  * lcml_fp8_attention (without a window) for groups of sequences that share
  * their first tokens' pages, which are read once for a group:
- *   group g is the sequences group_seq[g] .. group_seq[g+1]-1 (group_seq[0] = 0,
- *   rising; sequences from group_seq[groups] on share nothing); its first
+ *   group g is the sequences group_seq[g] .. group_seq[g+1]-1 (rising; sequences
+ *   before the first group and after the last share nothing); its first
  *   prefix_len[g] tokens (0: none) lie in the pages prefix_table[g][..]
  *   ([groups] rows of prefix_cols pages, row pitch prefix_stride), in tokens'
  *   order as in block_table.

@@ -296,11 +296,15 @@ __device__ inline int64_t part_at(const Split &sp, int64_t row, int32_t split) {
 __device__ inline SeqRows group_rows(const AttentionArgs &a, int32_t g) {
     SeqRows s{0, 0, 0, 0};
     if (g >= a.groups) return s;
-    const int32_t b0 = a.group_seq[g], b1 = a.group_seq[g + 1], len = a.prefix_len[g];
-    if (b0 < 0 || b1 < b0 || b1 > a.t.seqs || len <= 0) return s;
-    const int32_t row0 = a.t.cu[b0], end = a.t.cu[b1];
-    if (row0 < 0 || end > a.t.tokens || end < row0) return s;
-    return SeqRows{row0, end - row0, len, len};
+    int32_t b0 = a.group_seq[g], b1 = a.group_seq[g + 1];
+    const int32_t len = a.prefix_len[g];
+    // (cut to what there is: a sequence out of range must not take the others'
+    // parts with it)
+    b0 = b0 > 0 ? b0 : 0, b1 = b1 < a.t.seqs ? b1 : a.t.seqs;
+    if (b1 <= b0 || len <= 0) return s;
+    int32_t row0 = a.t.cu[b0], end = a.t.cu[b1];
+    row0 = row0 > 0 ? row0 : 0, end = end < a.t.tokens ? end : a.t.tokens;
+    return end > row0 ? SeqRows{row0, end - row0, len, len} : s;
 }
 
 // the tokens that sequence b reads with its group; 0: none, also where its rows
@@ -311,7 +315,7 @@ __device__ inline int32_t shared_tokens(const AttentionArgs &a, int32_t b, const
     for (int32_t g0 = 0; g0 < a.groups; g0 += 64) {
         const int32_t g = g0 + lane;
         const bool in = g < a.groups;
-        const int32_t end = in ? a.group_seq[g + 1] : 0x7fffffff, own = in ? a.prefix_len[g] : 0;
+        const int32_t end = in ? a.group_seq[g + 1] : 0x7fffffff, own = in && b >= a.group_seq[g] ? a.prefix_len[g] : 0;
         const uint64_t over = __builtin_amdgcn_ballot_w64(end > b);  // b's group, and those after it
         if (!over) continue;
         len = __builtin_amdgcn_readlane(own, __builtin_ctzll(over));
@@ -330,7 +334,7 @@ __device__ inline int32_t shared_tokens_of_lane(const AttentionArgs &a, int32_t 
         else
             lo = m + 1;
     }
-    const int32_t len = lo < a.groups ? a.prefix_len[lo] : 0;
+    const int32_t len = lo < a.groups && b >= a.group_seq[lo] ? a.prefix_len[lo] : 0;
     return len > 0 && s.pos0 >= len ? len : 0;
 }
 

@@ -128,6 +128,24 @@ def test_more_groups_than_lanes(dev, groups):
     run(dev, [(16 * (g % 3 + 1), [g % 5 + 1, 3]) for g in range(groups)], 1, 16, 1, 2, 32, seed=groups)
 
 
+@pytest.mark.parametrize("n", [1, 40])
+def test_sequences_outside_groups_and_rows_out_of_range(dev, n):
+    """A first group that does not begin at the first sequence; one that ends past
+    the last; a sequence whose rows pass the batch's counts as none, and its
+    group's others are as they were."""
+    def change(q, cache, table, kv, first, pt, plen):
+        return np.array([1, 3, 9]), np.concatenate([pt[:1], pt[:1]]), np.array([64, 64])
+    run(dev, [(64, [40, 50, 41, 70, 45])], n, 16, 1, 4, 64, change=change)
+    cache, table, kv, first, pt, plen = batch([(64, [40, 50, 41])], 16, 1, 64, 0)
+    q = torch.from_numpy(synth.normal(7, (2 * n, 4, 64))).to(dev)
+    out = torch.full_like(q, 5.0)
+    capi.attention_shared(q, *cache.to(dev), i32(table, dev), i32(kv, dev), i32([0, n, 2 * n, 2 * n + 3], dev), i32(first, dev),
+                          i32(pt, dev), i32(plen, dev), n, 50, 64, 0.125, out=out)
+    torch.cuda.synchronize()
+    dc.check_attention(out.double().cpu().numpy(), q.cpu().numpy(), cache, table[:2], kv[:2], [0, n, 2 * n], 1, 0.125, False,
+                       shared=(first, pt, plen))
+
+
 def test_no_groups(dev):
     def change(q, cache, table, kv, first, pt, plen):
         return np.array([0]), np.zeros((0, 1)), np.array([], dtype=np.int32)
