@@ -45,23 +45,32 @@ inline void cap_parts(Plan &p) {
     p.sp.splits = kMostParts;
 }
 
-// The parts of a prefix that many rows read, beside workgroups of few rows: as
-// many as make one workgroup a CU, which leaves the rest of it to those, or two,
-// which they follow; of four steps at least.  By measurement a step takes 1.8 us
-// alone and 2.3 beside another.  64 queries behind 16384 tokens: 16 parts 51 us,
-// 17 (272 workgroups) 56, 24 55, 32 62; 560 rows of 3 groups behind 6000: 3 parts
-// 70 us, 6 53, 8 64.
-inline void beside_few(Plan &p, const Plan &own, int64_t span) {
+// The parts of a prefix that many rows read: as many as make the least of, in
+// us by measurement (heads of 128, others by their columns),
+//   a step, 1.8 for a workgroup alone on its CU and 1.15 for each of several;
+//   a start and an end for every two of a CU's, which overlap;
+//   what the parts write and the join reads back, at 3.5 TB/s;
+//   the own tokens' workgroups of few rows, which run beside one workgroup a CU
+//   but after several.
+// 64 queries behind 16384 tokens (16 row tiles): 16 parts 51 us, 17 (272
+// workgroups) 56, 24 55, 32 62; 560 rows of 3 groups behind 6000 (74 tiles): 3
+// parts 70 us, 6 53, 8 64; 8 x 100 rows behind 8192 (200 tiles): 3 parts 201 us,
+// 5 174.
+inline void divide_prefix(Plan &p, const Plan &own, int64_t dim, int64_t span) {
     const int64_t groups = p.groups / p.sp.splits, steps = (span + 63) / 64;
-    const auto parts = [&](int64_t each) {
-        const int64_t n = each / groups, most = steps / 4;
-        return n > most ? (most > 1 ? most : 1) : n > 1 ? n : 1;
-    };
+    const int64_t most = steps / 4 > kMostParts ? kMostParts : steps / 4;  // four steps at least
+    const double width = many_width_of(dim), scale = width < 96 ? 0.67 : width / 128;
+    const double own_us = own.few ? 3.5 + 2.5 * ((own.sp.chunk / 64 + kFewWaves - 1) / kFewWaves) : 0.0;
     const auto length = [&](int64_t n) { return (steps + n - 1) / n; };
-    const double own_us = 3.5 + 2.5 * ((own.sp.chunk / 64 + kFewWaves - 1) / kFewWaves);
-    const int64_t one = parts(256), two = parts(512);
-    const int64_t n = 1.8 * length(one) < 2.3 * length(two) + own_us ? one : two;
-    p.sp.splits = (int32_t)n, p.sp.chunk = (int32_t)(length(n) * 64), p.groups = groups * n;
+    int64_t best = 1;
+    double least = 0.0;
+    for (int64_t n = 1; n <= most || n == 1; ++n) {
+        const int64_t each = (groups * n + 255) / 256;  // workgroups of a CU
+        const double us = length(n) * scale * (each == 1 ? 1.8 : 1.15 * each) + 8.0 * ((each + 1) / 2) +
+                          groups * n * (kManyRows * 8.0 / 3.5e6) * dim + (each == 1 ? 0.0 : own_us);
+        if (n == 1 || us < least) best = n, least = us;
+    }
+    p.sp.splits = (int32_t)best, p.sp.chunk = (int32_t)(length(best) * 64), p.groups = groups * best;
 }
 
 struct SharedPlan {
@@ -77,7 +86,7 @@ inline SharedPlan make_shared_plan(int64_t tokens, int64_t seqs, int64_t groups,
     // the tiles of all groups' rows, and one more for each group that ends inside a tile
     const int64_t rows = tokens * (q_heads / kv_heads);
     s.prefix = divide(s.own.few && few_rows(kv_heads, dim, rows, max_prefix), kv_heads, rows, max_prefix);
-    if (s.own.few && !s.prefix.few) beside_few(s.prefix, s.own, max_prefix);
+    if (!s.prefix.few) divide_prefix(s.prefix, s.own, dim, max_prefix);
     cap_parts(s.prefix);
     s.prefix.sp.tiles += (int32_t)(groups - 1);
     s.prefix.groups = kv_heads * s.prefix.sp.tiles * s.prefix.sp.splits;
