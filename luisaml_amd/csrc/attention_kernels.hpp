@@ -819,8 +819,8 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
 // repeated by each of the four), and reads K's codes in half the bytes (K
 // widened as well: 2% slower).  32x32x16 instructions.
 //
-// A prompt of 8192 tokens, 32 heads over 8 of 128, 0.55 TFLOP: 610 us, 900
-// TFLOP/s, where a product of 8192^3 in bf16 reaches 1190.  A step's 32 matrix
+// A prompt of 8192 tokens, 32 heads over 8 of 128, 0.55 TFLOP: 588 to 605 us,
+// 920 TFLOP/s, where a product of 8192^3 in bf16 reaches 1190.  A step's 32 matrix
 // instructions take 1024 cycles of a SIMD, its 320 vector ones 1280, and two
 // wavefronts a SIMD overlap them to two thirds of the sum.  (Two groups of
 // wavefronts half a step apart: 1075 us, for the registers spilled.)  D > 128

@@ -11,6 +11,10 @@
 // One workgroup does it all where there is little to write; else it leaves the
 // sums, and a second launch writes the new columns and the rows, each finding
 // its sequence by bisection in LDS.
+//
+// Measured: 64 sequences of a decode step 4.0 us in a graph, 5.2 where pages
+// come back (one round trip more), 256 4.7, 1024 7.0, 4096 17; 48 prompts, 196 000
+// rows, 7.7 in two launches, 13 with 4400 pages that come back.
 #include "kv_cache.hpp"
 #include "lcml_internal.hpp"
 
