@@ -95,9 +95,10 @@ inline SharedPlan make_shared_plan(int64_t tokens, int64_t seqs, int64_t groups,
     return s;
 }
 
+// (own tokens that many rows have: none of their workgroups)
 template <int DP, int NQ, int NP>
 void start_shared(const AttentionArgs &prefix, const AttentionArgs &own, const SharedPlan &p, hipStream_t s) {
-    const dim3 grid((unsigned)(p.prefix.groups + p.own.groups)), block(256);
+    const dim3 grid((unsigned)(p.prefix.groups + (p.own.few ? p.own.groups : 0))), block(256);
     const uint32_t first = (uint32_t)p.prefix.groups;
     if (p.prefix.few)
         hipLaunchKernelGGL((k_attention_shared<(DP == 96 ? 128 : DP), false, NQ, NP, false>), grid, block, 0, s, prefix, p.prefix.sp, own, p.own.sp, first);
@@ -110,17 +111,15 @@ void start_shared(const AttentionArgs &prefix, const AttentionArgs &own, const S
 template <int NQ, int NP>
 hipError_t launch_shared_t(const AttentionArgs &prefix, const AttentionArgs &own, const SharedPlan &p, hipStream_t s) {
     hipError_t err = hipSuccess;
-    if (p.own.few) {
+    if (p.own.few || p.prefix.groups) {
         const int width = many_width_of(own.t.dim);
         width == 64    ? start_shared<64, NQ, NP>(prefix, own, p, s)
         : width == 96  ? start_shared<96, NQ, NP>(prefix, own, p, s)
         : width == 128 ? start_shared<128, NQ, NP>(prefix, own, p, s)
                        : start_shared<256, NQ, NP>(prefix, own, p, s);
         err = hipGetLastError();
-    } else {
-        if (p.prefix.groups) err = start_attention_many<kPrefix, NQ, NP>(prefix, p.prefix, s);
-        if (err == hipSuccess) err = start_attention_many<kOwn, NQ, NP>(own, p.own, s);
     }
+    if (!p.own.few && err == hipSuccess) err = start_attention_many<kOwn, NQ, NP>(own, p.own, s);
     return err == hipSuccess ? start_join<kOwn, NP>(own, p.own.sp, p.own.sp.parts, s) : err;
 }
 
@@ -140,7 +139,7 @@ hipError_t launch_shared(const AttentionArgs &own, const int32_t *prefix_table, 
     set_divisors(p.own.sp, own);
     p.prefix.sp.o = p.own.sp.o = static_cast<float *>(work);
     p.prefix.sp.lse = p.own.sp.lse = p.own.sp.o + (int64_t)own.t.tokens * own.q_heads * p.own.sp.parts * own.t.dim;
-    *kernel = !p.own.few                         ? "attention_many, attention_many, attention_join"
+    *kernel = !p.own.few ? (p.prefix.groups ? "attention_shared_many, attention_many, attention_join" : "attention_many, attention_join")
               : !p.prefix.few && p.prefix.groups ? "attention_shared_many, attention_join"
                                                  : "attention_shared_few, attention_join";
     return own.o_bf16 ? launch_shared_t<NQ, 1>(prefix, own, p, s) : launch_shared_t<NQ, 2>(prefix, own, p, s);

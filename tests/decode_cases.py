@@ -125,7 +125,7 @@ def attention(q, cache, table, kv_len, cu, heads, scale, causal=True, window=0, 
             sees = there & (j <= p) if causal else there.copy()
             if window:
                 sees &= (j > p - window) | (j < sinks)
-            if p < 0 or not sees.any():
+            if not sees.any():
                 continue
             r = cu[b] + i
             for h in range(q_heads):

@@ -180,6 +180,7 @@ def test_missing_pages(dev, n):
 
 def test_not_causal(dev):
     run(dev, [(64, [30, 20, 40])], [30, 1, 4], 16, 2, 2, 64, causal=False)
+    run(dev, [(64, [30, 20, 40])], [100, 85, 4], 16, 2, 2, 64, causal=False)  # rows inside the prefix, and before it
 
 
 @pytest.mark.parametrize("D", [64, 80, 256])

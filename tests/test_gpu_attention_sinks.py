@@ -80,6 +80,7 @@ def test_no_window_no_sinks_is_attention(dev, max_q):
 @pytest.mark.parametrize("max_q", [None, MANY])
 def test_not_causal(dev, max_q):
     run(dev, [40, 1, 200, 77], [10, 1, 100, 1], 20, 6, 16, 2, 2, 64, causal=False, seed=3, max_q=max_q)
+    run(dev, [40, 1, 200, 77], [45, 3, 100, 1], 20, 6, 16, 2, 2, 64, causal=False, seed=3, max_q=max_q)  # rows before the first token
 
 
 @pytest.mark.parametrize("max_q", [None, MANY])
