@@ -11,9 +11,8 @@
 // token's heads in turn and keeps its cosines, sines and gammas.
 //
 // Measured: 32 + 8 heads of 128 in bf16, one token 2.5 us in a graph, 64 2.7, 8192
-// (172 MB) 38 on new data, 4.5 TB/s; with 100 of 128 elements rotated, which
-// leaves no runs of 16 bytes, 42 where 128 take 28; 1333 tokens of 32 heads of
-// 96 in fp32, neighbours, 33 MB, 8.6 (3.8 TB/s).
+// (172 MB) 38 on new data, 4.5 TB/s; 1333 tokens of 32 heads of 96 in fp32,
+// neighbours, 33 MB, 8.6 (3.8 TB/s).
 #include "lcml_internal.hpp"
 
 namespace lcml {
@@ -79,20 +78,16 @@ __device__ inline float group_sum(float v) {
     return v;
 }
 
-// how a pair lies in memory: halves of the rotated part, neighbours, or halves
-// that a lane's runs would straddle
-enum { kHalves = 0, kNeighbours = 1, kScattered = 2 };
+// how a pair lies in memory: in the halves of the rotated part, or neighbours
+enum { kHalves = 0, kNeighbours = 1 };
 
-// A lane's eight pairs are runs of RUN, of 16 bytes of input where the pairs
-// allow it: run g of lane u starts at pair g * D / 2 / RUNS + RUN * u, so that
-// every load of a wavefront is contiguous.
-template <int PAIRS, bool IB>
-constexpr int kRun = PAIRS == kScattered ? 1 : PAIRS == kNeighbours ? (IB ? 4 : 2) : (IB ? 8 : 4);
-
+// A lane's eight pairs are runs of RUN, of 16 bytes of input where the halves'
+// length is a multiple of that: run g of lane u starts at pair g * D / 2 / RUNS +
+// RUN * u, so that every load of a wavefront is contiguous.
 // LANES for each head; IB, OB: bf16 in and out
-template <int LANES, int PAIRS, bool IB, bool OB>
+template <int LANES, int PAIRS, int RUN, bool IB, bool OB>
 __global__ __launch_bounds__(kThreads) void k_qk_norm_rope(RopeArgs p) {
-    constexpr int ROWS = 64 / LANES, RUN = kRun<PAIRS, IB>, RUNS = 8 / RUN;
+    constexpr int ROWS = 64 / LANES, RUNS = 8 / RUN;
     const int lane = threadIdx.x & 63, u = lane % LANES, r = lane / LANES;
     const int32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t id = blockIdx.x * (kThreads / 64) + wave;
@@ -187,25 +182,30 @@ __global__ __launch_bounds__(kThreads) void k_qk_norm_rope(RopeArgs p) {
 
 int lanes_of(int32_t dim) { return dim <= 16 ? 1 : dim <= 32 ? 2 : dim <= 64 ? 4 : dim <= 128 ? 8 : 16; }
 
-template <int LANES, int PAIRS, bool IB, bool OB>
-void start_typed(const RopeArgs &p, dim3 grid, hipStream_t s) {
-    hipLaunchKernelGGL((k_qk_norm_rope<LANES, PAIRS, IB, OB>), grid, dim3(kThreads), 0, s, p);
-}
-template <int LANES, int PAIRS>
-void start(const RopeArgs &p, bool ib, bool ob, dim3 grid, hipStream_t s) {
-    if (ib)
-        ob ? start_typed<LANES, PAIRS, true, true>(p, grid, s) : start_typed<LANES, PAIRS, true, false>(p, grid, s);
+template <int LANES, int PAIRS, int RUN, bool IB>
+void start(const RopeArgs &p, bool ob, dim3 grid, hipStream_t s) {
+    if (ob)
+        hipLaunchKernelGGL((k_qk_norm_rope<LANES, PAIRS, RUN, IB, true>), grid, dim3(kThreads), 0, s, p);
     else
-        ob ? start_typed<LANES, PAIRS, false, true>(p, grid, s) : start_typed<LANES, PAIRS, false, false>(p, grid, s);
+        hipLaunchKernelGGL((k_qk_norm_rope<LANES, PAIRS, RUN, IB, false>), grid, dim3(kThreads), 0, s, p);
 }
+// the longest runs that no half's end cuts: 8192 tokens of 40 heads of 128 in bf16
+// with 128 elements rotated 28 us (runs of 8), 120 28 (4), 100 32 (2), 90 42 (1);
+// 4096 tokens in fp32 27 (4), 28 (2), 30 (1)
 template <int LANES>
 void start_lanes(const RopeArgs &p, bool ib, bool ob, dim3 grid, hipStream_t s) {
+    const int32_t half = p.rot >> 1;
     if (p.interleaved)
-        start<LANES, kNeighbours>(p, ib, ob, grid, s);
-    else if (p.rot % (ib ? 16 : 8) == 0)
-        start<LANES, kHalves>(p, ib, ob, grid, s);
+        ib ? start<LANES, kNeighbours, 4, true>(p, ob, grid, s) : start<LANES, kNeighbours, 2, false>(p, ob, grid, s);
+    else if (ib)
+        half % 8 == 0   ? start<LANES, kHalves, 8, true>(p, ob, grid, s)
+        : half % 4 == 0 ? start<LANES, kHalves, 4, true>(p, ob, grid, s)
+        : half % 2 == 0 ? start<LANES, kHalves, 2, true>(p, ob, grid, s)
+                        : start<LANES, kHalves, 1, true>(p, ob, grid, s);
     else
-        start<LANES, kScattered>(p, ib, ob, grid, s);
+        half % 4 == 0   ? start<LANES, kHalves, 4, false>(p, ob, grid, s)
+        : half % 2 == 0 ? start<LANES, kHalves, 2, false>(p, ob, grid, s)
+                        : start<LANES, kHalves, 1, false>(p, ob, grid, s);
 }
 
 }  // namespace
