@@ -151,6 +151,7 @@ def test_no_groups(dev):
         return np.array([0]), np.zeros((0, 1)), np.array([], dtype=np.int32)
     run(dev, [(64, [3, 20, 40])], 1, change=change)
     run(dev, [(64, [3, 200, 400])], 1, change=change, max_own=500)
+    run(dev, [(64, [3, 200, 400])], [3, 100, 130], change=change, max_own=500, max_q=1 << 15, kernel="attention_many, attention_join")
 
 
 def test_rows_that_do_not_lie_behind_the_prefix(dev):
