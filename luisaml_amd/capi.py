@@ -648,8 +648,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     """RMS norms of the heads of q [tokens, q_heads, head_dim] and k [tokens,
     k_heads, head_dim] (fp32/bf16, any token and head strides; no norm without a
     gamma) and the rotation of their first rot_dim elements by position, table
-    [rows, rot_dim] as from rope_table (None: no rotation).  Rows whose position is not in the
-    table are left as they were.  q_out may be q, k_out k.  Returns (q_out, k_out)."""
+    [rows, rot_dim] as from rope_table (None: no rotation).  Rows whose position
+    is not in the table are left as they were.  q_out may be q, k_out k.
+    Returns (q_out, k_out)."""
     if q_out is None:
         q_out = _empty(q.shape, out_dtype or q.dtype, q.device, stream)
     if k is not None and k_out is None:

@@ -64,9 +64,9 @@ def test_decode_of_many_sequences(dev, seqs):
     run(dev, n, held, 16, ended=ended, own=rng.integers(0, 3, seqs).tolist(), seed=seqs)
 
 
-@pytest.mark.parametrize("total", [2042, 2043, 2044, 70000])
+@pytest.mark.parametrize("total", [250, 251, 252, 2042, 2043, 2044, 70000])
 def test_prompts_around_the_change_of_kernels(dev, total):
-    run(dev, [total - 1000, 0, 1000], [3, 5, 1000], 16, seed=total)
+    run(dev, [total - total // 3, 0, total // 3], [3, 5, 1000], 16, ended=[0, 1, 0], seed=total)
 
 
 @pytest.mark.parametrize("free", [-4, 0, 1, 5, 12])
