@@ -279,6 +279,7 @@ def prepare(case, seed):
         st["prefix_len"] = _ints(_prefix(case))
         st["prefix_table"] = table[::case["seqs"], :max(prefix)]
         st["max_prefix"], st["max_own"] = max(_prefix(case)), max(x - s * T for x, s in zip(kv, shared))
+        st["max_group_q"] = max(cu[(g + 1) * case["seqs"]] - cu[g * case["seqs"]] for g in range(case["groups"]))
     for name in ("k", "v"):
         # a cache in use: pages of E4M3 values with the scale of their largest
         x = _activations(g, pages, hk, T, d)
@@ -418,7 +419,7 @@ def _pass_own(st):
                        out=st["o"])
     else:
         capi.attention_shared(st["q"], *cache, st["group_seq"], st["prefix_table"], st["prefix_len"], st["max_q"],
-                              st["max_own"], st["max_prefix"], st["sm_scale"], out=st["o"])
+                              st["max_own"], st["max_group_q"], st["max_prefix"], st["sm_scale"], out=st["o"])
 
 
 PLAIN = {"plan": _plain_plan, "rope": _plain_rope, "sinks": _plain_attend, "shared": _plain_attend}
