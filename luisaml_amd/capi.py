@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import importlib
+import operator
 import os
 import re
 
@@ -692,6 +693,23 @@ def _attention_shared_workspace(*sizes):
     return lib().lcml_fp8_attention_shared_workspace_bytes(*sizes)
 
 
+def _with_group_bound(call):
+    """Lets callers of attention_shared give a bound on a group's rows, by name
+    or between max_own and max_prefix.  By place it moves the scale to where
+    `causal` is otherwise, which is no float."""
+    @functools.wraps(call)
+    def given(*args, max_group_q: int | None = None, **kw):
+        if len(args) > 15 and not hasattr(args[15], "__index__") or len(args) == 15 and "scale" in kw:
+            if max_group_q is not None:
+                raise TypeError("attention_shared() got max_group_q twice")
+            args, max_group_q = args[:13] + args[14:], args[13]
+        if max_group_q is not None and operator.index(max_group_q) < 0:
+            raise ValueError(f"max_group_q: {max_group_q}")
+        return call(*args, **kw)
+    return given
+
+
+@_with_group_bound
 def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                      v_scale: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor, cu_q: torch.Tensor,
                      group_seq: torch.Tensor, prefix_table: torch.Tensor, prefix_len: torch.Tensor, max_q: int,
@@ -701,7 +719,10 @@ def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     is the sequences group_seq[g] .. group_seq[g+1]-1, and its first
     prefix_len[g] tokens are read once for all of them, from the pages
     prefix_table[g] (block_table's rows begin with the same ones).  max_own:
-    the most tokens that a sequence has behind them."""
+    the most tokens that a sequence has behind them.  A bound on the rows of a
+    group may stand between max_own and max_prefix (max_group_q=; the scale is
+    a float then): (.., max_q, max_own, max_group_q, max_prefix, scale, ..).  No
+    result depends on it, and the launches need none."""
     if out is None:
         out = _empty(q.shape, out_dtype or q.dtype, q.device, stream)
     if workspace is None:
