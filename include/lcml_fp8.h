@@ -630,7 +630,10 @@ LCML_API int lcml_fp8_attention_sinks(const void *q, int q_dtype, int64_t tokens
  * the order of sums.
  * group_seq, prefix_table and prefix_len are int32 on the device.  Host's
  * bounds, which divide the work (longer ones only take longer): max_own, of a
- * sequence's tokens behind its prefix, and max_prefix; max_q as ever.
+ * sequence's tokens behind its prefix, and max_prefix; max_q as ever.  A launch
+ * holds 2^24 workgroups, of which own tokens take as many as lcml_fp8_attention
+ * would, and the join of parts one for every 1024 / head_dim rows and heads of
+ * `tokens` (one for each where they are fewer than 512 or in more than 16 parts).
  * workspace: lcml_fp8_attention_shared_workspace_bytes(...) bytes, 16-byte
  * aligned, written before they are read.
  */

@@ -1276,24 +1276,77 @@ __device__ inline int32_t skipped(const AttentionArgs &a, const Split &sp, int32
     return 0;
 }
 
+// the first sequence that ends behind row t of the batch, or seqs (t the same
+// in all lanes, and all lanes active): every lane looks at one of 64 places,
+// between two of which a next round looks
+__device__ inline int32_t sequence_of(const AttentionArgs &a, int32_t t) {
+    int32_t lo = 0, hi = a.t.seqs;
+    while (hi > lo) {
+        const int32_t step = (hi - lo + 63) >> 6, up = lo + (int32_t)((threadIdx.x & 63) + 1) * step, at = up < hi ? up : hi;
+        const uint64_t over = __builtin_amdgcn_ballot_w64(a.t.cu[at] > t);
+        if (!over) return hi;
+        const int32_t f = __builtin_ctzll(over), end = lo + (f + 1) * step;
+        hi = (end < hi ? end : hi) - 1, lo += f * step;
+    }
+    return hi;
+}
+// the same for a row of a lane's own, at least `lo`
+__device__ inline int32_t sequence_of_lane(const AttentionArgs &a, int32_t lo, int32_t t) {
+    int32_t hi = a.t.seqs;
+    while (lo < hi) {
+        const int32_t m = (lo + hi) >> 1;
+        if (a.t.cu[m + 1] > t)
+            hi = m;
+        else
+            lo = m + 1;
+    }
+    return lo;
+}
+
 // Joins few parts of many rows: D / 4 threads a row, as many rows a workgroup
-// as fit, and no barriers; every thread weighs all of its row's parts.
+// as fit, and no barriers; every thread weighs all of its row's parts.  Rows
+// are max_q of each sequence, or (kPrefix, kOwn, which always join) those of the
+// batch, each of which looks for its sequence: beside one chunk of a prompt most
+// others would be empty (63 single queries and 2000, 32 heads of 128, behind
+// 2048: 505 us and 265 with attention; 8 x 100 behind 8192 177.5 and 179.5).
 template <bool BF16, Form F>
 __global__ __launch_bounds__(256) void k_attention_join_rows(AttentionArgs a, Split sp, uint32_t total) {
     const int32_t D = a.t.dim, q4 = D >> 2, per = 256 / q4;
     const int32_t grp = threadIdx.x / q4, d = (threadIdx.x - grp * q4) * 4;
-    const uint32_t id = blockIdx.x * (uint32_t)per + grp;
+    const uint32_t id0 = blockIdx.x * (uint32_t)per, id = id0 + grp;
+    const int32_t parts = parts_of<F>(sp);
+    float x[kRowsSplits];
+    auto load = [&](int64_t row) {
+#pragma unroll
+        for (int k = 0; k < kRowsSplits; ++k) x[k] = sp.lse[row * parts + (k < parts ? k : 0)];
+    };
+    int32_t b = 0, i, h;
+    if constexpr (kShares<F>) {
+        load(id < total ? id : id0);  // under way while the sequence is looked for
+        b = sequence_of(a, id0 / a.q_heads);
+    }
     if (grp >= per || id >= total) return;
-    const uint32_t per_seq = (uint32_t)(a.max_q * a.q_heads);
-    const int32_t b = id / per_seq, at = id - b * per_seq, i = at / a.q_heads, h = at - i * a.q_heads;
+    if constexpr (kShares<F>) {
+        i = id / a.q_heads, h = id - i * a.q_heads;
+        if (b < a.t.seqs && a.t.cu[b + 1] <= i) b = sequence_of_lane(a, b + 1, i);
+        if (b >= a.t.seqs) return;
+    } else {
+        const uint32_t per_seq = (uint32_t)(a.max_q * a.q_heads);
+        b = id / per_seq;
+        const int32_t at = id - b * per_seq;
+        i = at / a.q_heads, h = at - i * a.q_heads;
+    }
     const SeqRows s = seq_rows(a.t, b);
+    if constexpr (kShares<F>) {
+        i -= s.row0;
+        if (i < 0 || i >= a.max_q) return;
+    }
     if (i >= s.n) return;
     const int64_t row = ((int64_t)s.row0 + i) * a.q_heads + h;
-    const int32_t parts = parts_of<F>(sp), skip = skipped<F, true>(a, sp, b, s);
-    const float *lse = sp.lse + row * parts, *po = sp.o + row * parts * D + d;
-    float x[kRowsSplits], w[kRowsSplits], top = -kInf, sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kRowsSplits; ++k) x[k] = lse[k < parts ? k : 0];
+    const int32_t skip = skipped<F, true>(a, sp, b, s);
+    const float *po = sp.o + row * parts * D + d;
+    float w[kRowsSplits], top = -kInf, sum = 0.0f;
+    if (!kShares<F>) load(row);
     if (kShares<F>)
 #pragma unroll
         for (int k = 0; k < kRowsSplits; ++k) x[k] = k < skip || k >= parts ? -kInf : x[k];
@@ -1329,15 +1382,35 @@ __global__ __launch_bounds__(256) void k_attention_join(AttentionArgs a, Split s
     __shared__ float weight[kMostSplits];
     __shared__ f4 buf[256];
     const int32_t D = a.t.dim, q4 = D >> 2, lane = threadIdx.x & 63;
-    const int64_t per = a.max_q * a.q_heads;
-    const int32_t b = (int32_t)(blockIdx.x / per), i = (int32_t)(blockIdx.x % per / a.q_heads), h = (int32_t)(blockIdx.x % a.q_heads);
-    const SeqRows s = seq_rows(a.t, b);
+    const int32_t parts = parts_of<F>(sp);
+    int32_t b, i, h;
+    SeqRows s;
+    float x0 = -kInf, x1 = -kInf;
+    auto load = [&](int64_t row, int32_t skip) {
+        x0 = lane < parts && lane >= skip ? sp.lse[row * parts + lane] : -kInf;
+        x1 = lane + 64 < parts && lane + 64 >= skip ? sp.lse[row * parts + lane + 64] : -kInf;
+    };
+    if constexpr (kShares<F>) {
+        load(blockIdx.x, 0);  // under way while the sequence is looked for
+        i = blockIdx.x / a.q_heads, h = blockIdx.x - i * a.q_heads;
+        b = sequence_of(a, i);
+        if (b >= a.t.seqs) return;
+        s = seq_rows(a.t, b);
+        i -= s.row0;
+        if (i < 0 || i >= a.max_q) return;
+    } else {
+        const int64_t per = a.max_q * a.q_heads;
+        b = (int32_t)(blockIdx.x / per), i = (int32_t)(blockIdx.x % per / a.q_heads), h = (int32_t)(blockIdx.x % a.q_heads);
+        s = seq_rows(a.t, b);
+    }
     if (i >= s.n) return;
     const int64_t row = ((int64_t)s.row0 + i) * a.q_heads + h;
-    const int32_t parts = parts_of<F>(sp), skip = skipped<F, false>(a, sp, b, s);
-    const float *lse = sp.lse + row * parts, *po = sp.o + row * parts * D;
-    const float x0 = lane < parts && lane >= skip ? lse[lane] : -kInf;
-    const float x1 = lane + 64 < parts && lane + 64 >= skip ? lse[lane + 64] : -kInf;
+    const int32_t skip = skipped<F, false>(a, sp, b, s);
+    const float *po = sp.o + row * parts * D;
+    if constexpr (kShares<F>)
+        x0 = lane < skip ? -kInf : x0, x1 = lane + 64 < skip ? -kInf : x1;
+    else
+        load(row, skip);
     float top = fmaxf(x0, x1);
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
@@ -1496,17 +1569,27 @@ hipError_t start_attention_many(const AttentionArgs &a, const Plan &p, hipStream
     return hipGetLastError();
 }
 
+// rows that a join goes through, and its workgroups: from 512 rows on many rows
+// a workgroup (8 x 16 x 32 rows of 4 parts 40.5 us with attention, a workgroup a
+// row 44; 16384 rows of 2 parts 22 and 43; 128 rows of 16 parts 15.7 and 15.0,
+// before the parts' weights were divided)
+struct Join {
+    int64_t rows, groups;
+    bool many;
+};
+inline Join make_join(int64_t rows, int64_t parts, int64_t dim) {
+    const int64_t per = 1024 / dim;
+    const bool many = rows >= 512 && parts <= kRowsSplits;
+    return Join{rows, many ? (rows + per - 1) / per : rows, many};
+}
+
 template <Form F, int NP>
 hipError_t start_join(const AttentionArgs &a, const Split &sp, int32_t parts, hipStream_t s) {
-    const unsigned rows = (unsigned)((int64_t)a.t.seqs * a.max_q * a.q_heads);
-    const unsigned per = 1024u / a.t.dim;
-    // from 512 rows on many rows a workgroup (8 x 16 x 32 rows of 4 parts 40.5 us
-    // with attention, a workgroup a row 44; 16384 rows of 2 parts 22 and 43; 128
-    // rows of 16 parts 15.7 and 15.0, before the parts' weights were divided)
-    if (rows >= 512 && parts <= kRowsSplits)
-        hipLaunchKernelGGL((k_attention_join_rows<NP == 1, F>), dim3((rows + per - 1) / per), dim3(256), 0, s, a, sp, rows);
+    const Join j = make_join((kShares<F> ? a.t.tokens : a.t.seqs * a.max_q) * a.q_heads, parts, a.t.dim);
+    if (j.many)
+        hipLaunchKernelGGL((k_attention_join_rows<NP == 1, F>), dim3((unsigned)j.groups), dim3(256), 0, s, a, sp, (uint32_t)j.rows);
     else
-        hipLaunchKernelGGL((k_attention_join<NP == 1, F>), dim3(rows), dim3(256), 0, s, a, sp);
+        hipLaunchKernelGGL((k_attention_join<NP == 1, F>), dim3((unsigned)j.groups), dim3(256), 0, s, a, sp);
     return hipGetLastError();
 }
 

@@ -7,7 +7,8 @@ namespace lcml {
 int64_t attention_shared_workspace(int64_t tokens, int64_t seqs, int64_t groups, int64_t q_heads, int64_t kv_heads,
                                    int64_t dim, int64_t max_q, int64_t max_own, int64_t max_prefix, int64_t *workgroups) {
     const SharedPlan p = make_shared_plan(tokens, seqs, groups, q_heads, kv_heads, dim, max_q, max_own, max_prefix);
-    *workgroups = p.prefix.groups + p.own.groups;
+    const int64_t joined = make_join(tokens * q_heads, p.own.sp.parts, dim).groups, both = p.prefix.groups + p.own.groups;
+    *workgroups = both > joined ? both : joined;
     return tokens * q_heads * p.own.sp.parts * (dim + 1) * 4;
 }
 

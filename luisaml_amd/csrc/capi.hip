@@ -1181,7 +1181,7 @@ int lcml_fp8_attention_shared(const void *q, int q_dtype, int64_t tokens, int64_
         return fail(LCML_ERR_INVALID_ARG, "%s: NULL index array", fn);
     if (!aligned(group_seq, 4) || !aligned(prefix_len, 4) || !aligned(prefix_table, 4))
         return fail(LCML_ERR_INVALID_ARG, "%s: index arrays not 4-byte aligned", fn);
-    if (tokens * (q_heads / kv_heads) > kMostGroups * 16 || seqs * max_q >= kMostGroups / q_heads) return too_large(fn, c);
+    if (tokens * (q_heads / kv_heads) > kMostGroups * 16) return too_large(fn, c);
     int64_t workgroups = 0;
     const int64_t need = lcml::attention_shared_workspace(tokens, seqs, groups, q_heads, kv_heads, head_dim, max_q, max_own,
                                                           max_prefix, &workgroups);

@@ -172,7 +172,7 @@ int64_t attention_groups(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_
 hipError_t launch_attention(const AttentionArgs &a, void *work, hipStream_t s, const char **kernel);
 // window > 0 and sinks > 0
 hipError_t launch_attention_sinks(const AttentionArgs &a, void *work, hipStream_t s, const char **kernel);
-// a.max_kv: of a sequence's own tokens
+// a.max_kv: of a sequence's own tokens; *workgroups: of the larger of its launches
 int64_t attention_shared_workspace(int64_t tokens, int64_t seqs, int64_t groups, int64_t q_heads, int64_t kv_heads,
                                    int64_t dim, int64_t max_q, int64_t max_own, int64_t max_prefix, int64_t *workgroups);
 hipError_t launch_attention_shared(const AttentionArgs &a, const int32_t *prefix_table, int64_t prefix_stride,

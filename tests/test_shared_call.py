@@ -58,6 +58,26 @@ def test_refused(passed):
             call()
 
 
+P = 0x1000
+
+
+def entry(tokens, seqs, max_q, workspace=None, heads=32):
+    return capi.lib().lcml_fp8_attention_shared(
+        P, 16, tokens, heads, heads * 128, 128, P, 16, heads * 128, 128, P, P, P, P, 8, 8, 128, 16, P, 4, 4, P, P, seqs, P, P, 4, 4, P,
+        1, max_q, 800, 4096, 0.1, 1, workspace, 0, None)
+
+
+@pytest.mark.parametrize("tokens,seqs,max_q", [(8255, 64, 8192), (2303, 256, 2048), (100000, 64, 65536), (1000000, 4, 250000)])
+def test_single_tokens_beside_a_chunk_are_accepted(tokens, seqs, max_q):
+    """Up to the check of the workspace, which comes last."""
+    assert entry(tokens, seqs, max_q) == capi.ERR_INVALID_ARG and "workspace" in capi.last_error()
+
+
+@pytest.mark.parametrize("tokens,seqs,max_q", [(1 << 27, 1, 1 << 27), (1 << 20, 1 << 20, 1 << 20)])
+def test_sizes_past_a_launch(tokens, seqs, max_q):
+    assert entry(tokens, seqs, max_q) == capi.ERR_UNSUPPORTED and "exceeds one launch" in capi.last_error()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 40])
 def test_same_bits(dev, n):
