@@ -952,8 +952,10 @@ int lcml_fp8_kv_cache_plan(const int32_t *new_tokens, const int32_t *kv_len_in, 
     if (page_tokens < 16 || page_tokens > 256 || (page_tokens & (page_tokens - 1)))
         return fail(LCML_ERR_UNSUPPORTED, "%s: page_tokens=%lld (16, 32, 64, 128 or 256)", fn, (long long)page_tokens);
     const int64_t most = ((int64_t)1 << 31) - 1;
-    if (seqs >= most || pages > most || table_cols > most || tokens > most)
+    if (pages > most || table_cols > most || tokens > most)
         return fail(LCML_ERR_UNSUPPORTED, "%s: a size of 2^31 or more", fn);
+    if (seqs > (int64_t)1 << 30)  // indexes of sequences are added in 32 bits
+        return fail(LCML_ERR_UNSUPPORTED, "%s: seqs=%lld (2^30 at most)", fn, (long long)seqs);
     if (table_stride < table_cols)
         return fail(LCML_ERR_INVALID_ARG, "%s: table_stride=%lld < table_cols=%lld", fn, (long long)table_stride,
                     (long long)table_cols);

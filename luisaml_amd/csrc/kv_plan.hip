@@ -66,7 +66,7 @@ __device__ inline void block_scan(int64_t (&v)[N], int64_t (&total)[N], int64_t 
     }
 }
 
-// the last of at[0 .. n] (rising, at[0] <= i < at[n]) that is not above i
+// the last of at[0 .. n] (rising, at[0] <= i < at[n], n <= 2^30) that is not above i
 template <class T>
 __device__ inline int32_t find(const T *at, int32_t n, int64_t i) {
     int32_t lo = 0, hi = n;
