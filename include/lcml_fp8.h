@@ -520,7 +520,8 @@ LCML_API int lcml_fp8_kv_cache_read(const uint8_t *k_cache, const uint8_t *v_cac
  * Row cu_q[b] + i: positions = old + i, slots = page * page_tokens + position %
  * page_tokens, -1 where it has no page; rows from cu_q[seqs] up to `tokens` have
  * -1 in both.
- * Up to 2^30 sequences, other sizes below 2^31.
+ * Up to 2^30 sequences, other sizes below 2^31; lengths and offsets that would
+ * pass 2^31 - 1 stay there.
  * ended and first_own (all 0), positions and slots may be NULL; kv_len may be
  * kv_len_in, and left free_count: a captured step then runs on by itself.
  * workspace: lcml_fp8_kv_cache_plan_workspace_bytes(seqs, tokens) bytes, 8-byte

@@ -90,7 +90,7 @@ struct KvPlan {
     int32_t *positions;             // [tokens] or NULL
     int64_t *slots;                 // [tokens] or NULL
     int64_t tokens;
-    int64_t *work;  // [seqs + 2]: new columns before each sequence, all of them, the stack's height
+    int64_t *work;  // [seqs + 2]: new columns before each sequence, all of them, two words (kv_plan.hip)
 };
 
 // the smallest power of two s >= 2^-126 with a <= 448 s, for finite a >= 0:

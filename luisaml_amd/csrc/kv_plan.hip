@@ -80,7 +80,8 @@ __device__ inline int32_t find(const T *at, int32_t n, int64_t i) {
     return lo;
 }
 
-__device__ inline int32_t clamp32(int64_t v) { return (int32_t)(v < 0x7fffffff ? v : 0x7fffffff); }
+constexpr int32_t kMostRows = 0x7fffffff;  // of all sequences, and tokens of one: as far as int32 goes
+__device__ inline int32_t clamp32(int64_t v) { return (int32_t)(v < kMostRows ? v : kMostRows); }
 
 // columns of n tokens, as far as the table goes
 __device__ inline int32_t columns(const KvPlan &p, int32_t n) {
@@ -90,9 +91,10 @@ __device__ inline int32_t columns(const KvPlan &p, int32_t n) {
 
 // What is left to write once the sums are there: the new columns' pages, and
 // the rows' positions and slots.  cu: row offsets; need: new columns before
-// each sequence; both [seqs + 1]; kv: lengths.
+// each sequence; both [seqs + 1]; kv: lengths; cut: the first position of the
+// sequence whose rows end at kMostRows, where its offsets may not say it.
 __device__ inline void emit(const KvPlan &p, const int32_t *cu, const int64_t *need, const int32_t *kv, int32_t top,
-                            int64_t first, int64_t step) {
+                            int32_t cut, int64_t first, int64_t step) {
     const int64_t fresh = need[p.seqs], rows = p.positions || p.slots ? p.tokens : 0;
     const int64_t most = fresh > rows ? fresh : rows;
     for (int64_t i = first; i < most; i += step) {
@@ -107,7 +109,7 @@ __device__ inline void emit(const KvPlan &p, const int32_t *cu, const int64_t *n
         }
         if (i < rows && i < cu[p.seqs]) {
             const int32_t b = find(cu, p.seqs, i);
-            pos = kv[b] - (cu[b + 1] - (int32_t)i);
+            pos = cu[b + 1] < kMostRows ? kv[b] - (cu[b + 1] - (int32_t)i) : cut + ((int32_t)i - cu[b]);
             const int32_t c = pos >> p.tshift, old = columns(p, kv[b]) - (int32_t)(need[b + 1] - need[b]);
             if (p.slots && c < p.table_cols) {
                 const int64_t at = top - 1 - (need[b] + c - old);
@@ -138,7 +140,9 @@ __global__ __launch_bounds__(NT) void k_kv_plan(KvPlan p) {
     __shared__ int64_t lens[NT + 1];
     __shared__ int32_t firsts[NT], counts[2][kCounts];
     __shared__ int64_t s_need[ALL ? NT + 1 : 1];
-    __shared__ int32_t s_cu[ALL ? NT + 1 : 1], s_kv[ALL ? NT : 1];
+    __shared__ int32_t s_cu[ALL ? NT + 1 : 1], s_kv[ALL ? NT : 1], s_cut;
+    // work's last element: the stack's height, and `cut`
+    int32_t *const last = ALL ? nullptr : reinterpret_cast<int32_t *>(p.work + p.seqs + 1);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int turn = 0;
     int32_t top = p.free_in[0];
@@ -201,6 +205,7 @@ __global__ __launch_bounds__(NT) void k_kv_plan(KvPlan p) {
                 s_need[tid] = at[1], s_cu[tid] = row, s_kv[tid] = kv;
             else
                 p.work[b] = fresh + at[1];
+            if (row < kMostRows && rows + at[0] + (kv - old) >= kMostRows) (ALL ? &s_cut : last + 1)[0] = old;
         }
         rows += total[0], fresh += total[1];
     }
@@ -214,11 +219,11 @@ __global__ __launch_bounds__(NT) void k_kv_plan(KvPlan p) {
         if (ALL)
             s_need[p.seqs] = fresh, s_cu[p.seqs] = clamp32(rows);
         else
-            p.work[p.seqs] = fresh, p.work[p.seqs + 1] = top;
+            p.work[p.seqs] = fresh, last[0] = top;
     }
     if constexpr (ALL) {
         __syncthreads();  // and the returned pages
-        emit(p, s_cu, s_need, s_kv, top, tid, NT);
+        emit(p, s_cu, s_need, s_kv, top, s_cut, tid, NT);
     }
 }
 
@@ -226,7 +231,8 @@ template <bool LDS>
 __global__ __launch_bounds__(kEmitThreads) void k_kv_plan_emit(KvPlan p) {
     __shared__ int32_t cu[LDS ? kLdsSeqs + 1 : 1], kv[LDS ? kLdsSeqs : 1];
     __shared__ int64_t need[LDS ? kLdsSeqs + 1 : 1];
-    const int32_t top = (int32_t)p.work[p.seqs + 1];
+    const int32_t *const last = reinterpret_cast<const int32_t *>(p.work + p.seqs + 1);
+    const int32_t top = last[0], cut = last[1];
     const int64_t first = (int64_t)blockIdx.x * kEmitThreads + threadIdx.x, step = (int64_t)gridDim.x * kEmitThreads;
     if constexpr (LDS) {
         for (int32_t b = threadIdx.x; b <= p.seqs; b += kEmitThreads) {
@@ -234,9 +240,9 @@ __global__ __launch_bounds__(kEmitThreads) void k_kv_plan_emit(KvPlan p) {
             if (b < p.seqs) kv[b] = p.kv_len[b];
         }
         __syncthreads();
-        emit(p, cu, need, kv, top, first, step);
+        emit(p, cu, need, kv, top, cut, first, step);
     } else {
-        emit(p, p.cu_q, p.work, p.kv_len, top, first, step);
+        emit(p, p.cu_q, p.work, p.kv_len, top, cut, first, step);
     }
 }
 
