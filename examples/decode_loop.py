@@ -6,12 +6,16 @@
 The system prompt is prefilled once, as a sequence of its own; every request's
 row of the page table begins with its pages, and attention reads them once for
 all requests.  Without one, attention may instead look through a window beside
-which the first tokens stay visible, so that a request can go on for any length
-of time.  What a step needs from the host is how many tokens each request
-brings; a step of single tokens is captured in a HIP graph and replayed while
-requests grow, end and start, on a batch that is padded to the graph's rows.
+which the first tokens stay visible: a step then reads no more than these, while
+the pages that the window has passed stay with their request until it ends.  A
+request ends at --most tokens, as many as the page table and the table of
+rotations are made for.  What a step needs from the host is how many tokens each
+request brings; a step of single tokens is captured in a HIP graph and replayed
+on a batch that is padded to the graph's rows, and between replays requests end
+(a plan of its own, which takes their pages back) and start (their slot's first
+pages and length are written).
 
-    python examples/decode_loop.py [--window 512 --sinks 4] [--steps 200]
+    python examples/decode_loop.py [--window 512 --sinks 4] [--steps 200] [--most 8192]
 """
 from __future__ import annotations
 
@@ -41,7 +45,8 @@ class RotaryLayer(DecoderLayer):
     def __call__(self, x, add, batch: "Requests", max_q):
         rows = len(x)
         (q, k, v), h = self.project(x, add)
-        q, k = capi.qk_norm_rope(q, k, batch.positions[:rows], self.turns, self.q_gamma, self.k_gamma, self.eps)
+        # (in place: rows that the batch is padded with keep the projection's values)
+        q, k = capi.qk_norm_rope(q, k, batch.positions[:rows], self.turns, self.q_gamma, self.k_gamma, self.eps, q_out=q, k_out=k)
         capi.kv_cache_write(k, v, *batch.cache_args(), max_q)
         o = torch.zeros(rows, self.heads, self.dim, device=x.device)  # rows that the batch is padded with stay 0
         if batch.prefix:
@@ -83,7 +88,7 @@ class RotaryLayer(DecoderLayer):
 class Requests:
     """A layer's cache and the requests in it: a slot each, and one more sequence
     for the system prompt.  All of it lives on the device; the host only says
-    what each slot brings."""
+    what each slot brings, and counts along, as a request ends at `most` tokens."""
 
     def __init__(self, slots, prefix, most, pages, kv_heads, page_tokens, head_dim, rows, device):
         ints = lambda n, v=0: torch.full((n,), v, dtype=torch.int32, device=device)  # noqa: E731
@@ -99,6 +104,7 @@ class Requests:
         self.cu_q, self.positions = ints(slots + 2), ints(rows, -1)
         self.group_seq = torch.tensor([0, slots], dtype=torch.int32, device=device)
         self.prefix_len = ints(1, prefix)
+        self.held, self.bringing = [0] * (slots + 1), {}  # the host's count
 
     def cache_args(self):
         return (*self.cache, self.block_table, self.kv_len, self.cu_q)
@@ -111,9 +117,21 @@ class Requests:
         new = [0] * (self.slots + 1)
         for b, n in tokens.items():
             new[b] = n
+        self.bringing = dict(tokens)
         self.new.copy_(torch.tensor(new, dtype=torch.int32), non_blocking=True)
 
+    def grow(self):
+        """The host's count of a step: of each plan, and before each replay of a
+        captured one."""
+        for b, n in self.bringing.items():
+            if self.held[b] + n > self.most:
+                raise ValueError(f"slot {b} holds {self.held[b]} tokens and brings {n}: {self.most} at most")
+        for b, n in self.bringing.items():
+            self.held[b] += n
+
     def plan(self, rows):
+        if not torch.cuda.is_current_stream_capturing():
+            self.grow()
         capi.kv_cache_plan(self.new, self.kv_len, self.block_table, self.free_pages, self.left, self.T, ended=self.ended,
                            first_own=self.first_own, kv_len_out=self.kv_len, cu_q=self.cu_q, left=self.left,
                            positions=self.positions[:rows])
@@ -124,12 +142,16 @@ class Requests:
         self.ended[slots] = 1
         self.plan(0)
         self.ended.zero_()
+        for b in slots:
+            self.held[b] = 0
 
     def start(self, slots):
         """Empty slots begin behind the system prompt."""
         cols = self.prefix // self.T
         self.block_table[slots, :cols] = self.block_table[self.slots, :cols]
         self.kv_len[slots] = self.prefix
+        for b in slots:
+            self.held[b] = self.prefix
 
 
 def main():
@@ -138,12 +160,14 @@ def main():
     ap.add_argument("--window", type=int, default=0)
     ap.add_argument("--sinks", type=int, default=4)
     ap.add_argument("--steps", type=int, default=200)
+    ap.add_argument("--most", type=int, default=8192, help="tokens at which a request ends")
     args = ap.parse_args()
     dev = torch.device("cuda:0")
-    hidden, slots, T, most = 4096, 16, 64, 8192
+    hidden, slots, T, most = 4096, 16, 64, args.most
     prefix = 0 if args.window else args.prefix
     layer = RotaryLayer(hidden, 32, 8, 128, 11008, dev, most, args.window, args.sinks)
-    batch = Requests(slots, prefix, most, 2048, 8, T, 128, most, dev)
+    first = {b: 50 + 37 * b for b in range(slots)}
+    batch = Requests(slots, prefix, most, 2048, 8, T, 128, max(prefix, sum(first.values())), dev)
     g = torch.Generator(device=dev).manual_seed(1)
     tokens = lambda n: (torch.randn(n, hidden, device=dev, generator=g),  # noqa: E731
                         torch.zeros(n, hidden, device=dev, dtype=torch.bfloat16))
@@ -157,7 +181,7 @@ def main():
         prompt({slots: prefix})
     for b in range(slots):
         batch.start([b])
-    prompt({b: 50 + 37 * b for b in range(slots)})
+    prompt(first)
 
     x, add = tokens(slots)
     batch.brings(dict.fromkeys(range(slots), 1))
@@ -176,12 +200,15 @@ def main():
     torch.cuda.synchronize()
     spent = 0.0
     for i in range(args.steps):
-        if i % 20 == 10:  # one request ends, and another takes its slot
-            b = i // 20 % slots
-            batch.end([b])
-            batch.start([b])
-            prompt({b: 100})
+        gone = {b for b in range(slots) if batch.held[b] == most}
+        if i % 20 == 10:
+            gone.add(i // 20 % slots)
+        if gone:  # requests end, and others take their slots
+            batch.end(sorted(gone))
+            batch.start(sorted(gone))
+            prompt(dict.fromkeys(gone, 100))
             batch.brings(dict.fromkeys(range(slots), 1))
+        batch.grow()
         torch.cuda.synchronize()
         t = time.perf_counter()
         graph.replay()
