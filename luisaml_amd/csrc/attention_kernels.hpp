@@ -1530,8 +1530,8 @@ inline Plan make_plan(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t d
                       int64_t window, int64_t sinks) {
     const int64_t rows = max_q * (q_heads / kv_heads), pairs = seqs * kv_heads;
     int64_t span = max_kv;  // tokens that a row tile can see
-    if (window > 0 && window < span && window + sinks + max_q + 128 < span)
-        span = window + max_q + 64 + (sinks + 63) / 64 * 64;
+    const int64_t tile = window + max_q + 64 + (sinks + 63) / 64 * 64;
+    if (window > 0 && tile < span) span = tile;
     return divide(few_rows(pairs, dim, rows, max_kv), pairs, rows, span);
 }
 
