@@ -516,7 +516,10 @@ LCML_API int lcml_fp8_kv_cache_read(const uint8_t *k_cache, const uint8_t *v_cac
  * order, or -1 when there is none; other entries of block_table stay, and so do
  * entries of free_pages that nothing was put on.  left[0]: free pages that
  * remain, negative if as many were lacking (a later call's free_count; negative
- * counts as 0).  A page must not be in the stack twice, nor be its sequence's.
+ * counts as 0).  A column that got -1 is not looked at again, and its tokens
+ * count in kv_len: a sequence that found no page goes on by ending (`ended`, which
+ * puts the pages that it has on the stack) and bringing its tokens again.  A page
+ * must not be in the stack twice, nor be its sequence's.
  * Row cu_q[b] + i: positions = old + i, slots = page * page_tokens + position %
  * page_tokens, -1 where it has no page; rows from cu_q[seqs] up to `tokens` have
  * -1 in both.
@@ -552,10 +555,10 @@ LCML_API int lcml_fp8_kv_cache_plan(const int32_t *new_tokens, const int32_t *kv
  *   table: [table_rows][rot_dim] floats, row p the rot_dim / 2 cosines of
  *     position p and then its sines.
  *   positions: [tokens] int32.  A row whose position is negative or not below
- *     table_rows is left as it was.  (rot_dim 0: any position, and NULL takes
- *     every row.)
+ *     table_rows is left as it was.  (rot_dim 0: any that is not negative, and
+ *     NULL takes every row.)
  * head_dim 16 to 256 in steps of 16, rot_dim even.  A head whose sum of squares
- * overflows fp32 gives zeros, as the formula does.
+ * overflows fp32 gives zeros, as the formula in fp32 does.
  * No counterpart in the reference.
  */
 LCML_API int lcml_fp8_qk_norm_rope(const void *q, const void *k, int dtype, int64_t tokens, int64_t q_heads,

@@ -820,12 +820,13 @@ __global__ __launch_bounds__(NW * 64, DC <= 2 ? 2 : 1) void k_attention_few(Atte
 // widened as well: 2% slower).  32x32x16 instructions.
 //
 // A prompt of 8192 tokens, 32 heads over 8 of 128, 0.55 TFLOP: 588 to 605 us,
-// 920 TFLOP/s, where a product of 8192^3 in bf16 reaches 1190.  A step's 32 matrix
-// instructions take 1024 cycles of a SIMD, its 320 vector ones 1280, and two
-// wavefronts a SIMD overlap them to two thirds of the sum.  (Two groups of
-// wavefronts half a step apart: 1075 us, for the registers spilled.)  D > 128
-// has one wavefront a SIMD, and nothing to overlap LDS reads with: 220 TFLOP/s
-// on a prompt of 2048 tokens, 260 on one of 4000.  What happens around a step is
+// 920 TFLOP/s, where a library's product of 8192^3 in bf16 reaches 1190 to 1625 by
+// the order of its operands.  A step's 32 matrix instructions take 1024 cycles of
+// a SIMD, its 320 vector ones 1280, and two wavefronts a SIMD overlap them to two
+// thirds of the sum.  (Two groups of wavefronts half a step apart: 1075 us, for the
+// registers spilled.)  D > 128 has one wavefront a SIMD, and nothing to overlap LDS
+// reads with: 220 TFLOP/s on a prompt of 2048 tokens, 260 on one of 4000, 510 on one
+// of 8192 through a window of 2048 (heads of 256).  What happens around a step is
 // in three loops, always inlined: out of line, its registers lie in scratch.
 constexpr int kManyWaves = 4, kManyRows = 32 * kManyWaves;
 

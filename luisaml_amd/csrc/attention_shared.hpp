@@ -55,7 +55,13 @@ inline void cap_parts(Plan &p) {
 // 64 queries behind 16384 tokens (16 row tiles): 16 parts 51 us, 17 (272
 // workgroups) 56, 24 55, 32 62; 560 rows of 3 groups behind 6000 (74 tiles): 3
 // parts 70 us, 6 53, 8 64; 8 x 100 rows behind 8192 (200 tiles): 3 parts 201 us,
-// 5 174.
+// 5 174.  Other heads enter by a factor alone, and the model misses more there.
+// What it takes and the best of 1 to 48 parts, in us: 64 queries of 32 heads over
+// 8 behind 16384, heads of 64 40.5 and 36.3 (32 parts), 96 45.2 and 45.0, 128 50.0
+// both, 256 (16 over 4) 71.3 and 62.3 (24); 8 x 100 behind 8192 64 136 and 115 (5),
+// 96 162 and 148 (5), 256 241 both; 3 groups of 5 x 40 behind 6000 (16 over 2) 64
+// 47.1 and 44.8 (6), 96 60.8 and 58.5 (5), 256 172 and 163 (3), 128 in fp32 90.6
+// and 87.8 (6).
 inline void divide_prefix(Plan &p, const Plan &own, int64_t dim, int64_t span) {
     const int64_t groups = p.groups / p.sp.splits, steps = (span + 63) / 64;
     const int64_t most = steps / 4 > kMostParts ? kMostParts : steps / 4;  // four steps at least

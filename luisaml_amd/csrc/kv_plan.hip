@@ -12,9 +12,10 @@
 // sums, and a second launch writes the new columns and the rows, each finding
 // its sequence by bisection in LDS.
 //
-// Measured: 64 sequences of a decode step 4.0 us in a graph, 5.2 where pages
-// come back (one round trip more), 256 4.7, 1024 7.0, 4096 17; 48 prompts, 196 000
-// rows, 7.7 in two launches, 13 with 4400 pages that come back.
+// Measured: 64 sequences of a decode step 4.0 us in a graph, 5.4 where pages
+// come back (one round trip more), 256 4.3 and 6.5, 1024 6.5 and 9.9, 4096 17 and
+// 33; 48 prompts, 196 000 rows, 7.7 in two launches, 13 with 4400 pages that come
+// back.
 #include "kv_cache.hpp"
 #include "lcml_internal.hpp"
 
@@ -246,9 +247,9 @@ __global__ __launch_bounds__(kEmitThreads) void k_kv_plan_emit(KvPlan p) {
     }
 }
 
-// One launch or two, in us in a graph: 64 sequences of 512 rows in all 4.5 and 6.6,
-// 1024 5.4 and 6.7, 2048 6.4 and 6.7, 4096 8.5 and 6.9; 1000 of 2000 7.3 and 9.7; 8
-// of 4096 7.5 and 6.5.
+// One launch or two, in us in a graph: 64 sequences of 512 rows in all 5.1 and 6.7,
+// 1024 5.1 and 6.9, 2048 6.3 and 6.8, 4096 8.5 and 6.9; 1000 of 2000 7.9 and 9.5; 8
+// of 2048 5.6 and 6.7, of 4096 7.3 and 6.5.
 bool at_once(int64_t seqs, int64_t tokens) { return seqs <= kMostThreads && tokens <= 2 * kMostThreads; }
 
 }  // namespace
@@ -258,8 +259,9 @@ int64_t kv_plan_workspace(int64_t seqs, int64_t tokens) { return at_once(seqs, t
 hipError_t launch_kv_plan(const KvPlan &p, hipStream_t s, const char **kernel) {
     if (at_once(p.seqs, p.tokens)) {
         *kernel = "kv_plan";
-        // 64 sequences, 64 rows: 3.4 us with 256 threads, 4.4 with 1024; 256 and 256 4.1
-        // and 4.8, 200 and 400 4.7 both, 256 and 512 5.1 and 4.8
+        // 64 sequences, 64 rows: 4.0 us with 256 threads, 5.1 with 1024; 256 and 256 4.3
+        // and 5.5, 200 and 400 5.5 both, 256 and 512 5.5 both (where pages come back
+        // 5.4 and 7.3, 6.5 and 7.8, 7.1 and 7.8, 7.7 and 7.9)
         if (p.seqs <= 256 && p.tokens <= 256)
             hipLaunchKernelGGL((k_kv_plan<256, true>), dim3(1), dim3(256), 0, s, p);
         else
